@@ -192,6 +192,112 @@ KL_API kl_status kl_mx_quantize(const void* x, int32_t x_type, int64_t rows, int
 KL_API kl_status kl_nv_quantize(const void* x, int32_t x_type, int64_t rows, int64_t k, int64_t ldx, void* q,
                                 int64_t ldq, void* scales, float* global_scale, void* stream);
 
+/* ---- mixture-of-experts routing around the m-grouped GEMM -----------------------------------
+ * kl_moe_route chooses every token's experts and measures their balance; kl_moe_plan turns the ids
+ * into the row layout that kl_gemm takes with m_block_group, kl_moe_dispatch copies the tokens' rows
+ * into it and kl_moe_combine sums the experts' rows back. No counterpart in the reference. All are
+ * stream-ordered, allocate nothing and may be captured; the current device must be the stream's.
+ * Launches overlap the end of the kernel before them (programmatic dependent launch) and touch
+ * global memory only once it has completed. */
+
+typedef struct kl_moe_route_desc {
+  const void* logits;   /* device [tokens, ld_logits], logits_type KL_BF16, KL_F16 or KL_F32 */
+  int64_t ld_logits;
+  int64_t tokens;       /* below 2^26 */
+  int64_t experts;      /* 1 .. 1024 */
+  int64_t k;            /* experts of a token: 1 .. min(experts, 32) */
+  int32_t logits_type;
+  int32_t renormalize;  /* 0: weights are probabilities; 1: divided by their sum over the token's k */
+  const uint8_t* valid; /* device [tokens] or NULL: 0 = padding, not routed, its logits not read */
+  int32_t* ids;         /* device [tokens, k] */
+  float* weights;       /* device [tokens, k] */
+  int32_t* counts;      /* device [experts] */
+  int32_t* routed;      /* device [1] */
+  float* loss;          /* device [1] (unused by kl_moe_route_grad) */
+} kl_moe_route_desc;
+
+/* Bytes of device workspace (4-byte aligned, any contents) that kl_moe_route needs. */
+KL_API kl_status kl_moe_route_workspace_size(int64_t tokens, int64_t experts, size_t* bytes);
+
+/* p = softmax(logits) in fp32 over each token's experts; ids = its k largest logits, largest first,
+ * the lower expert first among equals; weights as `renormalize` says; counts[e] = slots that name e;
+ * *routed = N, the tokens that are routed; *loss = experts * sum_e (counts[e] / (k N)) * (mean over
+ * the routed tokens of p_e), 0 when N is 0 (a uniform router has loss 1). A logit of -inf closes an
+ * expert to the token: it is never chosen, and a slot with nothing left has id -1 and weight 0. A
+ * token whose logits are all -inf, or whose valid is 0, is not routed. The type's lowest finite value is
+ * an ordinary logit. A NaN or +inf logit makes its token's weights, and the loss, NaN (NaN is
+ * chosen first). Results do not depend on the timing of atomics. */
+KL_API kl_status kl_moe_route(const kl_moe_route_desc* desc, void* workspace, size_t workspace_bytes, void* stream);
+
+/* The gradient of the logits (logits_type, [tokens, ld_dlogits]; zeros for tokens not routed) from
+ * the gradients of weights (dweights, fp32 [tokens, k], NULL = 0; read only where the id is not -1)
+ * and of loss (dloss, device scalar, NULL = 0). desc is kl_moe_route's, with its outputs. The counts
+ * are constants here. dlogits may be the logits' own memory. */
+KL_API kl_status kl_moe_route_grad(const kl_moe_route_desc* desc, const float* dweights, const float* dloss, void* dlogits,
+                                   int64_t ld_dlogits, void* stream);
+
+/* Rows of the grouped layout that any split of `slots` rows over `experts` fits, each expert padded
+ * to `block` (128, or 256 for the CTA-pair kernel) rows: (slots + min(slots, experts) (block - 1)) /
+ * block * block. -1 for a bad argument. Host only. */
+KL_API int64_t kl_moe_rows(int64_t slots, int64_t experts, int32_t block);
+
+/* Sorts the slots (token t, j at t k + j) by expert, keeping their order within one: rows[slot] = its row
+ * of the layout (-1 where ids is not in [0, experts)), slots[row] = its slot (-1 = padding),
+ * m_block_group[i] = the expert of rows 128 i .. (-1 = none, behind the last expert). ids and rows:
+ * device [tokens, k]; m = a multiple of block, at least kl_moe_rows(tokens k, experts, block); slots:
+ * device [m]; m_block_group: device [m / 128]. experts up to 1024, k up to 32. */
+KL_API kl_status kl_moe_plan(const int32_t* ids, int64_t tokens, int64_t k, int64_t experts, int32_t block, int64_t m,
+                             int32_t* rows, int32_t* slots, int32_t* m_block_group, void* stream);
+
+/* a[row] = x[slots[row] / k], zeros for padding rows; x [tokens], a [m] in rows of row_bytes bytes, of any type,
+ * pitches in bytes. rows and slots are kl_moe_plan's. */
+KL_API kl_status kl_moe_dispatch(const void* x, int64_t ldx_bytes, int64_t tokens, int64_t row_bytes, int64_t k,
+                                 const int32_t* rows, const int32_t* slots, int64_t m, void* a, int64_t lda_bytes,
+                                 void* stream);
+
+/* out[t] = sum_j weights[t, j] y[rows[t, j]], summed in fp32 in the order of j and rounded once; a
+ * row outside [0, m) adds nothing. y [m, ldy], out [tokens, ldo] of `type` KL_BF16, KL_F16 or KL_F32;
+ * rows NULL: y is in slot order, m = tokens k; weights NULL: 1 (the gradient of kl_moe_dispatch). */
+KL_API kl_status kl_moe_combine(const void* y, int32_t type, int64_t ldy, int64_t m, const int32_t* rows,
+                                const float* weights, int64_t tokens, int64_t k, int64_t width, void* out, int64_t ldo,
+                                void* stream);
+
+/* The gradients of kl_moe_combine: dy[row] = weights[slots[row]] dout[slots[row] / k] (zeros for padding rows),
+ * dweights[t, j] = <dout[t], y[rows[t, j]]> in fp32 (0 where rows is -1; NULL = not wanted, y is then
+ * not read). rows and slots are kl_moe_plan's, or both NULL for slot order. dy must not be y. */
+KL_API kl_status kl_moe_combine_grad(const void* dout, int64_t ld_dout, const void* y, int32_t type, int64_t ldy,
+                                     int64_t m, const int32_t* rows, const int32_t* slots, const float* weights,
+                                     int64_t tokens, int64_t k, int64_t width, void* dy, int64_t ld_dy, float* dweights,
+                                     void* stream);
+
+/* ---- products with 4-bit weights and group scales (decode) -----------------------------------
+ * out[t, n] = sum_i x[t, i] (q[n, i] - zeros[n, i / group]) scales[n, i / group], summed in fp32,
+ * rounded once. With ids, one matrix per expert: out row t topk + j uses expert ids[t, j] (the
+ * experts' products for single tokens, straight from kl_moe_route's ids); an id outside [0, experts)
+ * gives zeros. The weights stream once for up to 32 tokens (16 of one expert). No counterpart in the
+ * reference. */
+typedef struct kl_int4_desc {
+  const void* x;        /* device [tokens, ldx], x_type KL_BF16 or KL_F16; 16-byte aligned, ldx % 8 == 0;
+                         * x_per_slot: [tokens topk, ldx] */
+  int64_t ldx;
+  const void* q;        /* device [n, ldq] bytes: two codes 0 .. 15 a byte, the lower K in the low nibble;
+                         * 16-byte aligned, ldq % 16 == 0; expert e at e * stride_q */
+  int64_t ldq, stride_q;
+  const void* scales;   /* device [n, ld_scales], one per `group` K-elements, x_type or KL_F32 */
+  int64_t ld_scales, stride_scales;
+  const uint8_t* zeros; /* device [n, ld_zeros], values 0 .. 127, or NULL: 8 everywhere */
+  int64_t ld_zeros, stride_zeros;
+  const int32_t* ids;   /* device [tokens, topk] or NULL: one matrix */
+  int64_t experts, topk; /* with ids: tokens * topk <= 8192 */
+  void* out;            /* device [tokens (* topk), ldo], x_type or KL_F32 */
+  int64_t ldo;
+  int64_t tokens, n, k; /* k a multiple of 32 */
+  int64_t group;        /* 32, 64 or a multiple of 128; the last group may be short */
+  int32_t x_type, scale_type, out_type, x_per_slot;
+} kl_int4_desc;
+
+KL_API kl_status kl_gemv_int4(const kl_int4_desc* desc, void* stream);
+
 /* Frees every workspace the library allocated for kl_gemm (the skinny kernel's per-device buffer,
  * the tile kernels' per-stream split-tail buffers), after synchronising each device that has one;
  * later calls allocate afresh. No launch that uses them may be in flight or captured in a CUDA

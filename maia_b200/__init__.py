@@ -38,7 +38,8 @@ EXPORTED = (
     "kl_mma_instr_desc_block_scaled", "kl_mx_scale_bytes", "kl_mx_pack_scales", "kl_block_scale_bytes",
     "kl_pack_block_scales", "kl_mx_quantize", "kl_nv_quantize",
     "kl_comm_get_unique_id", "kl_comm_init", "kl_comm_all_gather", "kl_comm_wait", "kl_comm_is_aborted",
-    "kl_comm_destroy",
+    "kl_comm_destroy", "kl_moe_route_workspace_size", "kl_moe_route", "kl_moe_route_grad", "kl_moe_rows", "kl_moe_plan",
+    "kl_moe_dispatch", "kl_moe_combine", "kl_moe_combine_grad", "kl_gemv_int4",
 )
 
 
@@ -71,6 +72,30 @@ class GemmDesc(ctypes.Structure):
         ("sfa", ctypes.c_void_p), ("sfb", ctypes.c_void_p),
         ("groups", ctypes.c_int32), ("launch_overlap", ctypes.c_int32),
         ("m_block_group", ctypes.c_void_p),
+    ]
+
+
+class MoeRouteDesc(ctypes.Structure):
+    _fields_ = [
+        ("logits", ctypes.c_void_p), ("ld_logits", ctypes.c_int64),
+        ("tokens", ctypes.c_int64), ("experts", ctypes.c_int64), ("k", ctypes.c_int64),
+        ("logits_type", ctypes.c_int32), ("renormalize", ctypes.c_int32),
+        ("valid", ctypes.c_void_p), ("ids", ctypes.c_void_p), ("weights", ctypes.c_void_p),
+        ("counts", ctypes.c_void_p), ("routed", ctypes.c_void_p), ("loss", ctypes.c_void_p),
+    ]
+
+
+class Int4Desc(ctypes.Structure):
+    _fields_ = [
+        ("x", ctypes.c_void_p), ("ldx", ctypes.c_int64),
+        ("q", ctypes.c_void_p), ("ldq", ctypes.c_int64), ("stride_q", ctypes.c_int64),
+        ("scales", ctypes.c_void_p), ("ld_scales", ctypes.c_int64), ("stride_scales", ctypes.c_int64),
+        ("zeros", ctypes.c_void_p), ("ld_zeros", ctypes.c_int64), ("stride_zeros", ctypes.c_int64),
+        ("ids", ctypes.c_void_p), ("experts", ctypes.c_int64), ("topk", ctypes.c_int64),
+        ("out", ctypes.c_void_p), ("ldo", ctypes.c_int64),
+        ("tokens", ctypes.c_int64), ("n", ctypes.c_int64), ("k", ctypes.c_int64), ("group", ctypes.c_int64),
+        ("x_type", ctypes.c_int32), ("scale_type", ctypes.c_int32), ("out_type", ctypes.c_int32),
+        ("x_per_slot", ctypes.c_int32),
     ]
 
 
@@ -132,6 +157,15 @@ def lib() -> ctypes.CDLL:
             "kl_comm_wait": (i32, [vp, vp, i64]),
             "kl_comm_is_aborted": (i32, [vp]),
             "kl_comm_destroy": (i32, [vp, i64]),
+            "kl_moe_route_workspace_size": (i32, [i64, i64, P(ctypes.c_size_t)]),
+            "kl_moe_route": (i32, [P(MoeRouteDesc), vp, ctypes.c_size_t, vp]),
+            "kl_moe_route_grad": (i32, [P(MoeRouteDesc), vp, vp, vp, i64, vp]),
+            "kl_moe_rows": (i64, [i64, i64, i32]),
+            "kl_moe_plan": (i32, [vp, i64, i64, i64, i32, i64, vp, vp, vp, vp]),
+            "kl_moe_dispatch": (i32, [vp, i64, i64, i64, i64, vp, vp, i64, vp, i64, vp]),
+            "kl_moe_combine": (i32, [vp, i32, i64, i64, vp, vp, i64, i64, i64, vp, i64, vp]),
+            "kl_moe_combine_grad": (i32, [vp, i64, vp, i32, i64, i64, vp, vp, vp, i64, i64, i64, vp, i64, vp, vp]),
+            "kl_gemv_int4": (i32, [P(Int4Desc), vp]),
         }
         for name, (res, args) in sig.items():
             fn = getattr(L, name)
@@ -607,3 +641,17 @@ def probe_wait_timeout(timeout_ns: int, stream=None) -> None:
 
     s = stream if stream is not None else torch.cuda.current_stream().cuda_stream
     check(lib().kl_probe_wait_timeout(int(timeout_ns), ctypes.c_void_p(s)))
+
+
+_EXPERTS = ("MoePlan", "MoeRoute", "gemv_int4", "moe_combine", "moe_combine_grad", "moe_dispatch", "moe_plan", "moe_route",
+            "moe_route_grad", "moe_rows")
+
+
+def __getattr__(name):
+    # The expert layer's calls (maia_b200.experts) load torch, which this module otherwise leaves to its functions.
+    if name not in _EXPERTS:
+        raise AttributeError(f"module {__name__!r} has no attribute {name!r}")
+    from . import experts
+
+    globals().update({n: getattr(experts, n) for n in _EXPERTS})
+    return globals()[name]

@@ -1,0 +1,490 @@
+// From a router's expert ids to the m-grouped GEMM's row layout and back: kl_moe_plan (counting
+// sort of the slots by expert, each expert padded to whole blocks), kl_moe_dispatch (copy every
+// token's row to its experts), kl_moe_combine (weighted sum of the experts' rows) and
+// kl_moe_combine_grad.
+
+#include <cooperative_groups.h>
+#include <cuda_runtime.h>
+
+#include <string>
+
+#include <kl/arch/griddep.hpp>
+#include <kl_gemm.h>
+
+#include "kl_internal.cuh"
+#include "kl_vec.cuh"
+
+namespace cg = cooperative_groups;
+
+namespace kl::capi {
+namespace {
+
+constexpr int kMaxExperts = 1024;
+constexpr int kMaxTopK = 32;
+constexpr int kPlanThreads = 1024;
+constexpr int kPlanWarps = kPlanThreads / 32;
+
+struct PlanArgs {
+  const int* ids;
+  long long total;  // slots
+  int experts;
+  int block;
+  long long m;      // rows of the layout
+  int* rows;        // [total]
+  int* slots;       // [m]
+  int* blocks;      // [m / 128]
+  long long warp_span;  // consecutive slots of a warp, a multiple of 32
+};
+
+// Inclusive sum over the block's 1024 threads.
+__device__ __forceinline__ int block_scan(int v, int* red) {
+  const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
+#pragma unroll
+  for (int o = 1; o < 32; o *= 2) {
+    const int u = __shfl_up_sync(0xFFFFFFFFu, v, o);
+    if (lane >= o) v += u;
+  }
+  if (lane == 31) red[warp] = v;
+  __syncthreads();
+  if (warp == 0) {
+    int w = red[lane];
+#pragma unroll
+    for (int o = 1; o < 32; o *= 2) {
+      const int u = __shfl_up_sync(0xFFFFFFFFu, w, o);
+      if (lane >= o) w += u;
+    }
+    red[lane] = w;
+  }
+  __syncthreads();
+  return warp > 0 ? v + red[warp - 1] : v;
+}
+
+// One cluster sorts all slots. Every warp counts the experts of its own run of consecutive slots;
+// sums over the warps, then (through distributed shared memory) over the blocks, give each (warp,
+// expert) the row of its first slot; a second walk over the same slots hands the rows out. Slots of
+// one expert keep their order, and nothing depends on the timing of atomics.
+__global__ void __launch_bounds__(kPlanThreads) plan_kernel(const PlanArgs a) {
+  extern __shared__ int hist[];  // [kPlanWarps][experts]
+  __shared__ int block_count[kMaxExperts];
+  __shared__ int red[32];
+  cg::cluster_group cluster = cg::this_cluster();
+  griddep_wait();
+  griddep_launch_dependents();
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  const int rank = int(cluster.block_rank()), ranks = int(cluster.num_blocks());
+  for (int i = threadIdx.x; i < kPlanWarps * a.experts; i += kPlanThreads) hist[i] = 0;
+  __syncthreads();
+  int* mine = hist + warp * a.experts;
+  const long long begin = ((long long)rank * kPlanWarps + warp) * a.warp_span;
+  const long long end = begin + a.warp_span < a.total ? begin + a.warp_span : a.total;
+  auto expert_at = [&](long long s) {
+    const int e = s < end ? a.ids[s] : -1;
+    return e >= 0 && e < a.experts ? e : -1;
+  };
+  for (long long s = begin; s < end; s += 32) {
+    const int e = expert_at(s + lane);
+    const unsigned same = __match_any_sync(0xFFFFFFFFu, e);
+    if (e >= 0 && lane == __ffs(same) - 1) mine[e] += __popc(same);
+    __syncwarp();
+  }
+  __syncthreads();
+  const int e = threadIdx.x;
+  if (e < a.experts) {
+    int run = 0;
+    for (int w = 0; w < kPlanWarps; ++w) {
+      const int c = hist[w * a.experts + e];
+      hist[w * a.experts + e] = run;
+      run += c;
+    }
+    block_count[e] = run;
+  }
+  cluster.sync();
+  int before = 0, all = 0;
+  if (e < a.experts)
+    for (int r = 0; r < ranks; ++r) {
+      const int c = cluster.map_shared_rank(block_count, r)[e];
+      before += r < rank ? c : 0;
+      all += c;
+    }
+  const int room = (all + a.block - 1) / a.block * a.block;
+  const int stop = block_scan(room, red);
+  const int start = stop - room;
+  if (e < a.experts)
+    for (int w = 0; w < kPlanWarps; ++w) hist[w * a.experts + e] += start + before;
+  // The padding behind each expert's rows, its blocks, and the blocks that nobody has.
+  if (e < a.experts && e % ranks == rank) {
+    for (int r = start + all; r < stop; ++r) a.slots[r] = -1;
+    for (int b = start / 128; b < stop / 128; ++b) a.blocks[b] = e;
+  }
+  __syncthreads();
+  const long long used = red[31];
+  for (long long r = used + rank * kPlanThreads + threadIdx.x; r < a.m; r += ranks * kPlanThreads) {
+    a.slots[r] = -1;
+    if (r % 128 == 0) a.blocks[r / 128] = -1;
+  }
+  for (long long s = begin; s < end; s += 32) {
+    const int x = expert_at(s + lane);
+    const unsigned same = __match_any_sync(0xFFFFFFFFu, x);
+    int row = -1;
+    if (x >= 0) row = mine[x] + __popc(same & ((1u << lane) - 1));
+    __syncwarp();
+    if (x >= 0 && lane == __ffs(same) - 1) mine[x] += __popc(same);
+    __syncwarp();
+    if (s + lane < end) a.rows[s + lane] = row;
+    if (row >= 0) a.slots[row] = int(s + lane);
+  }
+  cluster.sync();  // no block leaves while another may still read its counts
+}
+
+constexpr int kRowThreads = 256;
+
+struct RowArgs {
+  const void* src;      // dispatch: x [tokens]; combine: y [m]; combine_grad: y [m]
+  long long ld_src;     // row pitches in bytes
+  void* dst;            // dispatch: a [m]; combine: out [tokens]; combine_grad: dy [m]
+  long long ld_dst;
+  const void* dout;     // combine_grad: [tokens]
+  long long ld_dout;
+  const int* rows;      // [tokens, k], NULL = slot order
+  const int* slots;     // [m], NULL = slot order
+  const float* weights; // [tokens, k], NULL = 1
+  float* dweights;      // combine_grad: [tokens, k] or NULL
+  long long tokens, m;
+  int k;
+  long long width;      // vectors of a row (bytes / sizeof(V)), or elements
+};
+
+// Rows of the layout that hold no slot become zeros: blocks [0, pad_blocks) of the pad part take 32
+// rows each.
+constexpr int kPadRows = 32;
+template <class V>
+__device__ __forceinline__ void zero_padding(const RowArgs& a, long long part) {
+  for (int i = 0; i < kPadRows; ++i) {
+    const long long r = part * kPadRows + i;
+    if (r >= a.m) return;
+    if (a.slots[r] >= 0) continue;
+    V* dst = reinterpret_cast<V*>(static_cast<char*>(a.dst) + r * a.ld_dst);
+    for (long long c = threadIdx.x; c < a.width; c += kRowThreads) dst[c] = V{};
+  }
+}
+
+// A copy knows no element type: V is the widest of 16, 8, 4, 2 or 1 bytes that the row's bytes,
+// pitches and addresses allow. A token's row is read once and written to each of its experts.
+template <class V>
+__global__ void __launch_bounds__(kRowThreads) dispatch_kernel(const RowArgs a) {
+  griddep_wait();
+  griddep_launch_dependents();
+  if (blockIdx.x >= a.tokens) return zero_padding<V>(a, blockIdx.x - a.tokens);
+  const long long t = blockIdx.x;
+  const V* src = reinterpret_cast<const V*>(static_cast<const char*>(a.src) + t * a.ld_src);
+  for (long long c = threadIdx.x; c < a.width; c += kRowThreads) {
+    const V v = src[c];
+    for (int j = 0; j < a.k; ++j) {
+      const int r = a.rows[t * a.k + j];
+      if (r >= 0 && r < a.m) reinterpret_cast<V*>(static_cast<char*>(a.dst) + r * a.ld_dst)[c] = v;
+    }
+  }
+}
+
+// Vec: 16-byte vectors of T, else single elements.
+template <class T, bool Vec>
+struct Cells {
+  static constexpr int n = Vec ? kPerVec<T> : 1;
+  using type = std::conditional_t<Vec, uint4, T>;
+  static __device__ __forceinline__ void get(const type* p, float* v) {
+    if constexpr (Vec) unpack<T>(*p, v);
+    else v[0] = to_f32(*p);
+  }
+  static __device__ __forceinline__ void put(type* p, const float* v) {
+    if constexpr (Vec) *p = pack<T>(v);
+    else *p = from_f32<T>(v[0]);
+  }
+};
+
+__device__ __forceinline__ long long row_of(const RowArgs& a, long long slot) {
+  const long long r = a.rows != nullptr ? a.rows[slot] : slot;
+  return r >= 0 && r < a.m ? r : -1;
+}
+
+template <class T, bool Vec>
+__global__ void __launch_bounds__(kRowThreads) combine_kernel(const RowArgs a) {
+  using C = Cells<T, Vec>;
+  using V = typename C::type;
+  griddep_wait();
+  griddep_launch_dependents();
+  const long long t = blockIdx.x;
+  const long long c = (long long)blockIdx.y * kRowThreads + threadIdx.x;
+  if (c >= a.width) return;
+  float sum[C::n] = {};
+#pragma unroll 4
+  for (int j = 0; j < a.k; ++j) {
+    const long long r = row_of(a, t * a.k + j);
+    if (r < 0) continue;
+    const float w = a.weights != nullptr ? a.weights[t * a.k + j] : 1.0f;
+    float v[C::n];
+    C::get(reinterpret_cast<const V*>(static_cast<const char*>(a.src) + r * a.ld_src) + c, v);
+#pragma unroll
+    for (int i = 0; i < C::n; ++i) sum[i] += w * v[i];
+  }
+  C::put(reinterpret_cast<V*>(static_cast<char*>(a.dst) + t * a.ld_dst) + c, sum);
+}
+
+// dy and dw of one token: its dout is read once for kAtOnce slots at a time, each slot's y once.
+constexpr int kAtOnce = 8;
+template <class T, bool Vec>
+__global__ void __launch_bounds__(kRowThreads) combine_grad_kernel(const RowArgs a) {
+  using C = Cells<T, Vec>;
+  using V = typename C::type;
+  __shared__ float red[kAtOnce][kRowThreads / 32];
+  griddep_wait();
+  griddep_launch_dependents();
+  if (blockIdx.x >= a.tokens) return zero_padding<V>(a, blockIdx.x - a.tokens);
+  const long long t = blockIdx.x;
+  const V* dout = reinterpret_cast<const V*>(static_cast<const char*>(a.dout) + t * a.ld_dout);
+  for (int j0 = 0; j0 < a.k; j0 += kAtOnce) {
+    float dot[kAtOnce] = {};
+    for (long long c = threadIdx.x; c < a.width; c += kRowThreads) {
+      float g[C::n];
+      C::get(dout + c, g);
+#pragma unroll
+      for (int i = 0; i < kAtOnce; ++i) {
+        if (j0 + i >= a.k) break;
+        const long long s = t * a.k + j0 + i, r = row_of(a, s);
+        if (r < 0) continue;
+        float y[C::n];
+        if (a.dweights != nullptr) {
+          C::get(reinterpret_cast<const V*>(static_cast<const char*>(a.src) + r * a.ld_src) + c, y);
+#pragma unroll
+          for (int x = 0; x < C::n; ++x) dot[i] += g[x] * y[x];
+        }
+        if (a.slots == nullptr || a.slots[r] == s) {  // a row's gradient is written by its own slot alone
+          const float w = a.weights != nullptr ? a.weights[s] : 1.0f;
+#pragma unroll
+          for (int x = 0; x < C::n; ++x) y[x] = w * g[x];
+          C::put(reinterpret_cast<V*>(static_cast<char*>(a.dst) + r * a.ld_dst) + c, y);
+        }
+      }
+    }
+    if (a.dweights == nullptr) continue;
+#pragma unroll
+    for (int i = 0; i < kAtOnce; ++i) {
+#pragma unroll
+      for (int o = 16; o > 0; o /= 2) dot[i] += __shfl_xor_sync(0xFFFFFFFFu, dot[i], o);
+      if (threadIdx.x % 32 == 0) red[i][threadIdx.x / 32] = dot[i];
+    }
+    __syncthreads();
+    if (threadIdx.x < kAtOnce && j0 + int(threadIdx.x) < a.k) {
+      float s = 0.0f;
+      for (int w = 0; w < kRowThreads / 32; ++w) s += red[threadIdx.x][w];
+      a.dweights[t * a.k + j0 + threadIdx.x] = s;
+    }
+    __syncthreads();
+  }
+}
+
+cudaError_t launch(cudaStream_t stream, dim3 grid, int threads, size_t smem, int cluster, void const* kernel, void** args) {
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr[2];
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(unsigned(threads), 1, 1);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = unsigned(cluster);
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = cluster > 1 ? 2 : 1;
+  return cudaLaunchKernelExC(&cfg, kernel, args);
+}
+
+// Bytes that every one of the values is a multiple of: 16, 8, 4, 2 or 1.
+int common_granule(std::initializer_list<uint64_t> values) {
+  uint64_t all = 16;
+  for (uint64_t v : values) all |= v;
+  return int(all & (~all + 1));
+}
+
+int type_bytes(int32_t t) { return t == KL_F32 ? 4 : t == KL_BF16 || t == KL_F16 ? 2 : 0; }
+
+kl_status check_rows(char const* who, int64_t tokens, int64_t k, int64_t m, int64_t width) {
+  if (tokens < 0 || k < 1 || k > kMaxTopK || m < 0 || width < 0)
+    return fail(KL_ERR_INVALID_ARGUMENT, std::string(who) + ": extents must not be negative, k in [1, 32]");
+  if (tokens * k > INT32_MAX || m > INT32_MAX || tokens + (m + kPadRows - 1) / kPadRows > INT32_MAX)
+    return fail(KL_ERR_INVALID_ARGUMENT, std::string(who) + ": more than 2^31 - 1 rows");
+  return KL_OK;
+}
+
+}  // namespace
+}  // namespace kl::capi
+
+extern "C" int64_t kl_moe_rows(int64_t slots, int64_t experts, int32_t block) {
+  if (slots < 0 || experts < 1 || (block != 128 && block != 256)) return -1;
+  const int64_t holders = slots < experts ? slots : experts;
+  return (slots + holders * (block - 1)) / block * block;
+}
+
+extern "C" kl_status kl_moe_plan(const int32_t* ids, int64_t tokens, int64_t k, int64_t experts, int32_t block, int64_t m,
+                                 int32_t* rows, int32_t* slots, int32_t* m_block_group, void* stream) {
+  using namespace kl::capi;
+  kl_status s = check_rows("kl_moe_plan", tokens, k, m, 0);
+  if (s != KL_OK) return s;
+  if (experts < 1 || experts > kMaxExperts) return fail(KL_ERR_NOT_SUPPORTED, "kl_moe_plan: experts must be in [1, 1024]");
+  if (block != 128 && block != 256) return fail(KL_ERR_INVALID_ARGUMENT, "kl_moe_plan: block must be 128 or 256");
+  if (m % block != 0 || m < kl_moe_rows(tokens * k, experts, block))
+    return fail(KL_ERR_INVALID_ARGUMENT, "kl_moe_plan: m must be a multiple of block, at least kl_moe_rows(tokens * k, experts, block)");
+  if (m == 0) return KL_OK;
+  if ((tokens > 0 && (ids == nullptr || rows == nullptr)) || slots == nullptr || m_block_group == nullptr)
+    return fail(KL_ERR_INVALID_ARGUMENT, "kl_moe_plan: null pointer");
+  PlanArgs a = {};
+  a.ids = ids;
+  a.total = tokens * k;
+  a.experts = int(experts);
+  a.block = block;
+  a.m = m;
+  a.rows = rows;
+  a.slots = slots;
+  a.blocks = m_block_group;
+  // One block while it has at most four turns of 32 slots for each warp.
+  const int cluster = a.total <= 4 * 32 * kPlanWarps ? 1 : 8;
+  const long long warps = (long long)cluster * kPlanWarps;
+  a.warp_span = (a.total + warps * 32 - 1) / (warps * 32) * 32;
+  const size_t smem = size_t(kPlanWarps) * size_t(experts) * sizeof(int);
+  cudaError_t e = cudaFuncSetAttribute(plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem));
+  if (e != cudaSuccess) return cuda_fail(e, "kl_moe_plan shared memory");
+  void* args[] = {&a};
+  e = launch(static_cast<cudaStream_t>(stream), dim3(unsigned(cluster)), kPlanThreads, smem, cluster,
+             reinterpret_cast<void const*>(&plan_kernel), args);
+  return e == cudaSuccess ? KL_OK : cuda_fail(e, "kl_moe_plan launch");
+}
+
+extern "C" kl_status kl_moe_dispatch(const void* x, int64_t ldx_bytes, int64_t tokens, int64_t row_bytes, int64_t k,
+                                     const int32_t* rows, const int32_t* slots, int64_t m, void* a_out, int64_t lda_bytes,
+                                     void* stream) {
+  using namespace kl::capi;
+  kl_status s = check_rows("kl_moe_dispatch", tokens, k, m, row_bytes);
+  if (s != KL_OK) return s;
+  if (m == 0 || row_bytes == 0) return KL_OK;
+  if ((tokens > 0 && (x == nullptr || rows == nullptr)) || slots == nullptr || a_out == nullptr)
+    return fail(KL_ERR_INVALID_ARGUMENT, "kl_moe_dispatch: null pointer");
+  if (ldx_bytes < row_bytes || lda_bytes < row_bytes)
+    return fail(KL_ERR_INVALID_ARGUMENT, "kl_moe_dispatch: row pitch below the row's bytes");
+  RowArgs a = {};
+  a.src = x;
+  a.ld_src = ldx_bytes;
+  a.dst = a_out;
+  a.ld_dst = lda_bytes;
+  a.rows = rows;
+  a.slots = slots;
+  a.tokens = tokens;
+  a.m = m;
+  a.k = int(k);
+  const int g = common_granule({reinterpret_cast<uintptr_t>(x), reinterpret_cast<uintptr_t>(a_out), uint64_t(ldx_bytes),
+                                uint64_t(lda_bytes), uint64_t(row_bytes)});
+  a.width = row_bytes / g;
+  void const* kernel = g == 16 ? reinterpret_cast<void const*>(&dispatch_kernel<uint4>)
+                       : g == 8 ? reinterpret_cast<void const*>(&dispatch_kernel<uint2>)
+                       : g == 4 ? reinterpret_cast<void const*>(&dispatch_kernel<uint32_t>)
+                       : g == 2 ? reinterpret_cast<void const*>(&dispatch_kernel<uint16_t>)
+                                : reinterpret_cast<void const*>(&dispatch_kernel<uint8_t>);
+  void* args[] = {&a};
+  cudaError_t e = launch(static_cast<cudaStream_t>(stream), dim3(unsigned(tokens + (m + kPadRows - 1) / kPadRows)),
+                         kRowThreads, 0, 1, kernel, args);
+  return e == cudaSuccess ? KL_OK : cuda_fail(e, "kl_moe_dispatch launch");
+}
+
+namespace kl::capi {
+namespace {
+
+template <class F>
+void by_cells(int32_t type, bool vec, F&& f) {
+  if (type == KL_F32) vec ? f(float{}, std::true_type{}) : f(float{}, std::false_type{});
+  else if (type == KL_F16) vec ? f(__half{}, std::true_type{}) : f(__half{}, std::false_type{});
+  else vec ? f(__nv_bfloat16{}, std::true_type{}) : f(__nv_bfloat16{}, std::false_type{});
+}
+
+}  // namespace
+}  // namespace kl::capi
+
+extern "C" kl_status kl_moe_combine(const void* y, int32_t type, int64_t ldy, int64_t m, const int32_t* rows,
+                                    const float* weights, int64_t tokens, int64_t k, int64_t width, void* out, int64_t ldo,
+                                    void* stream) {
+  using namespace kl::capi;
+  kl_status s = check_rows("kl_moe_combine", tokens, k, m, width);
+  if (s != KL_OK) return s;
+  const int size = type_bytes(type);
+  if (size == 0) return fail(KL_ERR_NOT_SUPPORTED, "kl_moe_combine: rows must be bf16, f16 or f32");
+  if (tokens == 0 || width == 0) return KL_OK;
+  if (ldy < width || ldo < width) return fail(KL_ERR_INVALID_ARGUMENT, "kl_moe_combine: row pitch below the width");
+  if (rows == nullptr && m != tokens * k)
+    return fail(KL_ERR_INVALID_ARGUMENT, "kl_moe_combine: without rows, y has tokens * k rows");
+  if (out == nullptr || (m > 0 && y == nullptr)) return fail(KL_ERR_INVALID_ARGUMENT, "kl_moe_combine: null pointer");
+  RowArgs a = {};
+  a.src = y;
+  a.ld_src = ldy * size;
+  a.dst = out;
+  a.ld_dst = ldo * size;
+  a.rows = rows;
+  a.weights = weights;
+  a.tokens = tokens;
+  a.m = m;
+  a.k = int(k);
+  const bool vec = common_granule({reinterpret_cast<uintptr_t>(y), reinterpret_cast<uintptr_t>(out), uint64_t(a.ld_src),
+                                   uint64_t(a.ld_dst), uint64_t(width * size)}) == 16;
+  a.width = vec ? width * size / 16 : width;
+  const int64_t parts = (a.width + kRowThreads - 1) / kRowThreads;
+  if (parts > 65535) return fail(KL_ERR_INVALID_ARGUMENT, "kl_moe_combine: rows too wide");
+  cudaError_t e = cudaSuccess;
+  by_cells(type, vec, [&](auto t, auto v) {
+    void* args[] = {&a};
+    e = launch(static_cast<cudaStream_t>(stream), dim3(unsigned(tokens), unsigned(parts)), kRowThreads, 0, 1,
+               reinterpret_cast<void const*>(&combine_kernel<decltype(t), decltype(v)::value>), args);
+  });
+  return e == cudaSuccess ? KL_OK : cuda_fail(e, "kl_moe_combine launch");
+}
+
+extern "C" kl_status kl_moe_combine_grad(const void* dout, int64_t ld_dout, const void* y, int32_t type, int64_t ldy, int64_t m,
+                                         const int32_t* rows, const int32_t* slots, const float* weights, int64_t tokens,
+                                         int64_t k, int64_t width, void* dy, int64_t ld_dy, float* dweights, void* stream) {
+  using namespace kl::capi;
+  kl_status s = check_rows("kl_moe_combine_grad", tokens, k, m, width);
+  if (s != KL_OK) return s;
+  const int size = type_bytes(type);
+  if (size == 0) return fail(KL_ERR_NOT_SUPPORTED, "kl_moe_combine_grad: rows must be bf16, f16 or f32");
+  if ((rows == nullptr) != (slots == nullptr))
+    return fail(KL_ERR_INVALID_ARGUMENT, "kl_moe_combine_grad: rows and slots come together");
+  if (rows == nullptr && m != tokens * k)
+    return fail(KL_ERR_INVALID_ARGUMENT, "kl_moe_combine_grad: without rows, y has tokens * k rows");
+  if (ldy < width || ld_dout < width || ld_dy < width)
+    return fail(KL_ERR_INVALID_ARGUMENT, "kl_moe_combine_grad: row pitch below the width");
+  if (tokens == 0 && m == 0) return KL_OK;
+  if ((tokens > 0 && width > 0 && dout == nullptr) || (m > 0 && width > 0 && (dy == nullptr || (dweights != nullptr && y == nullptr))))
+    return fail(KL_ERR_INVALID_ARGUMENT, "kl_moe_combine_grad: null pointer");
+  RowArgs a = {};
+  a.src = y;
+  a.ld_src = ldy * size;
+  a.dst = dy;
+  a.ld_dst = ld_dy * size;
+  a.dout = dout;
+  a.ld_dout = ld_dout * size;
+  a.rows = rows;
+  a.slots = slots;
+  a.weights = weights;
+  a.dweights = dweights;
+  a.tokens = tokens;
+  a.m = m;
+  a.k = int(k);
+  const bool vec = common_granule({reinterpret_cast<uintptr_t>(y), reinterpret_cast<uintptr_t>(dy), reinterpret_cast<uintptr_t>(dout),
+                                   uint64_t(a.ld_src), uint64_t(a.ld_dst), uint64_t(a.ld_dout), uint64_t(width * size)}) == 16;
+  a.width = vec ? width * size / 16 : width;
+  const int64_t pad_parts = slots != nullptr ? (m + kPadRows - 1) / kPadRows : 0;
+  cudaError_t e = cudaSuccess;
+  by_cells(type, vec, [&](auto t, auto v) {
+    void* args[] = {&a};
+    e = launch(static_cast<cudaStream_t>(stream), dim3(unsigned(tokens + pad_parts)), kRowThreads, 0, 1,
+               reinterpret_cast<void const*>(&combine_grad_kernel<decltype(t), decltype(v)::value>), args);
+  });
+  return e == cudaSuccess ? KL_OK : cuda_fail(e, "kl_moe_combine_grad launch");
+}

@@ -1,0 +1,556 @@
+// Mixture-of-experts routing: the k experts of every token, their weights, the experts' counts and
+// the balance loss, and the gradient of the logits (kl_moe_route, kl_moe_route_grad).
+//
+// p = softmax(l) over a token's E logits; the k largest l are chosen (ties: the lower index);
+// w_j = p_{e_j}, or p_{e_j} / sum_i p_{e_i}. With c_e the number of slots that name e and N the
+// routed tokens, the loss is E sum_e (c_e / (k N)) (1/N sum_t p_te). The counts have no gradient:
+// with a_e = dL E c_e / (k N^2) and D = sum_j dw_j w_j,
+//   dl_te = p_te (a_e - sum_e' p_te' a_e' - [w = p] D) + [e = e_j] w_j (dw_j - [w normalised] D).
+
+#include <cuda_runtime.h>
+
+#include <string>
+
+#include <kl/arch/griddep.hpp>
+#include <kl_gemm.h>
+
+#include "kl_internal.cuh"
+#include "kl_vec.cuh"
+
+namespace kl::capi {
+namespace {
+
+constexpr int kRouteThreads = 256;
+constexpr int kRouteWarps = kRouteThreads / 32;
+constexpr int kMaxExperts = 1024;
+constexpr int kMaxTopK = 32;
+
+// Ordering keys: larger key = earlier choice. The value's bits in an order-preserving form sit above
+// 1023 - e, so one integer maximum gives the largest value and, among equals, the lowest expert.
+// 16-bit logits leave the low 12 bits of their fp32 form zero, so key and index share 32 bits. 0 is
+// "cannot be chosen" (-inf); NaN orders above everything.
+template <class T>
+struct RouteKey {
+  using type = uint32_t;
+};
+template <>
+struct RouteKey<float> {
+  using type = uint64_t;
+};
+
+__device__ __forceinline__ uint32_t ordered_bits(float v) {
+  const uint32_t u = __float_as_uint(v + 0.0f);  // -0 and +0 tie
+  return v != v ? 0xFFFFFFFFu : u ^ (u >> 31 ? 0xFFFFFFFFu : 0x80000000u);
+}
+__device__ __forceinline__ void make_key(float v, int e, uint32_t& k) {
+  k = v == -INFINITY ? 0u : (ordered_bits(v) & 0xFFFFF000u) | uint32_t(kMaxExperts - 1 - e);
+}
+__device__ __forceinline__ void make_key(float v, int e, uint64_t& k) {
+  k = v == -INFINITY ? 0ull : (uint64_t(ordered_bits(v)) << 32) | uint32_t(kMaxExperts - 1 - e);
+}
+__device__ __forceinline__ float value_of_bits(uint32_t o) {
+  return o == 0xFFFFFFFFu ? NAN : __uint_as_float(o & 0x80000000u ? o ^ 0x80000000u : ~o);
+}
+__device__ __forceinline__ float key_value(uint32_t k) {
+  const uint32_t o = k & 0xFFFFF000u;
+  return value_of_bits(o & 0x80000000u ? (o == 0xFFFFF000u ? 0xFFFFFFFFu : o) : o | 0xFFFu);
+}
+__device__ __forceinline__ float key_value(uint64_t k) { return value_of_bits(uint32_t(k >> 32)); }
+template <class K>
+__device__ __forceinline__ int key_expert(K k) {
+  return kMaxExperts - 1 - int(uint32_t(k) & (kMaxExperts - 1));
+}
+
+// L lanes share a token; lane i holds experts (v L + i) 8 + 0..7 for v < NV.
+template <int L>
+__device__ __forceinline__ float group_sum(float v) {
+#pragma unroll
+  for (int o = L / 2; o > 0; o /= 2) v += __shfl_xor_sync(0xFFFFFFFFu, v, o);
+  return v;
+}
+template <int L>
+__device__ __forceinline__ float group_max(float v) {
+#pragma unroll
+  for (int o = L / 2; o > 0; o /= 2) v = fmaxf(v, __shfl_xor_sync(0xFFFFFFFFu, v, o));
+  return v;
+}
+template <int L, class K>
+__device__ __forceinline__ K group_key_max(K k) {
+  if constexpr (L == 32 && sizeof(K) == 4) {
+    return __reduce_max_sync(0xFFFFFFFFu, k);
+  } else {
+#pragma unroll
+    for (int o = L / 2; o > 0; o /= 2) {
+      const K other = __shfl_xor_sync(0xFFFFFFFFu, k, o);
+      k = other > k ? other : k;
+    }
+    return k;
+  }
+}
+
+// A row's logits as fp32: whole 16-byte vectors where `vec` (aligned rows, E a multiple of 8), else
+// element by element; -inf outside the row.
+template <class T, int L, int NV>
+__device__ __forceinline__ void load_row(const T* row, int lane, int experts, bool vec, bool live, float (&v)[8 * NV]) {
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int e0 = (i * L + lane) * 8;
+    if (!live || e0 >= experts) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[8 * i + j] = -INFINITY;
+    } else if (vec) {
+      const uint4* p = reinterpret_cast<const uint4*>(row + e0);
+#pragma unroll
+      for (int j = 0; j < 8 / kPerVec<T>; ++j) unpack<T>(__ldg(p + j), v + 8 * i + j * kPerVec<T>);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[8 * i + j] = e0 + j < experts ? to_f32(row[e0 + j]) : -INFINITY;
+    }
+  }
+}
+
+struct RouteArgs {
+  const void* logits;
+  long long ld;
+  int tokens, experts, k;
+  int renormalize;
+  const uint8_t* valid;
+  int* ids;
+  float* weights;
+  int* counts;
+  int* routed;
+  float* loss;
+  // Partial sums of block b: share[b E + e], count[b E + e], routed_part[b]. Unused by one block.
+  float* share_part;
+  int* count_part;
+  int* routed_part;
+  int vec;
+};
+
+// The loss from the finished counts and probability sums: every thread brings its experts' terms
+// (sum over e of c_e s_e); the division by k N^2 comes last.
+__device__ __forceinline__ float block_total(float v, float* red) {
+#pragma unroll
+  for (int o = 16; o > 0; o /= 2) v += __shfl_xor_sync(0xFFFFFFFFu, v, o);
+  if (threadIdx.x % 32 == 0) red[threadIdx.x / 32] = v;
+  __syncthreads();
+  float t = 0.0f;
+  for (int w = 0; w < int(blockDim.x) / 32; ++w) t += red[w];
+  __syncthreads();
+  return t;
+}
+__device__ __forceinline__ float loss_of(float total, int experts, int k, int routed) {
+  return routed > 0 ? float(experts) * (total / (float(k) * float(routed))) / float(routed) : 0.0f;
+}
+
+template <class T, int L, int NV>
+__global__ void __launch_bounds__(kRouteThreads) route_kernel(const RouteArgs a) {
+  using K = typename RouteKey<T>::type;
+  constexpr int kGroups = 32 / L;  // tokens of a warp
+  constexpr int kPicks = L * 8 < kMaxTopK ? L * 8 : kMaxTopK;  // k is at most the number of experts
+  __shared__ K chosen[kRouteWarps * kGroups][kPicks];
+  __shared__ int count[L * 8 * NV];
+  __shared__ float share[kRouteWarps * L * 8 * NV];
+  __shared__ float red[32];
+  __shared__ int routed_here;
+  griddep_wait();
+  griddep_launch_dependents();
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % L, group = threadIdx.x % 32 / L;
+  for (int e = threadIdx.x; e < a.experts; e += kRouteThreads) count[e] = 0;
+  if (threadIdx.x == 0) routed_here = 0;
+  __syncthreads();
+  const T* logits = static_cast<const T*>(a.logits);
+  float acc[8 * NV];
+#pragma unroll
+  for (int i = 0; i < 8 * NV; ++i) acc[i] = 0.0f;
+  const int step = gridDim.x * kRouteWarps * kGroups;
+  K* mine = chosen[warp * kGroups + group];
+  int routed = 0;
+  // Whole warps leave the loop together: the shuffles take every lane.
+  for (long long first = (long long)(blockIdx.x * kRouteWarps + warp) * kGroups; first < a.tokens; first += step) {
+    const long long t = first + group;
+    const bool live = t < a.tokens && (a.valid == nullptr || a.valid[t] != 0);
+    float v[8 * NV];
+    load_row<T, L, NV>(logits + (t < a.tokens ? t : 0) * a.ld, lane, a.experts, a.vec, live, v);
+    K key[8 * NV];
+    float top = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < 8 * NV; ++i) {
+      make_key(v[i], (i / 8 * L + lane) * 8 + i % 8, key[i]);
+      top = fmaxf(top, v[i]);
+    }
+    top = group_max<L>(top);
+    // The k largest keys, one after another; each found key is struck out where it is held.
+    K first_key = 0;
+    for (int j = 0; j < a.k; ++j) {
+      K best = key[0];
+#pragma unroll
+      for (int i = 1; i < 8 * NV; ++i) best = key[i] > best ? key[i] : best;
+      best = group_key_max<L>(best);
+#pragma unroll
+      for (int i = 0; i < 8 * NV; ++i) key[i] = key[i] == best ? K(0) : key[i];
+      if (lane == 0) mine[j] = best;
+      if (j == 0) first_key = best;
+    }
+    const bool any = first_key != 0;
+    float sum = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 8 * NV; ++i) {
+      v[i] = v[i] == -INFINITY ? 0.0f : expf(v[i] - top);
+      sum += v[i];
+    }
+    sum = group_sum<L>(sum);
+    if (any) {
+      const float inv = 1.0f / sum;
+#pragma unroll
+      for (int i = 0; i < 8 * NV; ++i) acc[i] += v[i] * inv;
+      routed += lane == 0;
+    }
+    __syncwarp();
+    float part = 0.0f;
+    if (a.renormalize) {
+      for (int j = lane; j < a.k; j += L) part += mine[j] != 0 ? expf(key_value(mine[j]) - top) : 0.0f;
+      sum = group_sum<L>(part);
+    }
+    if (t < a.tokens) {
+      for (int j = lane; j < a.k; j += L) {
+        const K key_j = mine[j];
+        const int e = key_j != 0 ? key_expert(key_j) : -1;
+        a.ids[t * a.k + j] = e;
+        a.weights[t * a.k + j] = e >= 0 ? expf(key_value(key_j) - top) / sum : 0.0f;
+        if (e >= 0) atomicAdd(&count[e], 1);
+      }
+    }
+    __syncwarp();
+  }
+  // Block sums in a fixed order: the groups of a warp by shuffles, the warps one after another.
+  const int width = L * 8 * NV;
+#pragma unroll
+  for (int i = 0; i < 8 * NV; ++i) {
+#pragma unroll
+    for (int o = L; o < 32; o *= 2) acc[i] += __shfl_xor_sync(0xFFFFFFFFu, acc[i], o);
+    if (group == 0) share[warp * width + (i / 8 * L + lane) * 8 + i % 8] = acc[i];
+  }
+  if (routed) atomicAdd(&routed_here, routed);
+  __syncthreads();
+  float terms = 0.0f;
+  for (int e = threadIdx.x; e < a.experts; e += kRouteThreads) {
+    float s = 0.0f;
+    for (int w = 0; w < kRouteWarps; ++w) s += share[w * width + e];
+    if (gridDim.x == 1) {
+      a.counts[e] = count[e];
+      terms += s * float(count[e]);
+    } else {
+      a.share_part[(long long)blockIdx.x * a.experts + e] = s;
+      a.count_part[(long long)blockIdx.x * a.experts + e] = count[e];
+    }
+  }
+  if (gridDim.x == 1) {
+    const float total = block_total(terms, red);
+    if (threadIdx.x == 0) {
+      *a.routed = routed_here;
+      *a.loss = loss_of(total, a.experts, a.k, routed_here);
+    }
+  } else if (threadIdx.x == 0) {
+    a.routed_part[blockIdx.x] = routed_here;
+  }
+}
+
+// The blocks' partial sums, in block order.
+__global__ void __launch_bounds__(1024) route_finish_kernel(const RouteArgs a, int blocks) {
+  __shared__ float red[32];
+  griddep_wait();
+  griddep_launch_dependents();
+  float terms = 0.0f;
+  for (int e = threadIdx.x; e < a.experts; e += 1024) {
+    float s = 0.0f;
+    int c = 0;
+#pragma unroll 8
+    for (int b = 0; b < blocks; ++b) {
+      s += a.share_part[(long long)b * a.experts + e];
+      c += a.count_part[(long long)b * a.experts + e];
+    }
+    a.counts[e] = c;
+    terms += s * float(c);
+  }
+  const float total = block_total(terms, red);
+  if (threadIdx.x < 32) {
+    int n = 0;
+    for (int b = threadIdx.x; b < blocks; b += 32) n += a.routed_part[b];
+    n = __reduce_add_sync(0xFFFFFFFFu, n);
+    if (threadIdx.x == 0) {
+      *a.routed = n;
+      *a.loss = loss_of(total, a.experts, a.k, n);
+    }
+  }
+}
+
+struct RouteGradArgs {
+  const void* logits;
+  long long ld;
+  int tokens, experts, k;
+  int renormalize;
+  const uint8_t* valid;
+  const int* ids;
+  const float* weights;
+  const int* counts;
+  const int* routed;
+  const float* dweights;
+  const float* dloss;
+  void* dlogits;
+  long long ldd;
+  int vec;
+};
+
+template <class T, int L, int NV>
+__global__ void __launch_bounds__(kRouteThreads) route_grad_kernel(const RouteGradArgs a) {
+  constexpr int kGroups = 32 / L;
+  constexpr int kWidth = L * 8 * NV;
+  __shared__ float push[kWidth];                           // a_e
+  __shared__ float spot[kRouteWarps * kGroups][kWidth];    // the chosen experts' own terms, else 0
+  griddep_wait();
+  griddep_launch_dependents();
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % L, group = threadIdx.x % 32 / L;
+  const float n = float(*a.routed > 0 ? *a.routed : 1);
+  const float dloss = a.dloss != nullptr ? *a.dloss : 0.0f;
+  for (int e = threadIdx.x; e < kWidth; e += kRouteThreads)
+    push[e] = e < a.experts ? dloss * float(a.experts) * (float(a.counts[e]) / (float(a.k) * n)) / n : 0.0f;
+  for (int i = threadIdx.x; i < kRouteWarps * kGroups * kWidth; i += kRouteThreads) (&spot[0][0])[i] = 0.0f;
+  __syncthreads();
+  const T* logits = static_cast<const T*>(a.logits);
+  T* out = static_cast<T*>(a.dlogits);
+  float* mine = spot[warp * kGroups + group];
+  const int step = gridDim.x * kRouteWarps * kGroups;
+  for (long long first = (long long)(blockIdx.x * kRouteWarps + warp) * kGroups; first < a.tokens; first += step) {
+    const long long t = first + group;
+    const bool live = t < a.tokens && (a.valid == nullptr || a.valid[t] != 0);
+    float v[8 * NV];
+    load_row<T, L, NV>(logits + (t < a.tokens ? t : 0) * a.ld, lane, a.experts, a.vec, live, v);
+    float top = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < 8 * NV; ++i) top = fmaxf(top, v[i]);
+    top = group_max<L>(top);
+    float sum = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 8 * NV; ++i) {
+      v[i] = v[i] == -INFINITY ? 0.0f : expf(v[i] - top);
+      sum += v[i];
+    }
+    sum = group_sum<L>(sum);
+    const bool any = sum != 0.0f;  // else the row is not routed: zeros, whatever dloss and dweights hold
+    const float inv = any ? 1.0f / sum : 0.0f;
+    float level = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 8 * NV; ++i) {
+      v[i] *= inv;
+      level += v[i] * push[(i / 8 * L + lane) * 8 + i % 8];
+    }
+    level = group_sum<L>(level);
+    float pull = 0.0f;
+    if (live && a.dweights != nullptr)
+      for (int j = lane; j < a.k; j += L)
+        if (a.ids[t * a.k + j] >= 0) pull += a.weights[t * a.k + j] * a.dweights[t * a.k + j];
+    pull = group_sum<L>(pull);
+    if (live && a.dweights != nullptr)
+      for (int j = lane; j < a.k; j += L) {
+        const int e = a.ids[t * a.k + j];
+        if (e >= 0 && e < a.experts)
+          atomicAdd(&mine[e], a.weights[t * a.k + j] * (a.dweights[t * a.k + j] - (a.renormalize ? pull : 0.0f)));
+      }
+    __syncwarp();
+    const float base = level + (a.renormalize ? 0.0f : pull);
+    if (t < a.tokens) {
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        const int e0 = (i * L + lane) * 8;
+        float g[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) g[j] = any ? v[8 * i + j] * (push[e0 + j] - base) + mine[e0 + j] : 0.0f;
+        if (e0 >= a.experts) continue;
+        if (a.vec) {
+          uint4* p = reinterpret_cast<uint4*>(out + t * a.ldd + e0);
+#pragma unroll
+          for (int j = 0; j < 8 / kPerVec<T>; ++j) p[j] = pack<T>(g + j * kPerVec<T>);
+        } else {
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+            if (e0 + j < a.experts) out[t * a.ldd + e0 + j] = from_f32<T>(g[j]);
+        }
+      }
+    }
+    __syncwarp();
+    if (live && a.dweights != nullptr)
+      for (int j = lane; j < a.k; j += L) {
+        const int e = a.ids[t * a.k + j];
+        if (e >= 0 && e < a.experts) mine[e] = 0.0f;
+      }
+    __syncwarp();
+  }
+}
+
+// Lanes of a token: enough for 8 experts each, at most a warp; wider rows take more vectors a lane.
+template <class F>
+void by_width(int experts, F&& f) {
+  if (experts <= 8) f(std::integral_constant<int, 1>{}, std::integral_constant<int, 1>{});
+  else if (experts <= 16) f(std::integral_constant<int, 2>{}, std::integral_constant<int, 1>{});
+  else if (experts <= 32) f(std::integral_constant<int, 4>{}, std::integral_constant<int, 1>{});
+  else if (experts <= 64) f(std::integral_constant<int, 8>{}, std::integral_constant<int, 1>{});
+  else if (experts <= 128) f(std::integral_constant<int, 16>{}, std::integral_constant<int, 1>{});
+  else if (experts <= 256) f(std::integral_constant<int, 32>{}, std::integral_constant<int, 1>{});
+  else if (experts <= 512) f(std::integral_constant<int, 32>{}, std::integral_constant<int, 2>{});
+  else f(std::integral_constant<int, 32>{}, std::integral_constant<int, 4>{});
+}
+
+template <class F>
+void by_type(int32_t type, F&& f) {
+  if (type == KL_F32) f(float{});
+  else if (type == KL_F16) f(__half{});
+  else f(__nv_bfloat16{});
+}
+
+int lanes_of(int experts) {
+  int lanes = 1;
+  while (lanes < 32 && lanes * 8 < experts) lanes *= 2;
+  return lanes;
+}
+
+// Blocks of the routing kernel: one where its warps take all tokens in a few turns (no second
+// kernel then), else up to two for every SM of a 148-SM B200.
+int route_blocks(int64_t tokens, int experts) {
+  const int64_t turn = kRouteWarps * (32 / lanes_of(experts));  // tokens of one block at a time
+  if (tokens <= 4 * turn) return 1;
+  const int64_t blocks = (tokens + turn - 1) / turn;
+  return int(blocks < 296 ? blocks : 296);
+}
+
+kl_status check_route(char const* who, int64_t tokens, int64_t experts, int64_t k, int32_t type, int64_t ld) {
+  if (tokens < 0 || tokens > INT32_MAX / kMaxTopK) return fail(KL_ERR_INVALID_ARGUMENT, std::string(who) + ": tokens must be in [0, 2^26)");
+  if (experts < 1 || experts > kMaxExperts)
+    return fail(KL_ERR_NOT_SUPPORTED, std::string(who) + ": experts must be in [1, 1024]");
+  if (k < 1 || k > kMaxTopK || k > experts)
+    return fail(KL_ERR_INVALID_ARGUMENT, std::string(who) + ": k must be in [1, min(experts, 32)]");
+  if (type != KL_BF16 && type != KL_F16 && type != KL_F32)
+    return fail(KL_ERR_NOT_SUPPORTED, std::string(who) + ": logits must be bf16, f16 or f32");
+  if (ld < experts) return fail(KL_ERR_INVALID_ARGUMENT, std::string(who) + ": row pitch below the number of experts");
+  return KL_OK;
+}
+
+bool vector_rows(const void* p, int64_t ld, int64_t experts, int32_t type) {
+  const int64_t size = type == KL_F32 ? 4 : 2;
+  return aligned16(p) && ld * size % 16 == 0 && experts % 8 == 0;
+}
+
+cudaError_t launch(cudaStream_t stream, int grid, int threads, void const* kernel, void** args) {
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr[1];
+  cfg.gridDim = dim3(unsigned(grid), 1, 1);
+  cfg.blockDim = dim3(unsigned(threads), 1, 1);
+  cfg.stream = stream;
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelExC(&cfg, kernel, args);
+}
+
+}  // namespace
+}  // namespace kl::capi
+
+extern "C" kl_status kl_moe_route_workspace_size(int64_t tokens, int64_t experts, size_t* bytes) {
+  using namespace kl::capi;
+  if (bytes == nullptr) return fail(KL_ERR_INVALID_ARGUMENT, "kl_moe_route_workspace_size: null pointer");
+  kl_status s = check_route("kl_moe_route_workspace_size", tokens, experts, 1, KL_F32, experts);
+  if (s != KL_OK) return s;
+  const int blocks = route_blocks(tokens, int(experts));
+  *bytes = blocks == 1 ? 0 : size_t(blocks) * (2 * size_t(experts) + 1) * 4;
+  return KL_OK;
+}
+
+extern "C" kl_status kl_moe_route(const kl_moe_route_desc* d, void* workspace, size_t workspace_bytes, void* stream) {
+  using namespace kl::capi;
+  if (d == nullptr) return fail(KL_ERR_INVALID_ARGUMENT, "kl_moe_route: null descriptor");
+  kl_status s = check_route("kl_moe_route", d->tokens, d->experts, d->k, d->logits_type, d->ld_logits);
+  if (s != KL_OK) return s;
+  if (d->counts == nullptr || d->routed == nullptr || d->loss == nullptr ||
+      (d->tokens > 0 && (d->logits == nullptr || d->ids == nullptr || d->weights == nullptr)))
+    return fail(KL_ERR_INVALID_ARGUMENT, "kl_moe_route: null pointer");
+  const int blocks = route_blocks(d->tokens, int(d->experts));
+  size_t need = 0;
+  kl_moe_route_workspace_size(d->tokens, d->experts, &need);
+  if (need > 0 && (workspace == nullptr || workspace_bytes < need || reinterpret_cast<uintptr_t>(workspace) % 4 != 0))
+    return fail(KL_ERR_INVALID_ARGUMENT, "kl_moe_route: needs a 4-byte aligned workspace of " + std::to_string(need) + " bytes");
+  RouteArgs a = {};
+  a.logits = d->logits;
+  a.ld = d->ld_logits;
+  a.tokens = int(d->tokens);
+  a.experts = int(d->experts);
+  a.k = int(d->k);
+  a.renormalize = d->renormalize;
+  a.valid = d->valid;
+  a.ids = d->ids;
+  a.weights = d->weights;
+  a.counts = d->counts;
+  a.routed = d->routed;
+  a.loss = d->loss;
+  a.share_part = static_cast<float*>(workspace);
+  a.count_part = reinterpret_cast<int*>(a.share_part + size_t(blocks) * d->experts);
+  a.routed_part = a.count_part + size_t(blocks) * d->experts;
+  a.vec = vector_rows(d->logits, d->ld_logits, d->experts, d->logits_type);
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  cudaError_t e = cudaSuccess;
+  by_type(d->logits_type, [&](auto t) {
+    by_width(a.experts, [&](auto l, auto nv) {
+      void* args[] = {&a};
+      e = launch(st, blocks, kRouteThreads, reinterpret_cast<void const*>(&route_kernel<decltype(t), l(), nv()>), args);
+    });
+  });
+  if (e == cudaSuccess && blocks > 1) {
+    int b = blocks;
+    void* args[] = {&a, &b};
+    e = launch(st, 1, 1024, reinterpret_cast<void const*>(&route_finish_kernel), args);
+  }
+  return e == cudaSuccess ? KL_OK : cuda_fail(e, "kl_moe_route launch");
+}
+
+extern "C" kl_status kl_moe_route_grad(const kl_moe_route_desc* d, const float* dweights, const float* dloss,
+                                       void* dlogits, int64_t ld_dlogits, void* stream) {
+  using namespace kl::capi;
+  if (d == nullptr) return fail(KL_ERR_INVALID_ARGUMENT, "kl_moe_route_grad: null descriptor");
+  kl_status s = check_route("kl_moe_route_grad", d->tokens, d->experts, d->k, d->logits_type, d->ld_logits);
+  if (s != KL_OK) return s;
+  if (ld_dlogits < d->experts) return fail(KL_ERR_INVALID_ARGUMENT, "kl_moe_route_grad: row pitch below the number of experts");
+  if (d->tokens == 0) return KL_OK;
+  if (d->logits == nullptr || d->ids == nullptr || d->weights == nullptr || d->counts == nullptr || d->routed == nullptr ||
+      dlogits == nullptr)
+    return fail(KL_ERR_INVALID_ARGUMENT, "kl_moe_route_grad: null pointer");
+  RouteGradArgs a = {};
+  a.logits = d->logits;
+  a.ld = d->ld_logits;
+  a.tokens = int(d->tokens);
+  a.experts = int(d->experts);
+  a.k = int(d->k);
+  a.renormalize = d->renormalize;
+  a.valid = d->valid;
+  a.ids = d->ids;
+  a.weights = d->weights;
+  a.counts = d->counts;
+  a.routed = d->routed;
+  a.dweights = dweights;
+  a.dloss = dloss;
+  a.dlogits = dlogits;
+  a.ldd = ld_dlogits;
+  a.vec = vector_rows(d->logits, d->ld_logits, d->experts, d->logits_type) &&
+          vector_rows(dlogits, ld_dlogits, d->experts, d->logits_type);
+  const int64_t turn = kRouteWarps * (32 / lanes_of(a.experts));
+  const int64_t want = (d->tokens + turn - 1) / turn;
+  const int blocks = int(want < 592 ? want : 592);
+  cudaError_t e = cudaSuccess;
+  by_type(d->logits_type, [&](auto t) {
+    by_width(a.experts, [&](auto l, auto nv) {
+      void* args[] = {&a};
+      e = launch(static_cast<cudaStream_t>(stream), blocks, kRouteThreads,
+                 reinterpret_cast<void const*>(&route_grad_kernel<decltype(t), l(), nv()>), args);
+    });
+  });
+  return e == cudaSuccess ? KL_OK : cuda_fail(e, "kl_moe_route_grad launch");
+}
