@@ -14,11 +14,11 @@ through torch. No counterpart in the reference (kernel_lib has no GEMM and no ro
 from __future__ import annotations
 
 import ctypes
-from typing import NamedTuple, Optional
+from typing import NamedTuple
 
 import torch
 
-from . import (Int4Desc, KL_BF16, KL_F16, KL_F32, MoeRouteDesc, check, lib)
+from . import Int4Desc, KL_BF16, KL_F16, KL_F32, KL_OK, MoeRouteDesc, check, lib
 
 _FLOATS = {torch.bfloat16: KL_BF16, torch.float16: KL_F16, torch.float32: KL_F32}
 
@@ -37,51 +37,64 @@ class MoePlan(NamedTuple):
     m_block_group: torch.Tensor  # int32 [m / 128]: the expert of every 128-row block, -1 = none
 
 
+# torch's own cheap forms of current_stream(device).cuda_stream and current_device(): a decode step makes
+# a handful of calls of a few microseconds each.
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda i: torch.cuda.current_stream(i).cuda_stream)
+_current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
+
+
 def _refuse(ok: bool, message: str) -> None:
     if not ok:
         raise ValueError(message)
 
 
 def _matrix(name: str, t, dtypes=None) -> None:
-    _refuse(t.dim() == 2 and (t.stride(1) == 1 or t.shape[1] <= 1), f"{name} must be 2-D with a contiguous last dimension")
-    _refuse(dtypes is None or t.dtype in dtypes, f"{name} has the type {t.dtype}")
+    if t.dim() != 2 or (t.stride(1) != 1 and t.shape[1] > 1):
+        raise ValueError(f"{name} must be 2-D with a contiguous last dimension")
+    if dtypes is not None and t.dtype not in dtypes:
+        raise ValueError(f"{name} has the type {t.dtype}")
 
 
 def _whole(name: str, t, shape, dtype) -> None:
-    _refuse(tuple(t.shape) == tuple(shape) and t.dtype == dtype and t.is_contiguous(),
-            f"{name} must be a contiguous {dtype} tensor of shape {tuple(shape)}")
+    if t.shape != shape or t.dtype is not dtype or not t.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous {dtype} tensor of shape {tuple(shape)}")
 
 
 def _pitch(t) -> int:
     """Row pitch in elements; of a single row, whose stride torch leaves open, at least the row."""
-    return t.stride(-2) if t.shape[-2] > 1 else max(t.stride(-2), t.shape[-1])
+    pitch = t.stride(-2)
+    return pitch if pitch >= t.shape[-1] or t.shape[-2] > 1 else t.shape[-1]
 
 
 def _ptr(t):
     return None if t is None else t.data_ptr()
 
 
-def _queue(call, device, stream, owned=()):
-    """call(stream) with `device` current; `owned` tensors of this call outlive their use on a `stream` that is
-    not torch's current one."""
-    if device.type != "cuda":
-        raise ValueError("the tensors must be on a CUDA device")
-    current = torch.cuda.current_stream(device)
+def _device(*tensors) -> int:
+    """The one CUDA device of the tensors (None = not given)."""
+    found = {t.get_device() for t in tensors if t is not None}
+    index = found.pop()
+    if found or index < 0:
+        raise ValueError("the tensors must be on one CUDA device")
+    return index
+
+
+def _queue(device: int, stream, owned, fn, *args) -> None:
+    """fn(*args, stream) with `device` current; `owned` tensors of this call outlive their use on a `stream`
+    that is not torch's current one."""
+    current = _raw_stream(device)
     if stream is None:
-        stream = current.cuda_stream
-    elif stream != current.cuda_stream:
+        stream = current
+    elif stream != current:
         for t in owned:
-            t.record_stream(torch.cuda.ExternalStream(stream, device))
-    if device.index == torch.cuda.current_device():
-        check(call(stream))
+            t.record_stream(torch.cuda.ExternalStream(stream, torch.device("cuda", device)))
+    if device == _current_device():
+        status = fn(*args, stream)
     else:
         with torch.cuda.device(device):
-            check(call(stream))
-
-
-def _same_device(*tensors) -> None:
-    devices = {t.device for t in tensors if t is not None}
-    _refuse(len(devices) == 1, f"tensors on different devices: {sorted(map(str, devices))}")
+            status = fn(*args, stream)
+    if status != KL_OK:
+        check(status)
 
 
 def _route_desc(logits, k, renormalize, valid, ids, weights, counts, routed, loss):
@@ -108,20 +121,22 @@ def moe_route(logits, k: int, *, renormalize: bool = True, valid=None, stream=No
     _check_logits(logits, valid)
     tokens, experts = logits.shape
     _refuse(1 <= k <= experts, f"k must be in [1, {experts}]")
-    device = logits.device
-    need = ctypes.c_size_t()
-    check(lib().kl_moe_route_workspace_size(tokens, experts, ctypes.byref(need)))
-    ids = torch.empty((tokens, k), dtype=torch.int32, device=device)
-    weights = torch.empty((tokens, k), dtype=torch.float32, device=device)
-    counts = torch.empty((experts,), dtype=torch.int32, device=device)
-    routed = torch.empty((), dtype=torch.int32, device=device)
-    loss = torch.empty((), dtype=torch.float32, device=device)
-    work = torch.empty((need.value,), dtype=torch.uint8, device=device) if need.value else None
-    _same_device(logits, valid, loss)
-    d = _route_desc(logits, k, renormalize, valid, ids, weights, counts, routed, loss)
+    device = _device(logits, valid)
+    ids = logits.new_empty((tokens, k), dtype=torch.int32)
+    weights = logits.new_empty((tokens, k), dtype=torch.float32)
+    counts = logits.new_empty((experts,), dtype=torch.int32)
+    routed = logits.new_empty((), dtype=torch.int32)
+    loss = logits.new_empty((), dtype=torch.float32)
     out = MoeRoute(ids, weights, counts, routed, loss)
-    _queue(lambda s: lib().kl_moe_route(ctypes.byref(d), _ptr(work), need.value, s), device, stream,
-           out if work is None else (*out, work))
+    owned, work, size = out, None, 0
+    if tokens > 32:  # up to 32 tokens need no workspace
+        need = ctypes.c_size_t()
+        check(lib().kl_moe_route_workspace_size(tokens, experts, ctypes.byref(need)))
+        size = need.value
+        work = logits.new_empty((size,), dtype=torch.uint8)
+        owned = (*out, work)
+    d = _route_desc(logits, k, renormalize, valid, ids, weights, counts, routed, loss)
+    _queue(device, stream, owned, lib().kl_moe_route, ctypes.byref(d), _ptr(work), size)
     return out
 
 
@@ -143,13 +158,13 @@ def moe_route_grad(logits, route: MoeRoute, dweights=None, dloss=None, *, renorm
     if dloss is not None:
         _refuse(dloss.numel() == 1 and dloss.dtype == torch.float32, "dloss must be one fp32 value")
     if out is None:
-        out = torch.empty((tokens, experts), dtype=logits.dtype, device=logits.device)
+        out = logits.new_empty((tokens, experts))
     _matrix("out", out, (logits.dtype,))
     _refuse(out.shape == logits.shape, "out must have the logits' shape")
-    _same_device(logits, valid, route.ids, route.weights, route.counts, route.tokens, dweights, dloss, out)
+    device = _device(logits, valid, route.ids, route.weights, route.counts, route.tokens, dweights, dloss, out)
     d = _route_desc(logits, k, renormalize, valid, route.ids, route.weights, route.counts, route.tokens, None)
-    _queue(lambda s: lib().kl_moe_route_grad(ctypes.byref(d), _ptr(dweights), _ptr(dloss), out.data_ptr(), _pitch(out), s),
-           logits.device, stream, (out,))
+    _queue(device, stream, (out,), lib().kl_moe_route_grad, ctypes.byref(d), _ptr(dweights), _ptr(dloss), out.data_ptr(),
+           _pitch(out))
     return out
 
 
@@ -169,12 +184,11 @@ def moe_plan(ids, experts: int, *, block: int = 128, stream=None) -> MoePlan:
     _whole("ids", ids, ids.shape, torch.int32)
     tokens, k = ids.shape
     m = moe_rows(tokens * k, experts, block)
-    rows = torch.empty((tokens, k), dtype=torch.int32, device=ids.device)
-    slots = torch.empty((m,), dtype=torch.int32, device=ids.device)
-    groups = torch.empty((m // 128,), dtype=torch.int32, device=ids.device)
-    _queue(lambda s: lib().kl_moe_plan(ids.data_ptr(), tokens, k, int(experts), int(block), m, rows.data_ptr(),
-                                       slots.data_ptr(), groups.data_ptr(), s), ids.device, stream, (rows, slots, groups))
-    return MoePlan(rows, slots, groups)
+    device = _device(ids)
+    plan = MoePlan(ids.new_empty((tokens, k)), ids.new_empty((m,)), ids.new_empty((m // 128,)))
+    _queue(device, stream, plan, lib().kl_moe_plan, ids.data_ptr(), tokens, k, experts, block, m, plan.rows.data_ptr(),
+           plan.slots.data_ptr(), plan.m_block_group.data_ptr())
+    return plan
 
 
 def _check_plan(rows, slots) -> None:
@@ -186,55 +200,57 @@ def _check_plan(rows, slots) -> None:
 def moe_dispatch(x, plan: MoePlan, out=None, *, stream=None):
     """out[row] = x[slots[row] // k]: the tokens' rows (2-D, any type) in the m-grouped layout, every padding row
     zero. Its gradient is moe_combine(dout, rows=plan.rows)."""
+    rows, slots = plan.rows, plan.slots
     _matrix("x", x)
-    _check_plan(plan.rows, plan.slots)
-    tokens, k = plan.rows.shape
-    m = plan.slots.shape[0]
-    _refuse(x.shape[0] == tokens, f"x has {x.shape[0]} rows, the plan {tokens} tokens")
+    _check_plan(rows, slots)
+    tokens, k = rows.shape
+    m, width, size = slots.shape[0], x.shape[1], x.element_size()
+    if x.shape[0] != tokens:
+        raise ValueError(f"x has {x.shape[0]} rows, the plan {tokens} tokens")
     if out is None:
-        out = torch.empty((m, x.shape[1]), dtype=x.dtype, device=x.device)
-    _matrix("out", out, (x.dtype,))
-    _refuse(out.shape == (m, x.shape[1]), f"out must have the shape {(m, x.shape[1])}")
-    _same_device(x, plan.rows, plan.slots, out)
-    size = x.element_size()
-    _queue(lambda s: lib().kl_moe_dispatch(x.data_ptr(), _pitch(x) * size, tokens, x.shape[1] * size, max(k, 1),
-                                           plan.rows.data_ptr(), plan.slots.data_ptr(), m, out.data_ptr(),
-                                           _pitch(out) * size, s), x.device, stream, (out,))
+        out = x.new_empty((m, width))
+    else:
+        _matrix("out", out, (x.dtype,))
+        _refuse(out.shape == (m, width), f"out must have the shape {(m, width)}")
+    _queue(_device(x, rows, slots, out), stream, (out,), lib().kl_moe_dispatch, x.data_ptr(), _pitch(x) * size, tokens,
+           width * size, max(k, 1), rows.data_ptr(), slots.data_ptr(), m, out.data_ptr(), _pitch(out) * size)
     return out
 
 
 def _rows_of(y, rows, weights):
-    """y as a matrix, with (tokens, k), from its rows' indexes or its own [tokens, k, width]."""
+    """(tokens, k, rows of y, width, row pitch) from y's row indexes, or its own [tokens, k, width]."""
     if rows is None:
-        _refuse(y.dim() == 3, "without rows, y must be [tokens, k, width]")
-        tokens, k = y.shape[:2]
-        _refuse(y.is_contiguous(), "without rows, y must be contiguous")
-        y = y.view(tokens * k, y.shape[2])
+        if y.dim() != 3 or not y.is_contiguous() or y.dtype not in _FLOATS:
+            raise ValueError("without rows, y must be contiguous bf16, f16 or fp32 [tokens, k, width]")
+        tokens, k, width = y.shape
+        m, pitch = tokens * k, width
     else:
         _refuse(rows.dim() == 2, "rows must be 2-D")
         _whole("rows", rows, rows.shape, torch.int32)
+        _matrix("y", y, _FLOATS)
         tokens, k = rows.shape
-    _matrix("y", y, _FLOATS)
+        m, width = y.shape
+        pitch = _pitch(y)
     if weights is not None:
         _whole("weights", weights, (tokens, k), torch.float32)
-    return y, tokens, k
+    return tokens, k, m, width, pitch
 
 
 def moe_combine(y, weights=None, *, rows=None, out=None, stream=None):
     """out[t] = sum_j weights[t, j] * y[rows[t, j]] in fp32, rounded once to y's type (bf16, f16, fp32). y
     is [m, width] with int32 rows [tokens, k] (-1 adds nothing), or [tokens, k, width] without rows.
     weights: fp32 [tokens, k], None = 1."""
-    y, tokens, k = _rows_of(y, rows, weights)
-    width = y.shape[1]
+    tokens, k, m, width, pitch = _rows_of(y, rows, weights)
     if out is None:
-        out = torch.empty((tokens, width), dtype=y.dtype, device=y.device)
-    _matrix("out", out, (y.dtype,))
-    _refuse(out.shape == (tokens, width), f"out must have the shape {(tokens, width)}")
-    _same_device(y, rows, weights, out)
+        out = y.new_empty((tokens, width))
+    else:
+        _matrix("out", out, (y.dtype,))
+        _refuse(out.shape == (tokens, width), f"out must have the shape {(tokens, width)}")
+    device = _device(y, rows, weights, out)
     if k == 0:
         return out.zero_()
-    _queue(lambda s: lib().kl_moe_combine(y.data_ptr(), _FLOATS[y.dtype], _pitch(y), y.shape[0], _ptr(rows), _ptr(weights),
-                                          tokens, k, width, out.data_ptr(), _pitch(out), s), y.device, stream, (out,))
+    _queue(device, stream, (out,), lib().kl_moe_combine, y.data_ptr(), _FLOATS[y.dtype], pitch, m, _ptr(rows), _ptr(weights),
+           tokens, k, width, out.data_ptr(), _pitch(out))
     return out
 
 
@@ -242,21 +258,19 @@ def moe_combine_grad(dout, y, weights=None, *, rows=None, slots=None, stream=Non
     """(dy, dweights) of moe_combine from dout [tokens, width] of y's type: dy in y's shape and type,
     zero in padding rows; dweights fp32, or None where weights is None. rows and slots are moe_plan's, or
     both None."""
-    shape = y.shape
-    y, tokens, k = _rows_of(y, rows, weights)
+    tokens, k, m, width, pitch = _rows_of(y, rows, weights)
     _refuse((rows is None) == (slots is None), "rows and slots come together")
     if slots is not None:
-        _check_plan(rows, slots)
-        _refuse(slots.shape[0] == y.shape[0], "slots must have an entry for every row of y")
+        _whole("slots", slots, (m,), torch.int32)
     _matrix("dout", dout, (y.dtype,))
-    _refuse(dout.shape == (tokens, y.shape[1]), f"dout must have the shape {(tokens, y.shape[1])}")
-    _same_device(dout, y, weights, rows, slots)
-    dy = torch.empty(shape, dtype=y.dtype, device=y.device)
-    dweights = None if weights is None else torch.empty((tokens, k), dtype=torch.float32, device=y.device)
-    _queue(lambda s: lib().kl_moe_combine_grad(dout.data_ptr(), _pitch(dout), y.data_ptr(), _FLOATS[y.dtype], _pitch(y),
-                                               y.shape[0], _ptr(rows), _ptr(slots), _ptr(weights), tokens, max(k, 1),
-                                               y.shape[1], dy.data_ptr(), y.shape[1], _ptr(dweights), s),
-           y.device, stream, (dy,) if dweights is None else (dy, dweights))
+    if dout.shape != (tokens, width):
+        raise ValueError(f"dout must have the shape {(tokens, width)}")
+    device = _device(dout, y, weights, rows, slots)
+    dy = y.new_empty(y.shape)
+    dweights = None if weights is None else weights.new_empty((tokens, k))
+    _queue(device, stream, (dy,) if dweights is None else (dy, dweights), lib().kl_moe_combine_grad, dout.data_ptr(),
+           _pitch(dout), y.data_ptr(), _FLOATS[y.dtype], pitch, m, _ptr(rows), _ptr(slots), _ptr(weights), tokens, max(k, 1),
+           width, dy.data_ptr(), width, _ptr(dweights))
     return dy, dweights
 
 
@@ -267,39 +281,41 @@ def gemv_int4(x, q, scales, zeros=None, *, group: int = 128, ids=None, out=None,
     multiple of 32. With int32 ids [tokens, k]: q [E, N, K / 2], scales and zeros [E, N, ...], x [tokens, K]
     or [tokens, k, K], out [tokens, k, N] with expert ids[t, j] (rows of zeros for ids outside 0 .. E - 1). out in
     x's type or fp32; sums in fp32. Up to 32 tokens (16 of one expert) read the weights once."""
-    experts = ids is not None
-    _refuse(x.dtype in (torch.bfloat16, torch.float16), "x must be bf16 or f16")
-    _refuse(q.dtype == torch.uint8 and q.dim() == 2 + experts and q.stride(-1) == 1,
-            "q must be uint8 [N, K / 2], or [E, N, K / 2] with ids, its last dimension contiguous")
-    n, k = q.shape[-2], q.shape[-1] * 2
+    dtype, bits = x.dtype, x.dim()
+    if dtype is not torch.bfloat16 and dtype is not torch.float16:
+        raise ValueError("x must be bf16 or f16")
+    if q.dtype is not torch.uint8 or q.dim() != (2 if ids is None else 3) or (q.stride(-1) != 1 and q.shape[-1] > 1):
+        raise ValueError("q must be uint8 [N, K / 2], or [E, N, K / 2] with ids, its last dimension contiguous")
     _refuse(group > 0, "group must be positive")
-    shape = (*q.shape[:-1], -(-k // group))
-    for name, t in (("scales", scales), ("zeros", zeros)):
-        _refuse(t is None or (tuple(t.shape) == shape and (t.stride(-1) == 1 or shape[-1] <= 1)),
-                f"{name} must have the shape {shape}, its last dimension contiguous")
-    _refuse(scales.dtype in (x.dtype, torch.float32), "scales must have x's type or fp32")
-    _refuse(zeros is None or zeros.dtype == torch.uint8, "zeros must be uint8")
-    per_slot, topk = False, 1
-    if experts:
+    n, k = q.shape[-2], q.shape[-1] * 2
+    groups = -(-k // group)
+    shape = (n, groups) if ids is None else (q.shape[0], n, groups)
+    if scales.shape != shape or (scales.stride(-1) != 1 and groups > 1) or (scales.dtype is not dtype and scales.dtype is not torch.float32):
+        raise ValueError(f"scales must have the shape {shape}, its last dimension contiguous, and x's type or fp32")
+    if zeros is not None and (zeros.shape != shape or (zeros.stride(-1) != 1 and groups > 1) or zeros.dtype is not torch.uint8):
+        raise ValueError(f"zeros must be uint8 of the shape {shape}, its last dimension contiguous")
+    tokens = x.shape[0]
+    if ids is None:
+        if bits != 2 or x.shape[1] != k or (x.stride(1) != 1 and k > 1):
+            raise ValueError(f"x must be [tokens, {k}], its last dimension contiguous")
+        result, topk, per_slot, ldx = (tokens, n), 1, False, _pitch(x)
+    else:
         _refuse(ids.dim() == 2, "ids must be 2-D")
         _whole("ids", ids, ids.shape, torch.int32)
-        topk, per_slot = ids.shape[1], x.dim() == 3
-        _refuse(x.shape[:-1] == (ids.shape if per_slot else ids.shape[:1]), "x must be [tokens, K] or [tokens, k, K]")
-    else:
-        _refuse(x.dim() == 2, "x must be [tokens, K]")
-    _refuse(x.shape[-1] == k and (x.stride(-1) == 1 or k <= 1), f"x must have {k} contiguous columns")
-    _refuse(not per_slot or x.is_contiguous(), "x of [tokens, k, K] must be contiguous")
-    tokens = x.shape[0]
+        topk, per_slot = ids.shape[1], bits == 3
+        if x.shape != ((*ids.shape, k) if per_slot else (ids.shape[0], k)) or (x.stride(-1) != 1 and k > 1):
+            raise ValueError(f"x must be [tokens, {k}] or [tokens, k, {k}], its last dimension contiguous")
+        _refuse(not per_slot or x.is_contiguous(), "x of [tokens, k, K] must be contiguous")
+        result, ldx = (tokens, topk, n), k if per_slot else _pitch(x)
     if out is None:
-        out = torch.empty((*ids.shape, n) if experts else (tokens, n), dtype=out_dtype or x.dtype, device=x.device)
-    _refuse(tuple(out.shape) == ((*ids.shape, n) if experts else (tokens, n)) and out.dtype in (x.dtype, torch.float32),
-            "out must be [tokens, N] ([tokens, k, N] with ids) of x's type or fp32")
-    _refuse(out.is_contiguous() if experts else out.stride(-1) == 1 or n <= 1, "out must be contiguous in its last dimension")
-    _same_device(x, q, scales, zeros, ids, out)
-    d = Int4Desc(x.data_ptr(), k if per_slot else _pitch(x), q.data_ptr(), _pitch(q), q.stride(0) if experts else 0,
-                 scales.data_ptr(), _pitch(scales), scales.stride(0) if experts else 0,
-                 _ptr(zeros), 0 if zeros is None else _pitch(zeros), zeros.stride(0) if experts and zeros is not None else 0,
-                 _ptr(ids), q.shape[0] if experts else 0, topk, out.data_ptr(), n if experts else _pitch(out), tokens, n, k, group,
-                 _FLOATS[x.dtype], _FLOATS[scales.dtype], _FLOATS[out.dtype], int(per_slot))
-    _queue(lambda s: lib().kl_gemv_int4(ctypes.byref(d), s), x.device, stream, (out,))
+        out = x.new_empty(result, dtype=out_dtype or dtype)
+    if out.shape != result or (out.dtype is not dtype and out.dtype is not torch.float32):
+        raise ValueError(f"out must have the shape {result} and x's type or fp32")
+    _refuse(out.stride(-1) == 1 or n <= 1 if ids is None else out.is_contiguous(), "out must be contiguous in its last dimension")
+    d = Int4Desc(x.data_ptr(), ldx, q.data_ptr(), _pitch(q), 0 if ids is None else q.stride(0),
+                 scales.data_ptr(), _pitch(scales), 0 if ids is None else scales.stride(0),
+                 _ptr(zeros), 0 if zeros is None else _pitch(zeros), 0 if ids is None or zeros is None else zeros.stride(0),
+                 _ptr(ids), 0 if ids is None else q.shape[0], topk, out.data_ptr(), _pitch(out) if ids is None else n,
+                 tokens, n, k, group, _FLOATS[dtype], _FLOATS[scales.dtype], _FLOATS[out.dtype], per_slot)
+    _queue(_device(x, q, scales, zeros, ids, out), stream, (out,), lib().kl_gemv_int4, ctypes.byref(d))
     return out
