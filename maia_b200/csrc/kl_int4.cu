@@ -2,19 +2,34 @@
 //   out[t, n] = sum_g s[n, g] sum_{i in g} (q[n, i] - z[n, g]) x[t, i],
 // with one matrix, or one per expert and the expert of every (token, slot) in `ids`.
 //
-// The weights' bytes bound it: each is read once for up to 8 kTiles tokens. mma.sync.m16n8k16 takes
-// 16 weight rows as its A operand straight from registers and 8 tokens as its B, so up to 8 tokens
-// cost what one does. The codes become bf16 / f16 exactly: OR-ing a code into the mantissa of 128
-// (bf16) or 1024 (f16) gives 128 + q or 1024 + q, and subtracting 128 + z or 1024 + z leaves q - z
-// without rounding. Products are summed in fp32, group by group, and each group's sum is multiplied
-// by its scale in fp32.
+// The weights' bytes should bound it, so a code may cost little: at 6.5 TB/s an SM gets 46 codes a
+// cycle. Turned into bf16, eight codes cost eleven instructions and the SM, not the memory, sets the
+// time (measured: 2.0 TB/s). As unsigned bytes they cost three (two masks and a shift), so the products
+// are integer ones (mma.sync.m16n8k32, u8 x s8 -> s32): every block first writes x as fixed-point numbers
+// X = round(x 2^e), |X| <= 2^22, one e per token and scale group, in three signed digits of 8 bits,
+//   x ~ 2^-e (d_0 + 256 d_1 + 65536 d_2).
+// This rounding is at most 2^-22 of the group's largest |x|, what one addition in fp32 loses. The sums of a
+// group are exact: P_c = sum q d_c, and P_c - z sum d_c takes the zero point off without cancellation. Only
+// then come fp32 and the scales, sum_g s 2^-e 256^c (P_c - z D_c), accumulated in fp32 over the groups.
+//
+// Layout: a block per SM, 16 warps, each with its own ring of TMA loads (boxes of 16 rows x 128
+// bytes = 256 codes), refilled as soon as a slot has been read, so that no warp waits for another
+// while the weights stream. ldmatrix hands a lane eight codes of a row at a time. Where x's digits for all of K
+// would crowd out the ring, a cluster of 2, 4 or 8 blocks splits K and adds up through distributed
+// shared memory.
 
 #include <cooperative_groups.h>
+#include <cuda.h>
 #include <cuda_runtime.h>
 
+#include <atomic>
+#include <exception>
 #include <string>
 
 #include <kl/arch/griddep.hpp>
+#include <kl/arch/mbarrier.hpp>
+#include <kl/arch/tma.hpp>
+#include <kl/gemm/gemm.hpp>
 #include <kl_gemm.h>
 
 #include "kl_internal.cuh"
@@ -25,17 +40,20 @@ namespace cg = cooperative_groups;
 namespace kl::capi {
 namespace {
 
-constexpr int kThreads = 256;
-constexpr int kWarps = kThreads / 32;
-constexpr int kRows = 16;         // weight rows of a block
-constexpr int kChunk = 128;       // K-elements a warp takes at a time
-constexpr int kMaxSlots = 8192;   // (token, expert) pairs of a call with ids
+constexpr int kWarps = 16;
+constexpr int kThreads = 32 * kWarps;
+constexpr int kRows = 16;              // weight rows of a tile
+constexpr int kUnitK = 256;            // codes of a unit's row
+constexpr int kUnitBytes = kRows * kUnitK / 2;
+constexpr int kMaxExperts = 1024;
+constexpr int kMaxSlots = 4096;        // (token, expert) pairs of a call with ids
+constexpr int kMaxK = 65536;
+constexpr int kSmemLimit = 226 * 1024; // dynamic; 227 KB less the static arrays
 
 struct Int4Args {
+  CUtensorMap map;  // q as bytes [experts, n, k / 2]
   const void* x;
   long long ldx;
-  const uint8_t* q;
-  long long ldq, stride_q;  // bytes
   const void* scales;
   long long lds, stride_s;
   const uint8_t* zeros;
@@ -46,257 +64,713 @@ struct Int4Args {
   long long ldo;
   int n, k, group;
   int f32_scales, f32_out;
-  int by_slot;  // block row y of the grid: the y-th slot, if its expert's first; else expert y
+  int tiles;  // 16-row tiles of one matrix
+  int depth;  // slots of a warp's ring
+  int* status;
+  unsigned long long timeout_ns;
 };
 
-template <class T>
-struct Codes;
-
-// Four registers of two weights each from eight codes: register c holds codes c (low) and c + 4.
-template <>
-struct Codes<__nv_bfloat16> {
-  static __device__ __forceinline__ uint32_t offset(int z) {  // 128 + z, twice
-    return 0x43004300u | uint32_t(z) * 0x00010001u;
-  }
-  static __device__ __forceinline__ void expand(uint32_t w, uint32_t off, uint32_t (&r)[4]) {
-    const __nv_bfloat162 o = *reinterpret_cast<const __nv_bfloat162*>(&off);
-#pragma unroll
-    for (int c = 0; c < 4; ++c) {
-      uint32_t u = ((w >> (4 * c)) & 0x000F000Fu) | 0x43004300u;
-      const __nv_bfloat162 v = __hsub2(*reinterpret_cast<__nv_bfloat162*>(&u), o);
-      r[c] = *reinterpret_cast<const uint32_t*>(&v);
-    }
-  }
-  static __device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-    asm volatile(
-        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-  }
-};
-
-template <>
-struct Codes<__half> {
-  static __device__ __forceinline__ uint32_t offset(int z) {  // 1024 + z, twice
-    return 0x64006400u | uint32_t(z) * 0x00010001u;
-  }
-  static __device__ __forceinline__ void expand(uint32_t w, uint32_t off, uint32_t (&r)[4]) {
-    const __half2 o = *reinterpret_cast<const __half2*>(&off);
-#pragma unroll
-    for (int c = 0; c < 4; ++c) {
-      uint32_t u = ((w >> (4 * c)) & 0x000F000Fu) | 0x64006400u;
-      const __half2 v = __hsub2(*reinterpret_cast<__half2*>(&u), o);
-      r[c] = *reinterpret_cast<const uint32_t*>(&v);
-    }
-  }
-  static __device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-    asm volatile(
-        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-  }
-};
-
-// kWords consecutive 32-bit words of a lane belong to one scale group: 4 (groups of 128 and
-// multiples), 2 (64) or 1 (32). In a chunk of 128 K-elements, lane t of a row's four holds
-// K = 8 kWords (4 h + t) .. + 8 kWords for h = 0 .. 4 / kWords - 1: the four lanes of a row read
-// neighbouring words of one group, and x is read at the same K. The order of K inside an MMA is free
-// as long as both operands use it.
-template <int kWords>
-__device__ __forceinline__ void load_words(const uint8_t* p, bool ok, uint32_t* w) {
-  if constexpr (kWords == 4) {
-    const uint4 u = ok ? __ldg(reinterpret_cast<const uint4*>(p)) : make_uint4(0, 0, 0, 0);
-    w[0] = u.x; w[1] = u.y; w[2] = u.z; w[3] = u.w;
-  } else if constexpr (kWords == 2) {
-    const uint2 u = ok ? __ldg(reinterpret_cast<const uint2*>(p)) : make_uint2(0, 0);
-    w[0] = u.x; w[1] = u.y;
-  } else {
-    w[0] = ok ? __ldg(reinterpret_cast<const uint32_t*>(p)) : 0u;
-  }
+__device__ __forceinline__ void ldmatrix_x4(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
 }
 
-template <class T, int kWords, int kTiles>
-__global__ void __launch_bounds__(kThreads) gemv_int4_kernel(const Int4Args a) {
-  constexpr int kHops = 4 / kWords;
-  constexpr int kTok = 8 * kTiles;
-  __shared__ float red[kWarps][kRows * kTok];
-  extern __shared__ int list[];  // with ids: the slots of this block's expert
-  __shared__ int list_size;
+__device__ __forceinline__ void mma_u8s8(int (&d)[4], const uint32_t (&a)[4], uint2 b) {
+  asm("mma.sync.aligned.m16n8k32.row.col.s32.u8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+      : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b.x), "r"(b.y));
+}
+
+// With ids: the experts that some slot names, each with its slots, in shared memory.
+struct Lists {
+  int* base;        // [experts + 1]: token passes before an active expert
+  uint16_t* act;    // [experts]: its number
+  uint16_t* start;  // [experts + 1]: its first entry of `list`
+  uint16_t* list;   // [slots]
+  static __host__ __device__ size_t bytes(int experts, int slots) {
+    return (size_t(experts) + 1) * 4 + (size_t(experts) + 1) * 4 + size_t(slots) * 2;
+  }
+};
+
+// Counts the slots of every expert, packs the active ones and files the slots in their order: every block builds the
+// lists for itself, and all have to cut an expert's slots into the same passes.
+template <int kTok>
+__device__ void build_lists(const Int4Args& a, Lists const& l, int* hist, int* active_out) {
+  __shared__ unsigned long long warp_sum[kWarps];
+  const int tid = threadIdx.x, lane = tid % 32, warp = tid / 32;
+  for (int e = tid; e < a.experts; e += kThreads) hist[e] = 0;
+  __syncthreads();
+  for (int s = tid; s < a.slots; s += kThreads) {
+    const int e = a.ids[s];
+    if (e >= 0 && e < a.experts) atomicAdd(&hist[e], 1);
+  }
+  __syncthreads();
+  // Exclusive sums over the experts, two to a thread: active experts (bits 0-15), slots (16-31), passes (32-).
+  unsigned long long mine = 0, own[2];
+  int count[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int e = 2 * tid + i;
+    count[i] = e < a.experts ? hist[e] : 0;
+    own[i] = count[i] == 0 ? 0
+                           : 1ull | (unsigned long long)count[i] << 16 |
+                                 (unsigned long long)((count[i] + kTok - 1) / kTok) << 32;
+    mine += own[i];
+  }
+  unsigned long long sum = mine;
+#pragma unroll
+  for (int o = 1; o < 32; o *= 2) {
+    const unsigned long long u = __shfl_up_sync(0xFFFFFFFFu, sum, o);
+    if (lane >= o) sum += u;
+  }
+  if (lane == 31) warp_sum[warp] = sum;
+  __syncthreads();
+  unsigned long long before = sum - mine, total = 0;
+  for (int w = 0; w < kWarps; ++w) {
+    if (w < warp) before += warp_sum[w];
+    total += warp_sum[w];
+  }
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int e = 2 * tid + i;
+    if (count[i] > 0) {
+      const int at = int(before & 0xFFFF), first = int(before >> 16 & 0xFFFF);
+      l.act[at] = uint16_t(e);
+      l.start[at] = uint16_t(first);
+      l.base[at] = int(before >> 32);
+      hist[e] = first;
+    }
+    before += own[i];
+  }
+  const int active = int(total & 0xFFFF);
+  if (tid == 0) {
+    l.start[active] = uint16_t(total >> 16 & 0xFFFF);
+    l.base[active] = int(total >> 32);
+  }
+  __syncthreads();
+  if (warp == 0)
+    for (int s0 = 0; s0 < a.slots; s0 += 32) {
+      const int s = s0 + lane;
+      int e = s < a.slots ? a.ids[s] : -1;
+      if (e < 0 || e >= a.experts) e = -1;
+      const unsigned same = __match_any_sync(0xFFFFFFFFu, e);
+      if (e >= 0) l.list[hist[e] + __popc(same & ((1u << lane) - 1))] = uint16_t(s);
+      __syncwarp();
+      if (e >= 0 && lane == __ffs(same) - 1) hist[e] += __popc(same);
+      __syncwarp();
+    }
+  __syncthreads();
+  *active_out = active;
+}
+
+// Columns of the products. Three digits of 8 tokens are three 8-column tiles, digit c of token i in
+// column i of tile c, so a lane holds the digits of the same tokens; up to two tokens fit one tile, digit c of
+// token i in column 2 c + i, and the digits meet by shuffles.
+template <int NT>
+struct Columns {
+  static constexpr int kTokens = NT == 1 ? 2 : NT / 3 * 8;
+  static __device__ __forceinline__ int tile(int token, int digit) { return NT == 1 ? 0 : token / 8 * 3 + digit; }
+  static __device__ __forceinline__ int column(int token, int digit) { return NT == 1 ? 2 * digit + token : token % 8; }
+};
+
+// What a scale group of x contributes beside its digits. NT = 1: of a column, 2^-e 256^c and the digits' sum.
+struct __align__(8) ColumnFactor {
+  float scale;
+  int sum;
+};
+// NT = 3, 6: of a token, 2^-e and the sums of d_0 + 256 d_1 and of d_2.
+struct __align__(16) TokenFactor {
+  float scale;
+  int low, high, unused;
+};
+template <int NT>
+constexpr int kFactorBytes = NT == 1 ? 8 * int(sizeof(ColumnFactor)) : NT / 3 * 8 * int(sizeof(TokenFactor));  // of a group
+
+constexpr int kPieces = 2;  // tiles that a warp's run of units can touch
+template <int NT>
+constexpr int kPiece = Columns<NT>::kTokens * kRows;  // floats of a tile's sums
+
+// Shared memory, in order: rings, x's digits, factors, pieces, the block's sums, barriers, lists.
+template <int NG, int NT>
+struct Layout {
+  size_t digits, factors, pieces, sums, bars, lists, bytes;
+  __host__ __device__ Layout(int depth, int units, int cluster, bool ids, int experts, int slots) {
+    digits = size_t(kWarps) * depth * kUnitBytes;
+    factors = digits + size_t(units) * 8 * NT * 256;
+    pieces = factors + size_t(units) * NG * kFactorBytes<NT>;
+    sums = pieces + size_t(kWarps) * kPieces * kPiece<NT> * 4;
+    bars = sums + (cluster > 1 ? size_t(2) * kWarps * kPiece<NT> * 4 : 0);
+    lists = bars + size_t(kWarps) * depth * 8;
+    bytes = lists + (ids ? Lists::bytes(experts, slots) : 0);
+  }
+};
+
+// NG: scale groups of a unit's 256 codes (8, 4, 2 for groups of 32, 64, multiples of 128). NT: tiles of 8
+// columns.
+template <class T, int NG, int NT>
+__global__ void __launch_bounds__(kThreads, 1) gemv_int4_kernel(const __grid_constant__ Int4Args a) {
+  using Col = Columns<NT>;
+  constexpr int kTok = Col::kTokens;
+  constexpr int kPerGroup = 8 / NG;  // 32-code chunks of a group
+  constexpr int kHeld = NG > 4 ? 2 : 1;
+  constexpr uint32_t kNibbles = 0x0F0F0F0Fu;
+  extern __shared__ uint8_t raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) / 1024 * 1024);
   cg::cluster_group cluster = cg::this_cluster();
+  const int split = int(cluster.block_rank()), splits = int(cluster.num_blocks());
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, g = lane / 4, t = lane % 4;
+  // This block's share of K, in units; every block lays its memory out for the largest share.
+  const int kb_all = (a.k + kUnitK - 1) / kUnitK;
+  const int kb0 = kb_all * split / splits, kbs = kb_all * (split + 1) / splits - kb0;
+  const Layout<NG, NT> at(a.depth, (kb_all + splits - 1) / splits, splits, a.ids != nullptr, a.experts, a.slots);
+  const int depth = a.depth;
+  uint8_t* digits = smem + at.digits;
+  uint8_t* factors = smem + at.factors;
+  float* pieces = reinterpret_cast<float*>(smem + at.pieces);
+  float* sums = reinterpret_cast<float*>(smem + at.sums);
+  Lists l;
+  l.base = reinterpret_cast<int*>(smem + at.lists);
+  l.act = reinterpret_cast<uint16_t*>(l.base + a.experts + 1);
+  l.start = l.act + a.experts;
+  l.list = l.start + a.experts + 1;
+  const uint32_t bar0 = smem_addr(smem + at.bars) + warp * depth * 8;
+  const uint32_t ring0 = smem_addr(smem) + warp * depth * kUnitBytes;
+  if (lane == 0) {
+    for (int i = 0; i < depth; ++i) mbarrier_init(bar0 + 8 * i, 1);
+    fence_barrier_init();
+    if (warp == 0) tma_prefetch_map(&a.map);
+  }
+  __syncwarp();
   griddep_wait();
   griddep_launch_dependents();
-  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, g = lane / 4, t = lane % 4;
-  const int n0 = (blockIdx.x / cluster.num_blocks()) * kRows;
-  const int split = int(cluster.block_rank()), splits = int(cluster.num_blocks());
-  int expert = 0, first = 0, count = 0;
-  if (a.ids == nullptr) {
-    first = blockIdx.y * kTok;
-    count = a.slots - first < kTok ? a.slots - first : kTok;
-  } else {
-    // Every block of a cluster reads the same ids and so takes the same way.
-    auto id_at = [&](int s) {
-      const int e = a.ids[s];
-      return e >= 0 && e < a.experts ? e : a.experts;  // a.experts: no expert
-    };
-    expert = a.by_slot ? id_at(blockIdx.y) : int(blockIdx.y);
-    if (warp == 0) {
-      int found = 0;
-      for (int s0 = 0; s0 < a.slots; s0 += 32) {
-        const int s = s0 + lane;
-        const bool mine = s < a.slots && id_at(s) == expert;
-        const unsigned who = __ballot_sync(0xFFFFFFFFu, mine);
-        if (mine) list[found + __popc(who & ((1u << lane) - 1))] = s;
-        found += __popc(who);
-      }
-      if (lane == 0) list_size = found;
-    }
-    __syncthreads();
-    count = list_size;
-    if (count == 0 || (a.by_slot && list[0] != int(blockIdx.y))) return;
+
+  int passes = (a.slots + kTok - 1) / kTok, active = 0;
+  if (a.ids != nullptr) {
+    build_lists<kTok>(a, l, reinterpret_cast<int*>(digits), &active);
+    passes = l.base[active];
   }
-  const long long row_a = n0 + g < a.n ? n0 + g : a.n - 1, row_b = n0 + g + 8 < a.n ? n0 + g + 8 : a.n - 1;
-  const bool any = a.ids == nullptr || expert < a.experts;
-  const uint8_t* q = a.q + (any ? expert : 0) * a.stride_q;
-  const long long s_off = (any ? expert : 0) * a.stride_s;
-  const uint8_t* z = a.zeros != nullptr ? a.zeros + (any ? expert : 0) * a.stride_z : nullptr;
-  auto scale_at = [&](long long row, int gi) {
-    const long long i = s_off + row * a.lds + gi;
-    return a.f32_scales ? static_cast<const float*>(a.scales)[i] : to_f32(static_cast<const T*>(a.scales)[i]);
+  // The tokens and the matrix of a pass.
+  struct Pass {
+    int expert, first, count;
   };
-  const int chunks = (a.k + kChunk - 1) / kChunk;
-  for (int base = 0; base < count; base += kTok) {
-    const int here = count - base < kTok ? count - base : kTok;
-    const T* xp[kTiles];
-    bool live[kTiles];
-#pragma unroll
-    for (int j = 0; j < kTiles; ++j) {
-      live[j] = j * 8 + g < here;
-      const int slot = !live[j] ? 0 : a.ids == nullptr ? first + j * 8 + g : list[base + j * 8 + g];
-      xp[j] = static_cast<const T*>(a.x) + (long long)(slot / a.x_div) * a.ldx;
+  auto pass_of = [&](int pass) {
+    Pass p;
+    if (a.ids == nullptr) {
+      p.expert = 0;
+      p.first = pass * kTok;
+      p.count = a.slots - p.first;
+    } else {
+      int lo = 0, hi = active;  // the last active expert whose base is not above `pass`
+      while (hi - lo > 1) {
+        const int mid = (lo + hi) / 2;
+        if (l.base[mid] <= pass) lo = mid;
+        else hi = mid;
+      }
+      p.expert = l.act[lo];
+      p.first = l.start[lo] + (pass - l.base[lo]) * kTok;
+      p.count = l.start[lo + 1] - p.first;
     }
-    float acc[kTiles][4] = {};
-    if (any) {
-      for (int c = split * kWarps + warp; c < chunks; c += splits * kWarps) {
+    if (p.count > kTok) p.count = kTok;
+    return p;
+  };
+  auto slot_of = [&](int i) { return a.ids == nullptr ? i : int(l.list[i]); };
+
+  // The cluster's tiles [m0, m1) of all passes' tiles go in batches of up to 16 of one pass. A batch's units
+  // (tile, 256 codes of this block's K) are dealt to the warps in even, consecutive runs, so a run touches at
+  // most two tiles. A warp's share of one tile is a stretch.
+  const int clusters = int(gridDim.x) / splits, c = int(blockIdx.x) / splits;
+  const int m0 = int((long long)passes * a.tiles * c / clusters), m1 = int((long long)passes * a.tiles * (c + 1) / clusters);
+  struct Stretch {
+    int batch, count;  // the batch's first tile and its tiles; batch = m1: no more
+    int pass, row0;    // of its first tile
+    int tile, kb;      // the stretch: its tile, first unit and units
+    int units, left;   // left: of the run, behind the stretch
+  };
+  auto cut = [&](Stretch& s, int begin, int end) {
+    s.left = end - begin;
+    s.tile = s.kb = s.units = 0;
+    if (s.left > 0) {
+      s.tile = begin / kbs;
+      s.kb = begin - s.tile * kbs;
+      s.units = s.left < kbs - s.kb ? s.left : kbs - s.kb;
+      s.left -= s.units;
+    }
+  };
+  auto begin_batch = [&](Stretch& s) {
+    if (s.batch >= m1) return;
+    s.pass = s.batch / a.tiles;
+    const int first = s.batch - s.pass * a.tiles;
+    s.row0 = first * kRows;
+    s.count = min(kWarps, min(a.tiles - first, m1 - s.batch));
+    cut(s, s.count * kbs * warp / kWarps, s.count * kbs * (warp + 1) / kWarps);
+  };
+  auto next_batch = [&](Stretch& s) {
+    s.batch += s.count;
+    begin_batch(s);
+  };
+  auto second = [&](Stretch& s) {  // the run's next stretch, in the batch
+    s.units = s.left;
+    s.left = 0;
+    s.kb = 0;
+    ++s.tile;
+  };
+  auto next_stretch = [&](Stretch& s) {  // of whatever batch
+    if (s.left > 0) return second(s);
+    do next_batch(s);
+    while (s.batch < m1 && s.units == 0);
+  };
+
+  Stretch ahead = {};  // lane 0: where the next unit to load lies
+  ahead.batch = m0;
+  begin_batch(ahead);
+  if (ahead.units == 0) next_stretch(ahead);
+  int load_x = 0, load_y = 0, load_expert = 0, load_left = 0;
+  auto aim = [&]() {
+    if (ahead.batch >= m1) return;
+    load_x = (kb0 + ahead.kb) * (kUnitK / 2);
+    load_y = ahead.row0 + ahead.tile * kRows;
+    load_expert = pass_of(ahead.pass).expert;
+    load_left = ahead.units;
+  };
+  auto load = [&](uint32_t at_slot, uint32_t bar) {
+    if (load_left == 0) return;
+    mbarrier_arrive_expect_tx(bar, kUnitBytes);
+    tma_load_3d(at_slot, &a.map, bar, load_x, load_y, load_expert);
+    load_x += kUnitK / 2;
+    if (--load_left == 0) {
+      next_stretch(ahead);
+      aim();
+    }
+  };
+  if (lane == 0) {
+    aim();
+    for (int i = 0; i < depth; ++i) load(ring0 + i * kUnitBytes, bar0 + 8 * i);
+  }
+
+  // x of a pass as digits, a warp taking 128 K-elements of a token at a time, a lane 4 of them.
+  auto convert = [&](Pass const& p) {
+    constexpr int kLanes = 32 / (NG / 2);  // lanes of a scale group
+    for (int i = warp; i < p.count * kbs * 2; i += kWarps) {
+      const int token = i / (kbs * 2), block = i % (kbs * 2);
+      const int k = kb0 * kUnitK + block * 128 + lane * 4;
+      const T* src = static_cast<const T*>(a.x) + (long long)(slot_of(p.first + token) / a.x_div) * a.ldx + k;
+      T raw4[4] = {};
+      if (k < a.k) {
+        const uint2 u = *reinterpret_cast<const uint2*>(src);
+        memcpy(raw4, &u, 8);
+      }
+      float v[4], top = 0.0f;
+      bool odd = false;
 #pragma unroll
-        for (int h = 0; h < kHops; ++h) {
-          const int k0 = c * kChunk + 8 * kWords * (4 * h + t);
-          const bool ok = k0 < a.k;  // K is a multiple of 32 = the most that a lane holds
-          const int kg = c * kChunk + 32 * kWords * h;  // where the row's four lanes begin
-          if (kg >= a.k) break;
-          const int gi = kg / a.group;
-          uint32_t wa[kWords], wb[kWords];
-          load_words<kWords>(q + row_a * a.ldq + k0 / 2, ok, wa);
-          load_words<kWords>(q + row_b * a.ldq + k0 / 2, ok, wb);
-          const uint32_t off_a = Codes<T>::offset(z != nullptr ? z[row_a * a.ldz + gi] : 8);
-          const uint32_t off_b = Codes<T>::offset(z != nullptr ? z[row_b * a.ldz + gi] : 8);
-          const float sa = scale_at(row_a, gi), sb = scale_at(row_b, gi);
-          float part[kTiles][4] = {};
+      for (int j = 0; j < 4; ++j) {
+        v[j] = to_f32(raw4[j]);
+        top = fmaxf(top, fabsf(v[j]));
+        odd |= !(fabsf(v[j]) < INFINITY);
+      }
 #pragma unroll
-          for (int i = 0; i < kWords; ++i) {
-            uint32_t ra[4], rb[4];
-            Codes<T>::expand(wa[i], off_a, ra);
-            Codes<T>::expand(wb[i], off_b, rb);
-            const uint32_t a0[4] = {ra[0], rb[0], ra[1], rb[1]}, a1[4] = {ra[2], rb[2], ra[3], rb[3]};
+      for (int o = kLanes / 2; o > 0; o /= 2) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
+      // An infinity or a NaN makes the token's results NaN: its group's factor is NaN.
+      const unsigned who = __ballot_sync(0xFFFFFFFFu, odd);
+      const bool bad = (who >> (lane / kLanes * kLanes) & (kLanes == 32 ? 0xFFFFFFFFu : (1u << (kLanes % 32)) - 1)) != 0;
+      // Largest |X| in [2^21, 2^22]; below 2^-105 the steps stay at 2^-126.
+      int e = 21 + 127 - int(__float_as_uint(top) >> 23);
+      e = e < 126 ? e : 126;
+      const float up = __int_as_float((e + 127) << 23), down = bad ? NAN : __int_as_float((127 - e) << 23);
+      int d[3][4], low = 0, high = 0;  // digit sums: c = 0 and 1 in the halves of `low`
 #pragma unroll
-            for (int j = 0; j < kTiles; ++j) {
-              if (kTiles > 1 && j * 8 >= here) break;
-              uint4 u = make_uint4(0, 0, 0, 0);
-              if (live[j] && ok) u = __ldg(reinterpret_cast<const uint4*>(xp[j] + k0 + 8 * i));
-              Codes<T>::mma(part[j], a0, __byte_perm(u.x, u.z, 0x5410), __byte_perm(u.x, u.z, 0x7632));
-              Codes<T>::mma(part[j], a1, __byte_perm(u.y, u.w, 0x5410), __byte_perm(u.y, u.w, 0x7632));
-            }
-          }
+      for (int j = 0; j < 4; ++j) {
+        int x = bad ? 0 : __float2int_rn(v[j] * up);
 #pragma unroll
-          for (int j = 0; j < kTiles; ++j) {
-            acc[j][0] += sa * part[j][0];
-            acc[j][1] += sa * part[j][1];
-            acc[j][2] += sb * part[j][2];
-            acc[j][3] += sb * part[j][3];
-          }
+        for (int c = 0; c < 3; ++c) {
+          d[c][j] = int(int8_t(x));
+          x = (x - d[c][j]) >> 8;
+        }
+        low += d[0][j] + d[1][j] * 65536;
+        high += d[2][j];
+      }
+#pragma unroll
+      for (int o = kLanes / 2; o > 0; o /= 2) {
+        low += __shfl_xor_sync(0xFFFFFFFFu, low, o);
+        high += __shfl_xor_sync(0xFFFFFFFFu, high, o);
+      }
+      // Of a lane's eight codes the even ones (low nibbles) lie before the odd ones, as the masks leave them.
+      const int chunk = block * 4 + lane / 8;
+#pragma unroll
+      for (int c = 0; c < 3; ++c) {
+        uint8_t* to = digits + (size_t(chunk) * NT + Col::tile(token, c)) * 256 + Col::column(token, c) * 32 + lane % 8 / 2 * 8 +
+                      lane % 2 * 2;
+        *reinterpret_cast<uint16_t*>(to) = uint16_t((d[c][0] & 255) | (d[c][2] & 255) << 8);
+        *reinterpret_cast<uint16_t*>(to + 4) = uint16_t((d[c][1] & 255) | (d[c][3] & 255) << 8);
+      }
+      if (lane % kLanes == 0) {
+        uint8_t* to = factors + size_t(block * (NG / 2) + lane / kLanes) * kFactorBytes<NT>;
+        const int s0 = int(int16_t(low)), s1 = (low - s0) >> 16;
+        if constexpr (NT == 1) {
+          ColumnFactor* f = reinterpret_cast<ColumnFactor*>(to) + token;
+          f[0] = {down, s0};
+          f[2] = {down * 256.0f, s1};
+          f[4] = {down * 65536.0f, high};
+        } else {
+          reinterpret_cast<TokenFactor*>(to)[token] = {down, s0 + 256 * s1, high, 0};
         }
       }
     }
-    // The warps' sums, then the cluster's blocks' sums, each in a fixed order.
+  };
+
+  // A unit's scales and zero points, loaded one unit ahead: lane t of a row's four holds group t (and
+  // t + 4 of eight). Rows behind the matrix and groups behind K read the last ones: the first are not
+  // stored, the second multiply zeros.
+  struct Scales {
+    float s[2][kHeld];
+    int z[2][kHeld];
+  };
+  const int last_group = (a.k + a.group - 1) / a.group - 1, group_span = NG == 2 ? a.group / 128 : 1;
+  struct Rows {
+    const void* s[2];
+    const uint8_t* z[2];
+  };
+  const int scale_bytes = a.f32_scales ? 4 : 2;
+  auto rows_of = [&](int expert, int row0) {
+    Rows r;
 #pragma unroll
-    for (int j = 0; j < kTiles; ++j) {
-      float* r = red[warp] + (j * 8 + 2 * t) * kRows + g;  // [token][row]
-      r[0] = acc[j][0];
-      r[kRows] = acc[j][1];
-      r[8] = acc[j][2];
-      r[kRows + 8] = acc[j][3];
+    for (int i = 0; i < 2; ++i) {
+      const int row = min(row0 + i * 8 + g, a.n - 1);
+      r.s[i] = static_cast<const char*>(a.scales) + (expert * a.stride_s + row * a.lds) * scale_bytes;
+      r.z[i] = a.zeros + expert * a.stride_z + row * a.ldz;
     }
-    __syncthreads();
-    for (int i = threadIdx.x; i < kRows * kTok; i += kThreads) {
-      float s = red[0][i];
+    return r;
+  };
+  auto load_scales = [&](Rows const& rows, int kb, Scales& v) {
 #pragma unroll
-      for (int w = 1; w < kWarps; ++w) s += red[w][i];
-      red[0][i] = s;
-    }
-    if (splits > 1) cluster.sync();
-    else __syncthreads();
-    if (split == 0) {
-      for (int i = threadIdx.x; i < kRows * here; i += kThreads) {
-        float s = red[0][i];
-        for (int r = 1; r < splits; ++r) s += cluster.map_shared_rank(&red[0][0], r)[i];
-        const int n = n0 + i % kRows, tok = i / kRows;
-        if (n >= a.n) continue;
-        const long long o = (long long)(a.ids == nullptr ? first + tok : list[base + tok]) * a.ldo + n;
-        if (a.f32_out) static_cast<float*>(a.out)[o] = s;
-        else static_cast<T*>(a.out)[o] = from_f32<T>(s);
+    for (int h = 0; h < kHeld; ++h) {
+      int gi = kb * NG + (t + 4 * h) % NG;
+      if (NG == 2 && group_span != 1) gi /= group_span;
+      gi = min(gi, last_group);
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        v.s[r][h] = a.f32_scales ? static_cast<const float*>(rows.s[r])[gi] : to_f32(static_cast<const T*>(rows.s[r])[gi]);
+        v.z[r][h] = a.zeros != nullptr ? rows.z[r][gi] : 8;
       }
     }
-    if (splits > 1) cluster.sync();
-    else __syncthreads();
+  };
+
+  auto store = [&](int slot, int n, float v) {
+    const long long o = (long long)slot * a.ldo + n;
+    if (a.f32_out) static_cast<float*>(a.out)[o] = v;
+    else static_cast<T*>(a.out)[o] = from_f32<T>(v);
+  };
+
+  constexpr int kSets = NT == 1 ? 1 : NT / 3;  // groups of 8 tokens
+  Stretch cur = {};
+  cur.batch = m0;
+  begin_batch(cur);
+  Stretch peek = cur;
+  if (peek.batch < m1 && peek.units == 0) next_stretch(peek);
+  Scales now = {}, next = {};
+  Rows rows = {};
+  if (peek.batch < m1) {
+    rows = rows_of(pass_of(peek.pass).expert, peek.row0 + peek.tile * kRows);
+    load_scales(rows, kb0 + peek.kb, now);
   }
+  // Where a lane reads: its ldmatrix rows in a slot (swizzled by 16 bytes), its digits and factors in a unit.
+  uint32_t in_slot[4];
+#pragma unroll
+  for (int pair = 0; pair < 4; ++pair) in_slot[pair] = lane % 16 * 128 + (((pair * 2 + lane / 16) ^ (lane & 7)) * 16);
+  int slot = 0, pass = -1, flip = 0;
+  uint32_t parity = 0;
+  bool failed = false;
+  Pass p = {};
+  while (cur.batch < m1) {
+    if (cur.pass != pass) {
+      pass = cur.pass;
+      p = pass_of(pass);
+      convert(p);
+      __syncthreads();
+    }
+    int piece = 0;
+    while (cur.units > 0 && !failed) {
+      // The next stretch, whose first scales are loaded in this one's last unit.
+      if (peek.batch < m1) next_stretch(peek);
+      float acc[kSets][4] = {};
+      const uint2* b = reinterpret_cast<const uint2*>(digits + size_t(cur.kb) * 8 * NT * 256) + lane;
+      const uint4* fp = reinterpret_cast<const uint4*>(factors + size_t(cur.kb) * NG * kFactorBytes<NT>) + (NT == 1 ? t : 2 * t);
+      for (int u = 0; u < cur.units; ++u) {
+        if (u + 1 < cur.units) {
+          load_scales(rows, kb0 + cur.kb + u + 1, next);
+        } else if (peek.batch < m1) {
+          rows = rows_of(pass_of(peek.pass).expert, peek.row0 + peek.tile * kRows);
+          load_scales(rows, kb0 + peek.kb, next);
+        }
+        const uint32_t bar = bar0 + 8 * slot, base = ring0 + slot * kUnitBytes;
+        if (!mbarrier_wait(bar, parity, a.timeout_ns)) {
+          failed = true;
+          break;
+        }
+        int part[NT][4];
+#pragma unroll
+        for (int pair = 0; pair < 4; ++pair) {
+          // Matrices: rows 0-7 and 8-15 of chunk 2 pair, then of chunk 2 pair + 1.
+          uint32_t w[4];
+          ldmatrix_x4(w, base + in_slot[pair]);
+#pragma unroll
+          for (int cc = 0; cc < 2; ++cc) {
+            const int c8 = pair * 2 + cc;
+            const uint32_t f[4] = {w[2 * cc] & kNibbles, w[2 * cc + 1] & kNibbles, (w[2 * cc] >> 4) & kNibbles,
+                                   (w[2 * cc + 1] >> 4) & kNibbles};
+#pragma unroll
+            for (int j = 0; j < NT; ++j) {
+              if (c8 % kPerGroup == 0) part[j][0] = part[j][1] = part[j][2] = part[j][3] = 0;
+              if (j >= 3 && p.count <= 8) continue;
+              mma_u8s8(part[j], f, b[(c8 * NT + j) * 32]);
+            }
+            if (c8 % kPerGroup == kPerGroup - 1) {
+              const int gj = c8 / kPerGroup, from = (lane & 28) | (gj & 3);
+              float sc[2];
+              int z[2] = {8, 8};
+#pragma unroll
+              for (int r = 0; r < 2; ++r) {
+                sc[r] = __shfl_sync(0xFFFFFFFFu, now.s[r][gj / 4], from);
+                if (a.zeros != nullptr) z[r] = __shfl_sync(0xFFFFFFFFu, now.z[r][gj / 4], from);
+              }
+              if constexpr (NT == 1) {
+                const uint4 q = fp[gj * (kFactorBytes<NT> / 16)];
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                  acc[0][i] = fmaf(sc[i / 2] * __uint_as_float(i % 2 ? q.z : q.x),
+                                   float(part[0][i] - z[i / 2] * int(i % 2 ? q.w : q.y)), acc[0][i]);
+              } else {
+#pragma unroll
+                for (int set = 0; set < kSets; ++set) {
+                  if (set > 0 && p.count <= 8) continue;
+#pragma unroll
+                  for (int i = 0; i < 4; ++i) {
+                    const uint4 q = fp[gj * (kFactorBytes<NT> / 16) + set * 8 + i % 2];
+                    // |256 P_1 + P_0| and z times its sums stay below 2^30.
+                    const int low = part[3 * set + 1][i] * 256 + part[3 * set][i] - z[i / 2] * int(q.y);
+                    const int high = part[3 * set + 2][i] - z[i / 2] * int(q.z);
+                    acc[set][i] = fmaf(sc[i / 2] * __uint_as_float(q.x), fmaf(float(high), 65536.0f, float(low)), acc[set][i]);
+                  }
+                }
+              }
+            }
+          }
+        }
+        b += 8 * NT * 32;
+        fp += NG * (kFactorBytes<NT> / 16);
+        __syncwarp();
+        if (lane == 0) load(base, bar);
+        if (++slot == depth) {
+          slot = 0;
+          parity ^= 1;
+        }
+        now = next;
+      }
+      if (failed) break;
+      // This warp's part of the tile's sums, [token][row].
+      float* to = pieces + (warp * kPieces + piece) * kPiece<NT>;
+      ++piece;
+      if constexpr (NT == 1) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float v0 = __shfl_sync(0xFFFFFFFFu, acc[0][i], lane & 28), v1 = __shfl_sync(0xFFFFFFFFu, acc[0][i], (lane & 28) | 1),
+                      v2 = __shfl_sync(0xFFFFFFFFu, acc[0][i], (lane & 28) | 2);
+          if (t == 0) to[i % 2 * kRows + i / 2 * 8 + g] = v0 + v1 + v2;
+        }
+      } else {
+#pragma unroll
+        for (int set = 0; set < kSets; ++set)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) to[(set * 8 + 2 * t + i % 2) * kRows + i / 2 * 8 + g] = acc[set][i];
+      }
+      if (cur.left > 0) second(cur);
+      else cur.units = 0;
+    }
+    __syncthreads();
+    // The batch's tiles: the warps' parts in their order along K, then the cluster's blocks. Warp w's run is
+    // [count kbs w / 16, count kbs (w + 1) / 16), tile m's units [m kbs, (m + 1) kbs).
+    auto block_sum = [&](int i) {
+      const int m = i / kPiece<NT>, o = i % kPiece<NT>;
+      float sum = 0.0f;
+      for (int w = m * kWarps / cur.count; w < kWarps; ++w) {
+        const int lo = cur.count * kbs * w / kWarps, hi = cur.count * kbs * (w + 1) / kWarps;
+        if (lo >= (m + 1) * kbs) break;
+        if (lo >= hi || hi <= m * kbs) continue;
+        sum += pieces[(w * kPieces + (lo >= m * kbs ? 0 : 1)) * kPiece<NT> + o];  // 1: the run began in the tile before
+      }
+      return sum;
+    };
+    auto put = [&](int i, float v) {
+      const int m = i / kPiece<NT>, token = i % kPiece<NT> / kRows, n = cur.row0 + m * kRows + i % kRows;
+      if (token < p.count && n < a.n) store(slot_of(p.first + token), n, v);
+    };
+    const int cells = cur.count * kPiece<NT>;
+    if (splits == 1) {
+      for (int i = threadIdx.x; i < cells; i += kThreads) put(i, block_sum(i));
+      __syncthreads();
+    } else {
+      // Two buffers: a block writes one again only after a barrier that follows its readers' reads.
+      float* mine = sums + flip * kWarps * kPiece<NT>;
+      flip ^= 1;
+      for (int i = threadIdx.x; i < cells; i += kThreads) mine[i] = block_sum(i);
+      cluster.sync();
+      for (int i = threadIdx.x; i < cells; i += kThreads) {
+        if (i / kPiece<NT> % splits != split) continue;
+        float v = 0.0f;
+        for (int r = 0; r < splits; ++r) v += cluster.map_shared_rank(mine, r)[i];
+        put(i, v);
+      }
+    }
+    next_batch(cur);
+  }
+  if (splits > 1) cluster.sync();  // no block leaves while another may still read its sums
+  if (failed) {
+    // The loads still under way end, or are given up on, before the block leaves.
+    if (lane == 0) atomicOr(a.status, kl::gemm::kStatusProducerTimeout);
+    for (int i = 0; i < depth; ++i) {
+      mbarrier_wait(bar0 + 8 * slot, parity, a.timeout_ns);
+      if (++slot == depth) {
+        slot = 0;
+        parity ^= 1;
+      }
+    }
+  }
+  // Rows of slots without an expert.
+  if (a.ids != nullptr && l.start[active] < a.slots)
+    for (int s = blockIdx.x; s < a.slots; s += gridDim.x) {
+      const int e = a.ids[s];
+      if (e >= 0 && e < a.experts) continue;
+      for (int n = threadIdx.x; n < a.n; n += kThreads) store(s, n, 0.0f);
+    }
 }
 
-template <class T, int kWords, int kTiles>
-cudaError_t launch(Int4Args const& a, cudaStream_t stream) {
-  const int tiles = (a.n + kRows - 1) / kRows;
-  const int chunks = (a.k + kChunk - 1) / kChunk;
-  const long long rows_y = a.ids == nullptr ? (a.slots + 8 * kTiles - 1) / (8 * kTiles) : a.by_slot ? a.slots : a.experts + 1;
-  // K is split over the blocks of a cluster while there are too few blocks to fill the SMs and every
-  // warp still has a chunk.
-  int splits = 1;
-  while (splits < 8 && (long long)tiles * rows_y * splits < 4 * 148 && chunks >= 2 * splits * kWarps) splits *= 2;
+struct Fit {
+  int cluster, depth;
+  size_t bytes;
+};
+
+// The smallest cluster whose blocks keep x's digits in 80 KB, else 8, and the ring that the rest holds (at
+// most 8 slots a warp, 256 KB in flight). depth 0: does not fit.
+template <int NG, int NT>
+Fit fit(Int4Args const& a) {
+  Fit f = {1, 0, 0};
+  const int kb = (a.k + kUnitK - 1) / kUnitK;
+  auto units = [&] { return (kb + f.cluster - 1) / f.cluster; };
+  while (f.cluster < 8 && size_t(units()) * (NT * 2048 + NG * kFactorBytes<NT>) > 80 * 1024) f.cluster *= 2;
+  for (int depth = 2; depth <= 8; ++depth) {
+    const Layout<NG, NT> l(depth, units(), f.cluster, a.ids != nullptr, a.experts, a.slots);
+    if (l.bytes + 1024 > size_t(kSmemLimit)) break;
+    f.depth = depth;
+    f.bytes = l.bytes + 1024;
+  }
+  return f;
+}
+
+template <class T, int NG, int NT>
+kl_status launch(Int4Args& a, Fit const& f, int device, cudaStream_t stream) {
+  auto* kernel = gemv_int4_kernel<T, NG, NT>;
+  static std::atomic<int> resident[64][4];  // clusters of 1, 2, 4, 8 that fit the device at once
+  const int which = f.cluster == 1 ? 0 : f.cluster == 2 ? 1 : f.cluster == 4 ? 2 : 3;
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute attr[2];
-  cfg.gridDim = dim3(unsigned(tiles * splits), unsigned(rows_y), 1);
   cfg.blockDim = dim3(kThreads, 1, 1);
-  cfg.dynamicSmemBytes = a.ids != nullptr ? size_t(a.slots) * 4 : 0;
+  cfg.dynamicSmemBytes = f.bytes;
   cfg.stream = stream;
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  attr[1].id = cudaLaunchAttributeClusterDimension;
-  attr[1].val.clusterDim.x = unsigned(splits);
-  attr[1].val.clusterDim.y = 1;
-  attr[1].val.clusterDim.z = 1;
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = unsigned(f.cluster);
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
+  int most = resident[device][which].load(std::memory_order_acquire);
+  if (most == 0) {
+    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemLimit);
+    if (e != cudaSuccess) return cuda_fail(e, "kl_gemv_int4 shared memory");
+    cfg.gridDim = dim3(unsigned(f.cluster), 1, 1);
+    cfg.dynamicSmemBytes = kSmemLimit;
+    cfg.numAttrs = 1;
+    e = cudaOccupancyMaxActiveClusters(&most, kernel, &cfg);
+    if (e != cudaSuccess) return cuda_fail(e, "kl_gemv_int4 occupancy");
+    if (most <= 0) return fail(KL_ERR_CUDA, "kl_gemv_int4: no room for a block");
+    resident[device][which].store(most, std::memory_order_release);
+    cfg.dynamicSmemBytes = f.bytes;
+  }
+  const long long passes = a.ids != nullptr ? a.slots : (a.slots + Columns<NT>::kTokens - 1) / Columns<NT>::kTokens;
+  const long long work = passes * a.tiles;
+  if (work > INT32_MAX / 2) return fail(KL_ERR_NOT_SUPPORTED, "kl_gemv_int4: too many rows of out");
+  a.depth = f.depth;
+  cfg.gridDim = dim3(unsigned((work < most ? work : most) * f.cluster), 1, 1);
   cfg.numAttrs = 2;
-  auto* kernel = gemv_int4_kernel<T, kWords, kTiles>;
-  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxSlots * 4);
-  if (e != cudaSuccess) return e;
-  return cudaLaunchKernelEx(&cfg, kernel, a);
+  cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, a);
+  return e == cudaSuccess ? KL_OK : cuda_fail(e, "kl_gemv_int4 launch");
 }
 
-template <class T, int kWords>
-cudaError_t by_tiles(Int4Args const& a, cudaStream_t stream) {
-  if (a.ids != nullptr) return a.slots <= 8 ? launch<T, kWords, 1>(a, stream) : launch<T, kWords, 2>(a, stream);
-  if (a.slots <= 8) return launch<T, kWords, 1>(a, stream);
-  if (a.slots <= 16) return launch<T, kWords, 2>(a, stream);
-  return launch<T, kWords, 4>(a, stream);
+// Columns by the tokens that a matrix meets (with ids: on average), fewer where x's digits would not fit.
+template <class T, int NG>
+kl_status by_tokens(Int4Args& a, int device, cudaStream_t stream) {
+  const int tokens = a.ids != nullptr ? (a.slots + a.experts - 1) / a.experts : a.slots;
+  if (tokens > 8)
+    if (const Fit f = fit<NG, 6>(a); f.depth >= 3) return launch<T, NG, 6>(a, f, device, stream);
+  if (tokens > 2)
+    if (const Fit f = fit<NG, 3>(a); f.depth >= 3) return launch<T, NG, 3>(a, f, device, stream);
+  const Fit f = fit<NG, 1>(a);
+  if (f.depth == 0) return fail(KL_ERR_NOT_SUPPORTED, "kl_gemv_int4: k does not fit");
+  return launch<T, NG, 1>(a, f, device, stream);
 }
 
 template <class T>
-cudaError_t by_group(Int4Args const& a, cudaStream_t stream) {
-  if (a.group == 32) return by_tiles<T, 1>(a, stream);
-  if (a.group == 64) return by_tiles<T, 2>(a, stream);
-  return by_tiles<T, 4>(a, stream);
+kl_status by_group(Int4Args& a, int device, cudaStream_t stream) {
+  if (a.group == 32) return by_tokens<T, 8>(a, device, stream);
+  if (a.group == 64) return by_tokens<T, 4>(a, device, stream);
+  return by_tokens<T, 2>(a, device, stream);
+}
+
+kl_status run(kl_int4_desc const& d, int64_t slots, cudaStream_t stream) {
+  const bool by_expert = d.ids != nullptr;
+  int device = 0;
+  cudaError_t e = cudaGetDevice(&device);
+  if (e != cudaSuccess) return cuda_fail(e, "cudaGetDevice");
+  if (device < 0 || device >= 64) return fail(KL_ERR_NOT_SUPPORTED, "device index above 63");
+  Int4Args a = {};
+  const int64_t matrices = by_expert ? d.experts : 1;
+  if (d.k > 0) {
+    const int64_t shape[3] = {matrices, d.n, d.k / 2};
+    const int64_t stride[3] = {matrices > 1 ? d.stride_q : d.n * d.ldq, d.ldq, 1};
+    kl::TmaOptions opt;
+    opt.l2_promotion = CU_TENSOR_MAP_L2_PROMOTION_L2_256B;
+    kl::detail::encode_tma_map(&a.map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, CU_TENSOR_MAP_SWIZZLE_128B, 128, kRows, d.q, 3,
+                               shape, stride, opt);
+  }
+  a.x = d.x;
+  a.ldx = d.ldx;
+  a.scales = d.scales;
+  a.lds = d.ld_scales;
+  a.stride_s = matrices > 1 ? d.stride_scales : 0;
+  a.zeros = d.zeros;
+  a.ldz = d.ld_zeros;
+  a.stride_z = matrices > 1 ? d.stride_zeros : 0;
+  a.ids = d.ids;
+  a.experts = int(matrices);
+  a.slots = int(slots);
+  a.x_div = by_expert && !d.x_per_slot ? int(d.topk) : 1;
+  a.out = d.out;
+  a.ldo = d.ldo;
+  a.n = int(d.n);
+  a.k = int(d.k);
+  a.group = int(d.group);
+  a.f32_scales = d.scale_type == KL_F32;
+  a.f32_out = d.out_type == KL_F32;
+  a.tiles = (a.n + kRows - 1) / kRows;
+  a.timeout_ns = wait_timeout_ns();
+  kl_status s = device_status_ptr(&a.status);
+  if (s != KL_OK) return s;
+  return d.x_type == KL_BF16 ? by_group<__nv_bfloat16>(a, device, stream) : by_group<__half>(a, device, stream);
 }
 
 }  // namespace
 }  // namespace kl::capi
-
 extern "C" kl_status kl_gemv_int4(const kl_int4_desc* d, void* stream) {
   using namespace kl::capi;
   auto bad = [](char const* what) { return fail(KL_ERR_INVALID_ARGUMENT, std::string("kl_gemv_int4: ") + what); };
@@ -307,9 +781,8 @@ extern "C" kl_status kl_gemv_int4(const kl_int4_desc* d, void* stream) {
   const int64_t topk = by_expert ? d->topk : 1;
   if (d->tokens > INT32_MAX / 64 || d->n > INT32_MAX / 2 || d->k > INT32_MAX / 2 || topk > kMaxSlots) return bad("extent too large");
   const int64_t slots = d->tokens * topk;
-  if (by_expert && (slots > kMaxSlots || d->experts > 65534))
-    return fail(KL_ERR_NOT_SUPPORTED, "kl_gemv_int4: at most 8192 (token, expert) pairs and 65534 experts (more tokens: kl_moe_plan and the m-grouped GEMM)");
-  if (!by_expert && slots > 65535 * 8) return fail(KL_ERR_NOT_SUPPORTED, "kl_gemv_int4: at most 524280 tokens");
+  if (by_expert && (slots > kMaxSlots || d->experts > kMaxExperts))
+    return fail(KL_ERR_NOT_SUPPORTED, "kl_gemv_int4: at most 4096 (token, expert) pairs and 1024 experts (more tokens: kl_moe_plan and the m-grouped GEMM)");
   if (d->x_type != KL_BF16 && d->x_type != KL_F16) return fail(KL_ERR_NOT_SUPPORTED, "kl_gemv_int4: x must be bf16 or f16");
   if (d->scale_type != d->x_type && d->scale_type != KL_F32)
     return fail(KL_ERR_NOT_SUPPORTED, "kl_gemv_int4: scales must have x's type or f32");
@@ -318,6 +791,7 @@ extern "C" kl_status kl_gemv_int4(const kl_int4_desc* d, void* stream) {
   if (d->group != 32 && d->group != 64 && (d->group < 128 || d->group % 128 != 0))
     return bad("group must be 32, 64 or a multiple of 128");
   if (d->k % 32 != 0) return bad("k must be a multiple of 32");
+  if (d->k > kMaxK) return fail(KL_ERR_NOT_SUPPORTED, "kl_gemv_int4: k up to 65536");
   if (slots == 0 || d->n == 0) return KL_OK;
   const int64_t groups = (d->k + d->group - 1) / d->group;
   if (d->ldo < d->n || d->ldx < d->k || d->ldq < d->k / 2 || d->ld_scales < groups || (d->zeros != nullptr && d->ld_zeros < groups))
@@ -325,33 +799,11 @@ extern "C" kl_status kl_gemv_int4(const kl_int4_desc* d, void* stream) {
   if (d->out == nullptr || (d->k > 0 && (d->x == nullptr || d->q == nullptr || d->scales == nullptr))) return bad("null pointer");
   if (d->k > 0 && (!aligned16(d->x) || !aligned16(d->q) || d->ldx % 8 != 0 || d->ldq % 16 != 0))
     return bad("x and q must be 16-byte aligned with row pitches that are multiples of 16 bytes");
-  if (by_expert && d->experts > 1 && (d->stride_q % 16 != 0 || d->stride_q < 0 || d->stride_scales < 0 || d->stride_zeros < 0))
-    return bad("expert strides must not be negative, stride_q a multiple of 16 bytes");
-  Int4Args a = {};
-  a.x = d->x;
-  a.ldx = d->ldx;
-  a.q = static_cast<const uint8_t*>(d->q);
-  a.ldq = d->ldq;
-  a.stride_q = d->stride_q;
-  a.scales = d->scales;
-  a.lds = d->ld_scales;
-  a.stride_s = d->stride_scales;
-  a.zeros = d->zeros;
-  a.ldz = d->ld_zeros;
-  a.stride_z = d->stride_zeros;
-  a.ids = d->ids;
-  a.experts = by_expert ? int(d->experts) : 1;
-  a.slots = int(slots);
-  a.x_div = by_expert && !d->x_per_slot ? int(topk) : 1;
-  a.out = d->out;
-  a.ldo = d->ldo;
-  a.n = int(d->n);
-  a.k = int(d->k);
-  a.group = int(d->group);
-  a.f32_scales = d->scale_type == KL_F32;
-  a.f32_out = d->out_type == KL_F32;
-  a.by_slot = by_expert && slots <= d->experts;
-  cudaStream_t s = static_cast<cudaStream_t>(stream);
-  cudaError_t e = d->x_type == KL_BF16 ? by_group<__nv_bfloat16>(a, s) : by_group<__half>(a, s);
-  return e == cudaSuccess ? KL_OK : cuda_fail(e, "kl_gemv_int4 launch");
+  if (by_expert && d->experts > 1 && (d->stride_q % 16 != 0 || d->stride_q <= 0 || d->stride_scales < 0 || d->stride_zeros < 0))
+    return bad("expert strides must not be negative, stride_q a positive multiple of 16 bytes");
+  try {
+    return run(*d, slots, static_cast<cudaStream_t>(stream));
+  } catch (std::exception const& e) {
+    return bad(e.what());
+  }
 }

@@ -101,7 +101,7 @@ __device__ __forceinline__ void load_row(const T* row, int lane, int experts, bo
     } else if (vec) {
       const uint4* p = reinterpret_cast<const uint4*>(row + e0);
 #pragma unroll
-      for (int j = 0; j < 8 / kPerVec<T>; ++j) unpack<T>(__ldg(p + j), v + 8 * i + j * kPerVec<T>);
+      for (int j = 0; j < 8 / kPerVec<T>; ++j) unpack<T>(p[j], v + 8 * i + j * kPerVec<T>);
     } else {
 #pragma unroll
       for (int j = 0; j < 8; ++j) v[8 * i + j] = e0 + j < experts ? to_f32(row[e0 + j]) : -INFINITY;

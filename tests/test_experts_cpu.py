@@ -112,7 +112,7 @@ def test_row_movers_refusals():
     (dict(ldq=2056), "aligned"), (dict(x=None), "null"), (dict(q=None), "null"), (dict(scales=None), "null"),
     (dict(out=None), "null"), (dict(tokens=-1), "negative"), (dict(tokens=1 << 40), "too large"),
     (dict(ids=P, experts=0, topk=1), "experts"), (dict(ids=P, experts=4, topk=0), "topk"),
-    (dict(ids=P, experts=4, topk=8192, tokens=2), "8192"), (dict(ids=P, experts=65535, topk=1), "experts"),
+    (dict(ids=P, experts=4, topk=2049, tokens=2), "4096"), (dict(ids=P, experts=1025, topk=1), "1024 experts"),
     (dict(ids=P, experts=4, topk=1, stride_q=8), "stride"),
 ])
 def test_gemv_int4_refusals(over, what):
