@@ -6,14 +6,14 @@
 // cycle. Turned into bf16, eight codes cost eleven instructions and the SM, not the memory, sets the
 // time (measured: 2.0 TB/s). As unsigned bytes they cost three (two masks and a shift), so the products
 // are integer ones (mma.sync.m16n8k32, u8 x s8 -> s32): every block first writes x as fixed-point numbers
-// X = round(x 2^e), |X| <= 2^22, one e per token and scale group, in three signed digits of 8 bits,
+// X = round(x 2^e), |X| <= 2^22, one e for 128 K-elements of a token, in three signed digits of 8 bits,
 //   x ~ 2^-e (d_0 + 256 d_1 + 65536 d_2).
-// This rounding is at most 2^-22 of the group's largest |x|, what one addition in fp32 loses. The sums of a
-// group are exact: P_c = sum q d_c, and P_c - z sum d_c takes the zero point off without cancellation. Only
-// then come fp32 and the scales, sum_g s 2^-e 256^c (P_c - z D_c), accumulated in fp32 over the groups.
+// This rounding is at most 2^-22 of the 128 elements' largest |x|, what one addition in fp32 loses. The sums
+// of a scale group are exact: P_c = sum q d_c, and P_c - z D_c, D_c = sum d_c, takes the zero point off without
+// cancellation. Only then come fp32 and the scales: sum over the 128s of 2^-e sum_g s 256^c (P_c - z D_c).
 //
-// Layout: a block per SM, 16 warps, each with its own ring of TMA loads (boxes of 16 rows x 128
-// bytes = 256 codes), refilled as soon as a slot has been read, so that no warp waits for another
+// Layout: a block per SM, 16 warps, each with its own ring of TMA loads (units of 16 rows x 512
+// codes, two boxes of 128 bytes a row), refilled as soon as a slot has been read, so that no warp waits for another
 // while the weights stream. ldmatrix hands a lane eight codes of a row at a time. Where x's digits for all of K
 // would crowd out the ring, a cluster of 2, 4 or 8 blocks splits K and adds up through distributed
 // shared memory.
@@ -43,8 +43,9 @@ namespace {
 constexpr int kWarps = 16;
 constexpr int kThreads = 32 * kWarps;
 constexpr int kRows = 16;              // weight rows of a tile
-constexpr int kUnitK = 256;            // codes of a unit's row
-constexpr int kUnitBytes = kRows * kUnitK / 2;
+constexpr int kBoxBytes = kRows * 128;
+constexpr int kUnitK = 512;            // codes of a unit's row, in two boxes
+constexpr int kUnitBytes = 2 * kBoxBytes;
 constexpr int kMaxExperts = 1024;
 constexpr int kMaxSlots = 4096;        // (token, expert) pairs of a call with ids
 constexpr int kMaxK = 65536;
@@ -65,6 +66,7 @@ struct Int4Args {
   int n, k, group;
   int f32_scales, f32_out;
   int tiles;  // 16-row tiles of one matrix
+  int pair;   // NT = 1: a pass may have two tokens
   int depth;  // slots of a warp's ring
   int* status;
   unsigned long long timeout_ns;
@@ -77,10 +79,16 @@ __device__ __forceinline__ void ldmatrix_x4(uint32_t (&r)[4], uint32_t addr) {
                : "memory");
 }
 
-__device__ __forceinline__ void mma_u8s8(int (&d)[4], const uint32_t (&a)[4], uint2 b) {
-  asm("mma.sync.aligned.m16n8k32.row.col.s32.u8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-      : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3])
-      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b.x), "r"(b.y));
+// d = a b (+ d, unless `first`, a constant where it is called)
+__device__ __forceinline__ void mma_u8s8(int (&d)[4], const uint32_t (&a)[4], uint2 b, bool first) {
+  if (first)
+    asm("mma.sync.aligned.m16n8k32.row.col.s32.u8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"
+        : "=r"(d[0]), "=r"(d[1]), "=r"(d[2]), "=r"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b.x), "r"(b.y), "r"(0));
+  else
+    asm("mma.sync.aligned.m16n8k32.row.col.s32.u8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+        : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b.x), "r"(b.y));
 }
 
 // With ids: the experts that some slot names, each with its slots, in shared memory.
@@ -166,55 +174,54 @@ __device__ void build_lists(const Int4Args& a, Lists const& l, int* hist, int* a
 }
 
 // Columns of the products. Three digits of 8 tokens are three 8-column tiles, digit c of token i in
-// column i of tile c, so a lane holds the digits of the same tokens; up to two tokens fit one tile, digit c of
-// token i in column 2 c + i, and the digits meet by shuffles.
+// column i of tile c, so a lane holds the digits of the same tokens (NT = 3, 6); up to two tokens fit one tile, digit
+// c of token i in column 2 c + i, and the digits meet by shuffles (NT = 1).
 template <int NT>
-struct Columns {
-  static constexpr int kTokens = NT == 1 ? 2 : NT / 3 * 8;
-  static __device__ __forceinline__ int tile(int token, int digit) { return NT == 1 ? 0 : token / 8 * 3 + digit; }
-  static __device__ __forceinline__ int column(int token, int digit) { return NT == 1 ? 2 * digit + token : token % 8; }
-};
+constexpr int kTokens = NT == 1 ? 2 : NT / 3 * 8;
 
-// What a scale group of x contributes beside its digits. NT = 1: of a column, 2^-e 256^c and the digits' sum.
-struct __align__(8) ColumnFactor {
-  float scale;
-  int sum;
-};
-// NT = 3, 6: of a token, 2^-e and the sums of d_0 + 256 d_1 and of d_2.
-struct __align__(16) TokenFactor {
-  float scale;
-  int low, high, unused;
-};
+// x in shared memory. Digits: for every 32 K-elements a row of 32 bytes for each column (NT = 1: only the 3 or 6
+// that a launch uses). Sums D of a group: NT = 1: an int a column; else (D_0 + 256 D_1, D_2) a token.
+// Powers 2^-e of 128 elements: NT = 1: times 256^c, a float a column; else a float a token.
 template <int NT>
-constexpr int kFactorBytes = NT == 1 ? 8 * int(sizeof(ColumnFactor)) : NT / 3 * 8 * int(sizeof(TokenFactor));  // of a group
+__host__ __device__ constexpr int digit_bytes(int pair) {  // of 32 K-elements
+  return NT == 1 ? (pair ? 192 : 96) : NT * 256;
+}
+template <int NT>
+constexpr int kSumBytes = NT == 1 ? 32 : NT / 3 * 64;
+template <int NT>
+constexpr int kPowerBytes = NT == 1 ? 32 : NT / 3 * 32;
+template <int NG, int NT>
+__host__ __device__ constexpr int x_bytes(int pair) {  // of a unit
+  return 16 * digit_bytes<NT>(pair) + NG * kSumBytes<NT> + 4 * kPowerBytes<NT>;
+}
 
 constexpr int kPieces = 2;  // tiles that a warp's run of units can touch
 template <int NT>
-constexpr int kPiece = Columns<NT>::kTokens * kRows;  // floats of a tile's sums
+constexpr int kPiece = kTokens<NT> * kRows;  // floats of a tile's sums
 
-// Shared memory, in order: rings, x's digits, factors, pieces, the block's sums, barriers, lists.
+// Shared memory, in order: rings, x's digits, sums and powers, pieces, the block's sums, barriers, lists.
 template <int NG, int NT>
 struct Layout {
-  size_t digits, factors, pieces, sums, bars, lists, bytes;
-  __host__ __device__ Layout(int depth, int units, int cluster, bool ids, int experts, int slots) {
+  size_t digits, sums, powers, pieces, block, bars, lists, bytes;
+  __host__ __device__ Layout(int depth, int units, int pair, int cluster, bool ids, int experts, int slots) {
     digits = size_t(kWarps) * depth * kUnitBytes;
-    factors = digits + size_t(units) * 8 * NT * 256;
-    pieces = factors + size_t(units) * NG * kFactorBytes<NT>;
-    sums = pieces + size_t(kWarps) * kPieces * kPiece<NT> * 4;
-    bars = sums + (cluster > 1 ? size_t(2) * kWarps * kPiece<NT> * 4 : 0);
+    sums = digits + size_t(units) * 16 * digit_bytes<NT>(pair);
+    powers = sums + size_t(units) * NG * kSumBytes<NT>;
+    pieces = powers + size_t(units) * 4 * kPowerBytes<NT>;
+    block = pieces + size_t(kWarps) * kPieces * kPiece<NT> * 4;
+    bars = block + (cluster > 1 ? size_t(2) * kWarps * kPiece<NT> * 4 : 0);
     lists = bars + size_t(kWarps) * depth * 8;
     bytes = lists + (ids ? Lists::bytes(experts, slots) : 0);
   }
 };
 
-// NG: scale groups of a unit's 256 codes (8, 4, 2 for groups of 32, 64, multiples of 128). NT: tiles of 8
+// NG: scale groups of a unit's 512 codes (16, 8, 4 for groups of 32, 64, multiples of 128). NT: tiles of 8
 // columns.
 template <class T, int NG, int NT>
 __global__ void __launch_bounds__(kThreads, 1) gemv_int4_kernel(const __grid_constant__ Int4Args a) {
-  using Col = Columns<NT>;
-  constexpr int kTok = Col::kTokens;
-  constexpr int kPerGroup = 8 / NG;  // 32-code chunks of a group
-  constexpr int kHeld = NG > 4 ? 2 : 1;
+  constexpr int kTok = kTokens<NT>;
+  constexpr int kPerGroup = 16 / NG;  // 32-code chunks of a group
+  constexpr int kHeld = NG / 4;       // scales that a lane holds of each of its rows
   constexpr uint32_t kNibbles = 0x0F0F0F0Fu;
   extern __shared__ uint8_t raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) / 1024 * 1024);
@@ -224,12 +231,11 @@ __global__ void __launch_bounds__(kThreads, 1) gemv_int4_kernel(const __grid_con
   // This block's share of K, in units; every block lays its memory out for the largest share.
   const int kb_all = (a.k + kUnitK - 1) / kUnitK;
   const int kb0 = kb_all * split / splits, kbs = kb_all * (split + 1) / splits - kb0;
-  const Layout<NG, NT> at(a.depth, (kb_all + splits - 1) / splits, splits, a.ids != nullptr, a.experts, a.slots);
+  const Layout<NG, NT> at(a.depth, (kb_all + splits - 1) / splits, a.pair, splits, a.ids != nullptr, a.experts, a.slots);
   const int depth = a.depth;
   uint8_t* digits = smem + at.digits;
-  uint8_t* factors = smem + at.factors;
   float* pieces = reinterpret_cast<float*>(smem + at.pieces);
-  float* sums = reinterpret_cast<float*>(smem + at.sums);
+  float* block = reinterpret_cast<float*>(smem + at.block);
   Lists l;
   l.base = reinterpret_cast<int*>(smem + at.lists);
   l.act = reinterpret_cast<uint16_t*>(l.base + a.experts + 1);
@@ -278,7 +284,7 @@ __global__ void __launch_bounds__(kThreads, 1) gemv_int4_kernel(const __grid_con
   auto slot_of = [&](int i) { return a.ids == nullptr ? i : int(l.list[i]); };
 
   // The cluster's tiles [m0, m1) of all passes' tiles go in batches of up to 16 of one pass. A batch's units
-  // (tile, 256 codes of this block's K) are dealt to the warps in even, consecutive runs, so a run touches at
+  // (tile, 512 codes of this block's K) are dealt to the warps in even, consecutive runs, so a run touches at
   // most two tiles. A warp's share of one tile is a stretch.
   const int clusters = int(gridDim.x) / splits, c = int(blockIdx.x) / splits;
   const int m0 = int((long long)passes * a.tiles * c / clusters), m1 = int((long long)passes * a.tiles * (c + 1) / clusters);
@@ -338,6 +344,7 @@ __global__ void __launch_bounds__(kThreads, 1) gemv_int4_kernel(const __grid_con
     if (load_left == 0) return;
     mbarrier_arrive_expect_tx(bar, kUnitBytes);
     tma_load_3d(at_slot, &a.map, bar, load_x, load_y, load_expert);
+    tma_load_3d(at_slot + kBoxBytes, &a.map, bar, load_x + 128, load_y, load_expert);  // zeros behind K
     load_x += kUnitK / 2;
     if (--load_left == 0) {
       next_stretch(ahead);
@@ -349,84 +356,92 @@ __global__ void __launch_bounds__(kThreads, 1) gemv_int4_kernel(const __grid_con
     for (int i = 0; i < depth; ++i) load(ring0 + i * kUnitBytes, bar0 + 8 * i);
   }
 
-  // x of a pass as digits, a warp taking 128 K-elements of a token at a time, a lane 4 of them.
+  // x of a pass as digits: a warp takes 256 K-elements of a token at a time, a lane 8 of them.
+  const int digit_row = digit_bytes<NT>(a.pair);
   auto convert = [&](Pass const& p) {
-    constexpr int kLanes = 32 / (NG / 2);  // lanes of a scale group
+    constexpr int kLanes = 64 / NG;  // lanes of a scale group
     for (int i = warp; i < p.count * kbs * 2; i += kWarps) {
-      const int token = i / (kbs * 2), block = i % (kbs * 2);
-      const int k = kb0 * kUnitK + block * 128 + lane * 4;
-      const T* src = static_cast<const T*>(a.x) + (long long)(slot_of(p.first + token) / a.x_div) * a.ldx + k;
-      T raw4[4] = {};
-      if (k < a.k) {
-        const uint2 u = *reinterpret_cast<const uint2*>(src);
-        memcpy(raw4, &u, 8);
-      }
-      float v[4], top = 0.0f;
-      bool odd = false;
+      const int token = i / (kbs * 2), half = i - token * (kbs * 2);
+      const int k = kb0 * kUnitK + half * 256 + lane * 8;
+      uint4 u = make_uint4(0, 0, 0, 0);
+      if (k < a.k)
+        u = *reinterpret_cast<const uint4*>(static_cast<const T*>(a.x) + (long long)(slot_of(p.first + token) / a.x_div) * a.ldx + k);
+      // The largest |x|: both types order like their bits, with NaN above infinity.
+      uint32_t m = __vmaxu2(__vmaxu2(u.x & 0x7FFF7FFFu, u.y & 0x7FFF7FFFu), __vmaxu2(u.z & 0x7FFF7FFFu, u.w & 0x7FFF7FFFu));
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        v[j] = to_f32(raw4[j]);
-        top = fmaxf(top, fabsf(v[j]));
-        odd |= !(fabsf(v[j]) < INFINITY);
-      }
-#pragma unroll
-      for (int o = kLanes / 2; o > 0; o /= 2) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
-      // An infinity or a NaN makes the token's results NaN: its group's factor is NaN.
-      const unsigned who = __ballot_sync(0xFFFFFFFFu, odd);
-      const bool bad = (who >> (lane / kLanes * kLanes) & (kLanes == 32 ? 0xFFFFFFFFu : (1u << (kLanes % 32)) - 1)) != 0;
+      for (int o = 8; o > 0; o /= 2) m = __vmaxu2(m, __shfl_xor_sync(0xFFFFFFFFu, m, o));
+      const uint16_t top16 = uint16_t(max(m & 0xFFFFu, m >> 16));
+      T top_t;
+      memcpy(&top_t, &top16, 2);
+      const float top = to_f32(top_t);
+      const bool bad = !(top < INFINITY);  // an infinity or a NaN makes the token's results NaN
       // Largest |X| in [2^21, 2^22]; below 2^-105 the steps stay at 2^-126.
-      int e = 21 + 127 - int(__float_as_uint(top) >> 23);
-      e = e < 126 ? e : 126;
-      const float up = __int_as_float((e + 127) << 23), down = bad ? NAN : __int_as_float((127 - e) << 23);
-      int d[3][4], low = 0, high = 0;  // digit sums: c = 0 and 1 in the halves of `low`
+      const int e = min(21 + 127 - int(__float_as_uint(top) >> 23), 126);
+      const float up = bad ? 0.0f : __int_as_float((e + 127) << 23);
+      float v[8];
+      unpack<T>(u, v);
+      // 1.5 2^23 + X has X in its low bits; adding 0x80 to each byte and flipping its top bit leaves X's
+      // digits, each in [-128, 127], in three bytes.
+      uint32_t y[8];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        int x = bad ? 0 : __float2int_rn(v[j] * up);
-#pragma unroll
-        for (int c = 0; c < 3; ++c) {
-          d[c][j] = int(int8_t(x));
-          x = (x - d[c][j]) >> 8;
-        }
-        low += d[0][j] + d[1][j] * 65536;
-        high += d[2][j];
+      for (int j = 0; j < 8; ++j) {
+        const uint32_t x = __float_as_uint(fmaf(bad ? 0.0f : v[j], up, 12582912.0f));
+        y[j] = (x + (0x00808080u - 0x4B400000u)) ^ 0x00808080u;
       }
+      // By digit, the even elements (low nibbles) before the odd ones, as the masks leave the codes.
+      uint2 d[3];
+#pragma unroll
+      for (int odd = 0; odd < 2; ++odd) {
+        const uint32_t a01 = __byte_perm(y[odd], y[odd + 2], 0x5140), b01 = __byte_perm(y[odd + 4], y[odd + 6], 0x5140);
+        const uint32_t a2 = __byte_perm(y[odd], y[odd + 2], 0x7362), b2 = __byte_perm(y[odd + 4], y[odd + 6], 0x7362);
+        (odd ? d[0].y : d[0].x) = __byte_perm(a01, b01, 0x5410);
+        (odd ? d[1].y : d[1].x) = __byte_perm(a01, b01, 0x7632);
+        (odd ? d[2].y : d[2].x) = __byte_perm(a2, b2, 0x5410);
+      }
+      int sum[3];
+#pragma unroll
+      for (int c = 0; c < 3; ++c) sum[c] = __dp4a(int(d[c].x), 0x01010101, __dp4a(int(d[c].y), 0x01010101, 0));
+      int low = sum[0] + sum[1] * 65536, high = sum[2];
 #pragma unroll
       for (int o = kLanes / 2; o > 0; o /= 2) {
         low += __shfl_xor_sync(0xFFFFFFFFu, low, o);
         high += __shfl_xor_sync(0xFFFFFFFFu, high, o);
       }
-      // Of a lane's eight codes the even ones (low nibbles) lie before the odd ones, as the masks leave them.
-      const int chunk = block * 4 + lane / 8;
+      uint8_t* to = digits + size_t(half * 8 + lane / 4) * digit_row + lane % 4 * 8;
 #pragma unroll
-      for (int c = 0; c < 3; ++c) {
-        uint8_t* to = digits + (size_t(chunk) * NT + Col::tile(token, c)) * 256 + Col::column(token, c) * 32 + lane % 8 / 2 * 8 +
-                      lane % 2 * 2;
-        *reinterpret_cast<uint16_t*>(to) = uint16_t((d[c][0] & 255) | (d[c][2] & 255) << 8);
-        *reinterpret_cast<uint16_t*>(to + 4) = uint16_t((d[c][1] & 255) | (d[c][3] & 255) << 8);
-      }
+      for (int c = 0; c < 3; ++c)
+        *reinterpret_cast<uint2*>(to + (NT == 1 ? (a.pair ? 2 * c + token : c) * 32 : (token / 8 * 3 + c) * 256 + token % 8 * 32)) = d[c];
+      const int s0 = int(int16_t(low)), s1 = (low - s0) >> 16;
       if (lane % kLanes == 0) {
-        uint8_t* to = factors + size_t(block * (NG / 2) + lane / kLanes) * kFactorBytes<NT>;
-        const int s0 = int(int16_t(low)), s1 = (low - s0) >> 16;
+        uint8_t* to_sum = smem + at.sums + size_t(half * (NG / 2) + lane / kLanes) * kSumBytes<NT>;
         if constexpr (NT == 1) {
-          ColumnFactor* f = reinterpret_cast<ColumnFactor*>(to) + token;
-          f[0] = {down, s0};
-          f[2] = {down * 256.0f, s1};
-          f[4] = {down * 65536.0f, high};
+          int* f = reinterpret_cast<int*>(to_sum) + token;
+          f[0] = s0;
+          f[2] = s1;
+          f[4] = high;
         } else {
-          reinterpret_cast<TokenFactor*>(to)[token] = {down, s0 + 256 * s1, high, 0};
+          reinterpret_cast<int2*>(to_sum)[token] = make_int2(s0 + 256 * s1, high);
+        }
+      }
+      if (lane % 16 == 0) {
+        const float down = bad ? NAN : __int_as_float((127 - e) << 23);
+        float* f = reinterpret_cast<float*>(smem + at.powers + size_t(half * 2 + lane / 16) * kPowerBytes<NT>) + token;
+        f[0] = down;
+        if (NT == 1) {
+          f[2] = down * 256.0f;
+          f[4] = down * 65536.0f;
         }
       }
     }
   };
 
-  // A unit's scales and zero points, loaded one unit ahead: lane t of a row's four holds group t (and
-  // t + 4 of eight). Rows behind the matrix and groups behind K read the last ones: the first are not
+  // A unit's scales and zero points, loaded one unit ahead: lane t of a row's four holds groups t, t + 4, ... Rows behind the matrix and groups behind K read the last ones: the first are not
   // stored, the second multiply zeros.
   struct Scales {
     float s[2][kHeld];
     int z[2][kHeld];
   };
-  const int last_group = (a.k + a.group - 1) / a.group - 1, group_span = NG == 2 ? a.group / 128 : 1;
+  const int last_group = (a.k + a.group - 1) / a.group - 1, group_span = NG == 4 ? a.group / 128 : 1;
   struct Rows {
     const void* s[2];
     const uint8_t* z[2];
@@ -445,8 +460,8 @@ __global__ void __launch_bounds__(kThreads, 1) gemv_int4_kernel(const __grid_con
   auto load_scales = [&](Rows const& rows, int kb, Scales& v) {
 #pragma unroll
     for (int h = 0; h < kHeld; ++h) {
-      int gi = kb * NG + (t + 4 * h) % NG;
-      if (NG == 2 && group_span != 1) gi /= group_span;
+      int gi = kb * NG + t + 4 * h;
+      if (NG == 4 && group_span != 1) gi /= group_span;
       gi = min(gi, last_group);
 #pragma unroll
       for (int r = 0; r < 2; ++r) {
@@ -462,7 +477,7 @@ __global__ void __launch_bounds__(kThreads, 1) gemv_int4_kernel(const __grid_con
     else static_cast<T*>(a.out)[o] = from_f32<T>(v);
   };
 
-  constexpr int kSets = NT == 1 ? 1 : NT / 3;  // groups of 8 tokens
+  constexpr int kSets = NT == 1 ? 1 : NT / 3;  // tiles of 8 tokens
   Stretch cur = {};
   cur.batch = m0;
   begin_batch(cur);
@@ -474,10 +489,12 @@ __global__ void __launch_bounds__(kThreads, 1) gemv_int4_kernel(const __grid_con
     rows = rows_of(pass_of(peek.pass).expert, peek.row0 + peek.tile * kRows);
     load_scales(rows, kb0 + peek.kb, now);
   }
-  // Where a lane reads: its ldmatrix rows in a slot (swizzled by 16 bytes), its digits and factors in a unit.
-  uint32_t in_slot[4];
+  // Where a lane reads: its ldmatrix rows in a box (swizzled by 16 bytes), its column's digits (a column that
+  // nothing uses reads another's).
+  uint32_t in_box[4];
 #pragma unroll
-  for (int pair = 0; pair < 4; ++pair) in_slot[pair] = lane % 16 * 128 + (((pair * 2 + lane / 16) ^ (lane & 7)) * 16);
+  for (int i = 0; i < 4; ++i) in_box[i] = lane % 16 * 128 + (((i * 2 + lane / 16) ^ (lane & 7)) * 16);
+  const int digit_lane = t * 8 + (NT != 1 ? g * 32 : g >= 6 ? 0 : a.pair ? g * 32 : g % 2 ? 0 : g / 2 * 32);
   int slot = 0, pass = -1, flip = 0;
   uint32_t parity = 0;
   bool failed = false;
@@ -494,8 +511,9 @@ __global__ void __launch_bounds__(kThreads, 1) gemv_int4_kernel(const __grid_con
       // The next stretch, whose first scales are loaded in this one's last unit.
       if (peek.batch < m1) next_stretch(peek);
       float acc[kSets][4] = {};
-      const uint2* b = reinterpret_cast<const uint2*>(digits + size_t(cur.kb) * 8 * NT * 256) + lane;
-      const uint4* fp = reinterpret_cast<const uint4*>(factors + size_t(cur.kb) * NG * kFactorBytes<NT>) + (NT == 1 ? t : 2 * t);
+      const uint8_t* xd = digits + size_t(cur.kb) * 16 * digit_row + digit_lane;
+      const uint8_t* xs = smem + at.sums + size_t(cur.kb) * NG * kSumBytes<NT> + t * (NT == 1 ? 8 : 16);
+      const uint8_t* xp = smem + at.powers + size_t(cur.kb) * 4 * kPowerBytes<NT> + t * 8;
       for (int u = 0; u < cur.units; ++u) {
         if (u + 1 < cur.units) {
           load_scales(rows, kb0 + cur.kb + u + 1, next);
@@ -508,25 +526,30 @@ __global__ void __launch_bounds__(kThreads, 1) gemv_int4_kernel(const __grid_con
           failed = true;
           break;
         }
-        int part[NT][4];
+        const bool short_unit = (kb0 + cur.kb + u) * kUnitK + kUnitK / 2 >= a.k;
 #pragma unroll
-        for (int pair = 0; pair < 4; ++pair) {
-          // Matrices: rows 0-7 and 8-15 of chunk 2 pair, then of chunk 2 pair + 1.
-          uint32_t w[4];
-          ldmatrix_x4(w, base + in_slot[pair]);
+        for (int quarter = 0; quarter < 4; ++quarter) {  // 128 codes
+          if (quarter == 2 && short_unit) break;
+          int part[NT][4];
+          float sum[kSets][4] = {};
 #pragma unroll
-          for (int cc = 0; cc < 2; ++cc) {
-            const int c8 = pair * 2 + cc;
-            const uint32_t f[4] = {w[2 * cc] & kNibbles, w[2 * cc + 1] & kNibbles, (w[2 * cc] >> 4) & kNibbles,
-                                   (w[2 * cc + 1] >> 4) & kNibbles};
+          for (int pair = 0; pair < 2; ++pair) {
+            // Matrices: rows 0-7 and 8-15 of chunk 2 pair, then of chunk 2 pair + 1.
+            uint32_t w[4];
+            ldmatrix_x4(w, base + quarter / 2 * kBoxBytes + in_box[quarter % 2 * 2 + pair]);
 #pragma unroll
-            for (int j = 0; j < NT; ++j) {
-              if (c8 % kPerGroup == 0) part[j][0] = part[j][1] = part[j][2] = part[j][3] = 0;
-              if (j >= 3 && p.count <= 8) continue;
-              mma_u8s8(part[j], f, b[(c8 * NT + j) * 32]);
-            }
-            if (c8 % kPerGroup == kPerGroup - 1) {
-              const int gj = c8 / kPerGroup, from = (lane & 28) | (gj & 3);
+            for (int cc = 0; cc < 2; ++cc) {
+              const int c = quarter * 4 + pair * 2 + cc;
+              const uint32_t f[4] = {w[2 * cc] & kNibbles, w[2 * cc + 1] & kNibbles, (w[2 * cc] >> 4) & kNibbles,
+                                     (w[2 * cc + 1] >> 4) & kNibbles};
+              const uint8_t* xc = xd + c * digit_row;
+#pragma unroll
+              for (int j = 0; j < NT; ++j) {
+                if (j >= 3 && p.count <= 8) continue;
+                mma_u8s8(part[j], f, *reinterpret_cast<const uint2*>(xc + j * 256), c % kPerGroup == 0);
+              }
+              if (c % kPerGroup != kPerGroup - 1) continue;
+              const int gj = c / kPerGroup, from = (lane & 28) | (gj & 3);
               float sc[2];
               int z[2] = {8, 8};
 #pragma unroll
@@ -535,30 +558,35 @@ __global__ void __launch_bounds__(kThreads, 1) gemv_int4_kernel(const __grid_con
                 if (a.zeros != nullptr) z[r] = __shfl_sync(0xFFFFFFFFu, now.z[r][gj / 4], from);
               }
               if constexpr (NT == 1) {
-                const uint4 q = fp[gj * (kFactorBytes<NT> / 16)];
+                const int2 q = *reinterpret_cast<const int2*>(xs + gj * kSumBytes<NT>);
 #pragma unroll
-                for (int i = 0; i < 4; ++i)
-                  acc[0][i] = fmaf(sc[i / 2] * __uint_as_float(i % 2 ? q.z : q.x),
-                                   float(part[0][i] - z[i / 2] * int(i % 2 ? q.w : q.y)), acc[0][i]);
+                for (int i = 0; i < 4; ++i) sum[0][i] = fmaf(sc[i / 2], float(part[0][i] - z[i / 2] * (i % 2 ? q.y : q.x)), sum[0][i]);
               } else {
 #pragma unroll
                 for (int set = 0; set < kSets; ++set) {
                   if (set > 0 && p.count <= 8) continue;
+                  const int4 q = *reinterpret_cast<const int4*>(xs + gj * kSumBytes<NT> + set * 64);
 #pragma unroll
                   for (int i = 0; i < 4; ++i) {
-                    const uint4 q = fp[gj * (kFactorBytes<NT> / 16) + set * 8 + i % 2];
                     // |256 P_1 + P_0| and z times its sums stay below 2^30.
-                    const int low = part[3 * set + 1][i] * 256 + part[3 * set][i] - z[i / 2] * int(q.y);
-                    const int high = part[3 * set + 2][i] - z[i / 2] * int(q.z);
-                    acc[set][i] = fmaf(sc[i / 2] * __uint_as_float(q.x), fmaf(float(high), 65536.0f, float(low)), acc[set][i]);
+                    const int low = part[3 * set + 1][i] * 256 + part[3 * set][i] - z[i / 2] * (i % 2 ? q.z : q.x);
+                    const int high = part[3 * set + 2][i] - z[i / 2] * (i % 2 ? q.w : q.y);
+                    sum[set][i] = fmaf(sc[i / 2], fmaf(float(high), 65536.0f, float(low)), sum[set][i]);
                   }
                 }
               }
             }
           }
+#pragma unroll
+          for (int set = 0; set < kSets; ++set) {
+            const float2 q = *reinterpret_cast<const float2*>(xp + quarter * kPowerBytes<NT> + set * 32);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) acc[set][i] = fmaf(i % 2 ? q.y : q.x, sum[set][i], acc[set][i]);
+          }
         }
-        b += 8 * NT * 32;
-        fp += NG * (kFactorBytes<NT> / 16);
+        xd += 16 * digit_row;
+        xs += NG * kSumBytes<NT>;
+        xp += 4 * kPowerBytes<NT>;
         __syncwarp();
         if (lane == 0) load(base, bar);
         if (++slot == depth) {
@@ -611,7 +639,7 @@ __global__ void __launch_bounds__(kThreads, 1) gemv_int4_kernel(const __grid_con
       __syncthreads();
     } else {
       // Two buffers: a block writes one again only after a barrier that follows its readers' reads.
-      float* mine = sums + flip * kWarps * kPiece<NT>;
+      float* mine = block + flip * kWarps * kPiece<NT>;
       flip ^= 1;
       for (int i = threadIdx.x; i < cells; i += kThreads) mine[i] = block_sum(i);
       cluster.sync();
@@ -657,9 +685,9 @@ Fit fit(Int4Args const& a) {
   Fit f = {1, 0, 0};
   const int kb = (a.k + kUnitK - 1) / kUnitK;
   auto units = [&] { return (kb + f.cluster - 1) / f.cluster; };
-  while (f.cluster < 8 && size_t(units()) * (NT * 2048 + NG * kFactorBytes<NT>) > 80 * 1024) f.cluster *= 2;
+  while (f.cluster < 8 && size_t(units()) * x_bytes<NG, NT>(a.pair) > 80 * 1024) f.cluster *= 2;
   for (int depth = 2; depth <= 8; ++depth) {
-    const Layout<NG, NT> l(depth, units(), f.cluster, a.ids != nullptr, a.experts, a.slots);
+    const Layout<NG, NT> l(depth, units(), a.pair, f.cluster, a.ids != nullptr, a.experts, a.slots);
     if (l.bytes + 1024 > size_t(kSmemLimit)) break;
     f.depth = depth;
     f.bytes = l.bytes + 1024;
@@ -697,7 +725,7 @@ kl_status launch(Int4Args& a, Fit const& f, int device, cudaStream_t stream) {
     resident[device][which].store(most, std::memory_order_release);
     cfg.dynamicSmemBytes = f.bytes;
   }
-  const long long passes = a.ids != nullptr ? a.slots : (a.slots + Columns<NT>::kTokens - 1) / Columns<NT>::kTokens;
+  const long long passes = a.ids != nullptr ? a.slots : (a.slots + kTokens<NT> - 1) / kTokens<NT>;
   const long long work = passes * a.tiles;
   if (work > INT32_MAX / 2) return fail(KL_ERR_NOT_SUPPORTED, "kl_gemv_int4: too many rows of out");
   a.depth = f.depth;
@@ -712,9 +740,9 @@ template <class T, int NG>
 kl_status by_tokens(Int4Args& a, int device, cudaStream_t stream) {
   const int tokens = a.ids != nullptr ? (a.slots + a.experts - 1) / a.experts : a.slots;
   if (tokens > 8)
-    if (const Fit f = fit<NG, 6>(a); f.depth >= 3) return launch<T, NG, 6>(a, f, device, stream);
+    if (const Fit f = fit<NG, 6>(a); f.depth >= 2) return launch<T, NG, 6>(a, f, device, stream);
   if (tokens > 2)
-    if (const Fit f = fit<NG, 3>(a); f.depth >= 3) return launch<T, NG, 3>(a, f, device, stream);
+    if (const Fit f = fit<NG, 3>(a); f.depth >= 2) return launch<T, NG, 3>(a, f, device, stream);
   const Fit f = fit<NG, 1>(a);
   if (f.depth == 0) return fail(KL_ERR_NOT_SUPPORTED, "kl_gemv_int4: k does not fit");
   return launch<T, NG, 1>(a, f, device, stream);
@@ -722,9 +750,9 @@ kl_status by_tokens(Int4Args& a, int device, cudaStream_t stream) {
 
 template <class T>
 kl_status by_group(Int4Args& a, int device, cudaStream_t stream) {
-  if (a.group == 32) return by_tokens<T, 8>(a, device, stream);
-  if (a.group == 64) return by_tokens<T, 4>(a, device, stream);
-  return by_tokens<T, 2>(a, device, stream);
+  if (a.group == 32) return by_tokens<T, 16>(a, device, stream);
+  if (a.group == 64) return by_tokens<T, 8>(a, device, stream);
+  return by_tokens<T, 4>(a, device, stream);
 }
 
 kl_status run(kl_int4_desc const& d, int64_t slots, cudaStream_t stream) {
@@ -763,6 +791,7 @@ kl_status run(kl_int4_desc const& d, int64_t slots, cudaStream_t stream) {
   a.f32_scales = d.scale_type == KL_F32;
   a.f32_out = d.out_type == KL_F32;
   a.tiles = (a.n + kRows - 1) / kRows;
+  a.pair = a.slots > 1;
   a.timeout_ns = wait_timeout_ns();
   kl_status s = device_status_ptr(&a.status);
   if (s != KL_OK) return s;
