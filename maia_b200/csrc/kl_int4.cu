@@ -223,8 +223,8 @@ __global__ void __launch_bounds__(kThreads, 1) gemv_int4_kernel(const __grid_con
   constexpr int kPerGroup = 16 / NG;  // 32-code chunks of a group
   constexpr int kHeld = NG / 4;       // scales that a lane holds of each of its rows
   constexpr uint32_t kNibbles = 0x0F0F0F0Fu;
-  extern __shared__ uint8_t raw[];
-  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) / 1024 * 1024);
+  extern __shared__ uint8_t dynamic[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(dynamic) + 1023) / 1024 * 1024);
   cg::cluster_group cluster = cg::this_cluster();
   const int split = int(cluster.block_rank()), splits = int(cluster.num_blocks());
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, g = lane / 4, t = lane % 4;
@@ -249,11 +249,11 @@ __global__ void __launch_bounds__(kThreads, 1) gemv_int4_kernel(const __grid_con
     if (warp == 0) tma_prefetch_map(&a.map);
   }
   __syncwarp();
-  griddep_wait();
-  griddep_launch_dependents();
-
+  // Nothing of global memory is touched before the kernels before this one are done; what needs none of it
+  // (the whole schedule, for one matrix) is worked out in their shadow.
   int passes = (a.slots + kTok - 1) / kTok, active = 0;
   if (a.ids != nullptr) {
+    griddep_wait();
     build_lists<kTok>(a, l, reinterpret_cast<int*>(digits), &active);
     passes = l.base[active];
   }
@@ -287,7 +287,8 @@ __global__ void __launch_bounds__(kThreads, 1) gemv_int4_kernel(const __grid_con
   // (tile, 512 codes of this block's K) are dealt to the warps in even, consecutive runs, so a run touches at
   // most two tiles. A warp's share of one tile is a stretch.
   const int clusters = int(gridDim.x) / splits, c = int(blockIdx.x) / splits;
-  const int m0 = int((long long)passes * a.tiles * c / clusters), m1 = int((long long)passes * a.tiles * (c + 1) / clusters);
+  const int share = passes * a.tiles / clusters, extra = passes * a.tiles % clusters;
+  const int m0 = c * share + min(c, extra), m1 = m0 + share + (c < extra);
   struct Stretch {
     int batch, count;  // the batch's first tile and its tiles; batch = m1: no more
     int pass, row0;    // of its first tile
@@ -351,21 +352,32 @@ __global__ void __launch_bounds__(kThreads, 1) gemv_int4_kernel(const __grid_con
       aim();
     }
   };
-  if (lane == 0) {
-    aim();
-    for (int i = 0; i < depth; ++i) load(ring0 + i * kUnitBytes, bar0 + 8 * i);
-  }
-
-  // x of a pass as digits: a warp takes 256 K-elements of a token at a time, a lane 8 of them.
+  // x of a pass as digits: a warp takes 256 K-elements of a token at a time, a lane 8 of them; kEarly pieces
+  // are loaded before the first is worked on.
+  constexpr int kEarly = 2;
   const int digit_row = digit_bytes<NT>(a.pair);
-  auto convert = [&](Pass const& p) {
-    constexpr int kLanes = 64 / NG;  // lanes of a scale group
-    for (int i = warp; i < p.count * kbs * 2; i += kWarps) {
+  auto fetch = [&](Pass const& p, int i0, uint4 (&u)[kEarly]) {
+#pragma unroll
+    for (int n = 0; n < kEarly; ++n) {
+      const int i = i0 + n * kWarps;
+      u[n] = make_uint4(0, 0, 0, 0);
+      if (i >= p.count * kbs * 2) continue;
       const int token = i / (kbs * 2), half = i - token * (kbs * 2);
       const int k = kb0 * kUnitK + half * 256 + lane * 8;
-      uint4 u = make_uint4(0, 0, 0, 0);
       if (k < a.k)
-        u = *reinterpret_cast<const uint4*>(static_cast<const T*>(a.x) + (long long)(slot_of(p.first + token) / a.x_div) * a.ldx + k);
+        u[n] = *reinterpret_cast<const uint4*>(static_cast<const T*>(a.x) + (long long)(slot_of(p.first + token) / a.x_div) * a.ldx + k);
+    }
+  };
+  auto convert = [&](Pass const& p, uint4 (&early)[kEarly]) {
+    constexpr int kLanes = 64 / NG;  // lanes of a scale group
+    for (int i0 = warp; i0 < p.count * kbs * 2; i0 += kEarly * kWarps) {
+      if (i0 != warp) fetch(p, i0, early);
+#pragma unroll
+      for (int n = 0; n < kEarly; ++n) {
+      const int i = i0 + n * kWarps;
+      if (i >= p.count * kbs * 2) break;
+      const int token = i / (kbs * 2), half = i - token * (kbs * 2);
+      const uint4 u = early[n];
       // The largest |x|: both types order like their bits, with NaN above infinity.
       uint32_t m = __vmaxu2(__vmaxu2(u.x & 0x7FFF7FFFu, u.y & 0x7FFF7FFFu), __vmaxu2(u.z & 0x7FFF7FFFu, u.w & 0x7FFF7FFFu));
 #pragma unroll
@@ -432,14 +444,15 @@ __global__ void __launch_bounds__(kThreads, 1) gemv_int4_kernel(const __grid_con
           f[4] = down * 65536.0f;
         }
       }
+      }
     }
   };
 
   // A unit's scales and zero points, loaded one unit ahead: lane t of a row's four holds groups t, t + 4, ... Rows behind the matrix and groups behind K read the last ones: the first are not
   // stored, the second multiply zeros.
   struct Scales {
-    float s[2][kHeld];
-    int z[2][kHeld];
+    uint32_t s[2][kHeld];  // as loaded: nothing waits for them before the unit that uses them
+    uint32_t z[2][kHeld];
   };
   const int last_group = (a.k + a.group - 1) / a.group - 1, group_span = NG == 4 ? a.group / 128 : 1;
   struct Rows {
@@ -465,10 +478,35 @@ __global__ void __launch_bounds__(kThreads, 1) gemv_int4_kernel(const __grid_con
       gi = min(gi, last_group);
 #pragma unroll
       for (int r = 0; r < 2; ++r) {
-        v.s[r][h] = a.f32_scales ? static_cast<const float*>(rows.s[r])[gi] : to_f32(static_cast<const T*>(rows.s[r])[gi]);
-        v.z[r][h] = a.zeros != nullptr ? rows.z[r][gi] : 8;
+        v.s[r][h] = a.f32_scales ? static_cast<const uint32_t*>(rows.s[r])[gi] : static_cast<const uint16_t*>(rows.s[r])[gi];
+        if (a.zeros != nullptr) v.z[r][h] = rows.z[r][gi];
       }
     }
+  };
+
+  auto scale_of = [&](uint32_t bits) {
+    if (a.f32_scales) return __uint_as_float(bits);
+    const uint16_t b16 = uint16_t(bits);
+    T v;
+    memcpy(&v, &b16, 2);
+    return to_f32(v);
+  };
+  // The lines of a batch's scales and zero points into L2: behind the weights' queue to memory a plain load of
+  // them takes microseconds.
+  auto prefetch_batch = [&](Stretch const& s) {
+    if (s.batch >= m1) return;
+    const int expert = pass_of(s.pass).expert;
+    const int first = kb0 * NG / group_span, last = min((kb0 + kbs) * NG / group_span, last_group + 1);
+    auto lines = [&](const char* base, long long pitch, int size) {
+      const int bytes = (last - first) * size, per_row = bytes / 128 + 1;
+      for (int i = threadIdx.x; i < s.count * kRows * per_row; i += kThreads) {
+        const int row = s.row0 + i / per_row, at_byte = min(i % per_row * 128, bytes - 1);
+        if (row < a.n) asm volatile("prefetch.global.L2 [%0];" ::"l"(base + row * pitch + (long long)first * size + at_byte));
+      }
+    };
+    if (last <= first) return;
+    lines(static_cast<const char*>(a.scales) + expert * a.stride_s * scale_bytes, a.lds * scale_bytes, scale_bytes);
+    if (a.zeros != nullptr) lines(reinterpret_cast<const char*>(a.zeros) + expert * a.stride_z, a.ldz, 1);
   };
 
   auto store = [&](int slot, int n, float v) {
@@ -483,12 +521,26 @@ __global__ void __launch_bounds__(kThreads, 1) gemv_int4_kernel(const __grid_con
   begin_batch(cur);
   Stretch peek = cur;
   if (peek.batch < m1 && peek.units == 0) next_stretch(peek);
-  Scales now = {}, next = {};
+  if (a.ids == nullptr) griddep_wait();
+  griddep_launch_dependents();
+  // The first loads, those that the start waits for before the weights fill the queue to memory.
+  Pass p = {};
+  uint4 early[kEarly] = {};
+  Scales raw = {};
   Rows rows = {};
+  if (cur.batch < m1) {
+    p = pass_of(cur.pass);
+    fetch(p, warp, early);
+  }
   if (peek.batch < m1) {
     rows = rows_of(pass_of(peek.pass).expert, peek.row0 + peek.tile * kRows);
-    load_scales(rows, kb0 + peek.kb, now);
+    load_scales(rows, kb0 + peek.kb, raw);
   }
+  if (lane == 0) {
+    aim();
+    for (int i = 0; i < depth; ++i) load(ring0 + i * kUnitBytes, bar0 + 8 * i);
+  }
+  prefetch_batch(cur);
   // Where a lane reads: its ldmatrix rows in a box (swizzled by 16 bytes), its column's digits (a column that
   // nothing uses reads another's).
   uint32_t in_box[4];
@@ -498,14 +550,19 @@ __global__ void __launch_bounds__(kThreads, 1) gemv_int4_kernel(const __grid_con
   int slot = 0, pass = -1, flip = 0;
   uint32_t parity = 0;
   bool failed = false;
-  Pass p = {};
   while (cur.batch < m1) {
     if (cur.pass != pass) {
+      if (pass >= 0) {
+        p = pass_of(cur.pass);
+        fetch(p, warp, early);
+      }
       pass = cur.pass;
-      p = pass_of(pass);
-      convert(p);
+      convert(p, early);
       __syncthreads();
     }
+    Stretch then = cur;
+    next_batch(then);
+    prefetch_batch(then);
     int piece = 0;
     while (cur.units > 0 && !failed) {
       // The next stretch, whose first scales are loaded in this one's last unit.
@@ -515,11 +572,20 @@ __global__ void __launch_bounds__(kThreads, 1) gemv_int4_kernel(const __grid_con
       const uint8_t* xs = smem + at.sums + size_t(cur.kb) * NG * kSumBytes<NT> + t * (NT == 1 ? 8 : 16);
       const uint8_t* xp = smem + at.powers + size_t(cur.kb) * 4 * kPowerBytes<NT> + t * 8;
       for (int u = 0; u < cur.units; ++u) {
+        float s_now[2][kHeld];
+        uint32_t z_now[2][kHeld];
+#pragma unroll
+        for (int r = 0; r < 2; ++r)
+#pragma unroll
+          for (int h = 0; h < kHeld; ++h) {
+            s_now[r][h] = scale_of(raw.s[r][h]);
+            z_now[r][h] = raw.z[r][h];
+          }
         if (u + 1 < cur.units) {
-          load_scales(rows, kb0 + cur.kb + u + 1, next);
+          load_scales(rows, kb0 + cur.kb + u + 1, raw);
         } else if (peek.batch < m1) {
           rows = rows_of(pass_of(peek.pass).expert, peek.row0 + peek.tile * kRows);
-          load_scales(rows, kb0 + peek.kb, next);
+          load_scales(rows, kb0 + peek.kb, raw);
         }
         const uint32_t bar = bar0 + 8 * slot, base = ring0 + slot * kUnitBytes;
         if (!mbarrier_wait(bar, parity, a.timeout_ns)) {
@@ -554,8 +620,8 @@ __global__ void __launch_bounds__(kThreads, 1) gemv_int4_kernel(const __grid_con
               int z[2] = {8, 8};
 #pragma unroll
               for (int r = 0; r < 2; ++r) {
-                sc[r] = __shfl_sync(0xFFFFFFFFu, now.s[r][gj / 4], from);
-                if (a.zeros != nullptr) z[r] = __shfl_sync(0xFFFFFFFFu, now.z[r][gj / 4], from);
+                sc[r] = __shfl_sync(0xFFFFFFFFu, s_now[r][gj / 4], from);
+                if (a.zeros != nullptr) z[r] = int(__shfl_sync(0xFFFFFFFFu, z_now[r][gj / 4], from));
               }
               if constexpr (NT == 1) {
                 const int2 q = *reinterpret_cast<const int2*>(xs + gj * kSumBytes<NT>);
@@ -593,7 +659,6 @@ __global__ void __launch_bounds__(kThreads, 1) gemv_int4_kernel(const __grid_con
           slot = 0;
           parity ^= 1;
         }
-        now = next;
       }
       if (failed) break;
       // This warp's part of the tile's sums, [token][row].
