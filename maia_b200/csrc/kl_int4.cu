@@ -26,6 +26,7 @@
 #include <exception>
 #include <string>
 
+#include <kl/arch/cluster.hpp>
 #include <kl/arch/griddep.hpp>
 #include <kl/arch/mbarrier.hpp>
 #include <kl/arch/tma.hpp>
@@ -66,8 +67,9 @@ struct Int4Args {
   int n, k, group;
   int f32_scales, f32_out;
   int tiles;  // 16-row tiles of one matrix
-  int pair;   // NT = 1: a pass may have two tokens
   int depth;  // slots of a warp's ring
+  uint32_t digits, sums, powers, pieces, block, units, bars, lists;  // offsets in shared memory
+  int group_span, last_group;                           // 128-element runs of a group (groups of 128 and more); index of the last
   int* status;
   unsigned long long timeout_ns;
 };
@@ -104,7 +106,7 @@ struct Lists {
 
 // Counts the slots of every expert, packs the active ones and files the slots in their order: every block builds the
 // lists for itself, and all have to cut an expert's slots into the same passes.
-template <int kTok>
+template <int TOK>
 __device__ void build_lists(const Int4Args& a, Lists const& l, int* hist, int* active_out) {
   __shared__ unsigned long long warp_sum[kWarps];
   const int tid = threadIdx.x, lane = tid % 32, warp = tid / 32;
@@ -124,7 +126,7 @@ __device__ void build_lists(const Int4Args& a, Lists const& l, int* hist, int* a
     count[i] = e < a.experts ? hist[e] : 0;
     own[i] = count[i] == 0 ? 0
                            : 1ull | (unsigned long long)count[i] << 16 |
-                                 (unsigned long long)((count[i] + kTok - 1) / kTok) << 32;
+                                 (unsigned long long)((count[i] + TOK - 1) / TOK) << 32;
     mine += own[i];
   }
   unsigned long long sum = mine;
@@ -173,88 +175,92 @@ __device__ void build_lists(const Int4Args& a, Lists const& l, int* hist, int* a
   *active_out = active;
 }
 
-// Columns of the products. Three digits of 8 tokens are three 8-column tiles, digit c of token i in
-// column i of tile c, so a lane holds the digits of the same tokens (NT = 3, 6); up to two tokens fit one tile, digit
-// c of token i in column 2 c + i, and the digits meet by shuffles (NT = 1).
-template <int NT>
-constexpr int kTokens = NT == 1 ? 2 : NT / 3 * 8;
+// TOK: tokens of a pass, 1, 2, 8 or 16. Columns of the products: three digits of 8 tokens are three 8-column
+// tiles, digit c of token i in column i of tile c, so a lane holds the digits of the same tokens; up to two tokens
+// fit one tile, digit c of token i in column 2 c + i, and the digits meet by shuffles.
+template <int TOK>
+constexpr int kTiles = TOK <= 2 ? 1 : TOK / 8 * 3;
 
-// x in shared memory. Digits: for every 32 K-elements a row of 32 bytes for each column (NT = 1: only the 3 or 6
-// that a launch uses). Sums D of a group: NT = 1: an int a column; else (D_0 + 256 D_1, D_2) a token.
-// Powers 2^-e of 128 elements: NT = 1: times 256^c, a float a column; else a float a token.
-template <int NT>
-__host__ __device__ constexpr int digit_bytes(int pair) {  // of 32 K-elements
-  return NT == 1 ? (pair ? 192 : 96) : NT * 256;
-}
-template <int NT>
-constexpr int kSumBytes = NT == 1 ? 32 : NT / 3 * 64;
-template <int NT>
-constexpr int kPowerBytes = NT == 1 ? 32 : NT / 3 * 32;
-template <int NG, int NT>
-__host__ __device__ constexpr int x_bytes(int pair) {  // of a unit
-  return 16 * digit_bytes<NT>(pair) + NG * kSumBytes<NT> + 4 * kPowerBytes<NT>;
-}
+// x in shared memory. Digits: for every 32 K-elements a row of 32 bytes for each column that is used. Sums D of a
+// scale group: up to two tokens: an int a column; else (D_0 + 256 D_1, D_2) a token. Powers 2^-e of 128
+// elements: up to two tokens: times 256^c, a float a column; else a float a token.
+template <int TOK>
+constexpr int kDigitRow = TOK <= 2 ? TOK * 96 : kTiles<TOK> * 256;  // bytes of 32 K-elements
+template <int TOK>
+constexpr int kSumBytes = TOK <= 2 ? 32 : TOK * 8;  // of a group
+template <int TOK>
+constexpr int kPowerBytes = TOK <= 2 ? 32 : TOK * 4;  // of 128 K-elements
+template <int NG, int TOK>
+constexpr int kXBytes = 16 * kDigitRow<TOK> + NG * kSumBytes<TOK> + 4 * kPowerBytes<TOK>;  // of a unit
 
 constexpr int kPieces = 2;  // tiles that a warp's run of units can touch
-template <int NT>
-constexpr int kPiece = kTokens<NT> * kRows;  // floats of a tile's sums
+template <int TOK>
+constexpr int kPiece = TOK * kRows;  // floats of a tile's sums
 
-// Shared memory, in order: rings, x's digits, sums and powers, pieces, the block's sums, barriers, lists.
-template <int NG, int NT>
-struct Layout {
-  size_t digits, sums, powers, pieces, block, bars, lists, bytes;
-  __host__ __device__ Layout(int depth, int units, int pair, int cluster, bool ids, int experts, int slots) {
-    digits = size_t(kWarps) * depth * kUnitBytes;
-    sums = digits + size_t(units) * 16 * digit_bytes<NT>(pair);
-    powers = sums + size_t(units) * NG * kSumBytes<NT>;
-    pieces = powers + size_t(units) * 4 * kPowerBytes<NT>;
-    block = pieces + size_t(kWarps) * kPieces * kPiece<NT> * 4;
-    bars = block + (cluster > 1 ? size_t(2) * kWarps * kPiece<NT> * 4 : 0);
-    lists = bars + size_t(kWarps) * depth * 8;
-    bytes = lists + (ids ? Lists::bytes(experts, slots) : 0);
-  }
+// What a ring slot holds, and what its warp does around it.
+struct __align__(16) Unit {
+  int row0, kb, expert, flags;
+  int batch_row0, count, pass, unused;
 };
+constexpr int kFirst = 1;   // first unit of a stretch (the warp's share of a tile)
+constexpr int kLast = 2;    // last of it
+constexpr int kEnd = 4;     // last of the warp's run in the batch
+constexpr int kSecond = 8;  // the stretch is the run's second
+constexpr int kNone = 16;   // no unit: the warp has none in this batch
 
-// NG: scale groups of a unit's 512 codes (16, 8, 4 for groups of 32, 64, multiples of 128). NT: tiles of 8
-// columns.
-template <class T, int NG, int NT>
+// Shared memory, in order: rings, x's digits, sums and powers, pieces, the block's sums, unit records, barriers,
+// lists.
+template <int NG, int TOK>
+size_t lay_out(Int4Args& a, int depth, int units, int cluster) {
+  a.depth = depth;
+  size_t at = size_t(kWarps) * depth * kUnitBytes;
+  auto take = [&](uint32_t& offset, size_t bytes) {
+    offset = uint32_t(at);
+    at += bytes;
+  };
+  take(a.digits, size_t(units) * 16 * kDigitRow<TOK>);
+  take(a.sums, size_t(units) * NG * kSumBytes<TOK>);
+  take(a.powers, size_t(units) * 4 * kPowerBytes<TOK>);
+  take(a.pieces, size_t(kWarps) * kPieces * kPiece<TOK> * 4);
+  take(a.block, cluster > 1 ? size_t(2) * kWarps * kPiece<TOK> * 4 : 0);
+  take(a.units, size_t(kWarps) * depth * sizeof(Unit));
+  take(a.bars, size_t(kWarps) * depth * 8);
+  take(a.lists, a.ids != nullptr ? Lists::bytes(a.experts, a.slots) : 0);
+  return at + 1024;  // the base is rounded up to 1024
+}
+
+// NG: scale groups of a unit's 512 codes (16, 8, 4 for groups of 32, 64, multiples of 128).
+template <class T, int NG, int TOK>
 __global__ void __launch_bounds__(kThreads, 1) gemv_int4_kernel(const __grid_constant__ Int4Args a) {
-  constexpr int kTok = kTokens<NT>;
   constexpr int kPerGroup = 16 / NG;  // 32-code chunks of a group
   constexpr int kHeld = NG / 4;       // scales that a lane holds of each of its rows
   constexpr uint32_t kNibbles = 0x0F0F0F0Fu;
   extern __shared__ uint8_t dynamic[];
-  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(dynamic) + 1023) / 1024 * 1024);
+  uint8_t* smem = dynamic + (1024 - smem_addr(dynamic) % 1024) % 1024;  // still known to be shared memory
   cg::cluster_group cluster = cg::this_cluster();
   const int split = int(cluster.block_rank()), splits = int(cluster.num_blocks());
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, g = lane / 4, t = lane % 4;
-  // This block's share of K, in units; every block lays its memory out for the largest share.
-  const int kb_all = (a.k + kUnitK - 1) / kUnitK;
-  const int kb0 = kb_all * split / splits, kbs = kb_all * (split + 1) / splits - kb0;
-  const Layout<NG, NT> at(a.depth, (kb_all + splits - 1) / splits, a.pair, splits, a.ids != nullptr, a.experts, a.slots);
   const int depth = a.depth;
-  uint8_t* digits = smem + at.digits;
-  float* pieces = reinterpret_cast<float*>(smem + at.pieces);
-  float* block = reinterpret_cast<float*>(smem + at.block);
-  Lists l;
-  l.base = reinterpret_cast<int*>(smem + at.lists);
-  l.act = reinterpret_cast<uint16_t*>(l.base + a.experts + 1);
-  l.start = l.act + a.experts;
-  l.list = l.start + a.experts + 1;
-  const uint32_t bar0 = smem_addr(smem + at.bars) + warp * depth * 8;
+  const uint32_t bar0 = smem_addr(smem + a.bars) + warp * depth * 8;
   const uint32_t ring0 = smem_addr(smem) + warp * depth * kUnitBytes;
+  Unit* units = reinterpret_cast<Unit*>(smem + a.units) + warp * depth;
+  float* pieces = reinterpret_cast<float*>(smem + a.pieces);
   if (lane == 0) {
     for (int i = 0; i < depth; ++i) mbarrier_init(bar0 + 8 * i, 1);
     fence_barrier_init();
     if (warp == 0) tma_prefetch_map(&a.map);
   }
-  __syncwarp();
-  // Nothing of global memory is touched before the kernels before this one are done; what needs none of it
-  // (the whole schedule, for one matrix) is worked out in their shadow.
-  int passes = (a.slots + kTok - 1) / kTok, active = 0;
+  Lists l;
+  l.base = reinterpret_cast<int*>(smem + a.lists);
+  l.act = reinterpret_cast<uint16_t*>(l.base + a.experts + 1);
+  l.start = l.act + a.experts;
+  l.list = l.start + a.experts + 1;
+  // Nothing of global memory is touched before the kernels before this one are done.
+  griddep_wait();
+  griddep_launch_dependents();
+  int passes = (a.slots + TOK - 1) / TOK, active = 0;
   if (a.ids != nullptr) {
-    griddep_wait();
-    build_lists<kTok>(a, l, reinterpret_cast<int*>(digits), &active);
+    build_lists<TOK>(a, l, reinterpret_cast<int*>(smem + a.digits), &active);
     passes = l.base[active];
   }
   // The tokens and the matrix of a pass.
@@ -265,7 +271,7 @@ __global__ void __launch_bounds__(kThreads, 1) gemv_int4_kernel(const __grid_con
     Pass p;
     if (a.ids == nullptr) {
       p.expert = 0;
-      p.first = pass * kTok;
+      p.first = pass * TOK;
       p.count = a.slots - p.first;
     } else {
       int lo = 0, hi = active;  // the last active expert whose base is not above `pass`
@@ -275,109 +281,125 @@ __global__ void __launch_bounds__(kThreads, 1) gemv_int4_kernel(const __grid_con
         else hi = mid;
       }
       p.expert = l.act[lo];
-      p.first = l.start[lo] + (pass - l.base[lo]) * kTok;
+      p.first = l.start[lo] + (pass - l.base[lo]) * TOK;
       p.count = l.start[lo + 1] - p.first;
     }
-    if (p.count > kTok) p.count = kTok;
+    if (p.count > TOK) p.count = TOK;
     return p;
   };
   auto slot_of = [&](int i) { return a.ids == nullptr ? i : int(l.list[i]); };
-
-  // The cluster's tiles [m0, m1) of all passes' tiles go in batches of up to 16 of one pass. A batch's units
-  // (tile, 512 codes of this block's K) are dealt to the warps in even, consecutive runs, so a run touches at
-  // most two tiles. A warp's share of one tile is a stretch.
-  const int clusters = int(gridDim.x) / splits, c = int(blockIdx.x) / splits;
-  const int share = passes * a.tiles / clusters, extra = passes * a.tiles % clusters;
-  const int m0 = c * share + min(c, extra), m1 = m0 + share + (c < extra);
-  struct Stretch {
-    int batch, count;  // the batch's first tile and its tiles; batch = m1: no more
-    int pass, row0;    // of its first tile
-    int tile, kb;      // the stretch: its tile, first unit and units
-    int units, left;   // left: of the run, behind the stretch
-  };
-  auto cut = [&](Stretch& s, int begin, int end) {
-    s.left = end - begin;
-    s.tile = s.kb = s.units = 0;
-    if (s.left > 0) {
-      s.tile = begin / kbs;
-      s.kb = begin - s.tile * kbs;
-      s.units = s.left < kbs - s.kb ? s.left : kbs - s.kb;
-      s.left -= s.units;
-    }
-  };
-  auto begin_batch = [&](Stretch& s) {
-    if (s.batch >= m1) return;
-    s.pass = s.batch / a.tiles;
-    const int first = s.batch - s.pass * a.tiles;
-    s.row0 = first * kRows;
-    s.count = min(kWarps, min(a.tiles - first, m1 - s.batch));
-    cut(s, s.count * kbs * warp / kWarps, s.count * kbs * (warp + 1) / kWarps);
-  };
-  auto next_batch = [&](Stretch& s) {
-    s.batch += s.count;
-    begin_batch(s);
-  };
-  auto second = [&](Stretch& s) {  // the run's next stretch, in the batch
-    s.units = s.left;
-    s.left = 0;
-    s.kb = 0;
-    ++s.tile;
-  };
-  auto next_stretch = [&](Stretch& s) {  // of whatever batch
-    if (s.left > 0) return second(s);
-    do next_batch(s);
-    while (s.batch < m1 && s.units == 0);
+  auto row_of = [&](Pass const& p, int token) {  // of x
+    return static_cast<const T*>(a.x) + (long long)(slot_of(p.first + token) / a.x_div) * a.ldx;
   };
 
-  Stretch ahead = {};  // lane 0: where the next unit to load lies
-  ahead.batch = m0;
-  begin_batch(ahead);
-  if (ahead.units == 0) next_stretch(ahead);
-  int load_x = 0, load_y = 0, load_expert = 0, load_left = 0;
-  auto aim = [&]() {
-    if (ahead.batch >= m1) return;
-    load_x = (kb0 + ahead.kb) * (kUnitK / 2);
-    load_y = ahead.row0 + ahead.tile * kRows;
-    load_expert = pass_of(ahead.pass).expert;
-    load_left = ahead.units;
-  };
-  auto load = [&](uint32_t at_slot, uint32_t bar) {
-    if (load_left == 0) return;
-    mbarrier_arrive_expect_tx(bar, kUnitBytes);
-    tma_load_3d(at_slot, &a.map, bar, load_x, load_y, load_expert);
-    tma_load_3d(at_slot + kBoxBytes, &a.map, bar, load_x + 128, load_y, load_expert);  // zeros behind K
-    load_x += kUnitK / 2;
-    if (--load_left == 0) {
-      next_stretch(ahead);
-      aim();
+  // This block's share of K, in units, and its cluster's tiles of all passes' tiles: the `remaining` ones from
+  // tile `first` of pass `pass`. They go in batches of up to 16 of one pass. A batch's units (tile, 512 codes of this
+  // block's K) are dealt to the warps in even, consecutive runs, so a run touches at most two tiles:
+  // count kbs w / 16 units lie before warp w's, which begin in tile count w / 16.
+  const int kb_all = (a.k + kUnitK - 1) / kUnitK;
+  const int kb0 = kb_all * split / splits, kbs = kb_all * (split + 1) / splits - kb0;
+  const uint32_t clusters = gridDim.x / splits, c0 = blockIdx.x / splits, all = uint32_t(passes) * a.tiles;
+  const uint32_t share = all / clusters, extra = all % clusters, begin0 = c0 * share + min(c0, extra);
+  int remaining = int(share + (c0 < extra)), pass = int(begin0 / a.tiles), first = int(begin0 - pass * a.tiles);
+  int count = 0, run_left = 0, tile = 0, kb = 0, expert = -1, mark = 0;
+  bool failed = false;
+
+  // Puts the warp's next unit into ring slot `at`: its record, and its loads.
+  const int scale_bytes = a.f32_scales ? 4 : 2;
+  auto produce = [&](int at) {
+    Unit u;
+    u.flags = mark;
+    if (run_left == 0) {  // the next batch
+      first += count;
+      remaining -= count;
+      const bool turn = first == a.tiles;
+      if (turn) {
+        first = 0;
+        ++pass;
+      }
+      if (turn || expert < 0) {
+        // x of a pass is on its way to L2 before the weights' queue to memory fills: loads behind it take
+        // microseconds.
+        const Pass p = pass_of(pass);
+        expert = p.expert;
+        for (int token = 0; token < p.count; ++token) {
+          const char* x = reinterpret_cast<const char*>(row_of(p, token) + kb0 * kUnitK);
+          const int bytes = min(a.k - kb0 * kUnitK, kbs * kUnitK) * 2;
+          for (int i = threadIdx.x * 128; i < bytes; i += kThreads * 128) asm volatile("prefetch.global.L2 [%0];" ::"l"(x + i));
+        }
+      }
+      count = min(kWarps, min(a.tiles - first, remaining));
+      const int begin = count * kbs * warp / kWarps;
+      run_left = count * kbs * (warp + 1) / kWarps - begin;
+      tile = count * warp / kWarps;
+      kb = begin - tile * kbs;
+      u.flags = run_left == 0 ? kNone | kEnd : kFirst;
+      if (run_left > 0) {  // likewise the scales and zero points, a row of two tiles to a lane
+        const int row = min((first + tile) * kRows + lane, a.n - 1), g0 = kb0 * NG / a.group_span;
+        const int groups = min((kb0 + kbs) * NG / a.group_span, a.last_group + 1) - g0;
+        const char* s = static_cast<const char*>(a.scales) + (expert * a.stride_s + row * a.lds + g0) * scale_bytes;
+        for (int i = 0; i < groups * scale_bytes; i += 128) asm volatile("prefetch.global.L2 [%0];" ::"l"(s + i));
+        if (a.zeros != nullptr) {
+          const uint8_t* z = a.zeros + expert * a.stride_z + row * a.ldz + g0;
+          for (int i = 0; i < groups; i += 128) asm volatile("prefetch.global.L2 [%0];" ::"l"(z + i));
+        }
+      }
+    }
+    u.row0 = (first + tile) * kRows;
+    u.kb = kb;
+    u.expert = expert;
+    u.batch_row0 = first * kRows;
+    u.count = count;
+    u.pass = pass;
+    const bool load = (u.flags & kNone) == 0;
+    if (load) {
+      --run_left;
+      if (++kb == kbs || run_left == 0) u.flags |= kLast;
+      if (run_left == 0) u.flags |= kEnd;
+      mark &= kSecond;
+      if (kb == kbs) {
+        kb = 0;
+        ++tile;
+        mark = kFirst | kSecond;
+      }
+      if (run_left == 0) mark = 0;
+      else if ((u.flags & kSecond) != 0) mark |= kSecond;
+    }
+    if (lane == 0) {
+      units[at] = u;
+      const uint32_t bar = bar0 + 8 * at, to = ring0 + at * kUnitBytes;
+      if (load && !failed) {
+        mbarrier_arrive_expect_tx(bar, kUnitBytes);
+        tma_load_3d(to, &a.map, bar, (kb0 + u.kb) * (kUnitK / 2), u.row0, u.expert);
+        tma_load_3d(to + kBoxBytes, &a.map, bar, (kb0 + u.kb) * (kUnitK / 2) + 128, u.row0, u.expert);  // zeros behind K
+      } else {
+        mbarrier_arrive(bar);
+      }
     }
   };
-  // x of a pass as digits: a warp takes 256 K-elements of a token at a time, a lane 8 of them; kEarly pieces
-  // are loaded before the first is worked on.
-  constexpr int kEarly = 2;
-  const int digit_row = digit_bytes<NT>(a.pair);
-  auto fetch = [&](Pass const& p, int i0, uint4 (&u)[kEarly]) {
-#pragma unroll
-    for (int n = 0; n < kEarly; ++n) {
-      const int i = i0 + n * kWarps;
-      u[n] = make_uint4(0, 0, 0, 0);
-      if (i >= p.count * kbs * 2) continue;
-      const int token = i / (kbs * 2), half = i - token * (kbs * 2);
-      const int k = kb0 * kUnitK + half * 256 + lane * 8;
-      if (k < a.k)
-        u[n] = *reinterpret_cast<const uint4*>(static_cast<const T*>(a.x) + (long long)(slot_of(p.first + token) / a.x_div) * a.ldx + k);
-    }
-  };
-  auto convert = [&](Pass const& p, uint4 (&early)[kEarly]) {
+
+  // x of a pass as digits: a warp takes 256 K-elements of a token at a time, a lane 8 of them, and loads
+  // the next piece before it works on one.
+  auto convert = [&](Pass const& p) {
     constexpr int kLanes = 64 / NG;  // lanes of a scale group
-    for (int i0 = warp; i0 < p.count * kbs * 2; i0 += kEarly * kWarps) {
-      if (i0 != warp) fetch(p, i0, early);
-#pragma unroll
-      for (int n = 0; n < kEarly; ++n) {
-      const int i = i0 + n * kWarps;
-      if (i >= p.count * kbs * 2) break;
-      const int token = i / (kbs * 2), half = i - token * (kbs * 2);
-      const uint4 u = early[n];
+    int next_token = 0, next_half = warp;  // halves: kbs * 2 a token
+    uint4 next = make_uint4(0, 0, 0, 0);
+    auto fetch = [&] {
+      while (next_half >= kbs * 2) {
+        next_half -= kbs * 2;
+        ++next_token;
+      }
+      const int k = (kb0 * 2 + next_half) * 256 + lane * 8;
+      if (next_token < p.count)
+        next = k < a.k ? *reinterpret_cast<const uint4*>(row_of(p, next_token) + k) : make_uint4(0, 0, 0, 0);
+    };
+    fetch();
+#pragma unroll 1
+    while (next_token < p.count) {
+      const int token = next_token, half = next_half;
+      const uint4 u = next;
+      next_half += kWarps;
+      fetch();
       // The largest |x|: both types order like their bits, with NaN above infinity.
       uint32_t m = __vmaxu2(__vmaxu2(u.x & 0x7FFF7FFFu, u.y & 0x7FFF7FFFu), __vmaxu2(u.z & 0x7FFF7FFFu, u.w & 0x7FFF7FFFu));
 #pragma unroll
@@ -419,14 +441,14 @@ __global__ void __launch_bounds__(kThreads, 1) gemv_int4_kernel(const __grid_con
         low += __shfl_xor_sync(0xFFFFFFFFu, low, o);
         high += __shfl_xor_sync(0xFFFFFFFFu, high, o);
       }
-      uint8_t* to = digits + size_t(half * 8 + lane / 4) * digit_row + lane % 4 * 8;
+      uint8_t* to = smem + a.digits + (half * 8 + lane / 4) * kDigitRow<TOK> + lane % 4 * 8;
 #pragma unroll
       for (int c = 0; c < 3; ++c)
-        *reinterpret_cast<uint2*>(to + (NT == 1 ? (a.pair ? 2 * c + token : c) * 32 : (token / 8 * 3 + c) * 256 + token % 8 * 32)) = d[c];
+        *reinterpret_cast<uint2*>(to + (TOK <= 2 ? (c * TOK + token) * 32 : (token / 8 * 3 + c) * 256 + token % 8 * 32)) = d[c];
       const int s0 = int(int16_t(low)), s1 = (low - s0) >> 16;
       if (lane % kLanes == 0) {
-        uint8_t* to_sum = smem + at.sums + size_t(half * (NG / 2) + lane / kLanes) * kSumBytes<NT>;
-        if constexpr (NT == 1) {
+        uint8_t* to_sum = smem + a.sums + (half * (NG / 2) + lane / kLanes) * kSumBytes<TOK>;
+        if constexpr (TOK <= 2) {
           int* f = reinterpret_cast<int*>(to_sum) + token;
           f[0] = s0;
           f[2] = s1;
@@ -437,53 +459,39 @@ __global__ void __launch_bounds__(kThreads, 1) gemv_int4_kernel(const __grid_con
       }
       if (lane % 16 == 0) {
         const float down = bad ? NAN : __int_as_float((127 - e) << 23);
-        float* f = reinterpret_cast<float*>(smem + at.powers + size_t(half * 2 + lane / 16) * kPowerBytes<NT>) + token;
+        float* f = reinterpret_cast<float*>(smem + a.powers + (half * 2 + lane / 16) * kPowerBytes<TOK>) + token;
         f[0] = down;
-        if (NT == 1) {
+        if (TOK <= 2) {
           f[2] = down * 256.0f;
           f[4] = down * 65536.0f;
         }
       }
-      }
     }
   };
 
-  // A unit's scales and zero points, loaded one unit ahead: lane t of a row's four holds groups t, t + 4, ... Rows behind the matrix and groups behind K read the last ones: the first are not
-  // stored, the second multiply zeros.
+  // A unit's scales and zero points, loaded one unit ahead: lane t of a row's four holds groups t, t + 4, ...
+  // Rows behind the matrix and groups behind K read the last ones: the first are not stored, the second multiply
+  // zeros.
   struct Scales {
     uint32_t s[2][kHeld];  // as loaded: nothing waits for them before the unit that uses them
     uint32_t z[2][kHeld];
   };
-  const int last_group = (a.k + a.group - 1) / a.group - 1, group_span = NG == 4 ? a.group / 128 : 1;
-  struct Rows {
-    const void* s[2];
-    const uint8_t* z[2];
-  };
-  const int scale_bytes = a.f32_scales ? 4 : 2;
-  auto rows_of = [&](int expert, int row0) {
-    Rows r;
+  auto load_scales = [&](Unit const& u, Scales& v) {
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const int row = min(row0 + i * 8 + g, a.n - 1);
-      r.s[i] = static_cast<const char*>(a.scales) + (expert * a.stride_s + row * a.lds) * scale_bytes;
-      r.z[i] = a.zeros + expert * a.stride_z + row * a.ldz;
-    }
-    return r;
-  };
-  auto load_scales = [&](Rows const& rows, int kb, Scales& v) {
+    for (int r = 0; r < 2; ++r) {
+      const int row = min(u.row0 + r * 8 + g, a.n - 1);
+      const long long s_row = u.expert * a.stride_s + row * a.lds;
+      const uint8_t* z_row = a.zeros + u.expert * a.stride_z + row * a.ldz;
 #pragma unroll
-    for (int h = 0; h < kHeld; ++h) {
-      int gi = kb * NG + t + 4 * h;
-      if (NG == 4 && group_span != 1) gi /= group_span;
-      gi = min(gi, last_group);
-#pragma unroll
-      for (int r = 0; r < 2; ++r) {
-        v.s[r][h] = a.f32_scales ? static_cast<const uint32_t*>(rows.s[r])[gi] : static_cast<const uint16_t*>(rows.s[r])[gi];
-        if (a.zeros != nullptr) v.z[r][h] = rows.z[r][gi];
+      for (int h = 0; h < kHeld; ++h) {
+        int gi = (kb0 + u.kb) * NG + t + 4 * h;
+        if (NG == 4 && a.group_span != 1) gi /= a.group_span;
+        gi = min(gi, a.last_group);
+        v.s[r][h] = a.f32_scales ? static_cast<const uint32_t*>(a.scales)[s_row + gi] : static_cast<const uint16_t*>(a.scales)[s_row + gi];
+        if (a.zeros != nullptr) v.z[r][h] = z_row[gi];
       }
     }
   };
-
   auto scale_of = [&](uint32_t bits) {
     if (a.f32_scales) return __uint_as_float(bits);
     const uint16_t b16 = uint16_t(bits);
@@ -491,147 +499,115 @@ __global__ void __launch_bounds__(kThreads, 1) gemv_int4_kernel(const __grid_con
     memcpy(&v, &b16, 2);
     return to_f32(v);
   };
-  // The lines of a batch's scales and zero points into L2: behind the weights' queue to memory a plain load of
-  // them takes microseconds.
-  auto prefetch_batch = [&](Stretch const& s) {
-    if (s.batch >= m1) return;
-    const int expert = pass_of(s.pass).expert;
-    const int first = kb0 * NG / group_span, last = min((kb0 + kbs) * NG / group_span, last_group + 1);
-    auto lines = [&](const char* base, long long pitch, int size) {
-      const int bytes = (last - first) * size, per_row = bytes / 128 + 1;
-      for (int i = threadIdx.x; i < s.count * kRows * per_row; i += kThreads) {
-        const int row = s.row0 + i / per_row, at_byte = min(i % per_row * 128, bytes - 1);
-        if (row < a.n) asm volatile("prefetch.global.L2 [%0];" ::"l"(base + row * pitch + (long long)first * size + at_byte));
-      }
-    };
-    if (last <= first) return;
-    lines(static_cast<const char*>(a.scales) + expert * a.stride_s * scale_bytes, a.lds * scale_bytes, scale_bytes);
-    if (a.zeros != nullptr) lines(reinterpret_cast<const char*>(a.zeros) + expert * a.stride_z, a.ldz, 1);
-  };
-
   auto store = [&](int slot, int n, float v) {
     const long long o = (long long)slot * a.ldo + n;
     if (a.f32_out) static_cast<float*>(a.out)[o] = v;
     else static_cast<T*>(a.out)[o] = from_f32<T>(v);
   };
 
-  constexpr int kSets = NT == 1 ? 1 : NT / 3;  // tiles of 8 tokens
-  Stretch cur = {};
-  cur.batch = m0;
-  begin_batch(cur);
-  Stretch peek = cur;
-  if (peek.batch < m1 && peek.units == 0) next_stretch(peek);
-  if (a.ids == nullptr) griddep_wait();
-  griddep_launch_dependents();
-  // The first loads, those that the start waits for before the weights fill the queue to memory.
-  Pass p = {};
-  uint4 early[kEarly] = {};
-  Scales raw = {};
-  Rows rows = {};
-  if (cur.batch < m1) {
-    p = pass_of(cur.pass);
-    fetch(p, warp, early);
-  }
-  if (peek.batch < m1) {
-    rows = rows_of(pass_of(peek.pass).expert, peek.row0 + peek.tile * kRows);
-    load_scales(rows, kb0 + peek.kb, raw);
-  }
-  if (lane == 0) {
-    aim();
-    for (int i = 0; i < depth; ++i) load(ring0 + i * kUnitBytes, bar0 + 8 * i);
-  }
-  prefetch_batch(cur);
+  constexpr int kSets = TOK <= 2 ? 1 : TOK / 8;  // of up to 8 tokens
   // Where a lane reads: its ldmatrix rows in a box (swizzled by 16 bytes), its column's digits (a column that
   // nothing uses reads another's).
-  uint32_t in_box[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) in_box[i] = lane % 16 * 128 + (((i * 2 + lane / 16) ^ (lane & 7)) * 16);
-  const int digit_lane = t * 8 + (NT != 1 ? g * 32 : g >= 6 ? 0 : a.pair ? g * 32 : g % 2 ? 0 : g / 2 * 32);
-  int slot = 0, pass = -1, flip = 0;
-  uint32_t parity = 0;
-  bool failed = false;
-  while (cur.batch < m1) {
-    if (cur.pass != pass) {
-      if (pass >= 0) {
-        p = pass_of(cur.pass);
-        fetch(p, warp, early);
-      }
-      pass = cur.pass;
-      convert(p, early);
-      __syncthreads();
+  const uint32_t in_box = lane % 16 * 128 + ((lane / 16 ^ (lane & 7)) * 16);
+  const int digit_lane = t * 8 + (TOK > 2 ? g * 32 : g >= 6 ? 0 : TOK == 2 ? g * 32 : g % 2 ? 0 : g / 2 * 32);
+  // A batch's sums of the cluster's blocks, a tile to a block in turn. They are gathered a batch later, when the
+  // others' have long arrived; two buffers: by then every block has left the one that is written next.
+  Unit gathers = {};
+  Pass gathers_pass = {};
+  int flip = 0;
+  auto gather = [&] {
+    cluster_wait();
+    const float* mine = reinterpret_cast<const float*>(smem + a.block) + flip * kWarps * kPiece<TOK>;
+    for (int i = threadIdx.x; split + i / kPiece<TOK> * splits < gathers.count; i += kThreads) {
+      const int m = split + i / kPiece<TOK> * splits, o = i % kPiece<TOK>, token = o / kRows, n = gathers.batch_row0 + m * kRows + o % kRows;
+      if (token >= gathers_pass.count || n >= a.n) continue;
+      float v = 0.0f;
+      for (int r = 0; r < splits; ++r) v += cluster.map_shared_rank(mine, r)[m * kPiece<TOK> + o];
+      store(slot_of(gathers_pass.first + token), n, v);
     }
-    Stretch then = cur;
-    next_batch(then);
-    prefetch_batch(then);
-    int piece = 0;
-    while (cur.units > 0 && !failed) {
-      // The next stretch, whose first scales are loaded in this one's last unit.
-      if (peek.batch < m1) next_stretch(peek);
-      float acc[kSets][4] = {};
-      const uint8_t* xd = digits + size_t(cur.kb) * 16 * digit_row + digit_lane;
-      const uint8_t* xs = smem + at.sums + size_t(cur.kb) * NG * kSumBytes<NT> + t * (NT == 1 ? 8 : 16);
-      const uint8_t* xp = smem + at.powers + size_t(cur.kb) * 4 * kPowerBytes<NT> + t * 8;
-      for (int u = 0; u < cur.units; ++u) {
-        float s_now[2][kHeld];
-        uint32_t z_now[2][kHeld];
+    __syncwarp();
+  };
+  float acc[kSets][4] = {};
+  Scales raw = {};
+  Pass p = {};
+  int in = 0, out = depth - 1;      // ring slots: the next to fill, and that of unit `done`
+  int issued = 0, done = -1;        // units; before the first, a turn that only loads its scales
+  int at_pass = -1;
+  uint32_t parity = 1;
+#pragma unroll 1
+  while (true) {
+    // At first one unit a warp: what the start waits for does not queue behind a whole ring of weights.
+    while ((remaining > count || run_left > 0) && issued - max(done, 0) < (done < 0 ? 1 : depth)) {
+      produce(in);
+      in = in + 1 == depth ? 0 : in + 1;
+      ++issued;
+    }
+    if (done == issued) break;
+    __syncwarp();
+    float s_now[2][kHeld];
+    uint32_t z_now[2][kHeld];
 #pragma unroll
-        for (int r = 0; r < 2; ++r)
+    for (int r = 0; r < 2; ++r)
 #pragma unroll
-          for (int h = 0; h < kHeld; ++h) {
-            s_now[r][h] = scale_of(raw.s[r][h]);
-            z_now[r][h] = raw.z[r][h];
-          }
-        if (u + 1 < cur.units) {
-          load_scales(rows, kb0 + cur.kb + u + 1, raw);
-        } else if (peek.batch < m1) {
-          rows = rows_of(pass_of(peek.pass).expert, peek.row0 + peek.tile * kRows);
-          load_scales(rows, kb0 + peek.kb, raw);
-        }
-        const uint32_t bar = bar0 + 8 * slot, base = ring0 + slot * kUnitBytes;
-        if (!mbarrier_wait(bar, parity, a.timeout_ns)) {
-          failed = true;
-          break;
-        }
-        const bool short_unit = (kb0 + cur.kb + u) * kUnitK + kUnitK / 2 >= a.k;
+      for (int h = 0; h < kHeld; ++h) {
+        s_now[r][h] = scale_of(raw.s[r][h]);
+        z_now[r][h] = raw.z[r][h];
+      }
+    if (done + 1 < issued) load_scales(units[out + 1 == depth ? 0 : out + 1], raw);
+    if (done >= 0) {
+      const Unit u = units[out];
+      if ((u.flags & kFirst) != 0) {
+#pragma unroll
+        for (int set = 0; set < kSets; ++set) acc[set][0] = acc[set][1] = acc[set][2] = acc[set][3] = 0.0f;
+      }
+      if ((u.flags & kNone) == 0 && !failed)
+        failed = __any_sync(0xFFFFFFFFu, !mbarrier_wait(bar0 + 8 * out, parity, a.timeout_ns));
+      if ((u.flags & kNone) == 0 && !failed) {
+        const uint32_t base = ring0 + out * kUnitBytes + in_box;
+        const uint8_t* xd = smem + a.digits + u.kb * 16 * kDigitRow<TOK> + digit_lane;
+        const uint8_t* xs = smem + a.sums + u.kb * NG * kSumBytes<TOK> + t * (TOK <= 2 ? 8 : 16);
+        const uint8_t* xp = smem + a.powers + u.kb * 4 * kPowerBytes<TOK> + t * 8;
+        const int quarters = (kb0 + u.kb) * kUnitK + kUnitK / 2 >= a.k ? 2 : 4;
 #pragma unroll
         for (int quarter = 0; quarter < 4; ++quarter) {  // 128 codes
-          if (quarter == 2 && short_unit) break;
-          int part[NT][4];
+          if (quarter == quarters) break;
+          int part[kTiles<TOK>][4];
           float sum[kSets][4] = {};
 #pragma unroll
           for (int pair = 0; pair < 2; ++pair) {
             // Matrices: rows 0-7 and 8-15 of chunk 2 pair, then of chunk 2 pair + 1.
             uint32_t w[4];
-            ldmatrix_x4(w, base + quarter / 2 * kBoxBytes + in_box[quarter % 2 * 2 + pair]);
+            ldmatrix_x4(w, (base + quarter / 2 * kBoxBytes) ^ (quarter % 2 * 64 + pair * 32));
 #pragma unroll
             for (int cc = 0; cc < 2; ++cc) {
-              const int c = quarter * 4 + pair * 2 + cc;
+              constexpr int kGroups = 4 / kPerGroup;  // of a quarter
+              const int c = pair * 2 + cc;
               const uint32_t f[4] = {w[2 * cc] & kNibbles, w[2 * cc + 1] & kNibbles, (w[2 * cc] >> 4) & kNibbles,
                                      (w[2 * cc + 1] >> 4) & kNibbles};
-              const uint8_t* xc = xd + c * digit_row;
+              const uint8_t* xc = xd + c * kDigitRow<TOK>;
 #pragma unroll
-              for (int j = 0; j < NT; ++j) {
+              for (int j = 0; j < kTiles<TOK>; ++j) {
                 if (j >= 3 && p.count <= 8) continue;
                 mma_u8s8(part[j], f, *reinterpret_cast<const uint2*>(xc + j * 256), c % kPerGroup == 0);
               }
               if (c % kPerGroup != kPerGroup - 1) continue;
-              const int gj = c / kPerGroup, from = (lane & 28) | (gj & 3);
+              const int gj = c / kPerGroup, from = (lane & 28) | ((quarter * kGroups + gj) & 3);
               float sc[2];
               int z[2] = {8, 8};
 #pragma unroll
               for (int r = 0; r < 2; ++r) {
-                sc[r] = __shfl_sync(0xFFFFFFFFu, s_now[r][gj / 4], from);
-                if (a.zeros != nullptr) z[r] = int(__shfl_sync(0xFFFFFFFFu, z_now[r][gj / 4], from));
+                sc[r] = __shfl_sync(0xFFFFFFFFu, s_now[r][0], from);
+                if (a.zeros != nullptr) z[r] = int(__shfl_sync(0xFFFFFFFFu, z_now[r][0], from));
               }
-              if constexpr (NT == 1) {
-                const int2 q = *reinterpret_cast<const int2*>(xs + gj * kSumBytes<NT>);
+              if constexpr (TOK <= 2) {
+                const int2 q = *reinterpret_cast<const int2*>(xs + gj * kSumBytes<TOK>);
 #pragma unroll
                 for (int i = 0; i < 4; ++i) sum[0][i] = fmaf(sc[i / 2], float(part[0][i] - z[i / 2] * (i % 2 ? q.y : q.x)), sum[0][i]);
               } else {
 #pragma unroll
                 for (int set = 0; set < kSets; ++set) {
                   if (set > 0 && p.count <= 8) continue;
-                  const int4 q = *reinterpret_cast<const int4*>(xs + gj * kSumBytes<NT> + set * 64);
+                  const int4 q = *reinterpret_cast<const int4*>(xs + gj * kSumBytes<TOK> + set * 64);
 #pragma unroll
                   for (int i = 0; i < 4; ++i) {
                     // |256 P_1 + P_0| and z times its sums stay below 2^30.
@@ -645,89 +621,105 @@ __global__ void __launch_bounds__(kThreads, 1) gemv_int4_kernel(const __grid_con
           }
 #pragma unroll
           for (int set = 0; set < kSets; ++set) {
-            const float2 q = *reinterpret_cast<const float2*>(xp + quarter * kPowerBytes<NT> + set * 32);
+            const float2 q = *reinterpret_cast<const float2*>(xp + set * 32);
 #pragma unroll
             for (int i = 0; i < 4; ++i) acc[set][i] = fmaf(i % 2 ? q.y : q.x, sum[set][i], acc[set][i]);
           }
+          xd += 4 * kDigitRow<TOK>;
+          xs += NG / 4 * kSumBytes<TOK>;
+          xp += kPowerBytes<TOK>;
+          // The next quarter's groups in front, where this one's were a lane's last.
+          if (kHeld > 1 && (kHeld == 4 || quarter == 1)) {
+#pragma unroll
+            for (int r = 0; r < 2; ++r)
+#pragma unroll
+              for (int h = 0; h + 1 < kHeld; ++h) {
+                s_now[r][h] = s_now[r][h + 1];
+                z_now[r][h] = z_now[r][h + 1];
+              }
+          }
         }
-        xd += 16 * digit_row;
-        xs += NG * kSumBytes<NT>;
-        xp += 4 * kPowerBytes<NT>;
         __syncwarp();
-        if (lane == 0) load(base, bar);
-        if (++slot == depth) {
-          slot = 0;
-          parity ^= 1;
+        if ((u.flags & kLast) != 0) {
+          // This warp's part of the tile's sums, [token][row].
+          float* to = pieces + (warp * kPieces + ((u.flags & kSecond) != 0)) * kPiece<TOK>;
+          if constexpr (TOK <= 2) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const float v0 = __shfl_sync(0xFFFFFFFFu, acc[0][i], lane & 28), v1 = __shfl_sync(0xFFFFFFFFu, acc[0][i], (lane & 28) | 1),
+                          v2 = __shfl_sync(0xFFFFFFFFu, acc[0][i], (lane & 28) | 2);
+              if (t == 0 && i % 2 < TOK) to[i % 2 * kRows + i / 2 * 8 + g] = v0 + v1 + v2;
+            }
+          } else {
+#pragma unroll
+            for (int set = 0; set < kSets; ++set)
+#pragma unroll
+              for (int i = 0; i < 4; ++i) to[(set * 8 + 2 * t + i % 2) * kRows + i / 2 * 8 + g] = acc[set][i];
+          }
+          __syncwarp();
         }
       }
-      if (failed) break;
-      // This warp's part of the tile's sums, [token][row].
-      float* to = pieces + (warp * kPieces + piece) * kPiece<NT>;
-      ++piece;
-      if constexpr (NT == 1) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float v0 = __shfl_sync(0xFFFFFFFFu, acc[0][i], lane & 28), v1 = __shfl_sync(0xFFFFFFFFu, acc[0][i], (lane & 28) | 1),
-                      v2 = __shfl_sync(0xFFFFFFFFu, acc[0][i], (lane & 28) | 2);
-          if (t == 0) to[i % 2 * kRows + i / 2 * 8 + g] = v0 + v1 + v2;
+      if ((u.flags & kEnd) != 0) {
+        auto put = [&](int m, int o, float v) {
+          const int token = o / kRows, n = u.batch_row0 + m * kRows + o % kRows;
+          if (token < p.count && n < a.n) store(slot_of(p.first + token), n, v);
+        };
+        // A full batch is a tile a warp, whose sums (over this block's K) are the warp's own; else they are the
+        // sums of the warps' parts in their order along K: warp w's run is [count kbs w / 16, count kbs (w + 1) / 16),
+        // tile m's units [m kbs, (m + 1) kbs).
+        const bool full = u.count == kWarps;
+        if (!full) __syncthreads();
+        auto block_sum = [&](int m, int o) {
+          float sum = 0.0f;
+          for (int w = m * kWarps / u.count; w < kWarps; ++w) {
+            const int lo = u.count * kbs * w / kWarps, hi = u.count * kbs * (w + 1) / kWarps;
+            if (lo >= (m + 1) * kbs) break;
+            if (lo >= hi) continue;
+            sum += pieces[(w * kPieces + (lo >= m * kbs ? 0 : 1)) * kPiece<TOK> + o];  // 1: the run began in the tile before
+          }
+          return sum;
+        };
+        const int step = full ? 32 : kThreads, cells = (full ? 1 : u.count) * kPiece<TOK>;
+        if (splits > 1) {
+          if (gathers.count > 0) gather();
+          gathers = u;
+          gathers_pass = p;
+          flip ^= 1;
         }
-      } else {
-#pragma unroll
-        for (int set = 0; set < kSets; ++set)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) to[(set * 8 + 2 * t + i % 2) * kRows + i / 2 * 8 + g] = acc[set][i];
-      }
-      if (cur.left > 0) second(cur);
-      else cur.units = 0;
-    }
-    __syncthreads();
-    // The batch's tiles: the warps' parts in their order along K, then the cluster's blocks. Warp w's run is
-    // [count kbs w / 16, count kbs (w + 1) / 16), tile m's units [m kbs, (m + 1) kbs).
-    auto block_sum = [&](int i) {
-      const int m = i / kPiece<NT>, o = i % kPiece<NT>;
-      float sum = 0.0f;
-      for (int w = m * kWarps / cur.count; w < kWarps; ++w) {
-        const int lo = cur.count * kbs * w / kWarps, hi = cur.count * kbs * (w + 1) / kWarps;
-        if (lo >= (m + 1) * kbs) break;
-        if (lo >= hi || hi <= m * kbs) continue;
-        sum += pieces[(w * kPieces + (lo >= m * kbs ? 0 : 1)) * kPiece<NT> + o];  // 1: the run began in the tile before
-      }
-      return sum;
-    };
-    auto put = [&](int i, float v) {
-      const int m = i / kPiece<NT>, token = i % kPiece<NT> / kRows, n = cur.row0 + m * kRows + i % kRows;
-      if (token < p.count && n < a.n) store(slot_of(p.first + token), n, v);
-    };
-    const int cells = cur.count * kPiece<NT>;
-    if (splits == 1) {
-      for (int i = threadIdx.x; i < cells; i += kThreads) put(i, block_sum(i));
-      __syncthreads();
-    } else {
-      // Two buffers: a block writes one again only after a barrier that follows its readers' reads.
-      float* mine = block + flip * kWarps * kPiece<NT>;
-      flip ^= 1;
-      for (int i = threadIdx.x; i < cells; i += kThreads) mine[i] = block_sum(i);
-      cluster.sync();
-      for (int i = threadIdx.x; i < cells; i += kThreads) {
-        if (i / kPiece<NT> % splits != split) continue;
-        float v = 0.0f;
-        for (int r = 0; r < splits; ++r) v += cluster.map_shared_rank(mine, r)[i];
-        put(i, v);
+        float* mine = reinterpret_cast<float*>(smem + a.block) + flip * kWarps * kPiece<TOK>;
+        for (int i = full ? lane : int(threadIdx.x); i < cells; i += step) {
+          const int m = full ? warp : i / kPiece<TOK>, o = i % kPiece<TOK>;
+          const float v = block_sum(m, o);
+          if (splits > 1) mine[m * kPiece<TOK> + o] = v;
+          else put(m, o, v);
+        }
+        if (!full) __syncthreads();
+        else __syncwarp();
+        if (splits > 1) cluster_arrive();
       }
     }
-    next_batch(cur);
+    if (done + 1 < issued) {
+      const int next_pass = units[out + 1 == depth ? 0 : out + 1].pass;
+      if (next_pass != at_pass) {  // every warp has a record of every batch, so all come here together
+        if (at_pass >= 0) __syncthreads();
+        at_pass = next_pass;
+        p = pass_of(at_pass);
+        convert(p);
+        __syncthreads();
+      }
+    }
+    ++done;
+    out = out + 1 == depth ? 0 : out + 1;
+    if (out == 0) parity ^= 1;
   }
-  if (splits > 1) cluster.sync();  // no block leaves while another may still read its sums
+  if (splits > 1) {
+    if (gathers.count > 0) gather();
+    cluster_sync();  // no block leaves while another may still read its sums
+  }
   if (failed) {
     // The loads still under way end, or are given up on, before the block leaves.
     if (lane == 0) atomicOr(a.status, kl::gemm::kStatusProducerTimeout);
-    for (int i = 0; i < depth; ++i) {
-      mbarrier_wait(bar0 + 8 * slot, parity, a.timeout_ns);
-      if (++slot == depth) {
-        slot = 0;
-        parity ^= 1;
-      }
-    }
+    for (int i = 0; i < depth; ++i) mbarrier_wait(bar0 + 8 * i, i < out ? parity : parity ^ 1, a.timeout_ns);
   }
   // Rows of slots without an expert.
   if (a.ids != nullptr && l.start[active] < a.slots)
@@ -741,28 +733,32 @@ __global__ void __launch_bounds__(kThreads, 1) gemv_int4_kernel(const __grid_con
 struct Fit {
   int cluster, depth;
   size_t bytes;
+  Int4Args args;  // with the layout
 };
 
 // The smallest cluster whose blocks keep x's digits in 80 KB, else 8, and the ring that the rest holds (at
 // most 8 slots a warp, 256 KB in flight). depth 0: does not fit.
-template <int NG, int NT>
+template <int NG, int TOK>
 Fit fit(Int4Args const& a) {
-  Fit f = {1, 0, 0};
+  Fit f = {1, 0, 0, {}};
   const int kb = (a.k + kUnitK - 1) / kUnitK;
   auto units = [&] { return (kb + f.cluster - 1) / f.cluster; };
-  while (f.cluster < 8 && size_t(units()) * x_bytes<NG, NT>(a.pair) > 80 * 1024) f.cluster *= 2;
+  while (f.cluster < 8 && size_t(units()) * kXBytes<NG, TOK> > 80 * 1024) f.cluster *= 2;
+  Int4Args b = a;
   for (int depth = 2; depth <= 8; ++depth) {
-    const Layout<NG, NT> l(depth, units(), a.pair, f.cluster, a.ids != nullptr, a.experts, a.slots);
-    if (l.bytes + 1024 > size_t(kSmemLimit)) break;
+    const size_t bytes = lay_out<NG, TOK>(b, depth, units(), f.cluster);
+    if (bytes > size_t(kSmemLimit)) break;
     f.depth = depth;
-    f.bytes = l.bytes + 1024;
+    f.bytes = bytes;
+    f.args = b;
   }
   return f;
 }
 
-template <class T, int NG, int NT>
-kl_status launch(Int4Args& a, Fit const& f, int device, cudaStream_t stream) {
-  auto* kernel = gemv_int4_kernel<T, NG, NT>;
+template <class T, int NG, int TOK>
+kl_status launch(Fit const& f, int device, cudaStream_t stream) {
+  Int4Args const& a = f.args;
+  auto* kernel = gemv_int4_kernel<T, NG, TOK>;
   static std::atomic<int> resident[64][4];  // clusters of 1, 2, 4, 8 that fit the device at once
   const int which = f.cluster == 1 ? 0 : f.cluster == 2 ? 1 : f.cluster == 4 ? 2 : 3;
   cudaLaunchConfig_t cfg = {};
@@ -790,27 +786,28 @@ kl_status launch(Int4Args& a, Fit const& f, int device, cudaStream_t stream) {
     resident[device][which].store(most, std::memory_order_release);
     cfg.dynamicSmemBytes = f.bytes;
   }
-  const long long passes = a.ids != nullptr ? a.slots : (a.slots + kTokens<NT> - 1) / kTokens<NT>;
+  const long long passes = a.ids != nullptr ? a.slots : (a.slots + TOK - 1) / TOK;
   const long long work = passes * a.tiles;
   if (work > INT32_MAX / 2) return fail(KL_ERR_NOT_SUPPORTED, "kl_gemv_int4: too many rows of out");
-  a.depth = f.depth;
   cfg.gridDim = dim3(unsigned((work < most ? work : most) * f.cluster), 1, 1);
   cfg.numAttrs = 2;
   cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, a);
   return e == cudaSuccess ? KL_OK : cuda_fail(e, "kl_gemv_int4 launch");
 }
 
-// Columns by the tokens that a matrix meets (with ids: on average), fewer where x's digits would not fit.
+// Tokens of a pass by what a matrix meets (with ids: on average), fewer where x's digits would not fit.
 template <class T, int NG>
 kl_status by_tokens(Int4Args& a, int device, cudaStream_t stream) {
   const int tokens = a.ids != nullptr ? (a.slots + a.experts - 1) / a.experts : a.slots;
   if (tokens > 8)
-    if (const Fit f = fit<NG, 6>(a); f.depth >= 2) return launch<T, NG, 6>(a, f, device, stream);
+    if (const Fit f = fit<NG, 16>(a); f.depth >= 2) return launch<T, NG, 16>(f, device, stream);
   if (tokens > 2)
-    if (const Fit f = fit<NG, 3>(a); f.depth >= 2) return launch<T, NG, 3>(a, f, device, stream);
+    if (const Fit f = fit<NG, 8>(a); f.depth >= 2) return launch<T, NG, 8>(f, device, stream);
+  if (a.slots > 1)
+    if (const Fit f = fit<NG, 2>(a); f.depth >= 2) return launch<T, NG, 2>(f, device, stream);
   const Fit f = fit<NG, 1>(a);
-  if (f.depth == 0) return fail(KL_ERR_NOT_SUPPORTED, "kl_gemv_int4: k does not fit");
-  return launch<T, NG, 1>(a, f, device, stream);
+  if (f.depth < 2) return fail(KL_ERR_NOT_SUPPORTED, "kl_gemv_int4: k does not fit");
+  return launch<T, NG, 1>(f, device, stream);
 }
 
 template <class T>
@@ -828,14 +825,12 @@ kl_status run(kl_int4_desc const& d, int64_t slots, cudaStream_t stream) {
   if (device < 0 || device >= 64) return fail(KL_ERR_NOT_SUPPORTED, "device index above 63");
   Int4Args a = {};
   const int64_t matrices = by_expert ? d.experts : 1;
-  if (d.k > 0) {
-    const int64_t shape[3] = {matrices, d.n, d.k / 2};
-    const int64_t stride[3] = {matrices > 1 ? d.stride_q : d.n * d.ldq, d.ldq, 1};
-    kl::TmaOptions opt;
-    opt.l2_promotion = CU_TENSOR_MAP_L2_PROMOTION_L2_256B;
-    kl::detail::encode_tma_map(&a.map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, CU_TENSOR_MAP_SWIZZLE_128B, 128, kRows, d.q, 3,
-                               shape, stride, opt);
-  }
+  const int64_t shape[3] = {matrices, d.n, d.k / 2};
+  const int64_t stride[3] = {matrices > 1 ? d.stride_q : d.n * d.ldq, d.ldq, 1};
+  kl::TmaOptions opt;
+  opt.l2_promotion = CU_TENSOR_MAP_L2_PROMOTION_L2_256B;
+  kl::detail::encode_tma_map(&a.map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, CU_TENSOR_MAP_SWIZZLE_128B, 128, kRows, d.q, 3,
+                             shape, stride, opt);
   a.x = d.x;
   a.ldx = d.ldx;
   a.scales = d.scales;
@@ -856,7 +851,8 @@ kl_status run(kl_int4_desc const& d, int64_t slots, cudaStream_t stream) {
   a.f32_scales = d.scale_type == KL_F32;
   a.f32_out = d.out_type == KL_F32;
   a.tiles = (a.n + kRows - 1) / kRows;
-  a.pair = a.slots > 1;
+  a.group_span = a.group >= 128 ? a.group / 128 : 1;
+  a.last_group = (a.k + a.group - 1) / a.group - 1;
   a.timeout_ns = wait_timeout_ns();
   kl_status s = device_status_ptr(&a.status);
   if (s != KL_OK) return s;
@@ -895,6 +891,11 @@ extern "C" kl_status kl_gemv_int4(const kl_int4_desc* d, void* stream) {
     return bad("x and q must be 16-byte aligned with row pitches that are multiples of 16 bytes");
   if (by_expert && d->experts > 1 && (d->stride_q % 16 != 0 || d->stride_q <= 0 || d->stride_scales < 0 || d->stride_zeros < 0))
     return bad("expert strides must not be negative, stride_q a positive multiple of 16 bytes");
+  if (d->k == 0) {  // a sum of nothing
+    const size_t size = d->out_type == KL_F32 ? 4 : 2;
+    cudaError_t e = cudaMemset2DAsync(d->out, size_t(d->ldo) * size, 0, size_t(d->n) * size, size_t(slots), static_cast<cudaStream_t>(stream));
+    return e == cudaSuccess ? KL_OK : cuda_fail(e, "kl_gemv_int4 memset");
+  }
   try {
     return run(*d, slots, static_cast<cudaStream_t>(stream));
   } catch (std::exception const& e) {
