@@ -57,9 +57,11 @@ struct Int4Args {
   const void* x;
   long long ldx;
   const void* scales;
-  long long lds, stride_s;
+  int lds;
+  long long stride_s;
   const uint8_t* zeros;
-  long long ldz, stride_z;
+  int ldz;
+  long long stride_z;
   const int* ids;
   int experts, slots, x_div;  // slots: rows of out; x row = slot / x_div
   void* out;
@@ -337,10 +339,10 @@ __global__ void __launch_bounds__(kThreads, 1) gemv_int4_kernel(const __grid_con
       if (run_left > 0) {  // likewise the scales and zero points, a row of two tiles to a lane
         const int row = min((first + tile) * kRows + lane, a.n - 1), g0 = kb0 * NG / a.group_span;
         const int groups = min((kb0 + kbs) * NG / a.group_span, a.last_group + 1) - g0;
-        const char* s = static_cast<const char*>(a.scales) + (expert * a.stride_s + row * a.lds + g0) * scale_bytes;
+        const char* s = static_cast<const char*>(a.scales) + (expert * a.stride_s + (long long)row * a.lds + g0) * scale_bytes;
         for (int i = 0; i < groups * scale_bytes; i += 128) asm volatile("prefetch.global.L2 [%0];" ::"l"(s + i));
         if (a.zeros != nullptr) {
-          const uint8_t* z = a.zeros + expert * a.stride_z + row * a.ldz + g0;
+          const uint8_t* z = a.zeros + expert * a.stride_z + (long long)row * a.ldz + g0;
           for (int i = 0; i < groups; i += 128) asm volatile("prefetch.global.L2 [%0];" ::"l"(z + i));
         }
       }
@@ -476,18 +478,26 @@ __global__ void __launch_bounds__(kThreads, 1) gemv_int4_kernel(const __grid_con
     uint32_t s[2][kHeld];  // as loaded: nothing waits for them before the unit that uses them
     uint32_t z[2][kHeld];
   };
+  int base_expert = -1;
+  const char* s_base = nullptr;
+  const uint8_t* z_base = nullptr;
   auto load_scales = [&](Unit const& u, Scales& v) {
+    if (u.expert != base_expert) {
+      base_expert = u.expert;
+      s_base = static_cast<const char*>(a.scales) + u.expert * a.stride_s * scale_bytes;
+      z_base = a.zeros + u.expert * a.stride_z;
+    }
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
       const int row = min(u.row0 + r * 8 + g, a.n - 1);
-      const long long s_row = u.expert * a.stride_s + row * a.lds;
-      const uint8_t* z_row = a.zeros + u.expert * a.stride_z + row * a.ldz;
+      const char* s_row = s_base + (long long)row * (a.lds * scale_bytes);
+      const uint8_t* z_row = z_base + (long long)row * a.ldz;
 #pragma unroll
       for (int h = 0; h < kHeld; ++h) {
         int gi = (kb0 + u.kb) * NG + t + 4 * h;
         if (NG == 4 && a.group_span != 1) gi /= a.group_span;
         gi = min(gi, a.last_group);
-        v.s[r][h] = a.f32_scales ? static_cast<const uint32_t*>(a.scales)[s_row + gi] : static_cast<const uint16_t*>(a.scales)[s_row + gi];
+        v.s[r][h] = a.f32_scales ? reinterpret_cast<const uint32_t*>(s_row)[gi] : reinterpret_cast<const uint16_t*>(s_row)[gi];
         if (a.zeros != nullptr) v.z[r][h] = z_row[gi];
       }
     }
@@ -834,10 +844,10 @@ kl_status run(kl_int4_desc const& d, int64_t slots, cudaStream_t stream) {
   a.x = d.x;
   a.ldx = d.ldx;
   a.scales = d.scales;
-  a.lds = d.ld_scales;
+  a.lds = int(d.ld_scales);
   a.stride_s = matrices > 1 ? d.stride_scales : 0;
   a.zeros = d.zeros;
-  a.ldz = d.ld_zeros;
+  a.ldz = int(d.ld_zeros);
   a.stride_z = matrices > 1 ? d.stride_zeros : 0;
   a.ids = d.ids;
   a.experts = int(matrices);
@@ -886,6 +896,7 @@ extern "C" kl_status kl_gemv_int4(const kl_int4_desc* d, void* stream) {
   const int64_t groups = (d->k + d->group - 1) / d->group;
   if (d->ldo < d->n || d->ldx < d->k || d->ldq < d->k / 2 || d->ld_scales < groups || (d->zeros != nullptr && d->ld_zeros < groups))
     return bad("row pitch below the row's extent");
+  if (d->ld_scales > INT32_MAX / 4 || d->ld_zeros > INT32_MAX) return bad("row pitch too large");
   if (d->out == nullptr || (d->k > 0 && (d->x == nullptr || d->q == nullptr || d->scales == nullptr))) return bad("null pointer");
   if (d->k > 0 && (!aligned16(d->x) || !aligned16(d->q) || d->ldx % 8 != 0 || d->ldq % 16 != 0))
     return bad("x and q must be 16-byte aligned with row pitches that are multiples of 16 bytes");
