@@ -6,7 +6,13 @@
 // routed tokens, the loss is E sum_e (c_e / (k N)) (1/N sum_t p_te). The counts have no gradient:
 // with a_e = dL E c_e / (k N^2) and D = sum_j dw_j w_j,
 //   dl_te = p_te (a_e - sum_e' p_te' a_e' - [w = p] D) + [e = e_j] w_j (dw_j - [w normalised] D).
+//
+// Both kernels read a row once and keep it in registers, 8 experts to a lane. What bounds them is not
+// the memory but the instructions: at 256 bf16 logits a token, HBM would allow about 100 a token. So a lane sorts its
+// eight keys once (19 exchanges), after which each of the k rounds takes one warp-wide maximum and a shift in the lane that
+// held it.
 
+#include <cooperative_groups.h>
 #include <cuda_runtime.h>
 
 #include <string>
@@ -17,48 +23,70 @@
 #include "kl_internal.cuh"
 #include "kl_vec.cuh"
 
+namespace cg = cooperative_groups;
+
 namespace kl::capi {
 namespace {
 
-constexpr int kRouteThreads = 256;
+constexpr int kRouteThreads = 512;
 constexpr int kRouteWarps = kRouteThreads / 32;
 constexpr int kMaxExperts = 1024;
 constexpr int kMaxTopK = 32;
 
 // Ordering keys: larger key = earlier choice. The value's bits in an order-preserving form sit above
 // 1023 - e, so one integer maximum gives the largest value and, among equals, the lowest expert.
-// 16-bit logits leave the low 12 bits of their fp32 form zero, so key and index share 32 bits. 0 is
-// "cannot be chosen" (-inf); NaN orders above everything.
+// 16-bit logits leave the low 12 bits of their fp32 form zero, so key and index share 32 bits. Adding 0
+// makes both zeros +0 and every NaN the positive one, which orders above everything; keys up to
+// kClosed are -inf, which is never chosen.
 template <class T>
 struct RouteKey {
   using type = uint32_t;
+  static constexpr type kClosed = 0x007FFFFFu;
+  static __device__ __forceinline__ type make(uint32_t ordered, int e) {
+    return (ordered & 0xFFFFF000u) | uint32_t(kMaxExperts - 1 - e);
+  }
+  static __device__ __forceinline__ float value(type k) {
+    if (k >= 0xFFFFF000u) return NAN;
+    return __uint_as_float(k & 0x80000000u ? (k & 0x7FFFF000u) : ~(k | 0xFFFu));
+  }
 };
 template <>
 struct RouteKey<float> {
   using type = uint64_t;
+  static constexpr type kClosed = 0x007FFFFFFFFFFFFFull;
+  static __device__ __forceinline__ type make(uint32_t ordered, int e) {
+    return (uint64_t(ordered) << 32) | uint32_t(kMaxExperts - 1 - e);
+  }
+  static __device__ __forceinline__ float value(type k) {
+    const uint32_t o = uint32_t(k >> 32);
+    if (o == 0xFFFFFFFFu) return NAN;
+    return __uint_as_float(o & 0x80000000u ? o & 0x7FFFFFFFu : ~o);
+  }
 };
-
 __device__ __forceinline__ uint32_t ordered_bits(float v) {
-  const uint32_t u = __float_as_uint(v + 0.0f);  // -0 and +0 tie
-  return v != v ? 0xFFFFFFFFu : u ^ (u >> 31 ? 0xFFFFFFFFu : 0x80000000u);
+  const uint32_t u = __float_as_uint(v + 0.0f);
+  return u ^ (uint32_t(int32_t(u) >> 31) | 0x80000000u);
 }
-__device__ __forceinline__ void make_key(float v, int e, uint32_t& k) {
-  k = v == -INFINITY ? 0u : (ordered_bits(v) & 0xFFFFF000u) | uint32_t(kMaxExperts - 1 - e);
-}
-__device__ __forceinline__ void make_key(float v, int e, uint64_t& k) {
-  k = v == -INFINITY ? 0ull : (uint64_t(ordered_bits(v)) << 32) | uint32_t(kMaxExperts - 1 - e);
-}
-__device__ __forceinline__ float value_of_bits(uint32_t o) {
-  return o == 0xFFFFFFFFu ? NAN : __uint_as_float(o & 0x80000000u ? o ^ 0x80000000u : ~o);
-}
-__device__ __forceinline__ float key_value(uint32_t k) {
-  const uint32_t o = k & 0xFFFFF000u;
-  return value_of_bits(o & 0x80000000u ? (o == 0xFFFFF000u ? 0xFFFFFFFFu : o) : o | 0xFFFu);
-}
-__device__ __forceinline__ float key_value(uint64_t k) { return value_of_bits(uint32_t(k >> 32)); }
 template <class K>
 __device__ __forceinline__ int key_expert(K k) {
   return kMaxExperts - 1 - int(uint32_t(k) & (kMaxExperts - 1));
+}
+
+// Eight keys, largest first, by a sorting network of 19 exchanges.
+template <class K>
+__device__ __forceinline__ void sort8(K (&s)[8]) {
+  auto swap = [&](int i, int j) {
+    const K hi = s[i] > s[j] ? s[i] : s[j];
+    s[j] = s[i] > s[j] ? s[j] : s[i];
+    s[i] = hi;
+  };
+  swap(0, 1); swap(2, 3); swap(4, 5); swap(6, 7);
+  swap(0, 2); swap(1, 3); swap(4, 6); swap(5, 7);
+  swap(1, 2); swap(5, 6); swap(0, 4); swap(3, 7);
+  swap(1, 5); swap(2, 6);
+  swap(1, 4); swap(3, 6);
+  swap(2, 4); swap(3, 5);
+  swap(3, 4);
 }
 
 // L lanes share a token; lane i holds experts (v L + i) 8 + 0..7 for v < NV.
@@ -88,25 +116,45 @@ __device__ __forceinline__ K group_key_max(K k) {
   }
 }
 
-// A row's logits as fp32: whole 16-byte vectors where `vec` (aligned rows, E a multiple of 8), else
-// element by element; -inf outside the row.
+// A row's logits as they lie: whole 16-byte vectors where `vec` (aligned rows, E a multiple of 8), else
+// element by element; -inf outside the row, and for a row that is not `live`.
+template <class T, int NV>
+struct Row {
+  uint4 u[NV * 8 / kPerVec<T>];
+};
+template <class T>
+__device__ __forceinline__ T minus_infinity() { return from_f32<T>(-INFINITY); }
 template <class T, int L, int NV>
-__device__ __forceinline__ void load_row(const T* row, int lane, int experts, bool vec, bool live, float (&v)[8 * NV]) {
+__device__ __forceinline__ void load_row(const T* row, int lane, int experts, bool vec, bool live, Row<T, NV>& r) {
+  constexpr int kVecs = 8 / kPerVec<T>;
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
     const int e0 = (i * L + lane) * 8;
-    if (!live || e0 >= experts) {
+    if (vec && live && e0 < experts) {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) v[8 * i + j] = -INFINITY;
-    } else if (vec) {
-      const uint4* p = reinterpret_cast<const uint4*>(row + e0);
-#pragma unroll
-      for (int j = 0; j < 8 / kPerVec<T>; ++j) unpack<T>(p[j], v + 8 * i + j * kPerVec<T>);
+      for (int j = 0; j < kVecs; ++j) r.u[i * kVecs + j] = reinterpret_cast<const uint4*>(row + e0)[j];
     } else {
+      T v[8];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) v[8 * i + j] = e0 + j < experts ? to_f32(row[e0 + j]) : -INFINITY;
+      for (int j = 0; j < 8; ++j) v[j] = live && e0 + j < experts ? row[e0 + j] : minus_infinity<T>();
+      memcpy(&r.u[i * kVecs], v, sizeof(v));
     }
   }
+}
+template <class T, int NV>
+__device__ __forceinline__ void values(Row<T, NV> const& r, float (&v)[8 * NV]) {
+#pragma unroll
+  for (int i = 0; i < NV * 8 / kPerVec<T>; ++i) unpack<T>(r.u[i], v + i * kPerVec<T>);
+}
+
+// exp(x) for x <= 0: 2^(x log2 e) with the product's rounding made up for, so that the relative error
+// stays at a few 2^-24 for far values too.
+__device__ __forceinline__ float exp_neg(float x) {
+  const float hi = x * 1.44269502f;                                    // log2 e, rounded to fp32
+  const float lo = fmaf(x, 1.44269502f, -hi) + x * 1.92596303e-8f;     // and what that left out
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(hi));
+  return x < -104.0f ? 0.0f : fmaf(y * 0.693147182f, lo, y);
 }
 
 struct RouteArgs {
@@ -144,99 +192,114 @@ __device__ __forceinline__ float loss_of(float total, int experts, int k, int ro
 }
 
 template <class T, int L, int NV>
-__global__ void __launch_bounds__(kRouteThreads) route_kernel(const RouteArgs a) {
-  using K = typename RouteKey<T>::type;
+__global__ void __launch_bounds__(kRouteThreads, NV == 1 ? 2 : 1) route_kernel(const RouteArgs a) {
+  using Key = RouteKey<T>;
+  using K = typename Key::type;
   constexpr int kGroups = 32 / L;  // tokens of a warp
+  constexpr int kWidth = L * 8 * NV;
   constexpr int kPicks = L * 8 < kMaxTopK ? L * 8 : kMaxTopK;  // k is at most the number of experts
-  __shared__ K chosen[kRouteWarps * kGroups][kPicks];
-  __shared__ int count[L * 8 * NV];
-  __shared__ float share[kRouteWarps * L * 8 * NV];
+  constexpr int kHeld = kPicks / L > 0 ? kPicks / L : 1;       // picks of a lane: j = h L + lane
+  extern __shared__ float share[];                             // [kRouteWarps][kWidth]
+  __shared__ int count[kWidth];
   __shared__ float red[32];
   __shared__ int routed_here;
-  griddep_wait();
-  griddep_launch_dependents();
   const int warp = threadIdx.x / 32, lane = threadIdx.x % L, group = threadIdx.x % 32 / L;
   for (int e = threadIdx.x; e < a.experts; e += kRouteThreads) count[e] = 0;
   if (threadIdx.x == 0) routed_here = 0;
   __syncthreads();
+  griddep_wait();
+  griddep_launch_dependents();
   const T* logits = static_cast<const T*>(a.logits);
   float acc[8 * NV];
 #pragma unroll
   for (int i = 0; i < 8 * NV; ++i) acc[i] = 0.0f;
-  const int step = gridDim.x * kRouteWarps * kGroups;
-  K* mine = chosen[warp * kGroups + group];
+  const long long step = (long long)gridDim.x * kRouteWarps * kGroups;
+  auto is_live = [&](long long t) { return t < a.tokens && (a.valid == nullptr || a.valid[t] != 0); };
   int routed = 0;
+  long long t = (long long)(blockIdx.x * kRouteWarps + warp) * kGroups + group;
+  Row<T, NV> next;
+  load_row<T, L, NV>(logits + (t < a.tokens ? t : 0) * a.ld, lane, a.experts, a.vec, is_live(t), next);
   // Whole warps leave the loop together: the shuffles take every lane.
-  for (long long first = (long long)(blockIdx.x * kRouteWarps + warp) * kGroups; first < a.tokens; first += step) {
-    const long long t = first + group;
-    const bool live = t < a.tokens && (a.valid == nullptr || a.valid[t] != 0);
+  for (; t - group < a.tokens; t += step) {
     float v[8 * NV];
-    load_row<T, L, NV>(logits + (t < a.tokens ? t : 0) * a.ld, lane, a.experts, a.vec, live, v);
-    K key[8 * NV];
-    float top = -INFINITY;
+    values<T, NV>(next, v);
+    if (t - group + step < a.tokens)
+      load_row<T, L, NV>(logits + (t + step < a.tokens ? t + step : 0) * a.ld, lane, a.experts, a.vec, is_live(t + step), next);
+    K key[NV][8];
 #pragma unroll
-    for (int i = 0; i < 8 * NV; ++i) {
-      make_key(v[i], (i / 8 * L + lane) * 8 + i % 8, key[i]);
-      top = fmaxf(top, v[i]);
+    for (int i = 0; i < NV; ++i) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) key[i][j] = Key::make(ordered_bits(v[8 * i + j]), (i * L + lane) * 8 + j);
+      sort8(key[i]);
     }
-    top = group_max<L>(top);
-    // The k largest keys, one after another; each found key is struck out where it is held.
-    K first_key = 0;
+    // The k largest keys, one after another: the largest head of all lanes, taken off its list.
+    K pick[kHeld] = {};
+    K first = 0;
     for (int j = 0; j < a.k; ++j) {
-      K best = key[0];
+      K best = key[0][0];
 #pragma unroll
-      for (int i = 1; i < 8 * NV; ++i) best = key[i] > best ? key[i] : best;
+      for (int i = 1; i < NV; ++i) best = key[i][0] > best ? key[i][0] : best;
       best = group_key_max<L>(best);
 #pragma unroll
-      for (int i = 0; i < 8 * NV; ++i) key[i] = key[i] == best ? K(0) : key[i];
-      if (lane == 0) mine[j] = best;
-      if (j == 0) first_key = best;
+      for (int i = 0; i < NV; ++i) {
+        const bool here = key[i][0] == best;
+#pragma unroll
+        for (int x = 0; x < 7; ++x) key[i][x] = here ? key[i][x + 1] : key[i][x];
+        key[i][7] = here ? K(0) : key[i][7];
+      }
+#pragma unroll
+      for (int h = 0; h < kHeld; ++h) pick[h] = j == h * L + lane ? best : pick[h];
+      if (j == 0) first = best;
     }
-    const bool any = first_key != 0;
+    const bool any = first > Key::kClosed;
+    const float top = Key::value(first);
     float sum = 0.0f;
 #pragma unroll
     for (int i = 0; i < 8 * NV; ++i) {
-      v[i] = v[i] == -INFINITY ? 0.0f : expf(v[i] - top);
+      v[i] = exp_neg(v[i] - top);
       sum += v[i];
     }
     sum = group_sum<L>(sum);
     if (any) {
       const float inv = 1.0f / sum;
 #pragma unroll
-      for (int i = 0; i < 8 * NV; ++i) acc[i] += v[i] * inv;
+      for (int i = 0; i < 8 * NV; ++i) acc[i] = fmaf(v[i], inv, acc[i]);
       routed += lane == 0;
     }
-    __syncwarp();
-    float part = 0.0f;
-    if (a.renormalize) {
-      for (int j = lane; j < a.k; j += L) part += mine[j] != 0 ? expf(key_value(mine[j]) - top) : 0.0f;
-      sum = group_sum<L>(part);
+    float w[kHeld], part = 0.0f;
+#pragma unroll
+    for (int h = 0; h < kHeld; ++h) {
+      w[h] = h * L + lane < a.k && pick[h] > Key::kClosed ? exp_neg(Key::value(pick[h]) - top) : 0.0f;
+      part += w[h];
     }
+    if (a.renormalize) sum = group_sum<L>(part);
     if (t < a.tokens) {
-      for (int j = lane; j < a.k; j += L) {
-        const K key_j = mine[j];
-        const int e = key_j != 0 ? key_expert(key_j) : -1;
+#pragma unroll
+      for (int h = 0; h < kHeld; ++h) {
+        const int j = h * L + lane;
+        if (j >= a.k) break;
+        const bool open = pick[h] > Key::kClosed;
+        const int e = open ? key_expert(pick[h]) : -1;
         a.ids[t * a.k + j] = e;
-        a.weights[t * a.k + j] = e >= 0 ? expf(key_value(key_j) - top) / sum : 0.0f;
-        if (e >= 0) atomicAdd(&count[e], 1);
+        a.weights[t * a.k + j] = open ? w[h] / sum : 0.0f;
+        if (open) atomicAdd(&count[e], 1);
       }
     }
-    __syncwarp();
   }
   // Block sums in a fixed order: the groups of a warp by shuffles, the warps one after another.
-  const int width = L * 8 * NV;
 #pragma unroll
   for (int i = 0; i < 8 * NV; ++i) {
 #pragma unroll
     for (int o = L; o < 32; o *= 2) acc[i] += __shfl_xor_sync(0xFFFFFFFFu, acc[i], o);
-    if (group == 0) share[warp * width + (i / 8 * L + lane) * 8 + i % 8] = acc[i];
+    if (group == 0) share[warp * kWidth + (i / 8 * L + lane) * 8 + i % 8] = acc[i];
   }
   if (routed) atomicAdd(&routed_here, routed);
   __syncthreads();
   float terms = 0.0f;
   for (int e = threadIdx.x; e < a.experts; e += kRouteThreads) {
     float s = 0.0f;
-    for (int w = 0; w < kRouteWarps; ++w) s += share[w * width + e];
+#pragma unroll
+    for (int w = 0; w < kRouteWarps; ++w) s += share[w * kWidth + e];
     if (gridDim.x == 1) {
       a.counts[e] = count[e];
       terms += s * float(count[e]);
@@ -256,33 +319,68 @@ __global__ void __launch_bounds__(kRouteThreads) route_kernel(const RouteArgs a)
   }
 }
 
-// The blocks' partial sums, in block order.
-__global__ void __launch_bounds__(1024) route_finish_kernel(const RouteArgs a, int blocks) {
+// The blocks' partial sums by one cluster, in a fixed order: a thread takes every so-manieth block of
+// one expert; the threads of an expert meet in shared memory, the cluster's blocks in rank order.
+constexpr int kFinishBlocks = 8;
+constexpr int kFinishThreads = 1024;
+__global__ void __launch_bounds__(kFinishThreads) route_finish_kernel(const RouteArgs a, int blocks) {
+  __shared__ float share[kFinishThreads];
+  __shared__ int count[kFinishThreads];
+  __shared__ float term_sum;
   __shared__ float red[32];
+  cg::cluster_group cluster = cg::this_cluster();
+  const int rank = int(cluster.block_rank());
   griddep_wait();
   griddep_launch_dependents();
-  float terms = 0.0f;
-  for (int e = threadIdx.x; e < a.experts; e += 1024) {
-    float s = 0.0f;
-    int c = 0;
-#pragma unroll 8
-    for (int b = 0; b < blocks; ++b) {
+  const int rows = kFinishThreads / a.experts, row = threadIdx.x / a.experts, e = threadIdx.x % a.experts;  // experts <= 1024
+  float s = 0.0f;
+  int c = 0;
+  if (row < rows)
+#pragma unroll 4
+    for (int b = rank * rows + row; b < blocks; b += kFinishBlocks * rows) {
       s += a.share_part[(long long)b * a.experts + e];
       c += a.count_part[(long long)b * a.experts + e];
     }
-    a.counts[e] = c;
-    terms += s * float(c);
+  share[threadIdx.x] = s;
+  count[threadIdx.x] = c;
+  __syncthreads();
+  if (row == 0) {
+    for (int r = 1; r < rows; ++r) {
+      s += share[r * a.experts + e];
+      c += count[r * a.experts + e];
+    }
+    share[e] = s;
+    count[e] = c;
+  }
+  cluster.sync();
+  // Block `rank` ends the experts rank, rank + 8, ...
+  float terms = 0.0f;
+  const int mine = rank + kFinishBlocks * threadIdx.x;
+  if (mine < a.experts) {
+    s = 0.0f;
+    c = 0;
+    for (int r = 0; r < kFinishBlocks; ++r) {
+      s += cluster.map_shared_rank(share, r)[mine];
+      c += cluster.map_shared_rank(count, r)[mine];
+    }
+    a.counts[mine] = c;
+    terms = s * float(c);
   }
   const float total = block_total(terms, red);
-  if (threadIdx.x < 32) {
+  if (threadIdx.x == 0) term_sum = total;
+  cluster.sync();
+  if (rank == 0 && threadIdx.x < 32) {
     int n = 0;
     for (int b = threadIdx.x; b < blocks; b += 32) n += a.routed_part[b];
     n = __reduce_add_sync(0xFFFFFFFFu, n);
+    float all = 0.0f;
+    for (int r = 0; r < kFinishBlocks; ++r) all += *cluster.map_shared_rank(&term_sum, r);
     if (threadIdx.x == 0) {
       *a.routed = n;
-      *a.loss = loss_of(total, a.experts, a.k, n);
+      *a.loss = loss_of(all, a.experts, a.k, n);
     }
   }
+  cluster.sync();  // no block leaves while another may still read its sums
 }
 
 struct RouteGradArgs {
@@ -302,38 +400,53 @@ struct RouteGradArgs {
   int vec;
 };
 
+constexpr int kGradThreads = 256;
+constexpr int kGradWarps = kGradThreads / 32;
 template <class T, int L, int NV>
-__global__ void __launch_bounds__(kRouteThreads) route_grad_kernel(const RouteGradArgs a) {
+__global__ void __launch_bounds__(kGradThreads, NV == 1 ? 4 : 2) route_grad_kernel(const RouteGradArgs a) {
   constexpr int kGroups = 32 / L;
   constexpr int kWidth = L * 8 * NV;
-  __shared__ float push[kWidth];                           // a_e
-  __shared__ float spot[kRouteWarps * kGroups][kWidth];    // the chosen experts' own terms, else 0
+  __shared__ float spot[kGradWarps * kGroups][kWidth];  // the chosen experts' own terms, else 0
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % L, group = threadIdx.x % 32 / L;
+  for (int i = threadIdx.x; i < kGradWarps * kGroups * kWidth; i += kGradThreads) (&spot[0][0])[i] = 0.0f;
   griddep_wait();
   griddep_launch_dependents();
-  const int warp = threadIdx.x / 32, lane = threadIdx.x % L, group = threadIdx.x % 32 / L;
   const float n = float(*a.routed > 0 ? *a.routed : 1);
   const float dloss = a.dloss != nullptr ? *a.dloss : 0.0f;
-  for (int e = threadIdx.x; e < kWidth; e += kRouteThreads)
-    push[e] = e < a.experts ? dloss * float(a.experts) * (float(a.counts[e]) / (float(a.k) * n)) / n : 0.0f;
-  for (int i = threadIdx.x; i < kRouteWarps * kGroups * kWidth; i += kRouteThreads) (&spot[0][0])[i] = 0.0f;
+  float push[8 * NV];  // a_e of this lane's experts
+#pragma unroll
+  for (int i = 0; i < 8 * NV; ++i) {
+    const int e = (i / 8 * L + lane) * 8 + i % 8;
+    push[i] = e < a.experts ? dloss * float(a.experts) * (float(a.counts[e]) / (float(a.k) * n)) / n : 0.0f;
+  }
   __syncthreads();
   const T* logits = static_cast<const T*>(a.logits);
   T* out = static_cast<T*>(a.dlogits);
   float* mine = spot[warp * kGroups + group];
-  const int step = gridDim.x * kRouteWarps * kGroups;
-  for (long long first = (long long)(blockIdx.x * kRouteWarps + warp) * kGroups; first < a.tokens; first += step) {
-    const long long t = first + group;
-    const bool live = t < a.tokens && (a.valid == nullptr || a.valid[t] != 0);
+  const long long step = (long long)gridDim.x * kGradWarps * kGroups;
+  auto is_live = [&](long long t) { return t < a.tokens && (a.valid == nullptr || a.valid[t] != 0); };
+  long long t = (long long)(blockIdx.x * kGradWarps + warp) * kGroups + group;
+  Row<T, NV> next;
+  load_row<T, L, NV>(logits + (t < a.tokens ? t : 0) * a.ld, lane, a.experts, a.vec, is_live(t), next);
+  for (; t - group < a.tokens; t += step) {
+    const bool live = is_live(t);
     float v[8 * NV];
-    load_row<T, L, NV>(logits + (t < a.tokens ? t : 0) * a.ld, lane, a.experts, a.vec, live, v);
-    float top = -INFINITY;
+    values<T, NV>(next, v);
+    // What the chosen experts add: lane j has slot j (of more than L slots, also j + L, ...).
+    float pull = 0.0f;
+    if (live && a.dweights != nullptr)
+      for (int j = lane; j < a.k; j += L)
+        if (a.ids[t * a.k + j] >= 0) pull += a.weights[t * a.k + j] * a.dweights[t * a.k + j];
+    if (t - group + step < a.tokens)
+      load_row<T, L, NV>(logits + (t + step < a.tokens ? t + step : 0) * a.ld, lane, a.experts, a.vec, is_live(t + step), next);
+    float top = v[0];
 #pragma unroll
-    for (int i = 0; i < 8 * NV; ++i) top = fmaxf(top, v[i]);
+    for (int i = 1; i < 8 * NV; ++i) top = fmaxf(top, v[i]);
     top = group_max<L>(top);
     float sum = 0.0f;
 #pragma unroll
     for (int i = 0; i < 8 * NV; ++i) {
-      v[i] = v[i] == -INFINITY ? 0.0f : expf(v[i] - top);
+      v[i] = v[i] == -INFINITY ? 0.0f : exp_neg(v[i] - top);
       sum += v[i];
     }
     sum = group_sum<L>(sum);
@@ -343,29 +456,29 @@ __global__ void __launch_bounds__(kRouteThreads) route_grad_kernel(const RouteGr
 #pragma unroll
     for (int i = 0; i < 8 * NV; ++i) {
       v[i] *= inv;
-      level += v[i] * push[(i / 8 * L + lane) * 8 + i % 8];
+      level = fmaf(v[i], push[i], level);
     }
-    level = group_sum<L>(level);
-    float pull = 0.0f;
-    if (live && a.dweights != nullptr)
-      for (int j = lane; j < a.k; j += L)
-        if (a.ids[t * a.k + j] >= 0) pull += a.weights[t * a.k + j] * a.dweights[t * a.k + j];
-    pull = group_sum<L>(pull);
+    float base;
+    if (a.renormalize) {
+      pull = group_sum<L>(pull);
+      base = group_sum<L>(level);
+    } else {
+      base = group_sum<L>(level + pull);
+      pull = 0.0f;
+    }
     if (live && a.dweights != nullptr)
       for (int j = lane; j < a.k; j += L) {
         const int e = a.ids[t * a.k + j];
-        if (e >= 0 && e < a.experts)
-          atomicAdd(&mine[e], a.weights[t * a.k + j] * (a.dweights[t * a.k + j] - (a.renormalize ? pull : 0.0f)));
+        if (e >= 0 && e < a.experts) atomicAdd(&mine[e], a.weights[t * a.k + j] * (a.dweights[t * a.k + j] - pull));
       }
     __syncwarp();
-    const float base = level + (a.renormalize ? 0.0f : pull);
     if (t < a.tokens) {
 #pragma unroll
       for (int i = 0; i < NV; ++i) {
         const int e0 = (i * L + lane) * 8;
         float g[8];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) g[j] = any ? v[8 * i + j] * (push[e0 + j] - base) + mine[e0 + j] : 0.0f;
+        for (int j = 0; j < 8; ++j) g[j] = any ? fmaf(v[8 * i + j], push[8 * i + j] - base, mine[e0 + j]) : 0.0f;
         if (e0 >= a.experts) continue;
         if (a.vec) {
           uint4* p = reinterpret_cast<uint4*>(out + t * a.ldd + e0);
@@ -415,7 +528,7 @@ int lanes_of(int experts) {
 }
 
 // Blocks of the routing kernel: one where its warps take all tokens in a few turns (no second
-// kernel then), else up to two for every SM of a 148-SM B200.
+// kernel then), else up to the two that every SM of a 148-SM B200 holds.
 int route_blocks(int64_t tokens, int experts) {
   const int64_t turn = kRouteWarps * (32 / lanes_of(experts));  // tokens of one block at a time
   if (tokens <= 4 * turn) return 1;
@@ -440,16 +553,25 @@ bool vector_rows(const void* p, int64_t ld, int64_t experts, int32_t type) {
   return aligned16(p) && ld * size % 16 == 0 && experts % 8 == 0;
 }
 
-cudaError_t launch(cudaStream_t stream, int grid, int threads, void const* kernel, void** args) {
+cudaError_t launch(cudaStream_t stream, int grid, int threads, size_t smem, int cluster, void const* kernel, void** args) {
   cudaLaunchConfig_t cfg = {};
-  cudaLaunchAttribute attr[1];
+  cudaLaunchAttribute attr[2];
   cfg.gridDim = dim3(unsigned(grid), 1, 1);
   cfg.blockDim = dim3(unsigned(threads), 1, 1);
+  cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = unsigned(cluster);
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = 1;
+  cfg.numAttrs = cluster > 1 ? 2 : 1;
+  if (smem > 48 * 1024) {
+    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem));
+    if (e != cudaSuccess) return e;
+  }
   return cudaLaunchKernelExC(&cfg, kernel, args);
 }
 
@@ -501,13 +623,14 @@ extern "C" kl_status kl_moe_route(const kl_moe_route_desc* d, void* workspace, s
   by_type(d->logits_type, [&](auto t) {
     by_width(a.experts, [&](auto l, auto nv) {
       void* args[] = {&a};
-      e = launch(st, blocks, kRouteThreads, reinterpret_cast<void const*>(&route_kernel<decltype(t), l(), nv()>), args);
+      e = launch(st, blocks, kRouteThreads, size_t(kRouteWarps) * l() * 8 * nv() * sizeof(float), 1,
+                 reinterpret_cast<void const*>(&route_kernel<decltype(t), l(), nv()>), args);
     });
   });
   if (e == cudaSuccess && blocks > 1) {
     int b = blocks;
     void* args[] = {&a, &b};
-    e = launch(st, 1, 1024, reinterpret_cast<void const*>(&route_finish_kernel), args);
+    e = launch(st, kFinishBlocks, kFinishThreads, 0, kFinishBlocks, reinterpret_cast<void const*>(&route_finish_kernel), args);
   }
   return e == cudaSuccess ? KL_OK : cuda_fail(e, "kl_moe_route launch");
 }
@@ -541,14 +664,14 @@ extern "C" kl_status kl_moe_route_grad(const kl_moe_route_desc* d, const float* 
   a.ldd = ld_dlogits;
   a.vec = vector_rows(d->logits, d->ld_logits, d->experts, d->logits_type) &&
           vector_rows(dlogits, ld_dlogits, d->experts, d->logits_type);
-  const int64_t turn = kRouteWarps * (32 / lanes_of(a.experts));
+  const int64_t turn = kGradWarps * (32 / lanes_of(a.experts));
   const int64_t want = (d->tokens + turn - 1) / turn;
   const int blocks = int(want < 592 ? want : 592);
   cudaError_t e = cudaSuccess;
   by_type(d->logits_type, [&](auto t) {
     by_width(a.experts, [&](auto l, auto nv) {
       void* args[] = {&a};
-      e = launch(static_cast<cudaStream_t>(stream), blocks, kRouteThreads,
+      e = launch(static_cast<cudaStream_t>(stream), blocks, kGradThreads, 0, 1,
                  reinterpret_cast<void const*>(&route_grad_kernel<decltype(t), l(), nv()>), args);
     });
   });
