@@ -96,10 +96,16 @@ __device__ __forceinline__ float group_sum(float v) {
   for (int o = L / 2; o > 0; o /= 2) v += __shfl_xor_sync(0xFFFFFFFFu, v, o);
   return v;
 }
+// The larger, or NaN if either is.
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
 template <int L>
-__device__ __forceinline__ float group_max(float v) {
+__device__ __forceinline__ float group_max_nan(float v) {
 #pragma unroll
-  for (int o = L / 2; o > 0; o /= 2) v = fmaxf(v, __shfl_xor_sync(0xFFFFFFFFu, v, o));
+  for (int o = L / 2; o > 0; o /= 2) v = max_nan(v, __shfl_xor_sync(0xFFFFFFFFu, v, o));
   return v;
 }
 template <int L, class K>
@@ -147,14 +153,12 @@ __device__ __forceinline__ void values(Row<T, NV> const& r, float (&v)[8 * NV]) 
   for (int i = 0; i < NV * 8 / kPerVec<T>; ++i) unpack<T>(r.u[i], v + i * kPerVec<T>);
 }
 
-// exp(x) for x <= 0: 2^(x log2 e) with the product's rounding made up for, so that the relative error
-// stays at a few 2^-24 for far values too.
+// exp(x) for x <= 0 as one product and one ex2: off by |x| + 4 times 2^-24, relative. A row's large
+// probabilities have small |x|.
 __device__ __forceinline__ float exp_neg(float x) {
-  const float hi = x * 1.44269502f;                                    // log2 e, rounded to fp32
-  const float lo = fmaf(x, 1.44269502f, -hi) + x * 1.92596303e-8f;     // and what that left out
   float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(hi));
-  return x < -104.0f ? 0.0f : fmaf(y * 0.693147182f, lo, y);
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x * 1.44269504f));
+  return y;
 }
 
 struct RouteArgs {
@@ -191,14 +195,15 @@ __device__ __forceinline__ float loss_of(float total, int experts, int k, int ro
   return routed > 0 ? float(experts) * (total / (float(k) * float(routed))) / float(routed) : 0.0f;
 }
 
-template <class T, int L, int NV>
+// KMAX: the most rounds; the lists shrink as the rounds left do.
+template <class T, int L, int NV, int KMAX>
 __global__ void __launch_bounds__(kRouteThreads, NV == 1 ? 2 : 1) route_kernel(const RouteArgs a) {
   using Key = RouteKey<T>;
   using K = typename Key::type;
   constexpr int kGroups = 32 / L;  // tokens of a warp
   constexpr int kWidth = L * 8 * NV;
-  constexpr int kPicks = L * 8 < kMaxTopK ? L * 8 : kMaxTopK;  // k is at most the number of experts
-  constexpr int kHeld = kPicks / L > 0 ? kPicks / L : 1;       // picks of a lane: j = h L + lane
+  constexpr int kPicks = L * 8 < KMAX ? L * 8 : KMAX;  // k is at most the number of experts
+  constexpr int kHeld = (kPicks + L - 1) / L;          // picks of a lane: j = h L + lane
   extern __shared__ float share[];                             // [kRouteWarps][kWidth]
   __shared__ int count[kWidth];
   __shared__ float red[32];
@@ -235,20 +240,23 @@ __global__ void __launch_bounds__(kRouteThreads, NV == 1 ? 2 : 1) route_kernel(c
     // The k largest keys, one after another: the largest head of all lanes, taken off its list.
     K pick[kHeld] = {};
     K first = 0;
-    for (int j = 0; j < a.k; ++j) {
+#pragma unroll
+    for (int j = 0; j < kPicks; ++j) {
+      if (j >= a.k) break;
       K best = key[0][0];
 #pragma unroll
       for (int i = 1; i < NV; ++i) best = key[i][0] > best ? key[i][0] : best;
       best = group_key_max<L>(best);
 #pragma unroll
       for (int i = 0; i < NV; ++i) {
-        const bool here = key[i][0] == best;
+        if (key[i][0] == best) {
 #pragma unroll
-        for (int x = 0; x < 7; ++x) key[i][x] = here ? key[i][x + 1] : key[i][x];
-        key[i][7] = here ? K(0) : key[i][7];
+          for (int x = 0; x < 7; ++x)
+            if (x < kPicks - 1 - j) key[i][x] = key[i][x + 1];
+          if (7 < kPicks - 1 - j) key[i][7] = K(0);
+        }
       }
-#pragma unroll
-      for (int h = 0; h < kHeld; ++h) pick[h] = j == h * L + lane ? best : pick[h];
+      if (lane == j % L) pick[j / L] = best;
       if (j == 0) first = best;
     }
     const bool any = first > Key::kClosed;
@@ -260,8 +268,8 @@ __global__ void __launch_bounds__(kRouteThreads, NV == 1 ? 2 : 1) route_kernel(c
       sum += v[i];
     }
     sum = group_sum<L>(sum);
+    float inv = 1.0f / sum;
     if (any) {
-      const float inv = 1.0f / sum;
 #pragma unroll
       for (int i = 0; i < 8 * NV; ++i) acc[i] = fmaf(v[i], inv, acc[i]);
       routed += lane == 0;
@@ -272,7 +280,7 @@ __global__ void __launch_bounds__(kRouteThreads, NV == 1 ? 2 : 1) route_kernel(c
       w[h] = h * L + lane < a.k && pick[h] > Key::kClosed ? exp_neg(Key::value(pick[h]) - top) : 0.0f;
       part += w[h];
     }
-    if (a.renormalize) sum = group_sum<L>(part);
+    if (a.renormalize) inv = 1.0f / group_sum<L>(part);
     if (t < a.tokens) {
 #pragma unroll
       for (int h = 0; h < kHeld; ++h) {
@@ -281,7 +289,7 @@ __global__ void __launch_bounds__(kRouteThreads, NV == 1 ? 2 : 1) route_kernel(c
         const bool open = pick[h] > Key::kClosed;
         const int e = open ? key_expert(pick[h]) : -1;
         a.ids[t * a.k + j] = e;
-        a.weights[t * a.k + j] = open ? w[h] / sum : 0.0f;
+        a.weights[t * a.k + j] = open ? w[h] * inv : 0.0f;
         if (open) atomicAdd(&count[e], 1);
       }
     }
@@ -403,7 +411,7 @@ struct RouteGradArgs {
 constexpr int kGradThreads = 256;
 constexpr int kGradWarps = kGradThreads / 32;
 template <class T, int L, int NV>
-__global__ void __launch_bounds__(kGradThreads, NV == 1 ? 4 : 2) route_grad_kernel(const RouteGradArgs a) {
+__global__ void __launch_bounds__(kGradThreads, NV == 1 && L >= 8 ? 4 : 2) route_grad_kernel(const RouteGradArgs a) {
   constexpr int kGroups = 32 / L;
   constexpr int kWidth = L * 8 * NV;
   __shared__ float spot[kGradWarps * kGroups][kWidth];  // the chosen experts' own terms, else 0
@@ -425,33 +433,53 @@ __global__ void __launch_bounds__(kGradThreads, NV == 1 ? 4 : 2) route_grad_kern
   float* mine = spot[warp * kGroups + group];
   const long long step = (long long)gridDim.x * kGradWarps * kGroups;
   auto is_live = [&](long long t) { return t < a.tokens && (a.valid == nullptr || a.valid[t] != 0); };
-  long long t = (long long)(blockIdx.x * kGradWarps + warp) * kGroups + group;
+  // Lane j of a token has slot j (of more than L slots, also j + L, ...).
+  constexpr int kHeld = ((L * 8 < kMaxTopK ? L * 8 : kMaxTopK) + L - 1) / L;
+  struct Slot {
+    int e;  // -1: nothing to add
+    float w, dw;
+  };
+  Slot slots[kHeld];
   Row<T, NV> next;
-  load_row<T, L, NV>(logits + (t < a.tokens ? t : 0) * a.ld, lane, a.experts, a.vec, is_live(t), next);
-  for (; t - group < a.tokens; t += step) {
+  auto load = [&](long long t) {
     const bool live = is_live(t);
+    load_row<T, L, NV>(logits + (t < a.tokens ? t : 0) * a.ld, lane, a.experts, a.vec, live, next);
+#pragma unroll
+    for (int h = 0; h < kHeld; ++h) {
+      const int j = h * L + lane;
+      slots[h] = {-1, 0.0f, 0.0f};
+      if (live && a.dweights != nullptr && j < a.k) slots[h] = {a.ids[t * a.k + j], a.weights[t * a.k + j], a.dweights[t * a.k + j]};
+    }
+  };
+  long long t = (long long)(blockIdx.x * kGradWarps + warp) * kGroups + group;
+  load(t);
+  for (; t - group < a.tokens; t += step) {
     float v[8 * NV];
     values<T, NV>(next, v);
-    // What the chosen experts add: lane j has slot j (of more than L slots, also j + L, ...).
-    float pull = 0.0f;
-    if (live && a.dweights != nullptr)
-      for (int j = lane; j < a.k; j += L)
-        if (a.ids[t * a.k + j] >= 0) pull += a.weights[t * a.k + j] * a.dweights[t * a.k + j];
-    if (t - group + step < a.tokens)
-      load_row<T, L, NV>(logits + (t + step < a.tokens ? t + step : 0) * a.ld, lane, a.experts, a.vec, is_live(t + step), next);
+    int e_of[kHeld];
+    float pull_of[kHeld], w_of[kHeld], pull = 0.0f;
+#pragma unroll
+    for (int h = 0; h < kHeld; ++h) {
+      e_of[h] = slots[h].e < a.experts ? slots[h].e : -1;
+      w_of[h] = slots[h].w;
+      pull_of[h] = e_of[h] >= 0 ? slots[h].w * slots[h].dw : 0.0f;
+      pull += pull_of[h];
+    }
+    if (t - group + step < a.tokens) load(t + step);
     float top = v[0];
 #pragma unroll
-    for (int i = 1; i < 8 * NV; ++i) top = fmaxf(top, v[i]);
-    top = group_max<L>(top);
+    for (int i = 1; i < 8 * NV; ++i) top = max_nan(top, v[i]);
+    top = group_max_nan<L>(top);
     float sum = 0.0f;
 #pragma unroll
     for (int i = 0; i < 8 * NV; ++i) {
-      v[i] = v[i] == -INFINITY ? 0.0f : exp_neg(v[i] - top);
+      v[i] = exp_neg(v[i] - top);
       sum += v[i];
     }
     sum = group_sum<L>(sum);
-    const bool any = sum != 0.0f;  // else the row is not routed: zeros, whatever dloss and dweights hold
-    const float inv = any ? 1.0f / sum : 0.0f;
+    // A row of -inf alone is not routed: zeros, whatever dloss and dweights hold.
+    const bool any = top != -INFINITY;
+    const float inv = 1.0f / sum;
     float level = 0.0f;
 #pragma unroll
     for (int i = 0; i < 8 * NV; ++i) {
@@ -466,11 +494,9 @@ __global__ void __launch_bounds__(kGradThreads, NV == 1 ? 4 : 2) route_grad_kern
       base = group_sum<L>(level + pull);
       pull = 0.0f;
     }
-    if (live && a.dweights != nullptr)
-      for (int j = lane; j < a.k; j += L) {
-        const int e = a.ids[t * a.k + j];
-        if (e >= 0 && e < a.experts) atomicAdd(&mine[e], a.weights[t * a.k + j] * (a.dweights[t * a.k + j] - pull));
-      }
+#pragma unroll
+    for (int h = 0; h < kHeld; ++h)
+      if (e_of[h] >= 0) mine[e_of[h]] = fmaf(-w_of[h], pull, pull_of[h]);
     __syncwarp();
     if (t < a.tokens) {
 #pragma unroll
@@ -492,11 +518,9 @@ __global__ void __launch_bounds__(kGradThreads, NV == 1 ? 4 : 2) route_grad_kern
       }
     }
     __syncwarp();
-    if (live && a.dweights != nullptr)
-      for (int j = lane; j < a.k; j += L) {
-        const int e = a.ids[t * a.k + j];
-        if (e >= 0 && e < a.experts) mine[e] = 0.0f;
-      }
+#pragma unroll
+    for (int h = 0; h < kHeld; ++h)
+      if (e_of[h] >= 0) mine[e_of[h]] = 0.0f;
     __syncwarp();
   }
 }
@@ -623,8 +647,10 @@ extern "C" kl_status kl_moe_route(const kl_moe_route_desc* d, void* workspace, s
   by_type(d->logits_type, [&](auto t) {
     by_width(a.experts, [&](auto l, auto nv) {
       void* args[] = {&a};
-      e = launch(st, blocks, kRouteThreads, size_t(kRouteWarps) * l() * 8 * nv() * sizeof(float), 1,
-                 reinterpret_cast<void const*>(&route_kernel<decltype(t), l(), nv()>), args);
+      using T = decltype(t);
+      void const* kernel = a.k <= 8 ? reinterpret_cast<void const*>(&route_kernel<T, l(), nv(), 8>)
+                                    : reinterpret_cast<void const*>(&route_kernel<T, l(), nv(), kMaxTopK>);
+      e = launch(st, blocks, kRouteThreads, size_t(kRouteWarps) * l() * 8 * nv() * sizeof(float), 1, kernel, args);
     });
   });
   if (e == cudaSuccess && blocks > 1) {
