@@ -10,7 +10,7 @@
 // Both kernels read a row once and keep it in registers, 8 experts to a lane. What bounds them is not
 // the memory but the instructions: at 256 bf16 logits a token, HBM would allow about 100 a token. So a lane sorts its
 // eight keys once (19 exchanges), after which each of the k rounds takes one warp-wide maximum and a shift in the lane that
-// held it.
+// held it (two sorted keys a lane would do for four tokens of ten: measured slower).
 
 #include <cooperative_groups.h>
 #include <cuda_runtime.h>
@@ -230,6 +230,9 @@ __global__ void __launch_bounds__(kRouteThreads, NV == 1 ? 2 : 1) route_kernel(c
     values<T, NV>(next, v);
     if (t - group + step < a.tokens)
       load_row<T, L, NV>(logits + (t + step < a.tokens ? t + step : 0) * a.ld, lane, a.experts, a.vec, is_live(t + step), next);
+    // The k largest keys, one after another: the largest head of all lanes, taken off its lane's list.
+    K pick[kHeld] = {};
+    K first = 0;
     K key[NV][8];
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
@@ -237,9 +240,6 @@ __global__ void __launch_bounds__(kRouteThreads, NV == 1 ? 2 : 1) route_kernel(c
       for (int j = 0; j < 8; ++j) key[i][j] = Key::make(ordered_bits(v[8 * i + j]), (i * L + lane) * 8 + j);
       sort8(key[i]);
     }
-    // The k largest keys, one after another: the largest head of all lanes, taken off its list.
-    K pick[kHeld] = {};
-    K first = 0;
 #pragma unroll
     for (int j = 0; j < kPicks; ++j) {
       if (j >= a.k) break;
@@ -414,9 +414,11 @@ template <class T, int L, int NV>
 __global__ void __launch_bounds__(kGradThreads, NV == 1 && L >= 8 ? 4 : 2) route_grad_kernel(const RouteGradArgs a) {
   constexpr int kGroups = 32 / L;
   constexpr int kWidth = L * 8 * NV;
-  __shared__ float spot[kGradWarps * kGroups][kWidth];  // the chosen experts' own terms, else 0
+  // The chosen experts' own terms, else 0. A lane's eight lie in two vectors, each beside its neighbours' own.
+  __shared__ float4 spot[kGradWarps * kGroups][kWidth / 4];
+  auto place = [](int e) { return ((e / (8 * L) * 2 + e % 8 / 4) * L + e / 8 % L) * 4 + e % 4; };
   const int warp = threadIdx.x / 32, lane = threadIdx.x % L, group = threadIdx.x % 32 / L;
-  for (int i = threadIdx.x; i < kGradWarps * kGroups * kWidth; i += kGradThreads) (&spot[0][0])[i] = 0.0f;
+  for (int i = threadIdx.x; i < kGradWarps * kGroups * kWidth; i += kGradThreads) reinterpret_cast<float*>(spot)[i] = 0.0f;
   griddep_wait();
   griddep_launch_dependents();
   const float n = float(*a.routed > 0 ? *a.routed : 1);
@@ -430,7 +432,8 @@ __global__ void __launch_bounds__(kGradThreads, NV == 1 && L >= 8 ? 4 : 2) route
   __syncthreads();
   const T* logits = static_cast<const T*>(a.logits);
   T* out = static_cast<T*>(a.dlogits);
-  float* mine = spot[warp * kGroups + group];
+  float4* mine = spot[warp * kGroups + group];
+  float* mine_at = reinterpret_cast<float*>(mine);
   const long long step = (long long)gridDim.x * kGradWarps * kGroups;
   auto is_live = [&](long long t) { return t < a.tokens && (a.valid == nullptr || a.valid[t] != 0); };
   // Lane j of a token has slot j (of more than L slots, also j + L, ...).
@@ -496,15 +499,16 @@ __global__ void __launch_bounds__(kGradThreads, NV == 1 && L >= 8 ? 4 : 2) route
     }
 #pragma unroll
     for (int h = 0; h < kHeld; ++h)
-      if (e_of[h] >= 0) mine[e_of[h]] = fmaf(-w_of[h], pull, pull_of[h]);
+      if (e_of[h] >= 0) mine_at[place(e_of[h])] = fmaf(-w_of[h], pull, pull_of[h]);
     __syncwarp();
     if (t < a.tokens) {
 #pragma unroll
       for (int i = 0; i < NV; ++i) {
         const int e0 = (i * L + lane) * 8;
-        float g[8];
+        const float4 s0 = mine[i * 2 * L + lane], s1 = mine[(i * 2 + 1) * L + lane];
+        float g[8] = {s0.x, s0.y, s0.z, s0.w, s1.x, s1.y, s1.z, s1.w};
 #pragma unroll
-        for (int j = 0; j < 8; ++j) g[j] = any ? fmaf(v[8 * i + j], push[8 * i + j] - base, mine[e0 + j]) : 0.0f;
+        for (int j = 0; j < 8; ++j) g[j] = any ? fmaf(v[8 * i + j], push[8 * i + j] - base, g[j]) : 0.0f;
         if (e0 >= a.experts) continue;
         if (a.vec) {
           uint4* p = reinterpret_cast<uint4*>(out + t * a.ldd + e0);
@@ -520,7 +524,7 @@ __global__ void __launch_bounds__(kGradThreads, NV == 1 && L >= 8 ? 4 : 2) route
     __syncwarp();
 #pragma unroll
     for (int h = 0; h < kHeld; ++h)
-      if (e_of[h] >= 0) mine[e_of[h]] = 0.0f;
+      if (e_of[h] >= 0) mine_at[place(e_of[h])] = 0.0f;
     __syncwarp();
   }
 }
