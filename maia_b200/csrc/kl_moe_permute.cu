@@ -154,16 +154,15 @@ struct RowArgs {
   long long width;      // vectors of a row (bytes / sizeof(V)), or elements
 };
 
-// Rows of the layout that hold no slot become zeros: blocks [0, pad_blocks) of the pad part take 32
-// rows each.
+// Rows of the layout that hold no slot become zeros: each part takes 32 rows, whose slots a warp looks up
+// at once.
 constexpr int kPadRows = 32;
 template <class V>
 __device__ __forceinline__ void zero_padding(const RowArgs& a, long long part) {
-  for (int i = 0; i < kPadRows; ++i) {
-    const long long r = part * kPadRows + i;
-    if (r >= a.m) return;
-    if (a.slots[r] >= 0) continue;
-    V* dst = reinterpret_cast<V*>(static_cast<char*>(a.dst) + r * a.ld_dst);
+  const long long r0 = part * kPadRows, r = r0 + threadIdx.x % 32;
+  unsigned empty = __ballot_sync(0xFFFFFFFFu, r < a.m && a.slots[r] < 0);
+  for (; empty != 0; empty &= empty - 1) {
+    V* dst = reinterpret_cast<V*>(static_cast<char*>(a.dst) + (r0 + __ffs(empty) - 1) * a.ld_dst);
     for (long long c = threadIdx.x; c < a.width; c += kRowThreads) dst[c] = V{};
   }
 }
@@ -175,13 +174,21 @@ __global__ void __launch_bounds__(kRowThreads) dispatch_kernel(const RowArgs a) 
   griddep_wait();
   griddep_launch_dependents();
   if (blockIdx.x >= a.tokens) return zero_padding<V>(a, blockIdx.x - a.tokens);
+  __shared__ int row[kMaxTopK];
   const long long t = blockIdx.x;
   const V* src = reinterpret_cast<const V*>(static_cast<const char*>(a.src) + t * a.ld_src);
-  for (long long c = threadIdx.x; c < a.width; c += kRowThreads) {
-    const V v = src[c];
+  if (threadIdx.x < a.k) row[threadIdx.x] = a.rows[t * a.k + threadIdx.x];
+  __syncthreads();
+  // Two vectors at a time, so that a row of 8 KB is one turn of the block.
+  for (long long c = threadIdx.x; c < a.width; c += 2 * kRowThreads) {
+    const bool more = c + kRowThreads < a.width;
+    const V v0 = src[c], v1 = more ? src[c + kRowThreads] : V{};
     for (int j = 0; j < a.k; ++j) {
-      const int r = a.rows[t * a.k + j];
-      if (r >= 0 && r < a.m) reinterpret_cast<V*>(static_cast<char*>(a.dst) + r * a.ld_dst)[c] = v;
+      const long long r = row[j];
+      if (r < 0 || r >= a.m) continue;
+      V* dst = reinterpret_cast<V*>(static_cast<char*>(a.dst) + r * a.ld_dst);
+      dst[c] = v0;
+      if (more) dst[c + kRowThreads] = v1;
     }
   }
 }
@@ -229,40 +236,57 @@ __global__ void __launch_bounds__(kRowThreads) combine_kernel(const RowArgs a) {
   C::put(reinterpret_cast<V*>(static_cast<char*>(a.dst) + t * a.ld_dst) + c, sum);
 }
 
-// dy and dw of one token: its dout is read once for kAtOnce slots at a time, each slot's y once.
-constexpr int kAtOnce = 8;
+// dy and dw of one token: its dout is read once for kAtOnce slots at a time, each slot's y once. The slots' rows
+// are looked up before the loop, and a turn's loads go out together.
+constexpr int kAtOnce = 4;
 template <class T, bool Vec>
 __global__ void __launch_bounds__(kRowThreads) combine_grad_kernel(const RowArgs a) {
   using C = Cells<T, Vec>;
   using V = typename C::type;
   __shared__ float red[kAtOnce][kRowThreads / 32];
+  __shared__ long long row[kMaxTopK];
+  __shared__ float weight[kMaxTopK];
+  __shared__ bool writes[kMaxTopK];
   griddep_wait();
   griddep_launch_dependents();
   if (blockIdx.x >= a.tokens) return zero_padding<V>(a, blockIdx.x - a.tokens);
   const long long t = blockIdx.x;
+  if (threadIdx.x < a.k) {
+    const long long s = t * a.k + threadIdx.x, r = row_of(a, s);
+    row[threadIdx.x] = r;
+    weight[threadIdx.x] = a.weights != nullptr ? a.weights[s] : 1.0f;
+    // A row's gradient is written by its own slot alone.
+    writes[threadIdx.x] = r >= 0 && (a.slots == nullptr || a.slots[r] == s);
+  }
+  __syncthreads();
   const V* dout = reinterpret_cast<const V*>(static_cast<const char*>(a.dout) + t * a.ld_dout);
   for (int j0 = 0; j0 < a.k; j0 += kAtOnce) {
     float dot[kAtOnce] = {};
     for (long long c = threadIdx.x; c < a.width; c += kRowThreads) {
-      float g[C::n];
-      C::get(dout + c, g);
+      V y[kAtOnce];
+      const V d = dout[c];
 #pragma unroll
       for (int i = 0; i < kAtOnce; ++i) {
-        if (j0 + i >= a.k) break;
-        const long long s = t * a.k + j0 + i, r = row_of(a, s);
-        if (r < 0) continue;
-        float y[C::n];
-        if (a.dweights != nullptr) {
-          C::get(reinterpret_cast<const V*>(static_cast<const char*>(a.src) + r * a.ld_src) + c, y);
+        y[i] = V{};
+        if (a.dweights != nullptr && j0 + i < a.k && row[j0 + i] >= 0)
+          y[i] = reinterpret_cast<const V*>(static_cast<const char*>(a.src) + row[j0 + i] * a.ld_src)[c];
+      }
+      float g[C::n];
+      C::get(&d, g);
 #pragma unroll
-          for (int x = 0; x < C::n; ++x) dot[i] += g[x] * y[x];
-        }
-        if (a.slots == nullptr || a.slots[r] == s) {  // a row's gradient is written by its own slot alone
-          const float w = a.weights != nullptr ? a.weights[s] : 1.0f;
+      for (int i = 0; i < kAtOnce; ++i) {
+        if (j0 + i >= a.k || row[j0 + i] < 0) continue;
+        float v[C::n];
+        C::get(&y[i], v);
 #pragma unroll
-          for (int x = 0; x < C::n; ++x) y[x] = w * g[x];
-          C::put(reinterpret_cast<V*>(static_cast<char*>(a.dst) + r * a.ld_dst) + c, y);
-        }
+        for (int x = 0; x < C::n; ++x) dot[i] += g[x] * v[x];
+        if (!writes[j0 + i]) continue;
+        const float w = weight[j0 + i];
+#pragma unroll
+        for (int x = 0; x < C::n; ++x) v[x] = w * g[x];
+        V o;
+        C::put(&o, v);
+        reinterpret_cast<V*>(static_cast<char*>(a.dst) + row[j0 + i] * a.ld_dst)[c] = o;
       }
     }
     if (a.dweights == nullptr) continue;
