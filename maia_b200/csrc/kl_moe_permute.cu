@@ -23,6 +23,7 @@ constexpr int kMaxExperts = 1024;
 constexpr int kMaxTopK = 32;
 constexpr int kPlanThreads = 1024;
 constexpr int kPlanWarps = kPlanThreads / 32;
+constexpr int kPlanBlocks = 8;  // of the cluster, where one does not do
 
 struct PlanArgs {
   const int* ids;
@@ -65,7 +66,7 @@ __device__ __forceinline__ int block_scan(int v, int* red) {
 // one expert keep their order, and nothing depends on the timing of atomics.
 __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const PlanArgs a) {
   extern __shared__ int hist[];  // [kPlanWarps][experts]
-  __shared__ int block_count[kMaxExperts];
+  __shared__ int block_count[kMaxExperts], starts[kMaxExperts], counts[kMaxExperts];
   __shared__ int red[32];
   cg::cluster_group cluster = cg::this_cluster();
   griddep_wait();
@@ -81,49 +82,67 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const PlanArgs a) {
     const int e = s < end ? a.ids[s] : -1;
     return e >= 0 && e < a.experts ? e : -1;
   };
-  for (long long s = begin; s < end; s += 32) {
-    const int e = expert_at(s + lane);
+  // The first kKept turns' ids stay in registers for the second walk; they load together.
+  constexpr int kKept = 8;
+  int kept[kKept];
+#pragma unroll
+  for (int i = 0; i < kKept; ++i) kept[i] = expert_at(begin + i * 32 + lane);
+  auto count = [&](int e) {
     const unsigned same = __match_any_sync(0xFFFFFFFFu, e);
     if (e >= 0 && lane == __ffs(same) - 1) mine[e] += __popc(same);
     __syncwarp();
-  }
+  };
+#pragma unroll
+  for (int i = 0; i < kKept; ++i)
+    if (begin + i * 32 < end) count(kept[i]);
+  for (long long s = begin + kKept * 32; s < end; s += 32) count(expert_at(s + lane));
   __syncthreads();
   const int e = threadIdx.x;
   if (e < a.experts) {
-    int run = 0;
+    int run = 0, c[kPlanWarps];
+#pragma unroll
+    for (int w = 0; w < kPlanWarps; ++w) c[w] = hist[w * a.experts + e];
+#pragma unroll
     for (int w = 0; w < kPlanWarps; ++w) {
-      const int c = hist[w * a.experts + e];
       hist[w * a.experts + e] = run;
-      run += c;
+      run += c[w];
     }
     block_count[e] = run;
   }
   cluster.sync();
   int before = 0, all = 0;
-  if (e < a.experts)
-    for (int r = 0; r < ranks; ++r) {
-      const int c = cluster.map_shared_rank(block_count, r)[e];
-      before += r < rank ? c : 0;
-      all += c;
+  if (e < a.experts) {
+    int c[kPlanBlocks];
+#pragma unroll
+    for (int r = 0; r < kPlanBlocks; ++r) c[r] = r < ranks ? cluster.map_shared_rank(block_count, r)[e] : 0;
+#pragma unroll
+    for (int r = 0; r < kPlanBlocks; ++r) {
+      before += r < rank ? c[r] : 0;
+      all += c[r];
     }
+  }
   const int room = (all + a.block - 1) / a.block * a.block;
   const int stop = block_scan(room, red);
   const int start = stop - room;
   if (e < a.experts)
     for (int w = 0; w < kPlanWarps; ++w) hist[w * a.experts + e] += start + before;
-  // The padding behind each expert's rows, its blocks, and the blocks that nobody has.
-  if (e < a.experts && e % ranks == rank) {
-    for (int r = start + all; r < stop; ++r) a.slots[r] = -1;
-    for (int b = start / 128; b < stop / 128; ++b) a.blocks[b] = e;
+  // The padding behind each expert's rows, its blocks (a warp an expert), and the blocks that nobody has.
+  if (e < a.experts) {
+    starts[e] = start;
+    counts[e] = all;
   }
   __syncthreads();
+  for (int x = rank * kPlanWarps + warp; x < a.experts; x += ranks * kPlanWarps) {
+    const int s0 = starts[x], n = counts[x], s1 = s0 + (n + a.block - 1) / a.block * a.block;
+    for (int r = s0 + n + lane; r < s1; r += 32) a.slots[r] = -1;
+    for (int b = s0 / 128 + lane; b < s1 / 128; b += 32) a.blocks[b] = x;
+  }
   const long long used = red[31];
   for (long long r = used + rank * kPlanThreads + threadIdx.x; r < a.m; r += ranks * kPlanThreads) {
     a.slots[r] = -1;
     if (r % 128 == 0) a.blocks[r / 128] = -1;
   }
-  for (long long s = begin; s < end; s += 32) {
-    const int x = expert_at(s + lane);
+  auto hand_out = [&](long long s, int x) {
     const unsigned same = __match_any_sync(0xFFFFFFFFu, x);
     int row = -1;
     if (x >= 0) row = mine[x] + __popc(same & ((1u << lane) - 1));
@@ -132,7 +151,11 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const PlanArgs a) {
     __syncwarp();
     if (s + lane < end) a.rows[s + lane] = row;
     if (row >= 0) a.slots[row] = int(s + lane);
-  }
+  };
+#pragma unroll
+  for (int i = 0; i < kKept; ++i)
+    if (begin + i * 32 < end) hand_out(begin + i * 32, kept[i]);
+  for (long long s = begin + kKept * 32; s < end; s += 32) hand_out(s, expert_at(s + lane));
   cluster.sync();  // no block leaves while another may still read its counts
 }
 
@@ -372,7 +395,7 @@ extern "C" kl_status kl_moe_plan(const int32_t* ids, int64_t tokens, int64_t k, 
   a.slots = slots;
   a.blocks = m_block_group;
   // One block while it has at most four turns of 32 slots for each warp.
-  const int cluster = a.total <= 4 * 32 * kPlanWarps ? 1 : 8;
+  const int cluster = a.total <= 4 * 32 * kPlanWarps ? 1 : kPlanBlocks;
   const long long warps = (long long)cluster * kPlanWarps;
   a.warp_span = (a.total + warps * 32 - 1) / (warps * 32) * 32;
   const size_t smem = size_t(kPlanWarps) * size_t(experts) * sizeof(int);
