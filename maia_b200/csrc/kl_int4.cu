@@ -70,7 +70,7 @@ struct Int4Args {
   int f32_scales, f32_out;
   int tiles;  // 16-row tiles of one matrix
   int depth;  // slots of a warp's ring
-  uint32_t digits, sums, powers, pieces, block, units, bars, lists;  // offsets in shared memory
+  uint32_t digits, sums, powers, pieces, block, records, bars, lists;  // offsets in shared memory
   int group_span, last_group;                           // 128-element runs of a group (groups of 128 and more); index of the last
   int* status;
   unsigned long long timeout_ns;
@@ -199,18 +199,17 @@ constexpr int kPieces = 2;  // tiles that a warp's run of units can touch
 template <int TOK>
 constexpr int kPiece = TOK * kRows;  // floats of a tile's sums
 
-// What a ring slot holds, and what its warp does around it.
-struct __align__(16) Unit {
-  int row0, kb, expert, flags;
-  int batch_row0, count, pass, unused;
+// A stretch: a warp's share of one tile, consecutive units of K. Its record lies with the ring slot of its first
+// unit.
+struct __align__(16) Stretch {
+  int row0, kb, units, flags;  // kb: of this block's K
+  int batch_row0, count, pass, expert;
 };
-constexpr int kFirst = 1;   // first unit of a stretch (the warp's share of a tile)
-constexpr int kLast = 2;    // last of it
-constexpr int kEnd = 4;     // last of the warp's run in the batch
-constexpr int kSecond = 8;  // the stretch is the run's second
-constexpr int kNone = 16;   // no unit: the warp has none in this batch
+constexpr int kEnd = 1;     // the last of the warp's run in the batch
+constexpr int kSecond = 2;  // the run's second
+constexpr int kNone = 4;    // the warp has no unit in this batch: a slot without loads
 
-// Shared memory, in order: rings, x's digits, sums and powers, pieces, the block's sums, unit records, barriers,
+// Shared memory, in order: rings, x's digits, sums and powers, pieces, the block's sums, stretch records, barriers,
 // lists.
 template <int NG, int TOK>
 size_t lay_out(Int4Args& a, int depth, int units, int cluster) {
@@ -225,14 +224,14 @@ size_t lay_out(Int4Args& a, int depth, int units, int cluster) {
   take(a.powers, size_t(units) * 4 * kPowerBytes<TOK>);
   take(a.pieces, size_t(kWarps) * kPieces * kPiece<TOK> * 4);
   take(a.block, cluster > 1 ? size_t(2) * kWarps * kPiece<TOK> * 4 : 0);
-  take(a.units, size_t(kWarps) * depth * sizeof(Unit));
+  take(a.records, size_t(kWarps) * depth * sizeof(Stretch));
   take(a.bars, size_t(kWarps) * depth * 8);
   take(a.lists, a.ids != nullptr ? Lists::bytes(a.experts, a.slots) : 0);
   return at + 1024;  // the base is rounded up to 1024
 }
 
 // NG: scale groups of a unit's 512 codes (16, 8, 4 for groups of 32, 64, multiples of 128).
-template <class T, int NG, int TOK>
+template <class T, int NG, int TOK, bool kZeros>
 __global__ void __launch_bounds__(kThreads, 1) gemv_int4_kernel(const __grid_constant__ Int4Args a) {
   constexpr int kPerGroup = 16 / NG;  // 32-code chunks of a group
   constexpr int kHeld = NG / 4;       // scales that a lane holds of each of its rows
@@ -245,7 +244,7 @@ __global__ void __launch_bounds__(kThreads, 1) gemv_int4_kernel(const __grid_con
   const int depth = a.depth;
   const uint32_t bar0 = smem_addr(smem + a.bars) + warp * depth * 8;
   const uint32_t ring0 = smem_addr(smem) + warp * depth * kUnitBytes;
-  Unit* units = reinterpret_cast<Unit*>(smem + a.units) + warp * depth;
+  Stretch* records = reinterpret_cast<Stretch*>(smem + a.records) + warp * depth;
   float* pieces = reinterpret_cast<float*>(smem + a.pieces);
   if (lane == 0) {
     for (int i = 0; i < depth; ++i) mbarrier_init(bar0 + 8 * i, 1);
@@ -303,15 +302,21 @@ __global__ void __launch_bounds__(kThreads, 1) gemv_int4_kernel(const __grid_con
   const uint32_t clusters = gridDim.x / splits, c0 = blockIdx.x / splits, all = uint32_t(passes) * a.tiles;
   const uint32_t share = all / clusters, extra = all % clusters, begin0 = c0 * share + min(c0, extra);
   int remaining = int(share + (c0 < extra)), pass = int(begin0 / a.tiles), first = int(begin0 - pass * a.tiles);
-  int count = 0, run_left = 0, tile = 0, kb = 0, expert = -1, mark = 0;
+  int count = 0, run_left = 0, tile = 0, kb = 0, expert = -1, left = 0;  // run_left: units of the run behind the stretch
+  int load_x = 0, load_y = 0;
   bool failed = false;
 
-  // Puts the warp's next unit into ring slot `at`: its record, and its loads.
+  // Begins the warp's next stretch in ring slot `at`.
   const int scale_bytes = a.f32_scales ? 4 : 2;
-  auto produce = [&](int at) {
-    Unit u;
-    u.flags = mark;
-    if (run_left == 0) {  // the next batch
+  auto begin_stretch = [&](int at) {
+    Stretch s;
+    s.flags = 0;
+    if (run_left > 0) {
+      kb = 0;
+      ++tile;
+      left = run_left;
+      s.flags = kSecond;
+    } else {  // the next batch
       first += count;
       remaining -= count;
       const bool turn = first == a.tiles;
@@ -335,49 +340,54 @@ __global__ void __launch_bounds__(kThreads, 1) gemv_int4_kernel(const __grid_con
       run_left = count * kbs * (warp + 1) / kWarps - begin;
       tile = count * warp / kWarps;
       kb = begin - tile * kbs;
-      u.flags = run_left == 0 ? kNone | kEnd : kFirst;
+      left = min(run_left, kbs - kb);
       if (run_left > 0) {  // likewise the scales and zero points, a row of two tiles to a lane
         const int row = min((first + tile) * kRows + lane, a.n - 1), g0 = kb0 * NG / a.group_span;
         const int groups = min((kb0 + kbs) * NG / a.group_span, a.last_group + 1) - g0;
-        const char* s = static_cast<const char*>(a.scales) + (expert * a.stride_s + (long long)row * a.lds + g0) * scale_bytes;
-        for (int i = 0; i < groups * scale_bytes; i += 128) asm volatile("prefetch.global.L2 [%0];" ::"l"(s + i));
-        if (a.zeros != nullptr) {
+        const char* x = static_cast<const char*>(a.scales) + (expert * a.stride_s + (long long)row * a.lds + g0) * scale_bytes;
+        for (int i = 0; i < groups * scale_bytes; i += 128) asm volatile("prefetch.global.L2 [%0];" ::"l"(x + i));
+        if (kZeros) {
           const uint8_t* z = a.zeros + expert * a.stride_z + (long long)row * a.ldz + g0;
           for (int i = 0; i < groups; i += 128) asm volatile("prefetch.global.L2 [%0];" ::"l"(z + i));
         }
-      }
-    }
-    u.row0 = (first + tile) * kRows;
-    u.kb = kb;
-    u.expert = expert;
-    u.batch_row0 = first * kRows;
-    u.count = count;
-    u.pass = pass;
-    const bool load = (u.flags & kNone) == 0;
-    if (load) {
-      --run_left;
-      if (++kb == kbs || run_left == 0) u.flags |= kLast;
-      if (run_left == 0) u.flags |= kEnd;
-      mark &= kSecond;
-      if (kb == kbs) {
-        kb = 0;
-        ++tile;
-        mark = kFirst | kSecond;
-      }
-      if (run_left == 0) mark = 0;
-      else if ((u.flags & kSecond) != 0) mark |= kSecond;
-    }
-    if (lane == 0) {
-      units[at] = u;
-      const uint32_t bar = bar0 + 8 * at, to = ring0 + at * kUnitBytes;
-      if (load && !failed) {
-        mbarrier_arrive_expect_tx(bar, kUnitBytes);
-        tma_load_3d(to, &a.map, bar, (kb0 + u.kb) * (kUnitK / 2), u.row0, u.expert);
-        tma_load_3d(to + kBoxBytes, &a.map, bar, (kb0 + u.kb) * (kUnitK / 2) + 128, u.row0, u.expert);  // zeros behind K
       } else {
-        mbarrier_arrive(bar);
+        s.flags = kNone;
       }
     }
+    run_left -= left;
+    if (run_left == 0) s.flags |= kEnd;
+    load_x = (kb0 + kb) * (kUnitK / 2);
+    load_y = (first + tile) * kRows;
+    s.row0 = load_y;
+    s.kb = kb;
+    s.units = left;
+    s.batch_row0 = first * kRows;
+    s.count = count;
+    s.pass = pass;
+    s.expert = expert;
+    if (lane == 0) records[at] = s;
+  };
+  // Fills ring slot `at` with the warp's next unit.
+  auto produce = [&](int at) {
+    const uint32_t bar = bar0 + 8 * at, to = ring0 + at * kUnitBytes;
+    if (left == 0) {
+      begin_stretch(at);
+      if (left == 0) {  // nothing to load: the slot's barrier goes on to its next phase all the same
+        if (lane == 0) mbarrier_arrive(bar);
+        return;
+      }
+    }
+    --left;
+    if (lane == 0) {
+      if (failed) {
+        mbarrier_arrive(bar);
+      } else {
+        mbarrier_arrive_expect_tx(bar, kUnitBytes);
+        tma_load_3d(to, &a.map, bar, load_x, load_y, expert);
+        tma_load_3d(to + kBoxBytes, &a.map, bar, load_x + 128, load_y, expert);  // zeros behind K
+      }
+    }
+    load_x += kUnitK / 2;
   };
 
   // x of a pass as digits: a warp takes 256 K-elements of a token at a time, a lane 8 of them, and loads
@@ -478,29 +488,33 @@ __global__ void __launch_bounds__(kThreads, 1) gemv_int4_kernel(const __grid_con
     uint32_t s[2][kHeld];  // as loaded: nothing waits for them before the unit that uses them
     uint32_t z[2][kHeld];
   };
-  int base_expert = -1;
-  const char* s_base = nullptr;
-  const uint8_t* z_base = nullptr;
-  auto load_scales = [&](Unit const& u, Scales& v) {
-    if (u.expert != base_expert) {
-      base_expert = u.expert;
-      s_base = static_cast<const char*>(a.scales) + u.expert * a.stride_s * scale_bytes;
-      z_base = a.zeros + u.expert * a.stride_z;
-    }
+  const char* s_row[2] = {};
+  const uint8_t* z_row[2] = {};
+  int s_kb = 0;  // the unit whose scales are loaded next
+  Scales raw = {};
+  auto aim_scales = [&](Stretch const& s) {
+    s_kb = kb0 + s.kb;
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
-      const int row = min(u.row0 + r * 8 + g, a.n - 1);
-      const char* s_row = s_base + (long long)row * (a.lds * scale_bytes);
-      const uint8_t* z_row = z_base + (long long)row * a.ldz;
+      const int row = min(s.row0 + r * 8 + g, a.n - 1);
+      s_row[r] = static_cast<const char*>(a.scales) + (s.expert * a.stride_s + (long long)row * a.lds) * scale_bytes;
+      if (kZeros) z_row[r] = a.zeros + s.expert * a.stride_z + (long long)row * a.ldz;
+    }
+  };
+  auto load_scales = [&] {
 #pragma unroll
-      for (int h = 0; h < kHeld; ++h) {
-        int gi = (kb0 + u.kb) * NG + t + 4 * h;
-        if (NG == 4 && a.group_span != 1) gi /= a.group_span;
-        gi = min(gi, a.last_group);
-        v.s[r][h] = a.f32_scales ? reinterpret_cast<const uint32_t*>(s_row)[gi] : reinterpret_cast<const uint16_t*>(s_row)[gi];
-        if (a.zeros != nullptr) v.z[r][h] = z_row[gi];
+    for (int h = 0; h < kHeld; ++h) {
+      int gi = s_kb * NG + t + 4 * h;
+      if (NG == 4 && a.group_span != 1) gi /= a.group_span;
+      gi = min(gi, a.last_group);
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        if (a.f32_scales) raw.s[r][h] = reinterpret_cast<const uint32_t*>(s_row[r])[gi];
+        else raw.s[r][h] = reinterpret_cast<const uint16_t*>(s_row[r])[gi];
+        if (kZeros) raw.z[r][h] = z_row[r][gi];
       }
     }
+    ++s_kb;
   };
   auto scale_of = [&](uint32_t bits) {
     if (a.f32_scales) return __uint_as_float(bits);
@@ -522,7 +536,7 @@ __global__ void __launch_bounds__(kThreads, 1) gemv_int4_kernel(const __grid_con
   const int digit_lane = t * 8 + (TOK > 2 ? g * 32 : g >= 6 ? 0 : TOK == 2 ? g * 32 : g % 2 ? 0 : g / 2 * 32);
   // A batch's sums of the cluster's blocks, a tile to a block in turn. They are gathered a batch later, when the
   // others' have long arrived; two buffers: by then every block has left the one that is written next.
-  Unit gathers = {};
+  Stretch gathers = {};
   Pass gathers_pass = {};
   int flip = 0;
   auto gather = [&] {
@@ -538,22 +552,47 @@ __global__ void __launch_bounds__(kThreads, 1) gemv_int4_kernel(const __grid_con
     __syncwarp();
   };
   float acc[kSets][4] = {};
-  Scales raw = {};
   Pass p = {};
-  int in = 0, out = depth - 1;      // ring slots: the next to fill, and that of unit `done`
-  int issued = 0, done = -1;        // units; before the first, a turn that only loads its scales
-  int at_pass = -1;
-  uint32_t parity = 1;
+  Stretch u = {};
+  int in = 0, out = 0, issued = 0, done = 0;  // ring slots to fill next and of unit `done`; units
+  int now_left = 0, at_pass = -1;             // units left of the stretch at hand
+  uint32_t parity = 0;
+  const uint8_t *xd = smem, *xs = smem, *xp = smem;
+  int k_at = 0;
 #pragma unroll 1
   while (true) {
     // At first one unit a warp: what the start waits for does not queue behind a whole ring of weights.
-    while ((remaining > count || run_left > 0) && issued - max(done, 0) < (done < 0 ? 1 : depth)) {
+    while ((left > 0 || run_left > 0 || remaining > count) && issued - done < (at_pass < 0 ? 1 : depth)) {
       produce(in);
       in = in + 1 == depth ? 0 : in + 1;
       ++issued;
     }
     if (done == issued) break;
-    __syncwarp();
+    if (now_left == 0) {
+      __syncwarp();
+      u = records[out];
+      if (u.pass != at_pass) {  // every warp has a record of every batch, so all come here together
+        const bool start = at_pass < 0;
+        if (start) {
+          aim_scales(u);
+          load_scales();
+        } else {
+          __syncthreads();
+        }
+        at_pass = u.pass;
+        p = pass_of(at_pass);
+        convert(p);
+        __syncthreads();
+        if (start) continue;  // to fill the ring
+      }
+      now_left = max(u.units, 1);
+      k_at = (kb0 + u.kb) * kUnitK;
+      xd = smem + a.digits + u.kb * 16 * kDigitRow<TOK> + digit_lane;
+      xs = smem + a.sums + u.kb * NG * kSumBytes<TOK> + t * (TOK <= 2 ? 8 : 16);
+      xp = smem + a.powers + u.kb * 4 * kPowerBytes<TOK> + t * 8;
+#pragma unroll
+      for (int set = 0; set < kSets; ++set) acc[set][0] = acc[set][1] = acc[set][2] = acc[set][3] = 0.0f;
+    }
     float s_now[2][kHeld];
     uint32_t z_now[2][kHeld];
 #pragma unroll
@@ -563,24 +602,21 @@ __global__ void __launch_bounds__(kThreads, 1) gemv_int4_kernel(const __grid_con
         s_now[r][h] = scale_of(raw.s[r][h]);
         z_now[r][h] = raw.z[r][h];
       }
-    if (done + 1 < issued) load_scales(units[out + 1 == depth ? 0 : out + 1], raw);
-    if (done >= 0) {
-      const Unit u = units[out];
-      if ((u.flags & kFirst) != 0) {
-#pragma unroll
-        for (int set = 0; set < kSets; ++set) acc[set][0] = acc[set][1] = acc[set][2] = acc[set][3] = 0.0f;
-      }
-      if ((u.flags & kNone) == 0 && !failed)
-        failed = __any_sync(0xFFFFFFFFu, !mbarrier_wait(bar0 + 8 * out, parity, a.timeout_ns));
-      if ((u.flags & kNone) == 0 && !failed) {
+    if (now_left > 1) {
+      load_scales();
+    } else if (done + 1 < issued) {
+      __syncwarp();
+      aim_scales(records[out + 1 == depth ? 0 : out + 1]);
+      load_scales();
+    }
+    if ((u.flags & kNone) == 0) {
+      if (!failed) failed = __any_sync(0xFFFFFFFFu, !mbarrier_wait(bar0 + 8 * out, parity, a.timeout_ns));
+      if (!failed) {
         const uint32_t base = ring0 + out * kUnitBytes + in_box;
-        const uint8_t* xd = smem + a.digits + u.kb * 16 * kDigitRow<TOK> + digit_lane;
-        const uint8_t* xs = smem + a.sums + u.kb * NG * kSumBytes<TOK> + t * (TOK <= 2 ? 8 : 16);
-        const uint8_t* xp = smem + a.powers + u.kb * 4 * kPowerBytes<TOK> + t * 8;
-        const int quarters = (kb0 + u.kb) * kUnitK + kUnitK / 2 >= a.k ? 2 : 4;
+        const bool whole = k_at + kUnitK / 2 < a.k;
 #pragma unroll
         for (int quarter = 0; quarter < 4; ++quarter) {  // 128 codes
-          if (quarter == quarters) break;
+          if (quarter == 2 && !whole) break;
           int part[kTiles<TOK>][4];
           float sum[kSets][4] = {};
 #pragma unroll
@@ -594,7 +630,7 @@ __global__ void __launch_bounds__(kThreads, 1) gemv_int4_kernel(const __grid_con
               const int c = pair * 2 + cc;
               const uint32_t f[4] = {w[2 * cc] & kNibbles, w[2 * cc + 1] & kNibbles, (w[2 * cc] >> 4) & kNibbles,
                                      (w[2 * cc + 1] >> 4) & kNibbles};
-              const uint8_t* xc = xd + c * kDigitRow<TOK>;
+              const uint8_t* xc = xd + (quarter * 4 + c) * kDigitRow<TOK>;
 #pragma unroll
               for (int j = 0; j < kTiles<TOK>; ++j) {
                 if (j >= 3 && p.count <= 8) continue;
@@ -607,17 +643,17 @@ __global__ void __launch_bounds__(kThreads, 1) gemv_int4_kernel(const __grid_con
 #pragma unroll
               for (int r = 0; r < 2; ++r) {
                 sc[r] = __shfl_sync(0xFFFFFFFFu, s_now[r][0], from);
-                if (a.zeros != nullptr) z[r] = int(__shfl_sync(0xFFFFFFFFu, z_now[r][0], from));
+                if (kZeros) z[r] = int(__shfl_sync(0xFFFFFFFFu, z_now[r][0], from));
               }
               if constexpr (TOK <= 2) {
-                const int2 q = *reinterpret_cast<const int2*>(xs + gj * kSumBytes<TOK>);
+                const int2 q = *reinterpret_cast<const int2*>(xs + (quarter * kGroups + gj) * kSumBytes<TOK>);
 #pragma unroll
                 for (int i = 0; i < 4; ++i) sum[0][i] = fmaf(sc[i / 2], float(part[0][i] - z[i / 2] * (i % 2 ? q.y : q.x)), sum[0][i]);
               } else {
 #pragma unroll
                 for (int set = 0; set < kSets; ++set) {
                   if (set > 0 && p.count <= 8) continue;
-                  const int4 q = *reinterpret_cast<const int4*>(xs + gj * kSumBytes<TOK> + set * 64);
+                  const int4 q = *reinterpret_cast<const int4*>(xs + (quarter * kGroups + gj) * kSumBytes<TOK> + set * 64);
 #pragma unroll
                   for (int i = 0; i < 4; ++i) {
                     // |256 P_1 + P_0| and z times its sums stay below 2^30.
@@ -631,13 +667,10 @@ __global__ void __launch_bounds__(kThreads, 1) gemv_int4_kernel(const __grid_con
           }
 #pragma unroll
           for (int set = 0; set < kSets; ++set) {
-            const float2 q = *reinterpret_cast<const float2*>(xp + set * 32);
+            const float2 q = *reinterpret_cast<const float2*>(xp + quarter * kPowerBytes<TOK> + set * 32);
 #pragma unroll
             for (int i = 0; i < 4; ++i) acc[set][i] = fmaf(i % 2 ? q.y : q.x, sum[set][i], acc[set][i]);
           }
-          xd += 4 * kDigitRow<TOK>;
-          xs += NG / 4 * kSumBytes<TOK>;
-          xp += kPowerBytes<TOK>;
           // The next quarter's groups in front, where this one's were a lane's last.
           if (kHeld > 1 && (kHeld == 4 || quarter == 1)) {
 #pragma unroll
@@ -649,8 +682,12 @@ __global__ void __launch_bounds__(kThreads, 1) gemv_int4_kernel(const __grid_con
               }
           }
         }
-        __syncwarp();
-        if ((u.flags & kLast) != 0) {
+        xd += 16 * kDigitRow<TOK>;
+        xs += NG * kSumBytes<TOK>;
+        xp += 4 * kPowerBytes<TOK>;
+        k_at += kUnitK;
+        __syncwarp();  // the slot is read
+        if (now_left == 1) {
           // This warp's part of the tile's sums, [token][row].
           float* to = pieces + (warp * kPieces + ((u.flags & kSecond) != 0)) * kPiece<TOK>;
           if constexpr (TOK <= 2) {
@@ -669,6 +706,8 @@ __global__ void __launch_bounds__(kThreads, 1) gemv_int4_kernel(const __grid_con
           __syncwarp();
         }
       }
+    }
+    if (--now_left == 0) {
       if ((u.flags & kEnd) != 0) {
         auto put = [&](int m, int o, float v) {
           const int token = o / kRows, n = u.batch_row0 + m * kRows + o % kRows;
@@ -706,16 +745,6 @@ __global__ void __launch_bounds__(kThreads, 1) gemv_int4_kernel(const __grid_con
         if (!full) __syncthreads();
         else __syncwarp();
         if (splits > 1) cluster_arrive();
-      }
-    }
-    if (done + 1 < issued) {
-      const int next_pass = units[out + 1 == depth ? 0 : out + 1].pass;
-      if (next_pass != at_pass) {  // every warp has a record of every batch, so all come here together
-        if (at_pass >= 0) __syncthreads();
-        at_pass = next_pass;
-        p = pass_of(at_pass);
-        convert(p);
-        __syncthreads();
       }
     }
     ++done;
@@ -765,10 +794,10 @@ Fit fit(Int4Args const& a) {
   return f;
 }
 
-template <class T, int NG, int TOK>
+template <class T, int NG, int TOK, bool kZeros>
 kl_status launch(Fit const& f, int device, cudaStream_t stream) {
   Int4Args const& a = f.args;
-  auto* kernel = gemv_int4_kernel<T, NG, TOK>;
+  auto* kernel = gemv_int4_kernel<T, NG, TOK, kZeros>;
   static std::atomic<int> resident[64][4];  // clusters of 1, 2, 4, 8 that fit the device at once
   const int which = f.cluster == 1 ? 0 : f.cluster == 2 ? 1 : f.cluster == 4 ? 2 : 3;
   cudaLaunchConfig_t cfg = {};
@@ -806,25 +835,30 @@ kl_status launch(Fit const& f, int device, cudaStream_t stream) {
 }
 
 // Tokens of a pass by what a matrix meets (with ids: on average), fewer where x's digits would not fit.
-template <class T, int NG>
+template <class T, int NG, bool kZeros>
 kl_status by_tokens(Int4Args& a, int device, cudaStream_t stream) {
   const int tokens = a.ids != nullptr ? (a.slots + a.experts - 1) / a.experts : a.slots;
   if (tokens > 8)
-    if (const Fit f = fit<NG, 16>(a); f.depth >= 2) return launch<T, NG, 16>(f, device, stream);
+    if (const Fit f = fit<NG, 16>(a); f.depth >= 2) return launch<T, NG, 16, kZeros>(f, device, stream);
   if (tokens > 2)
-    if (const Fit f = fit<NG, 8>(a); f.depth >= 2) return launch<T, NG, 8>(f, device, stream);
+    if (const Fit f = fit<NG, 8>(a); f.depth >= 2) return launch<T, NG, 8, kZeros>(f, device, stream);
   if (a.slots > 1)
-    if (const Fit f = fit<NG, 2>(a); f.depth >= 2) return launch<T, NG, 2>(f, device, stream);
+    if (const Fit f = fit<NG, 2>(a); f.depth >= 2) return launch<T, NG, 2, kZeros>(f, device, stream);
   const Fit f = fit<NG, 1>(a);
   if (f.depth < 2) return fail(KL_ERR_NOT_SUPPORTED, "kl_gemv_int4: k does not fit");
-  return launch<T, NG, 1>(f, device, stream);
+  return launch<T, NG, 1, kZeros>(f, device, stream);
+}
+
+template <class T, bool kZeros>
+kl_status by_group(Int4Args& a, int device, cudaStream_t stream) {
+  if (a.group == 32) return by_tokens<T, 16, kZeros>(a, device, stream);
+  if (a.group == 64) return by_tokens<T, 8, kZeros>(a, device, stream);
+  return by_tokens<T, 4, kZeros>(a, device, stream);
 }
 
 template <class T>
-kl_status by_group(Int4Args& a, int device, cudaStream_t stream) {
-  if (a.group == 32) return by_tokens<T, 16>(a, device, stream);
-  if (a.group == 64) return by_tokens<T, 8>(a, device, stream);
-  return by_tokens<T, 4>(a, device, stream);
+kl_status by_zeros(Int4Args& a, int device, cudaStream_t stream) {
+  return a.zeros != nullptr ? by_group<T, true>(a, device, stream) : by_group<T, false>(a, device, stream);
 }
 
 kl_status run(kl_int4_desc const& d, int64_t slots, cudaStream_t stream) {
@@ -866,7 +900,7 @@ kl_status run(kl_int4_desc const& d, int64_t slots, cudaStream_t stream) {
   a.timeout_ns = wait_timeout_ns();
   kl_status s = device_status_ptr(&a.status);
   if (s != KL_OK) return s;
-  return d.x_type == KL_BF16 ? by_group<__nv_bfloat16>(a, device, stream) : by_group<__half>(a, device, stream);
+  return d.x_type == KL_BF16 ? by_zeros<__nv_bfloat16>(a, device, stream) : by_zeros<__half>(a, device, stream);
 }
 
 }  // namespace
