@@ -687,63 +687,65 @@ __global__ void __launch_bounds__(kThreads, 1) gemv_int4_kernel(const __grid_con
         xp += 4 * kPowerBytes<TOK>;
         k_at += kUnitK;
         __syncwarp();  // the slot is read
-        if (now_left == 1) {
-          // This warp's part of the tile's sums, [token][row].
-          float* to = pieces + (warp * kPieces + ((u.flags & kSecond) != 0)) * kPiece<TOK>;
-          if constexpr (TOK <= 2) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const float v0 = __shfl_sync(0xFFFFFFFFu, acc[0][i], lane & 28), v1 = __shfl_sync(0xFFFFFFFFu, acc[0][i], (lane & 28) | 1),
-                          v2 = __shfl_sync(0xFFFFFFFFu, acc[0][i], (lane & 28) | 2);
-              if (t == 0 && i % 2 < TOK) to[i % 2 * kRows + i / 2 * 8 + g] = v0 + v1 + v2;
-            }
-          } else {
-#pragma unroll
-            for (int set = 0; set < kSets; ++set)
-#pragma unroll
-              for (int i = 0; i < 4; ++i) to[(set * 8 + 2 * t + i % 2) * kRows + i / 2 * 8 + g] = acc[set][i];
-          }
-          __syncwarp();
-        }
       }
     }
     if (--now_left == 0) {
+      // The stretch ends. In a full batch a tile is a warp's own, all of this block's K; else the warps leave their
+      // parts, [token][row], and add them up in their order along K: warp w's run is [count kbs w / 16,
+      // count kbs (w + 1) / 16), tile m's units [m kbs, (m + 1) kbs).
+      const bool full = u.count == kWarps;
+      auto spread = [&](auto&& f) {  // f(cell, sum) for this lane's cells of the tile
+        if constexpr (TOK <= 2) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float v0 = __shfl_sync(0xFFFFFFFFu, acc[0][i], lane & 28), v1 = __shfl_sync(0xFFFFFFFFu, acc[0][i], (lane & 28) | 1),
+                        v2 = __shfl_sync(0xFFFFFFFFu, acc[0][i], (lane & 28) | 2);
+            if (t == 0 && i % 2 < TOK) f(i % 2 * kRows + i / 2 * 8 + g, v0 + v1 + v2);
+          }
+        } else {
+#pragma unroll
+          for (int set = 0; set < kSets; ++set)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) f((set * 8 + 2 * t + i % 2) * kRows + i / 2 * 8 + g, acc[set][i]);
+        }
+      };
+      if (!full && (u.flags & kNone) == 0) {
+        float* to = pieces + (warp * kPieces + ((u.flags & kSecond) != 0)) * kPiece<TOK>;
+        spread([&](int o, float v) { to[o] = v; });
+      }
       if ((u.flags & kEnd) != 0) {
         auto put = [&](int m, int o, float v) {
           const int token = o / kRows, n = u.batch_row0 + m * kRows + o % kRows;
           if (token < p.count && n < a.n) store(slot_of(p.first + token), n, v);
         };
-        // A full batch is a tile a warp, whose sums (over this block's K) are the warp's own; else they are the
-        // sums of the warps' parts in their order along K: warp w's run is [count kbs w / 16, count kbs (w + 1) / 16),
-        // tile m's units [m kbs, (m + 1) kbs).
-        const bool full = u.count == kWarps;
-        if (!full) __syncthreads();
-        auto block_sum = [&](int m, int o) {
-          float sum = 0.0f;
-          for (int w = m * kWarps / u.count; w < kWarps; ++w) {
-            const int lo = u.count * kbs * w / kWarps, hi = u.count * kbs * (w + 1) / kWarps;
-            if (lo >= (m + 1) * kbs) break;
-            if (lo >= hi) continue;
-            sum += pieces[(w * kPieces + (lo >= m * kbs ? 0 : 1)) * kPiece<TOK> + o];  // 1: the run began in the tile before
-          }
-          return sum;
-        };
-        const int step = full ? 32 : kThreads, cells = (full ? 1 : u.count) * kPiece<TOK>;
         if (splits > 1) {
+          __syncwarp();
           if (gathers.count > 0) gather();
           gathers = u;
           gathers_pass = p;
           flip ^= 1;
         }
         float* mine = reinterpret_cast<float*>(smem + a.block) + flip * kWarps * kPiece<TOK>;
-        for (int i = full ? lane : int(threadIdx.x); i < cells; i += step) {
-          const int m = full ? warp : i / kPiece<TOK>, o = i % kPiece<TOK>;
-          const float v = block_sum(m, o);
-          if (splits > 1) mine[m * kPiece<TOK> + o] = v;
-          else put(m, o, v);
+        if (full) {
+          if (splits > 1) spread([&](int o, float v) { mine[warp * kPiece<TOK> + o] = v; });
+          else spread([&](int o, float v) { put(warp, o, v); });
+        } else {
+          __syncthreads();
+          for (int i = threadIdx.x; i < u.count * kPiece<TOK>; i += kThreads) {
+            const int m = i / kPiece<TOK>, o = i % kPiece<TOK>;
+            float sum = 0.0f;
+            for (int w = m * kWarps / u.count; w < kWarps; ++w) {
+              const int lo = u.count * kbs * w / kWarps, hi = u.count * kbs * (w + 1) / kWarps;
+              if (lo >= (m + 1) * kbs) break;
+              if (lo >= hi) continue;
+              sum += pieces[(w * kPieces + (lo >= m * kbs ? 0 : 1)) * kPiece<TOK> + o];  // 1: the run began in the tile before
+            }
+            if (splits > 1) mine[i] = sum;
+            else put(m, o, sum);
+          }
+          __syncthreads();
         }
-        if (!full) __syncthreads();
-        else __syncwarp();
+        __syncwarp();
         if (splits > 1) cluster_arrive();
       }
     }
