@@ -737,7 +737,7 @@ __global__ void __launch_bounds__(kThreads, 1) gemv_int4_kernel(const __grid_con
             for (int w = m * kWarps / u.count; w < kWarps; ++w) {
               const int lo = u.count * kbs * w / kWarps, hi = u.count * kbs * (w + 1) / kWarps;
               if (lo >= (m + 1) * kbs) break;
-              if (lo >= hi) continue;
+              if (lo >= hi || hi <= m * kbs) continue;  // no units, or none of this tile
               sum += pieces[(w * kPieces + (lo >= m * kbs ? 0 : 1)) * kPiece<TOK> + o];  // 1: the run began in the tile before
             }
             if (splits > 1) mine[i] = sum;

@@ -346,6 +346,8 @@ def gemv_tol(x, w, want, k, dtype):
     summed exactly; each group's sum takes 3 roundings to scale and 3 to join its three digits, then at
     most k / 32 sums, 16 warps and 8 blocks are added in fp32; one rounding to the type."""
     x = x.to(F64).abs()
+    if x.shape[0] == 0:
+        return torch.zeros_like(want)
     fixed = 2.0 ** -22 * x.max(-1, keepdim=True)[0] * w.abs().sum(1)
     size = x @ w.abs().T
     return fixed + (size + fixed) * (k / 32 + 32) * U + want.abs() * HALF[dtype] * 1.001 + torch.finfo(dtype).smallest_normal * HALF[dtype] * 2
@@ -364,6 +366,48 @@ def test_gemv_int4(cuda, dtype, group, tokens, n, k):
         close(kl.gemv_int4(x.to(cuda), q, s, z, group=group), want, gemv_tol(x, w, want, k, dtype), f"zeros {zeros}")
     got = kl.gemv_int4(x.to(cuda), q, s.float(), z, group=group, out_dtype=torch.float32)
     close(got, want, gemv_tol(x, w, want, k, torch.float32), "fp32 scales and out")
+
+
+@pytest.mark.parametrize("tokens, n, k, group", [
+    (1, 16 * 148 * 14 + 5, 2048, 128),    # every block has several tiles, cut between the warps
+    (2, 16 * 148 * 21, 512, 32),          # a full batch of 16 tiles and a rest, one unit a tile
+    (1, 16 * 148 * 3, 1536, 64), (5, 16 * 300 + 1, 2560, 64), (13, 10007, 4128, 64), (16, 16 * 700, 8192, 128),
+    (33, 16 * 200, 1056, 32), (3, 40, 16384, 128), (16, 64, 32768, 32), (1, 32, 65536, 64), (2, 8192, 8192, 256),
+])
+def test_gemv_int4_many_tiles(cuda, tokens, n, k, group):
+    """Sizes at which blocks have several tiles, tiles are shared between warps, K is split over a cluster."""
+    g = torch.Generator("cuda").manual_seed(n + k)
+    q = torch.randint(0, 256, (n, k // 2), generator=g, device=cuda, dtype=torch.uint8)
+    s = (torch.rand((n, -(-k // group)), generator=g, device=cuda) * 0.02 + 0.001).bfloat16()
+    z = torch.randint(0, 16, s.shape, generator=g, device=cuda, dtype=torch.uint8)
+    x = torch.randn((tokens, k), generator=g, device=cuda).bfloat16()
+    codes = torch.stack([q & 15, q >> 4], -1).flatten(-2).double()
+    at = torch.arange(k, device=cuda) // group
+    w = (codes - z.double()[:, at]) * s.double()[:, at]
+    want = x.double() @ w.T
+    tol = gemv_tol(x, w, want, k, torch.bfloat16)
+    for _ in range(2):
+        close(kl.gemv_int4(x, q, s, z, group=group), want.cpu(), tol.cpu())
+
+
+def test_gemv_int4_by_expert_many_tiles(cuda):
+    """Blocks whose tiles belong to several experts, experts with several passes of tokens."""
+    g = torch.Generator("cuda").manual_seed(5)
+    for tokens, k, experts, n, width, group in ((1, 8, 64, 4096, 2048, 128), (16, 4, 64, 2064, 1536, 32), (40, 2, 3, 1000, 768, 64),
+                                                (300, 2, 5, 500, 512, 128)):
+        q = torch.randint(0, 256, (experts, n, width // 2), generator=g, device=cuda, dtype=torch.uint8)
+        s = (torch.rand((experts, n, -(-width // group)), generator=g, device=cuda) * 0.02 + 0.001).half()
+        ids = torch.randint(-1, experts, (tokens, k), generator=g, device=cuda, dtype=torch.int32)
+        x = torch.randn((tokens, k, width), generator=g, device=cuda).half()
+        got = kl.gemv_int4(x, q, s, group=group, ids=ids)
+        at = torch.arange(width, device=cuda) // group
+        assert (got[ids < 0] == 0).all()
+        for e in range(experts):
+            mine = ids == e
+            codes = torch.stack([q[e] & 15, q[e] >> 4], -1).flatten(-2).double()
+            w = (codes - 8) * s[e].double()[:, at]
+            want = x[mine].double() @ w.T
+            close(got[mine], want.cpu(), gemv_tol(x[mine], w, want, width, torch.float16).cpu(), f"expert {e}")
 
 
 def test_gemv_int4_every_code(cuda):
