@@ -399,7 +399,8 @@ extern "C" kl_status kl_moe_plan(const int32_t* ids, int64_t tokens, int64_t k, 
   const long long warps = (long long)cluster * kPlanWarps;
   a.warp_span = (a.total + warps * 32 - 1) / (warps * 32) * 32;
   const size_t smem = size_t(kPlanWarps) * size_t(experts) * sizeof(int);
-  cudaError_t e = cudaFuncSetAttribute(plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem));
+  cudaError_t e = cudaSuccess;
+  if (smem > 32 * 1024) e = cudaFuncSetAttribute(plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem));
   if (e != cudaSuccess) return cuda_fail(e, "kl_moe_plan shared memory");
   void* args[] = {&a};
   e = launch(static_cast<cudaStream_t>(stream), dim3(unsigned(cluster)), kPlanThreads, smem, cluster,

@@ -14,6 +14,7 @@ through torch. No counterpart in the reference (kernel_lib has no GEMM and no ro
 from __future__ import annotations
 
 import ctypes
+from functools import lru_cache
 from typing import NamedTuple
 
 import torch
@@ -97,6 +98,13 @@ def _queue(device: int, stream, owned, fn, *args) -> None:
         check(status)
 
 
+@lru_cache(maxsize=4096)
+def _route_workspace(tokens: int, experts: int) -> int:
+    need = ctypes.c_size_t()
+    check(lib().kl_moe_route_workspace_size(tokens, experts, ctypes.byref(need)))
+    return need.value
+
+
 def _route_desc(logits, k, renormalize, valid, ids, weights, counts, routed, loss):
     return MoeRouteDesc(logits.data_ptr(), _pitch(logits), logits.shape[0], logits.shape[1], k, _FLOATS[logits.dtype],
                         int(bool(renormalize)), _ptr(valid), ids.data_ptr(), weights.data_ptr(), counts.data_ptr(),
@@ -128,11 +136,8 @@ def moe_route(logits, k: int, *, renormalize: bool = True, valid=None, stream=No
     routed = logits.new_empty((), dtype=torch.int32)
     loss = logits.new_empty((), dtype=torch.float32)
     out = MoeRoute(ids, weights, counts, routed, loss)
-    owned, work, size = out, None, 0
-    if tokens > 32:  # up to 32 tokens need no workspace
-        need = ctypes.c_size_t()
-        check(lib().kl_moe_route_workspace_size(tokens, experts, ctypes.byref(need)))
-        size = need.value
+    owned, work, size = out, None, _route_workspace(tokens, experts)
+    if size:
         work = logits.new_empty((size,), dtype=torch.uint8)
         owned = (*out, work)
     d = _route_desc(logits, k, renormalize, valid, ids, weights, counts, routed, loss)
@@ -169,10 +174,9 @@ def moe_route_grad(logits, route: MoeRoute, dweights=None, dloss=None, *, renorm
 
 
 def moe_rows(slots: int, experts: int, block: int = 128) -> int:
-    """Rows of the grouped layout that any split of `slots` rows over the experts fits."""
-    rows = int(lib().kl_moe_rows(int(slots), int(experts), int(block)))
-    _refuse(rows >= 0, "slots must not be negative, experts positive, block 128 or 256")
-    return rows
+    """Rows of the grouped layout that any split of `slots` rows over the experts fits (kl_moe_rows)."""
+    _refuse(slots >= 0 and experts >= 1 and block in (128, 256), "slots must not be negative, experts positive, block 128 or 256")
+    return (slots + min(slots, experts) * (block - 1)) // block * block
 
 
 def moe_plan(ids, experts: int, *, block: int = 128, stream=None) -> MoePlan:

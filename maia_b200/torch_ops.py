@@ -1,5 +1,6 @@
 """PyTorch operators over the C ABI: torch.ops.kl.gemm, torch.ops.kl.gemm_fp8,
-torch.ops.kl.gemm_block_scaled and torch.ops.kl.gemm_grouped.
+torch.ops.kl.gemm_block_scaled and torch.ops.kl.gemm_grouped; around the last the expert layer's
+torch.ops.kl.moe_route, moe_plan, moe_dispatch and moe_combine, with gradients, and torch.ops.kl.gemv_int4.
 
 Registered with torch.library so they compose with the rest of a PyTorch program (fake tensors
 for shape inference, the dispatcher, torch.compile graphs that call them as opaque ops). The work
@@ -8,11 +9,11 @@ is the library's own kernels, launched on the tensors' current CUDA stream.
 
 from __future__ import annotations
 
-from typing import Optional
+from typing import Optional, Tuple
 
 import torch
 
-from . import ALGO_1CTA, ALGO_2CTA, ALGO_AUTO, gemm as _kl_gemm, gemm_grouped as _kl_gemm_grouped
+from . import ALGO_1CTA, ALGO_2CTA, ALGO_AUTO, experts as _experts, gemm as _kl_gemm, gemm_grouped as _kl_gemm_grouped
 
 
 @torch.library.custom_op("kl::gemm", mutates_args=())
@@ -78,3 +79,144 @@ def gemm_grouped(a: torch.Tensor, b: torch.Tensor, m_block_group: torch.Tensor,
 @gemm_grouped.register_fake
 def _(a, b, m_block_group, out_dtype=torch.bfloat16, pairs=False):
     return a.new_empty((a.shape[0], b.shape[1]), dtype=out_dtype)
+
+
+@torch.library.custom_op("kl::moe_route", mutates_args=())
+def moe_route(logits: torch.Tensor, k: int, renormalize: bool = True, valid: Optional[torch.Tensor] = None
+              ) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
+    """(ids, weights, counts, routed tokens, balance loss) of logits [tokens, experts]: maia_b200.moe_route.
+    Differentiable in weights and loss; the choice of experts and the counts are constants."""
+    return tuple(_experts.moe_route(logits, k, renormalize=renormalize, valid=valid))
+
+
+@moe_route.register_fake
+def _(logits, k, renormalize=True, valid=None):
+    tokens, experts = logits.shape
+    whole = dict(dtype=torch.int32)
+    return (logits.new_empty((tokens, k), **whole), logits.new_empty((tokens, k), dtype=torch.float32),
+            logits.new_empty((experts,), **whole), logits.new_empty((), **whole), logits.new_empty((), dtype=torch.float32))
+
+
+@torch.library.custom_op("kl::moe_route_grad", mutates_args=())
+def moe_route_grad(logits: torch.Tensor, ids: torch.Tensor, weights: torch.Tensor, counts: torch.Tensor, tokens: torch.Tensor,
+                   dweights: Optional[torch.Tensor], dloss: Optional[torch.Tensor], renormalize: bool,
+                   valid: Optional[torch.Tensor]) -> torch.Tensor:
+    """The gradient of kl::moe_route's logits: maia_b200.moe_route_grad."""
+    route = _experts.MoeRoute(ids, weights, counts, tokens, None)
+    return _experts.moe_route_grad(logits, route, dweights, dloss, renormalize=renormalize, valid=valid)
+
+
+@moe_route_grad.register_fake
+def _(logits, ids, weights, counts, tokens, dweights, dloss, renormalize, valid):
+    return logits.new_empty(logits.shape)
+
+
+def _route_context(ctx, inputs, output):
+    logits, _, ctx.renormalize, valid = inputs
+    ids, weights, counts, tokens, _ = output
+    ctx.save_for_backward(logits, ids, weights, counts, tokens, valid)
+    ctx.mark_non_differentiable(ids, counts, tokens)
+
+
+def _route_backward(ctx, _ids, dweights, _counts, _tokens, dloss):
+    logits, ids, weights, counts, tokens, valid = ctx.saved_tensors
+    dlogits = torch.ops.kl.moe_route_grad(logits, ids, weights, counts, tokens,
+                                          None if dweights is None else dweights.contiguous(),
+                                          None if dloss is None else dloss.contiguous(), ctx.renormalize, valid)
+    return dlogits, None, None, None
+
+
+moe_route.register_autograd(_route_backward, setup_context=_route_context)
+
+
+@torch.library.custom_op("kl::moe_plan", mutates_args=())
+def moe_plan(ids: torch.Tensor, experts: int, block: int = 128) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """(rows, slots, m_block_group) of int32 ids [tokens, k]: maia_b200.moe_plan."""
+    return tuple(_experts.moe_plan(ids, experts, block=block))
+
+
+@moe_plan.register_fake
+def _(ids, experts, block=128):
+    m = _experts.moe_rows(ids.shape[0] * ids.shape[1], experts, block)
+    return ids.new_empty(ids.shape), ids.new_empty((m,)), ids.new_empty((m // 128,))
+
+
+@torch.library.custom_op("kl::moe_dispatch", mutates_args=())
+def moe_dispatch(x: torch.Tensor, rows: torch.Tensor, slots: torch.Tensor) -> torch.Tensor:
+    """x's rows in the m-grouped layout of kl::moe_plan's rows and slots: maia_b200.moe_dispatch."""
+    return _experts.moe_dispatch(x, _experts.MoePlan(rows, slots, None))
+
+
+@moe_dispatch.register_fake
+def _(x, rows, slots):
+    return x.new_empty((slots.shape[0], x.shape[1]))
+
+
+def _dispatch_context(ctx, inputs, output):
+    ctx.save_for_backward(inputs[1])
+
+
+def _dispatch_backward(ctx, da):
+    (rows,) = ctx.saved_tensors
+    return torch.ops.kl.moe_combine(da.contiguous(), None, rows, None), None, None
+
+
+moe_dispatch.register_autograd(_dispatch_backward, setup_context=_dispatch_context)
+
+
+@torch.library.custom_op("kl::moe_combine", mutates_args=())
+def moe_combine(y: torch.Tensor, weights: Optional[torch.Tensor] = None, rows: Optional[torch.Tensor] = None,
+                slots: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """The weighted sum of each token's rows of y: maia_b200.moe_combine. Differentiable in y and weights; with rows
+    that takes kl::moe_plan's slots too."""
+    return _experts.moe_combine(y, weights, rows=rows)
+
+
+@moe_combine.register_fake
+def _(y, weights=None, rows=None, slots=None):
+    return y.new_empty((y.shape[0] if rows is None else rows.shape[0], y.shape[-1]))
+
+
+@torch.library.custom_op("kl::moe_combine_grad", mutates_args=())
+def moe_combine_grad(dout: torch.Tensor, y: torch.Tensor, weights: torch.Tensor, rows: Optional[torch.Tensor],
+                     slots: Optional[torch.Tensor]) -> Tuple[torch.Tensor, torch.Tensor]:
+    """The gradients of kl::moe_combine's y and weights: maia_b200.moe_combine_grad."""
+    return tuple(_experts.moe_combine_grad(dout, y, weights, rows=rows, slots=slots))
+
+
+@moe_combine_grad.register_fake
+def _(dout, y, weights, rows, slots):
+    return y.new_empty(y.shape), weights.new_empty(weights.shape)
+
+
+def _combine_context(ctx, inputs, output):
+    ctx.save_for_backward(*inputs)
+
+
+def _combine_backward(ctx, dout):
+    y, weights, rows, slots = ctx.saved_tensors
+    if rows is not None and slots is None:
+        raise RuntimeError("kl::moe_combine with rows needs kl::moe_plan's slots for its gradient")
+    plain = weights is None
+    if plain:
+        tokens, k = y.shape[:2] if rows is None else rows.shape
+        weights = torch.ones((tokens, k), dtype=torch.float32, device=y.device)
+    dy, dweights = torch.ops.kl.moe_combine_grad(dout.contiguous(), y, weights, rows, slots)
+    return dy, None if plain else dweights, None, None
+
+
+moe_combine.register_autograd(_combine_backward, setup_context=_combine_context)
+
+
+@torch.library.custom_op("kl::gemv_int4", mutates_args=())
+def gemv_int4(x: torch.Tensor, q: torch.Tensor, scales: torch.Tensor, zeros: Optional[torch.Tensor] = None, group: int = 128,
+              ids: Optional[torch.Tensor] = None, out_dtype: Optional[torch.dtype] = None) -> torch.Tensor:
+    """Products of few tokens with 4-bit weights, of one matrix or of the experts that `ids` names:
+    maia_b200.gemv_int4. For inference: no gradient."""
+    return _experts.gemv_int4(x, q, scales, zeros, group=group, ids=ids, out_dtype=out_dtype)
+
+
+@gemv_int4.register_fake
+def _(x, q, scales, zeros=None, group=128, ids=None, out_dtype=None):
+    shape = (x.shape[0], q.shape[0]) if ids is None else (*ids.shape, q.shape[1])
+    return x.new_empty(shape, dtype=out_dtype or x.dtype)

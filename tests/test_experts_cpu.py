@@ -63,6 +63,8 @@ def test_rows_of_the_layout():
     for args in ((-1, 8, 128), (1, 0, 128), (1, 8, 64)):
         with pytest.raises(ValueError):
             kl.moe_rows(*args)
+    for slots, experts, block in ((0, 8, 128), (1, 8, 128), (77, 5, 256), (1000, 1024, 128)):
+        assert kl.moe_rows(slots, experts, block) == kl.lib().kl_moe_rows(slots, experts, block)
     # Never too small: the worst split puts one row into the last block of every expert.
     for slots in range(1, 600, 7):
         for experts in (1, 2, 5):
@@ -167,3 +169,26 @@ def test_binding_imports_without_torch():
     code = "import sys; sys.modules['torch'] = None; import maia_b200 as kl; print(kl.lib().kl_moe_rows(1, 1, 128))"
     out = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, check=True)
     assert out.stdout.strip() == "128"
+
+
+def test_fake_tensor_shapes():
+    import maia_b200.torch_ops  # noqa: F401
+    from torch._subclasses.fake_tensor import FakeTensorMode
+
+    with FakeTensorMode():
+        logits = torch.empty((10, 8), dtype=torch.bfloat16)
+        ids, weights, counts, tokens, loss = torch.ops.kl.moe_route(logits, 2)
+        assert ids.shape == weights.shape == (10, 2) and ids.dtype == torch.int32 and weights.dtype == torch.float32
+        assert counts.shape == (8,) and tokens.shape == loss.shape == ()
+        rows, slots, groups = torch.ops.kl.moe_plan(ids, 8)
+        m = kl.moe_rows(20, 8)
+        assert rows.shape == (10, 2) and slots.shape == (m,) and groups.shape == (m // 128,)
+        a = torch.ops.kl.moe_dispatch(torch.empty((10, 64), dtype=torch.float16), rows, slots)
+        assert a.shape == (m, 64) and a.dtype == torch.float16
+        assert torch.ops.kl.moe_combine(a, weights, rows, slots).shape == (10, 64)
+        assert torch.ops.kl.moe_combine(torch.empty((10, 2, 32)), weights).shape == (10, 32)
+        x, q, s = torch.empty((3, 64), dtype=torch.bfloat16), torch.empty((40, 32), dtype=torch.uint8), torch.empty((40, 1))
+        assert torch.ops.kl.gemv_int4(x, q, s, None, 64).shape == (3, 40)
+        ids = torch.empty((3, 2), dtype=torch.int32)
+        y = torch.ops.kl.gemv_int4(x, q[None], s[None], None, 64, ids, torch.float32)
+        assert y.shape == (3, 2, 40) and y.dtype == torch.float32

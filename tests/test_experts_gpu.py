@@ -582,3 +582,63 @@ def test_routed_experts_with_4_bit_weights(cuda):
     close(y, want_y, fixed + size * 64 * U + want_y.abs() * HALF[torch.bfloat16] * 1.001, "y")
     terms = r.weights.cpu().to(F64)[..., None] * y.cpu().to(F64)
     close(out, terms.sum(1), terms.abs().sum(1) * 4 * U + terms.sum(1).abs() * HALF[torch.bfloat16] * 1.001, "out")
+
+
+# ------------------------------------------------------------------------------------ torch.ops.kl with gradients
+
+@pytest.mark.parametrize("renormalize", [True, False])
+def test_layer_gradients_through_torch_ops(cuda, renormalize):
+    """A training step through torch.ops.kl: route, plan, dispatch, the experts (torch), combine and the balance
+    loss; every gradient against torch's autograd over the same layer in float64, the choice held fixed."""
+    import maia_b200.torch_ops  # noqa: F401
+
+    tokens, experts, k, width, n = 70, 6, 2, 48, 40
+    logits = torch.randn((tokens, experts), generator=gen(1)).to(cuda).requires_grad_()
+    x = torch.randn((tokens, width), generator=gen(2)).to(cuda).requires_grad_()
+    w = (torch.randn((experts, n, width), generator=gen(3)) / 7).to(cuda).requires_grad_()
+    head = torch.randn((tokens, n), generator=gen(4)).to(cuda)
+    ids, weights, counts, routed, loss = torch.ops.kl.moe_route(logits, k, renormalize)
+    assert not ids.requires_grad and not counts.requires_grad and loss.requires_grad
+    rows, slots, groups = torch.ops.kl.moe_plan(ids, experts)
+    a = torch.ops.kl.moe_dispatch(x, rows, slots)
+    y = torch.cat([a[128 * i:128 * i + 128] @ (w[g].T if g >= 0 else 0 * w[0].T) for i, g in enumerate(groups.tolist())])
+    out = torch.ops.kl.moe_combine(y, weights, rows, slots)
+    ((out * head).sum() + 0.3 * loss).backward()
+
+    l64, x64, w64 = (t.detach().double().requires_grad_() for t in (logits, x, w))
+    p = torch.softmax(l64, 1)
+    sel = p.gather(1, ids.long())
+    if renormalize:
+        sel = sel / sel.sum(1, keepdim=True)
+    out64 = (sel[..., None] * torch.einsum("tw,tjnw->tjn", x64, w64[ids.long()])).sum(1)
+    loss64 = experts * (counts.double() / (k * tokens) * p.mean(0)).sum()
+    ((out64 * head.double()).sum() + 0.3 * loss64).backward()
+    # fp32 throughout, torch's own products among it: sums of up to tokens * k * width terms of size 1.
+    for name, mine, theirs in (("logits", logits, l64), ("x", x, x64), ("w", w, w64)):
+        close(mine.grad, theirs.grad.cpu(), 256 * U * theirs.grad.abs().max().item() * 8, name)
+    close(loss, loss64.detach().cpu(), 1e-5, "loss")
+
+
+def test_gradients_that_only_one_output_uses(cuda):
+    import maia_b200.torch_ops  # noqa: F401
+
+    logits = torch.randn((40, 8), generator=gen(1)).to(cuda).requires_grad_()
+    _, weights, _, _, loss = torch.ops.kl.moe_route(logits, 2)
+    (g,) = torch.autograd.grad(loss, logits, retain_graph=True)
+    check_grad(g, logits.detach(), 2, None, 1.0, True)
+    dw = torch.randn((40, 2), generator=gen(2)).to(cuda)
+    (g,) = torch.autograd.grad(weights, logits, dw)
+    check_grad(g, logits.detach(), 2, dw, None, True)
+    # Rows without slots: the sum runs, its gradient is refused.
+    rows = torch.arange(8, dtype=torch.int32, device=cuda).view(4, 2)
+    y = torch.randn((8, 16), device=cuda, requires_grad=True)
+    out = torch.ops.kl.moe_combine(y, None, rows)
+    with pytest.raises(RuntimeError, match="slots"):
+        out.sum().backward()
+    # Slot order, no weights: a broadcast gradient.
+    y = torch.randn((4, 2, 16), device=cuda, requires_grad=True)
+    torch.ops.kl.moe_combine(y).sum().backward()
+    assert (y.grad == 1).all()
+    q, s, _ = int4_case(cuda, 16, 64, 32, torch.bfloat16, None)
+    x = torch.randn((2, 64), generator=gen(3)).bfloat16().to(cuda)
+    assert torch.equal(torch.ops.kl.gemv_int4(x, q, s, None, 32), kl.gemv_int4(x, q, s, group=32))
