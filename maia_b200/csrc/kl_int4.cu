@@ -256,11 +256,11 @@ __global__ void __launch_bounds__(kThreads, 1) gemv_int4_kernel(const __grid_con
   l.act = reinterpret_cast<uint16_t*>(l.base + a.experts + 1);
   l.start = l.act + a.experts;
   l.list = l.start + a.experts + 1;
-  // Nothing of global memory is touched before the kernels before this one are done.
-  griddep_wait();
-  griddep_launch_dependents();
+  // Nothing of global memory is touched before the kernels before this one are done; for one matrix the
+  // schedule is worked out in their shadow.
   int passes = (a.slots + TOK - 1) / TOK, active = 0;
   if (a.ids != nullptr) {
+    griddep_wait();
     build_lists<TOK>(a, l, reinterpret_cast<int*>(smem + a.digits), &active);
     passes = l.base[active];
   }
@@ -392,26 +392,30 @@ __global__ void __launch_bounds__(kThreads, 1) gemv_int4_kernel(const __grid_con
 
   // x of a pass as digits: a warp takes 256 K-elements of a token at a time, a lane 8 of them, and loads
   // the next piece before it works on one.
+  int x_token = 0, x_half = 0;  // of the piece that is loaded; halves of a unit: kbs * 2 a token
+  uint4 x_piece = make_uint4(0, 0, 0, 0);
+  auto fetch = [&](Pass const& p) {
+    while (x_half >= kbs * 2) {
+      x_half -= kbs * 2;
+      ++x_token;
+    }
+    const int k = (kb0 * 2 + x_half) * 256 + lane * 8;
+    if (x_token < p.count)
+      x_piece = k < a.k ? *reinterpret_cast<const uint4*>(row_of(p, x_token) + k) : make_uint4(0, 0, 0, 0);
+  };
+  auto begin_x = [&](Pass const& p) {
+    x_token = 0;
+    x_half = warp;
+    fetch(p);
+  };
   auto convert = [&](Pass const& p) {
     constexpr int kLanes = 64 / NG;  // lanes of a scale group
-    int next_token = 0, next_half = warp;  // halves: kbs * 2 a token
-    uint4 next = make_uint4(0, 0, 0, 0);
-    auto fetch = [&] {
-      while (next_half >= kbs * 2) {
-        next_half -= kbs * 2;
-        ++next_token;
-      }
-      const int k = (kb0 * 2 + next_half) * 256 + lane * 8;
-      if (next_token < p.count)
-        next = k < a.k ? *reinterpret_cast<const uint4*>(row_of(p, next_token) + k) : make_uint4(0, 0, 0, 0);
-    };
-    fetch();
 #pragma unroll 1
-    while (next_token < p.count) {
-      const int token = next_token, half = next_half;
-      const uint4 u = next;
-      next_half += kWarps;
-      fetch();
+    while (x_token < p.count) {
+      const int token = x_token, half = x_half;
+      const uint4 u = x_piece;
+      x_half += kWarps;
+      fetch(p);
       // The largest |x|: both types order like their bits, with NaN above infinity.
       uint32_t m = __vmaxu2(__vmaxu2(u.x & 0x7FFF7FFFu, u.y & 0x7FFF7FFFu), __vmaxu2(u.z & 0x7FFF7FFFu, u.w & 0x7FFF7FFFu));
 #pragma unroll
@@ -559,6 +563,12 @@ __global__ void __launch_bounds__(kThreads, 1) gemv_int4_kernel(const __grid_con
   uint32_t parity = 0;
   const uint8_t *xd = smem, *xs = smem, *xp = smem;
   int k_at = 0;
+  if (a.ids == nullptr) griddep_wait();
+  griddep_launch_dependents();
+  if (remaining > 0) {  // x first: what the start waits for goes before the weights
+    p = pass_of(pass);
+    begin_x(p);
+  }
 #pragma unroll 1
   while (true) {
     // At first one unit a warp: what the start waits for does not queue behind a whole ring of weights.
@@ -573,14 +583,15 @@ __global__ void __launch_bounds__(kThreads, 1) gemv_int4_kernel(const __grid_con
       u = records[out];
       if (u.pass != at_pass) {  // every warp has a record of every batch, so all come here together
         const bool start = at_pass < 0;
+        at_pass = u.pass;
         if (start) {
           aim_scales(u);
           load_scales();
         } else {
+          p = pass_of(at_pass);
+          begin_x(p);
           __syncthreads();
         }
-        at_pass = u.pass;
-        p = pass_of(at_pass);
         convert(p);
         __syncthreads();
         if (start) continue;  // to fill the ring
