@@ -71,12 +71,14 @@ def _ptr(t):
     return None if t is None else t.data_ptr()
 
 
-def _device(*tensors) -> int:
+def _device(first, *others) -> int:
     """The one CUDA device of the tensors (None = not given)."""
-    found = {t.get_device() for t in tensors if t is not None}
-    index = found.pop()
-    if found or index < 0:
-        raise ValueError("the tensors must be on one CUDA device")
+    index = first.get_device()
+    for t in others:
+        if t is not None and t.get_device() != index:
+            raise ValueError("the tensors must be on one CUDA device")
+    if index < 0:
+        raise ValueError("the tensors must be on a CUDA device")
     return index
 
 
@@ -128,7 +130,8 @@ def moe_route(logits, k: int, *, renormalize: bool = True, valid=None, stream=No
     padding tokens hold is not read. For gradients: moe_route_grad, or torch.ops.kl.moe_route."""
     _check_logits(logits, valid)
     tokens, experts = logits.shape
-    _refuse(1 <= k <= experts, f"k must be in [1, {experts}]")
+    if not 1 <= k <= experts:
+        raise ValueError(f"k must be in [1, {experts}]")
     device = _device(logits, valid)
     ids = logits.new_empty((tokens, k), dtype=torch.int32)
     weights = logits.new_empty((tokens, k), dtype=torch.float32)
@@ -175,7 +178,8 @@ def moe_route_grad(logits, route: MoeRoute, dweights=None, dloss=None, *, renorm
 
 def moe_rows(slots: int, experts: int, block: int = 128) -> int:
     """Rows of the grouped layout that any split of `slots` rows over the experts fits (kl_moe_rows)."""
-    _refuse(slots >= 0 and experts >= 1 and block in (128, 256), "slots must not be negative, experts positive, block 128 or 256")
+    if slots < 0 or experts < 1 or block not in (128, 256):
+        raise ValueError("slots must not be negative, experts positive, block 128 or 256")
     return (slots + min(slots, experts) * (block - 1)) // block * block
 
 
@@ -189,16 +193,16 @@ def moe_plan(ids, experts: int, *, block: int = 128, stream=None) -> MoePlan:
     tokens, k = ids.shape
     m = moe_rows(tokens * k, experts, block)
     device = _device(ids)
-    plan = MoePlan(ids.new_empty((tokens, k)), ids.new_empty((m,)), ids.new_empty((m // 128,)))
+    plan = MoePlan(torch.empty_like(ids), ids.new_empty((m,)), ids.new_empty((m // 128,)))
     _queue(device, stream, plan, lib().kl_moe_plan, ids.data_ptr(), tokens, k, experts, block, m, plan.rows.data_ptr(),
            plan.slots.data_ptr(), plan.m_block_group.data_ptr())
     return plan
 
 
 def _check_plan(rows, slots) -> None:
-    _refuse(rows.dim() == 2 and slots.dim() == 1, "rows must be 2-D and slots 1-D, as moe_plan makes them")
-    _whole("rows", rows, rows.shape, torch.int32)
-    _whole("slots", slots, slots.shape, torch.int32)
+    if (rows.dim() != 2 or slots.dim() != 1 or rows.dtype is not torch.int32 or slots.dtype is not torch.int32
+            or not rows.is_contiguous() or not slots.is_contiguous()):
+        raise ValueError("rows must be 2-D and slots 1-D, contiguous int32, as moe_plan makes them")
 
 
 def moe_dispatch(x, plan: MoePlan, out=None, *, stream=None):
@@ -271,7 +275,7 @@ def moe_combine_grad(dout, y, weights=None, *, rows=None, slots=None, stream=Non
         raise ValueError(f"dout must have the shape {(tokens, width)}")
     device = _device(dout, y, weights, rows, slots)
     dy = y.new_empty(y.shape)
-    dweights = None if weights is None else weights.new_empty((tokens, k))
+    dweights = None if weights is None else torch.empty_like(weights)
     _queue(device, stream, (dy,) if dweights is None else (dy, dweights), lib().kl_moe_combine_grad, dout.data_ptr(),
            _pitch(dout), y.data_ptr(), _FLOATS[y.dtype], pitch, m, _ptr(rows), _ptr(slots), _ptr(weights), tokens, max(k, 1),
            width, dy.data_ptr(), width, _ptr(dweights))
