@@ -216,7 +216,8 @@ typedef struct kl_moe_route_desc {
   float* loss;          /* device [1] (unused by kl_moe_route_grad) */
 } kl_moe_route_desc;
 
-/* Bytes of device workspace (4-byte aligned, any contents) that kl_moe_route needs. */
+/* Bytes of device workspace (4-byte aligned, any contents) that kl_moe_route needs; 0 for a few
+ * tokens. Calls that may overlap on the GPU, two captured graphs among them, take one each. */
 KL_API kl_status kl_moe_route_workspace_size(int64_t tokens, int64_t experts, size_t* bytes);
 
 /* p = softmax(logits) in fp32 over each token's experts; ids = its k largest logits, largest first,
@@ -230,9 +231,10 @@ KL_API kl_status kl_moe_route_workspace_size(int64_t tokens, int64_t experts, si
 KL_API kl_status kl_moe_route(const kl_moe_route_desc* desc, void* workspace, size_t workspace_bytes, void* stream);
 
 /* The gradient of the logits (logits_type, [tokens, ld_dlogits]; zeros for tokens not routed) from
- * the gradients of weights (dweights, fp32 [tokens, k], NULL = 0; read only where the id is not -1)
- * and of loss (dloss, device scalar, NULL = 0). desc is kl_moe_route's, with its outputs. The counts
- * are constants here. dlogits may be the logits' own memory. */
+ * the gradients of weights (dweights, fp32 [tokens, k], NULL = 0; its values count only where the id
+ * is not -1) and of loss (dloss, device scalar, NULL = 0). desc is kl_moe_route's, with its outputs as
+ * it left them (a token's ids are distinct). The counts are constants here. dlogits may be the logits'
+ * own memory. */
 KL_API kl_status kl_moe_route_grad(const kl_moe_route_desc* desc, const float* dweights, const float* dloss, void* dlogits,
                                    int64_t ld_dlogits, void* stream);
 
@@ -271,11 +273,14 @@ KL_API kl_status kl_moe_combine_grad(const void* dout, int64_t ld_dout, const vo
                                      void* stream);
 
 /* ---- products with 4-bit weights and group scales (decode) -----------------------------------
- * out[t, n] = sum_i x[t, i] (q[n, i] - zeros[n, i / group]) scales[n, i / group], summed in fp32,
- * rounded once. With ids, one matrix per expert: out row t topk + j uses expert ids[t, j] (the
- * experts' products for single tokens, straight from kl_moe_route's ids); an id outside [0, experts)
- * gives zeros. The weights stream once for up to 32 tokens (16 of one expert). No counterpart in the
- * reference. */
+ * out[t, n] = sum_i x[t, i] (q[n, i] - zeros[n, i / group]) scales[n, i / group], rounded once. With
+ * ids, one matrix per expert: out row t topk + j uses expert ids[t, j] (the experts' products for
+ * single tokens, straight from kl_moe_route's ids; an id may repeat); an id outside [0, experts)
+ * gives zeros. x enters as a fixed-point number with 22 bits below the largest of its 128 neighbours
+ * (what an fp32 sum with that neighbour would keep); the products of a scale group are summed exactly,
+ * the groups in fp32. A NaN or infinity in a row of x makes that row of out NaN, and no other. The weights
+ * stream once for up to 16 tokens of a matrix; more take a pass for every 16. Allocates nothing, keeps
+ * nothing; stream-ordered; may be captured. No counterpart in the reference. */
 typedef struct kl_int4_desc {
   const void* x;        /* device [tokens, ldx], x_type KL_BF16 or KL_F16; 16-byte aligned, ldx % 8 == 0;
                          * x_per_slot: [tokens topk, ldx] */
@@ -291,7 +296,7 @@ typedef struct kl_int4_desc {
   int64_t experts, topk; /* with ids: tokens * topk <= 4096, experts <= 1024 */
   void* out;            /* device [tokens (* topk), ldo], x_type or KL_F32 */
   int64_t ldo;
-  int64_t tokens, n, k; /* k a multiple of 32 */
+  int64_t tokens, n, k; /* k a multiple of 32, at most 65536 */
   int64_t group;        /* 32, 64 or a multiple of 128; the last group may be short */
   int32_t x_type, scale_type, out_type, x_per_slot;
 } kl_int4_desc;
