@@ -329,10 +329,14 @@ __global__ void __launch_bounds__(kThreads, 1) gemv_int4_kernel(const __grid_con
         // microseconds.
         const Pass p = pass_of(pass);
         expert = p.expert;
-        for (int token = 0; token < p.count; ++token) {
+        // A token has 16 / TOK warps.
+        constexpr int kTokenWarps = TOK < kWarps ? kWarps / TOK : 1;
+        const int token = warp / kTokenWarps;
+        if (token < p.count) {
           const char* x = reinterpret_cast<const char*>(row_of(p, token) + kb0 * kUnitK);
           const int bytes = min(a.k - kb0 * kUnitK, kbs * kUnitK) * 2;
-          for (int i = threadIdx.x * 128; i < bytes; i += kThreads * 128) asm volatile("prefetch.global.L2 [%0];" ::"l"(x + i));
+          for (int i = (warp % kTokenWarps * 32 + lane) * 128; i < bytes; i += kTokenWarps * 32 * 128)
+            asm volatile("prefetch.global.L2 [%0];" ::"l"(x + i));
         }
       }
       count = min(kWarps, min(a.tiles - first, remaining));
