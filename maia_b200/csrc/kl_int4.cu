@@ -45,8 +45,6 @@ constexpr int kWarps = 16;
 constexpr int kThreads = 32 * kWarps;
 constexpr int kRows = 16;              // weight rows of a tile
 constexpr int kBoxBytes = kRows * 128;
-constexpr int kUnitK = 512;            // codes of a unit's row, in two boxes
-constexpr int kUnitBytes = 2 * kBoxBytes;
 constexpr int kMaxExperts = 1024;
 constexpr int kMaxSlots = 4096;        // (token, expert) pairs of a call with ids
 constexpr int kMaxK = 65536;
@@ -183,6 +181,13 @@ __device__ void build_lists(const Int4Args& a, Lists const& l, int* hist, int* a
 template <int TOK>
 constexpr int kTiles = TOK <= 2 ? 1 : TOK / 8 * 3;
 
+// Codes of a unit's row: two boxes' worth; with 16 tokens, whose digits and sums take most of the shared
+// memory, one.
+template <int TOK>
+constexpr int kUnitK = TOK <= 8 ? 512 : 256;
+template <int TOK>
+constexpr int kUnitBytes = kRows * kUnitK<TOK> / 2;
+
 // x in shared memory. Digits: for every 32 K-elements a row of 32 bytes for each column that is used. Sums D of a
 // scale group: up to two tokens: an int a column; else (D_0 + 256 D_1, D_2) a token. Powers 2^-e of 128
 // elements: up to two tokens: times 256^c, a float a column; else a float a token.
@@ -193,7 +198,7 @@ constexpr int kSumBytes = TOK <= 2 ? 32 : TOK * 8;  // of a group
 template <int TOK>
 constexpr int kPowerBytes = TOK <= 2 ? 32 : TOK * 4;  // of 128 K-elements
 template <int NG, int TOK>
-constexpr int kXBytes = 16 * kDigitRow<TOK> + NG * kSumBytes<TOK> + 4 * kPowerBytes<TOK>;  // of a unit
+constexpr int kXBytes = kUnitK<TOK> / 32 * kDigitRow<TOK> + NG * kSumBytes<TOK> + kUnitK<TOK> / 128 * kPowerBytes<TOK>;  // of a unit
 
 constexpr int kPieces = 2;  // tiles that a warp's run of units can touch
 template <int TOK>
@@ -214,14 +219,14 @@ constexpr int kNone = 4;    // the warp has no unit in this batch: a slot withou
 template <int NG, int TOK>
 size_t lay_out(Int4Args& a, int depth, int units, int cluster) {
   a.depth = depth;
-  size_t at = size_t(kWarps) * depth * kUnitBytes;
+  size_t at = size_t(kWarps) * depth * kUnitBytes<TOK>;
   auto take = [&](uint32_t& offset, size_t bytes) {
     offset = uint32_t(at);
     at += bytes;
   };
-  take(a.digits, size_t(units) * 16 * kDigitRow<TOK>);
+  take(a.digits, size_t(units) * (kUnitK<TOK> / 32) * kDigitRow<TOK>);
   take(a.sums, size_t(units) * NG * kSumBytes<TOK>);
-  take(a.powers, size_t(units) * 4 * kPowerBytes<TOK>);
+  take(a.powers, size_t(units) * (kUnitK<TOK> / 128) * kPowerBytes<TOK>);
   take(a.pieces, size_t(kWarps) * kPieces * kPiece<TOK> * 4);
   take(a.block, cluster > 1 ? size_t(2) * kWarps * kPiece<TOK> * 4 : 0);
   take(a.records, size_t(kWarps) * depth * sizeof(Stretch));
@@ -230,11 +235,12 @@ size_t lay_out(Int4Args& a, int depth, int units, int cluster) {
   return at + 1024;  // the base is rounded up to 1024
 }
 
-// NG: scale groups of a unit's 512 codes (16, 8, 4 for groups of 32, 64, multiples of 128).
+// NG: scale groups of a unit (of 512 codes 16, 8, 4 for groups of 32, 64, multiples of 128).
 template <class T, int NG, int TOK, bool kZeros>
 __global__ void __launch_bounds__(kThreads, 1) gemv_int4_kernel(const __grid_constant__ Int4Args a) {
-  constexpr int kPerGroup = 16 / NG;  // 32-code chunks of a group
-  constexpr int kHeld = NG / 4;       // scales that a lane holds of each of its rows
+  constexpr int kPerGroup = kUnitK<TOK> / 32 / NG;  // 32-code chunks of a group
+  constexpr int kHeld = NG >= 4 ? NG / 4 : 1;       // scales that a lane holds of each of its rows
+  constexpr int kHalves = kUnitK<TOK> / 256;
   constexpr uint32_t kNibbles = 0x0F0F0F0Fu;
   extern __shared__ uint8_t dynamic[];
   uint8_t* smem = dynamic + (1024 - smem_addr(dynamic) % 1024) % 1024;  // still known to be shared memory
@@ -243,7 +249,7 @@ __global__ void __launch_bounds__(kThreads, 1) gemv_int4_kernel(const __grid_con
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, g = lane / 4, t = lane % 4;
   const int depth = a.depth;
   const uint32_t bar0 = smem_addr(smem + a.bars) + warp * depth * 8;
-  const uint32_t ring0 = smem_addr(smem) + warp * depth * kUnitBytes;
+  const uint32_t ring0 = smem_addr(smem) + warp * depth * kUnitBytes<TOK>;
   Stretch* records = reinterpret_cast<Stretch*>(smem + a.records) + warp * depth;
   float* pieces = reinterpret_cast<float*>(smem + a.pieces);
   if (lane == 0) {
@@ -290,14 +296,14 @@ __global__ void __launch_bounds__(kThreads, 1) gemv_int4_kernel(const __grid_con
   };
   auto slot_of = [&](int i) { return a.ids == nullptr ? i : int(l.list[i]); };
   auto row_of = [&](Pass const& p, int token) {  // of x
-    return static_cast<const T*>(a.x) + (long long)(slot_of(p.first + token) / a.x_div) * a.ldx;
+    return static_cast<const T*>(a.x) + (long long)(a.x_div == 1 ? slot_of(p.first + token) : slot_of(p.first + token) / a.x_div) * a.ldx;
   };
 
   // This block's share of K, in units, and its cluster's tiles of all passes' tiles: the `remaining` ones from
-  // tile `first` of pass `pass`. They go in batches of up to 16 of one pass. A batch's units (tile, 512 codes of this
+  // tile `first` of pass `pass`. They go in batches of up to 16 of one pass. A batch's units (tile, 512 or 256 codes of this
   // block's K) are dealt to the warps in even, consecutive runs, so a run touches at most two tiles:
   // count kbs w / 16 units lie before warp w's, which begin in tile count w / 16.
-  const int kb_all = (a.k + kUnitK - 1) / kUnitK;
+  const int kb_all = (a.k + kUnitK<TOK> - 1) / kUnitK<TOK>;
   const int kb0 = kb_all * split / splits, kbs = kb_all * (split + 1) / splits - kb0;
   const uint32_t clusters = gridDim.x / splits, c0 = blockIdx.x / splits, all = uint32_t(passes) * a.tiles;
   const uint32_t share = all / clusters, extra = all % clusters, begin0 = c0 * share + min(c0, extra);
@@ -333,8 +339,8 @@ __global__ void __launch_bounds__(kThreads, 1) gemv_int4_kernel(const __grid_con
         constexpr int kTokenWarps = TOK < kWarps ? kWarps / TOK : 1;
         const int token = warp / kTokenWarps;
         if (token < p.count) {
-          const char* x = reinterpret_cast<const char*>(row_of(p, token) + kb0 * kUnitK);
-          const int bytes = min(a.k - kb0 * kUnitK, kbs * kUnitK) * 2;
+          const char* x = reinterpret_cast<const char*>(row_of(p, token) + kb0 * kUnitK<TOK>);
+          const int bytes = min(a.k - kb0 * kUnitK<TOK>, kbs * kUnitK<TOK>) * 2;
           for (int i = (warp % kTokenWarps * 32 + lane) * 128; i < bytes; i += kTokenWarps * 32 * 128)
             asm volatile("prefetch.global.L2 [%0];" ::"l"(x + i));
         }
@@ -360,7 +366,7 @@ __global__ void __launch_bounds__(kThreads, 1) gemv_int4_kernel(const __grid_con
     }
     run_left -= left;
     if (run_left == 0) s.flags |= kEnd;
-    load_x = (kb0 + kb) * (kUnitK / 2);
+    load_x = (kb0 + kb) * (kUnitK<TOK> / 2);
     load_y = (first + tile) * kRows;
     s.row0 = load_y;
     s.kb = kb;
@@ -373,7 +379,7 @@ __global__ void __launch_bounds__(kThreads, 1) gemv_int4_kernel(const __grid_con
   };
   // Fills ring slot `at` with the warp's next unit.
   auto produce = [&](int at) {
-    const uint32_t bar = bar0 + 8 * at, to = ring0 + at * kUnitBytes;
+    const uint32_t bar = bar0 + 8 * at, to = ring0 + at * kUnitBytes<TOK>;
     if (left == 0) {
       begin_stretch(at);
       if (left == 0) {  // nothing to load: the slot's barrier goes on to its next phase all the same
@@ -386,24 +392,25 @@ __global__ void __launch_bounds__(kThreads, 1) gemv_int4_kernel(const __grid_con
       if (failed) {
         mbarrier_arrive(bar);
       } else {
-        mbarrier_arrive_expect_tx(bar, kUnitBytes);
-        tma_load_3d(to, &a.map, bar, load_x, load_y, expert);
-        tma_load_3d(to + kBoxBytes, &a.map, bar, load_x + 128, load_y, expert);  // zeros behind K
+        mbarrier_arrive_expect_tx(bar, kUnitBytes<TOK>);
+#pragma unroll
+        for (int i = 0; i < kHalves; ++i)  // zeros behind K
+          tma_load_3d(to + i * kBoxBytes, &a.map, bar, load_x + i * 128, load_y, expert);
       }
     }
-    load_x += kUnitK / 2;
+    load_x += kUnitK<TOK> / 2;
   };
 
   // x of a pass as digits: a warp takes 256 K-elements of a token at a time, a lane 8 of them, and loads
   // the next piece before it works on one.
-  int x_token = 0, x_half = 0;  // of the piece that is loaded; halves of a unit: kbs * 2 a token
+  int x_token = 0, x_half = 0;  // of the piece that is loaded; halves of a unit: kbs * kHalves a token
   uint4 x_piece = make_uint4(0, 0, 0, 0);
   auto fetch = [&](Pass const& p) {
-    while (x_half >= kbs * 2) {
-      x_half -= kbs * 2;
+    while (x_half >= kbs * kHalves) {
+      x_half -= kbs * kHalves;
       ++x_token;
     }
-    const int k = (kb0 * 2 + x_half) * 256 + lane * 8;
+    const int k = (kb0 * kHalves + x_half) * 256 + lane * 8;
     if (x_token < p.count)
       x_piece = k < a.k ? *reinterpret_cast<const uint4*>(row_of(p, x_token) + k) : make_uint4(0, 0, 0, 0);
   };
@@ -413,7 +420,7 @@ __global__ void __launch_bounds__(kThreads, 1) gemv_int4_kernel(const __grid_con
     fetch(p);
   };
   auto convert = [&](Pass const& p) {
-    constexpr int kLanes = 64 / NG;  // lanes of a scale group
+    constexpr int kLanes = kUnitK<TOK> / NG / 8;  // lanes of a scale group
 #pragma unroll 1
     while (x_token < p.count) {
       const int token = x_token, half = x_half;
@@ -467,7 +474,7 @@ __global__ void __launch_bounds__(kThreads, 1) gemv_int4_kernel(const __grid_con
         *reinterpret_cast<uint2*>(to + (TOK <= 2 ? (c * TOK + token) * 32 : (token / 8 * 3 + c) * 256 + token % 8 * 32)) = d[c];
       const int s0 = int(int16_t(low)), s1 = (low - s0) >> 16;
       if (lane % kLanes == 0) {
-        uint8_t* to_sum = smem + a.sums + (half * (NG / 2) + lane / kLanes) * kSumBytes<TOK>;
+        uint8_t* to_sum = smem + a.sums + (half * (32 / kLanes) + lane / kLanes) * kSumBytes<TOK>;
         if constexpr (TOK <= 2) {
           int* f = reinterpret_cast<int*>(to_sum) + token;
           f[0] = s0;
@@ -513,7 +520,7 @@ __global__ void __launch_bounds__(kThreads, 1) gemv_int4_kernel(const __grid_con
 #pragma unroll
     for (int h = 0; h < kHeld; ++h) {
       int gi = s_kb * NG + t + 4 * h;
-      if (NG == 4 && a.group_span != 1) gi /= a.group_span;
+      if (kPerGroup == 4 && a.group_span != 1) gi /= a.group_span;
       gi = min(gi, a.last_group);
 #pragma unroll
       for (int r = 0; r < 2; ++r) {
@@ -601,10 +608,10 @@ __global__ void __launch_bounds__(kThreads, 1) gemv_int4_kernel(const __grid_con
         if (start) continue;  // to fill the ring
       }
       now_left = max(u.units, 1);
-      k_at = (kb0 + u.kb) * kUnitK;
-      xd = smem + a.digits + u.kb * 16 * kDigitRow<TOK> + digit_lane;
+      k_at = (kb0 + u.kb) * kUnitK<TOK>;
+      xd = smem + a.digits + u.kb * (kUnitK<TOK> / 32) * kDigitRow<TOK> + digit_lane;
       xs = smem + a.sums + u.kb * NG * kSumBytes<TOK> + t * (TOK <= 2 ? 8 : 16);
-      xp = smem + a.powers + u.kb * 4 * kPowerBytes<TOK> + t * 8;
+      xp = smem + a.powers + u.kb * (kUnitK<TOK> / 128) * kPowerBytes<TOK> + t * 8;
 #pragma unroll
       for (int set = 0; set < kSets; ++set) acc[set][0] = acc[set][1] = acc[set][2] = acc[set][3] = 0.0f;
     }
@@ -627,10 +634,10 @@ __global__ void __launch_bounds__(kThreads, 1) gemv_int4_kernel(const __grid_con
     if ((u.flags & kNone) == 0) {
       if (!failed) failed = __any_sync(0xFFFFFFFFu, !mbarrier_wait(bar0 + 8 * out, parity, a.timeout_ns));
       if (!failed) {
-        const uint32_t base = ring0 + out * kUnitBytes + in_box;
-        const bool whole = k_at + kUnitK / 2 < a.k;
+        const uint32_t base = ring0 + out * kUnitBytes<TOK> + in_box;
+        const bool whole = kHalves == 1 || k_at + 256 < a.k;
 #pragma unroll
-        for (int quarter = 0; quarter < 4; ++quarter) {  // 128 codes
+        for (int quarter = 0; quarter < kUnitK<TOK> / 128; ++quarter) {  // 128 codes
           if (quarter == 2 && !whole) break;
           int part[kTiles<TOK>][4];
           float sum[kSets][4] = {};
@@ -687,7 +694,7 @@ __global__ void __launch_bounds__(kThreads, 1) gemv_int4_kernel(const __grid_con
             for (int i = 0; i < 4; ++i) acc[set][i] = fmaf(i % 2 ? q.y : q.x, sum[set][i], acc[set][i]);
           }
           // The next quarter's groups in front, where this one's were a lane's last.
-          if (kHeld > 1 && (kHeld == 4 || quarter == 1)) {
+          if (kHeld > 1 && (quarter + 1) * (4 / kPerGroup) % 4 == 0) {
 #pragma unroll
             for (int r = 0; r < 2; ++r)
 #pragma unroll
@@ -697,10 +704,10 @@ __global__ void __launch_bounds__(kThreads, 1) gemv_int4_kernel(const __grid_con
               }
           }
         }
-        xd += 16 * kDigitRow<TOK>;
+        xd += kUnitK<TOK> / 32 * kDigitRow<TOK>;
         xs += NG * kSumBytes<TOK>;
-        xp += 4 * kPowerBytes<TOK>;
-        k_at += kUnitK;
+        xp += kUnitK<TOK> / 128 * kPowerBytes<TOK>;
+        k_at += kUnitK<TOK>;
         __syncwarp();  // the slot is read
       }
     }
@@ -797,7 +804,7 @@ struct Fit {
 template <int NG, int TOK>
 Fit fit(Int4Args const& a) {
   Fit f = {1, 0, 0, {}};
-  const int kb = (a.k + kUnitK - 1) / kUnitK;
+  const int kb = (a.k + kUnitK<TOK> - 1) / kUnitK<TOK>;
   auto units = [&] { return (kb + f.cluster - 1) / f.cluster; };
   while (f.cluster < 8 && size_t(units()) * kXBytes<NG, TOK> > 80 * 1024) f.cluster *= 2;
   Int4Args b = a;
@@ -852,25 +859,25 @@ kl_status launch(Fit const& f, int device, cudaStream_t stream) {
 }
 
 // Tokens of a pass by what a matrix meets (with ids: on average), fewer where x's digits would not fit.
-template <class T, int NG, bool kZeros>
+template <class T, int GROUP, bool kZeros>
 kl_status by_tokens(Int4Args& a, int device, cudaStream_t stream) {
   const int tokens = a.ids != nullptr ? (a.slots + a.experts - 1) / a.experts : a.slots;
   if (tokens > 8)
-    if (const Fit f = fit<NG, 16>(a); f.depth >= 2) return launch<T, NG, 16, kZeros>(f, device, stream);
+    if (const Fit f = fit<kUnitK<16> / GROUP, 16>(a); f.depth >= 2) return launch<T, kUnitK<16> / GROUP, 16, kZeros>(f, device, stream);
   if (tokens > 2)
-    if (const Fit f = fit<NG, 8>(a); f.depth >= 2) return launch<T, NG, 8, kZeros>(f, device, stream);
+    if (const Fit f = fit<kUnitK<8> / GROUP, 8>(a); f.depth >= 2) return launch<T, kUnitK<8> / GROUP, 8, kZeros>(f, device, stream);
   if (a.slots > 1)
-    if (const Fit f = fit<NG, 2>(a); f.depth >= 2) return launch<T, NG, 2, kZeros>(f, device, stream);
-  const Fit f = fit<NG, 1>(a);
+    if (const Fit f = fit<kUnitK<2> / GROUP, 2>(a); f.depth >= 2) return launch<T, kUnitK<2> / GROUP, 2, kZeros>(f, device, stream);
+  const Fit f = fit<kUnitK<1> / GROUP, 1>(a);
   if (f.depth < 2) return fail(KL_ERR_NOT_SUPPORTED, "kl_gemv_int4: k does not fit");
-  return launch<T, NG, 1, kZeros>(f, device, stream);
+  return launch<T, kUnitK<1> / GROUP, 1, kZeros>(f, device, stream);
 }
 
 template <class T, bool kZeros>
 kl_status by_group(Int4Args& a, int device, cudaStream_t stream) {
-  if (a.group == 32) return by_tokens<T, 16, kZeros>(a, device, stream);
-  if (a.group == 64) return by_tokens<T, 8, kZeros>(a, device, stream);
-  return by_tokens<T, 4, kZeros>(a, device, stream);
+  if (a.group == 32) return by_tokens<T, 32, kZeros>(a, device, stream);
+  if (a.group == 64) return by_tokens<T, 64, kZeros>(a, device, stream);
+  return by_tokens<T, 128, kZeros>(a, device, stream);
 }
 
 template <class T>
