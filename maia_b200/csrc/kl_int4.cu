@@ -93,6 +93,91 @@ __device__ __forceinline__ void mma_u8s8(int (&d)[4], const uint32_t (&a)[4], ui
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b.x), "r"(b.y));
 }
 
+template <class T>
+__device__ __forceinline__ void mma_16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, bool first) {
+  constexpr bool kBf16 = std::is_same_v<T, __nv_bfloat16>;
+#define KL_MMA(TYPE)                                                                                                  \
+  if (first)                                                                                                          \
+    asm("mma.sync.aligned.m16n8k16.row.col.f32." TYPE "." TYPE                                                        \
+        ".f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"                                    \
+        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])                                                              \
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.0f));                                   \
+  else                                                                                                                \
+    asm("mma.sync.aligned.m16n8k16.row.col.f32." TYPE "." TYPE                                                        \
+        ".f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"                                        \
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])                                                              \
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1))
+  if constexpr (kBf16) {
+    KL_MMA("bf16");
+  } else {
+    KL_MMA("f16");
+  }
+#undef KL_MMA
+}
+
+// Zero point z (z2: with 16 bits a value) as the unpacking below takes it off, and codes - z of a word's eight codes,
+// exactly, in pairs (0, 4), (1, 5), (2, 6), (3, 7). A code's bits below those of 128 (bf16) or 1024 (f16) make 128 + q
+// or 1024 + q; f16 has room for 1024 + 16 q too, which spares shifts.
+__device__ __forceinline__ uint32_t and_or(uint32_t a, uint32_t mask, uint32_t bits) {
+  uint32_t r;
+  asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(r) : "r"(a), "r"(mask), "r"(bits));
+  return r;
+}
+__device__ __forceinline__ uint32_t fma_bf16(uint32_t a, uint32_t b, uint32_t c) {
+  uint32_t r;
+  asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(a), "r"(b), "r"(c));
+  return r;
+}
+__device__ __forceinline__ uint32_t fma_f16(uint32_t a, uint32_t b, uint32_t c) {
+  uint32_t r;
+  asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(a), "r"(b), "r"(c));
+  return r;
+}
+template <class T>
+__device__ __forceinline__ uint32_t pack_two(float v) {
+  const T b = from_f32<T>(v);
+  uint16_t u;
+  memcpy(&u, &b, 2);
+  return u * 0x10001u;
+}
+// A constant that stays in its register: else the compiler makes it anew for every use, at an instruction each.
+__device__ __forceinline__ uint32_t held(uint32_t v) {
+  uint32_t r;
+  asm volatile("mov.b32 %0, %1;" : "=r"(r) : "r"(v));
+  return r;
+}
+template <class T>
+struct Codes;
+template <>
+struct Codes<__nv_bfloat16> {
+  uint32_t mask = held(0x000F000Fu), bits = held(0x43004300u), one = held(0x3F803F80u);
+  struct Zero {
+    uint32_t z;  // -(128 + z)
+  };
+  __device__ __forceinline__ Zero zero(uint32_t z2) const { return {0xC300C300u | z2}; }
+  __device__ __forceinline__ void minus(uint32_t w, Zero z, uint32_t (&r)[4]) const {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) r[i] = fma_bf16(and_or(w >> 4 * i, mask, bits), one, z.z);
+  }
+};
+template <>
+struct Codes<__half> {
+  uint32_t mask = held(0x000F000Fu), mask16 = held(0x00F000F0u), bits = held(0x64006400u), one = held(0x3C003C00u),
+           sixteenth = held(0x2C002C00u);
+  struct Zero {
+    uint32_t z, z16;  // -(1024 + z), -(64 + z)
+  };
+  __device__ __forceinline__ Zero zero(uint32_t z2) const { return {0xE400E400u | z2, fma_f16(0xE400E400u | z2, one, 0x63806380u)}; }
+  __device__ __forceinline__ void minus(uint32_t w, Zero z, uint32_t (&r)[4]) const {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const uint32_t v = w >> 8 * i;
+      r[2 * i] = fma_f16(and_or(v, mask, bits), one, z.z);
+      r[2 * i + 1] = fma_f16(and_or(v, mask16, bits), sixteenth, z.z16);
+    }
+  }
+};
+
 // With ids: the experts that some slot names, each with its slots, in shared memory.
 struct Lists {
   int* base;        // [experts + 1]: token passes before an active expert
@@ -175,30 +260,29 @@ __device__ void build_lists(const Int4Args& a, Lists const& l, int* hist, int* a
   *active_out = active;
 }
 
-// TOK: tokens of a pass, 1, 2, 8 or 16. Columns of the products: three digits of 8 tokens are three 8-column
-// tiles, digit c of token i in column i of tile c, so a lane holds the digits of the same tokens; up to two tokens
-// fit one tile, digit c of token i in column 2 c + i, and the digits meet by shuffles.
+// TOK: tokens of a pass, 1, 2, 8 or 16. Up to two go by the integer products: three digits of two tokens fit one
+// 8-column tile, digit c of token i in column 2 c + i, and the digits meet by shuffles. 8 and 16 would take three and six
+// tiles; with them the codes are turned into x's type and each 8 tokens are one tile.
 template <int TOK>
-constexpr int kTiles = TOK <= 2 ? 1 : TOK / 8 * 3;
+constexpr bool kDigits = TOK <= 2;
 
-// Codes of a unit's row: two boxes' worth; with 16 tokens, whose digits and sums take most of the shared
-// memory, one.
+// Codes of a unit's row: two boxes' worth; with 16 tokens one.
 template <int TOK>
 constexpr int kUnitK = TOK <= 8 ? 512 : 256;
 template <int TOK>
 constexpr int kUnitBytes = kRows * kUnitK<TOK> / 2;
 
-// x in shared memory. Digits: for every 32 K-elements a row of 32 bytes for each column that is used. Sums D of a
-// scale group: up to two tokens: an int a column; else (D_0 + 256 D_1, D_2) a token. Powers 2^-e of 128
-// elements: up to two tokens: times 256^c, a float a column; else a float a token.
+// x in shared memory, by 32 K-elements. Digits: a row of 32 bytes for each column that is used; sums D of a scale
+// group, an int a column; powers 2^-e of 128 elements, times 256^c, a float a column. Else: 64 bytes a token, every eight
+// elements in the order of the codes' pairs.
 template <int TOK>
-constexpr int kDigitRow = TOK <= 2 ? TOK * 96 : kTiles<TOK> * 256;  // bytes of 32 K-elements
+constexpr int kXRow = kDigits<TOK> ? TOK * 96 : TOK * 64;  // bytes of 32 K-elements
 template <int TOK>
-constexpr int kSumBytes = TOK <= 2 ? 32 : TOK * 8;  // of a group
+constexpr int kSumBytes = kDigits<TOK> ? 32 : 0;  // of a group
 template <int TOK>
-constexpr int kPowerBytes = TOK <= 2 ? 32 : TOK * 4;  // of 128 K-elements
+constexpr int kPowerBytes = kDigits<TOK> ? 32 : 0;  // of 128 K-elements
 template <int NG, int TOK>
-constexpr int kXBytes = kUnitK<TOK> / 32 * kDigitRow<TOK> + NG * kSumBytes<TOK> + kUnitK<TOK> / 128 * kPowerBytes<TOK>;  // of a unit
+constexpr int kXBytes = kUnitK<TOK> / 32 * kXRow<TOK> + NG * kSumBytes<TOK> + kUnitK<TOK> / 128 * kPowerBytes<TOK>;  // of a unit
 
 constexpr int kPieces = 2;  // tiles that a warp's run of units can touch
 template <int TOK>
@@ -224,7 +308,7 @@ size_t lay_out(Int4Args& a, int depth, int units, int cluster) {
     offset = uint32_t(at);
     at += bytes;
   };
-  take(a.digits, size_t(units) * (kUnitK<TOK> / 32) * kDigitRow<TOK>);
+  take(a.digits, size_t(units) * (kUnitK<TOK> / 32) * kXRow<TOK>);
   take(a.sums, size_t(units) * NG * kSumBytes<TOK>);
   take(a.powers, size_t(units) * (kUnitK<TOK> / 128) * kPowerBytes<TOK>);
   take(a.pieces, size_t(kWarps) * kPieces * kPiece<TOK> * 4);
@@ -427,6 +511,12 @@ __global__ void __launch_bounds__(kThreads, 1) gemv_int4_kernel(const __grid_con
       const uint4 u = x_piece;
       x_half += kWarps;
       fetch(p);
+      uint8_t* to = smem + a.digits + (half * 8 + lane / 4) * kXRow<TOK>;
+      if constexpr (!kDigits<TOK>) {
+        *reinterpret_cast<uint4*>(to + token * 64 + lane % 4 * 16) =
+            make_uint4(__byte_perm(u.x, u.z, 0x5410), __byte_perm(u.x, u.z, 0x7632), __byte_perm(u.y, u.w, 0x5410), __byte_perm(u.y, u.w, 0x7632));
+        continue;
+      }
       // The largest |x|: both types order like their bits, with NaN above infinity.
       uint32_t m = __vmaxu2(__vmaxu2(u.x & 0x7FFF7FFFu, u.y & 0x7FFF7FFFu), __vmaxu2(u.z & 0x7FFF7FFFu, u.w & 0x7FFF7FFFu));
 #pragma unroll
@@ -468,30 +558,21 @@ __global__ void __launch_bounds__(kThreads, 1) gemv_int4_kernel(const __grid_con
         low += __shfl_xor_sync(0xFFFFFFFFu, low, o);
         high += __shfl_xor_sync(0xFFFFFFFFu, high, o);
       }
-      uint8_t* to = smem + a.digits + (half * 8 + lane / 4) * kDigitRow<TOK> + lane % 4 * 8;
 #pragma unroll
-      for (int c = 0; c < 3; ++c)
-        *reinterpret_cast<uint2*>(to + (TOK <= 2 ? (c * TOK + token) * 32 : (token / 8 * 3 + c) * 256 + token % 8 * 32)) = d[c];
+      for (int c = 0; c < 3; ++c) *reinterpret_cast<uint2*>(to + (c * TOK + token) * 32 + lane % 4 * 8) = d[c];
       const int s0 = int(int16_t(low)), s1 = (low - s0) >> 16;
       if (lane % kLanes == 0) {
-        uint8_t* to_sum = smem + a.sums + (half * (32 / kLanes) + lane / kLanes) * kSumBytes<TOK>;
-        if constexpr (TOK <= 2) {
-          int* f = reinterpret_cast<int*>(to_sum) + token;
-          f[0] = s0;
-          f[2] = s1;
-          f[4] = high;
-        } else {
-          reinterpret_cast<int2*>(to_sum)[token] = make_int2(s0 + 256 * s1, high);
-        }
+        int* f = reinterpret_cast<int*>(smem + a.sums + (half * (32 / kLanes) + lane / kLanes) * kSumBytes<TOK>) + token;
+        f[0] = s0;
+        f[2] = s1;
+        f[4] = high;
       }
       if (lane % 16 == 0) {
         const float down = bad ? NAN : __int_as_float((127 - e) << 23);
         float* f = reinterpret_cast<float*>(smem + a.powers + (half * 2 + lane / 16) * kPowerBytes<TOK>) + token;
         f[0] = down;
-        if (TOK <= 2) {
-          f[2] = down * 256.0f;
-          f[4] = down * 65536.0f;
-        }
+        f[2] = down * 256.0f;
+        f[4] = down * 65536.0f;
       }
     }
   };
@@ -544,11 +625,11 @@ __global__ void __launch_bounds__(kThreads, 1) gemv_int4_kernel(const __grid_con
     else static_cast<T*>(a.out)[o] = from_f32<T>(v);
   };
 
-  constexpr int kSets = TOK <= 2 ? 1 : TOK / 8;  // of up to 8 tokens
+  constexpr int kSets = TOK <= 8 ? 1 : TOK / 8;  // of up to 8 tokens
   // Where a lane reads: its ldmatrix rows in a box (swizzled by 16 bytes), its column's digits (a column that
-  // nothing uses reads another's).
+  // nothing uses reads another's) or its token's elements.
   const uint32_t in_box = lane % 16 * 128 + ((lane / 16 ^ (lane & 7)) * 16);
-  const int digit_lane = t * 8 + (TOK > 2 ? g * 32 : g >= 6 ? 0 : TOK == 2 ? g * 32 : g % 2 ? 0 : g / 2 * 32);
+  const int x_lane = !kDigits<TOK> ? lane * 16 : t * 8 + (g >= 6 ? 0 : TOK == 2 ? g * 32 : g % 2 ? 0 : g / 2 * 32);
   // A batch's sums of the cluster's blocks, a tile to a block in turn. They are gathered a batch later, when the
   // others' have long arrived; two buffers: by then every block has left the one that is written next.
   Stretch gathers = {};
@@ -566,6 +647,7 @@ __global__ void __launch_bounds__(kThreads, 1) gemv_int4_kernel(const __grid_con
     }
     __syncwarp();
   };
+  const Codes<T> codes;
   float acc[kSets][4] = {};
   Pass p = {};
   Stretch u = {};
@@ -609,8 +691,8 @@ __global__ void __launch_bounds__(kThreads, 1) gemv_int4_kernel(const __grid_con
       }
       now_left = max(u.units, 1);
       k_at = (kb0 + u.kb) * kUnitK<TOK>;
-      xd = smem + a.digits + u.kb * (kUnitK<TOK> / 32) * kDigitRow<TOK> + digit_lane;
-      xs = smem + a.sums + u.kb * NG * kSumBytes<TOK> + t * (TOK <= 2 ? 8 : 16);
+      xd = smem + a.digits + u.kb * (kUnitK<TOK> / 32) * kXRow<TOK> + x_lane;
+      xs = smem + a.sums + u.kb * NG * kSumBytes<TOK> + t * 8;
       xp = smem + a.powers + u.kb * (kUnitK<TOK> / 128) * kPowerBytes<TOK> + t * 8;
 #pragma unroll
       for (int set = 0; set < kSets; ++set) acc[set][0] = acc[set][1] = acc[set][2] = acc[set][3] = 0.0f;
@@ -639,8 +721,12 @@ __global__ void __launch_bounds__(kThreads, 1) gemv_int4_kernel(const __grid_con
 #pragma unroll
         for (int quarter = 0; quarter < kUnitK<TOK> / 128; ++quarter) {  // 128 codes
           if (quarter == 2 && !whole) break;
-          int part[kTiles<TOK>][4];
-          float sum[kSets][4] = {};
+          constexpr int kGroups = 4 / kPerGroup;  // of a quarter
+          int part[4];                            // of a group
+          float sum[4] = {};                      // of the quarter
+          float dot[kSets][4];                    // of a group
+          float sc[2];
+          uint32_t z[2] = {8, 8};
 #pragma unroll
           for (int pair = 0; pair < 2; ++pair) {
             // Matrices: rows 0-7 and 8-15 of chunk 2 pair, then of chunk 2 pair + 1.
@@ -648,50 +734,61 @@ __global__ void __launch_bounds__(kThreads, 1) gemv_int4_kernel(const __grid_con
             ldmatrix_x4(w, (base + quarter / 2 * kBoxBytes) ^ (quarter % 2 * 64 + pair * 32));
 #pragma unroll
             for (int cc = 0; cc < 2; ++cc) {
-              constexpr int kGroups = 4 / kPerGroup;  // of a quarter
-              const int c = pair * 2 + cc;
-              const uint32_t f[4] = {w[2 * cc] & kNibbles, w[2 * cc + 1] & kNibbles, (w[2 * cc] >> 4) & kNibbles,
-                                     (w[2 * cc + 1] >> 4) & kNibbles};
-              const uint8_t* xc = xd + (quarter * 4 + c) * kDigitRow<TOK>;
+              const int c = pair * 2 + cc, gj = c / kPerGroup;
+              const bool begins = c % kPerGroup == 0, ends = c % kPerGroup == kPerGroup - 1;
+              const uint8_t* xc = xd + (quarter * 4 + c) * kXRow<TOK>;
+              if (begins) {
+                const int from = (lane & 28) | ((quarter * kGroups + gj) & 3);
 #pragma unroll
-              for (int j = 0; j < kTiles<TOK>; ++j) {
-                if (j >= 3 && p.count <= 8) continue;
-                mma_u8s8(part[j], f, *reinterpret_cast<const uint2*>(xc + j * 256), c % kPerGroup == 0);
+                for (int r = 0; r < 2; ++r) {
+                  sc[r] = __shfl_sync(0xFFFFFFFFu, s_now[r][0], from);
+                  if (kZeros) z[r] = __shfl_sync(0xFFFFFFFFu, z_now[r][0], from);
+                }
               }
-              if (c % kPerGroup != kPerGroup - 1) continue;
-              const int gj = c / kPerGroup, from = (lane & 28) | ((quarter * kGroups + gj) & 3);
-              float sc[2];
-              int z[2] = {8, 8};
-#pragma unroll
-              for (int r = 0; r < 2; ++r) {
-                sc[r] = __shfl_sync(0xFFFFFFFFu, s_now[r][0], from);
-                if (kZeros) z[r] = int(__shfl_sync(0xFFFFFFFFu, z_now[r][0], from));
-              }
-              if constexpr (TOK <= 2) {
+              if constexpr (kDigits<TOK>) {
+                const uint32_t f[4] = {w[2 * cc] & kNibbles, w[2 * cc + 1] & kNibbles, (w[2 * cc] >> 4) & kNibbles,
+                                       (w[2 * cc + 1] >> 4) & kNibbles};
+                mma_u8s8(part, f, *reinterpret_cast<const uint2*>(xc), begins);
+                if (!ends) continue;
                 const int2 q = *reinterpret_cast<const int2*>(xs + (quarter * kGroups + gj) * kSumBytes<TOK>);
 #pragma unroll
-                for (int i = 0; i < 4; ++i) sum[0][i] = fmaf(sc[i / 2], float(part[0][i] - z[i / 2] * (i % 2 ? q.y : q.x)), sum[0][i]);
+                for (int i = 0; i < 4; ++i) sum[i] = fmaf(sc[i / 2], float(part[i] - int(z[i / 2]) * (i % 2 ? q.y : q.x)), sum[i]);
               } else {
+                // bf16 has 128 + z for z up to 127; what is above goes into a product of its own.
+                constexpr uint32_t kMaxZ = std::is_same_v<T, __nv_bfloat16> ? 127 : 255;
+                const auto z0 = codes.zero(kZeros ? min(z[0], kMaxZ) * 0x10001u : 0x00080008u);
+                const auto z1 = codes.zero(kZeros ? min(z[1], kMaxZ) * 0x10001u : 0x00080008u);
+                uint32_t f0[4], f1[4];
+                codes.minus(w[2 * cc], z0, f0);
+                codes.minus(w[2 * cc + 1], z1, f1);
+                const uint32_t fa[4] = {f0[0], f1[0], f0[1], f1[1]}, fb[4] = {f0[2], f1[2], f0[3], f1[3]};
+                bool more = false;
+                if (kZeros && kMaxZ < 255) more = __any_sync(0xFFFFFFFFu, max(z[0], z[1]) > kMaxZ);
 #pragma unroll
                 for (int set = 0; set < kSets; ++set) {
                   if (set > 0 && p.count <= 8) continue;
-                  const int4 q = *reinterpret_cast<const int4*>(xs + (quarter * kGroups + gj) * kSumBytes<TOK> + set * 64);
+                  const uint4 q = *reinterpret_cast<const uint4*>(xc + set * 512);
+                  mma_16<T>(dot[set], fa, q.x, q.y, begins);
+                  mma_16<T>(dot[set], fb, q.z, q.w, false);
+                  if (more) {
+                    uint32_t rest[2];
 #pragma unroll
-                  for (int i = 0; i < 4; ++i) {
-                    // |256 P_1 + P_0| and z times its sums stay below 2^30.
-                    const int low = part[3 * set + 1][i] * 256 + part[3 * set][i] - z[i / 2] * (i % 2 ? q.z : q.x);
-                    const int high = part[3 * set + 2][i] - z[i / 2] * (i % 2 ? q.w : q.y);
-                    sum[set][i] = fmaf(sc[i / 2], fmaf(float(high), 65536.0f, float(low)), sum[set][i]);
+                    for (int r = 0; r < 2; ++r) rest[r] = pack_two<T>(-float(max(z[r], kMaxZ) - kMaxZ));
+                    const uint32_t fr[4] = {rest[0], rest[1], rest[0], rest[1]};
+                    mma_16<T>(dot[set], fr, q.x, q.y, false);
+                    mma_16<T>(dot[set], fr, q.z, q.w, false);
                   }
+                  if (!ends) continue;
+#pragma unroll
+                  for (int i = 0; i < 4; ++i) acc[set][i] = fmaf(sc[i / 2], dot[set][i], acc[set][i]);
                 }
               }
             }
           }
+          if constexpr (kDigits<TOK>) {
+            const float2 q = *reinterpret_cast<const float2*>(xp + quarter * kPowerBytes<TOK>);
 #pragma unroll
-          for (int set = 0; set < kSets; ++set) {
-            const float2 q = *reinterpret_cast<const float2*>(xp + quarter * kPowerBytes<TOK> + set * 32);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) acc[set][i] = fmaf(i % 2 ? q.y : q.x, sum[set][i], acc[set][i]);
+            for (int i = 0; i < 4; ++i) acc[0][i] = fmaf(i % 2 ? q.y : q.x, sum[i], acc[0][i]);
           }
           // The next quarter's groups in front, where this one's were a lane's last.
           if (kHeld > 1 && (quarter + 1) * (4 / kPerGroup) % 4 == 0) {
@@ -704,7 +801,7 @@ __global__ void __launch_bounds__(kThreads, 1) gemv_int4_kernel(const __grid_con
               }
           }
         }
-        xd += kUnitK<TOK> / 32 * kDigitRow<TOK>;
+        xd += kUnitK<TOK> / 32 * kXRow<TOK>;
         xs += NG * kSumBytes<TOK>;
         xp += kUnitK<TOK> / 128 * kPowerBytes<TOK>;
         k_at += kUnitK<TOK>;
@@ -717,7 +814,7 @@ __global__ void __launch_bounds__(kThreads, 1) gemv_int4_kernel(const __grid_con
       // count kbs (w + 1) / 16), tile m's units [m kbs, (m + 1) kbs).
       const bool full = u.count == kWarps;
       auto spread = [&](auto&& f) {  // f(cell, sum) for this lane's cells of the tile
-        if constexpr (TOK <= 2) {
+        if constexpr (kDigits<TOK>) {
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             const float v0 = __shfl_sync(0xFFFFFFFFu, acc[0][i], lane & 28), v1 = __shfl_sync(0xFFFFFFFFu, acc[0][i], (lane & 28) | 1),
@@ -799,23 +896,25 @@ struct Fit {
   Int4Args args;  // with the layout
 };
 
-// The smallest cluster whose blocks keep x's digits in 80 KB, else 8, and the ring that the rest holds (at
-// most 8 slots a warp, 256 KB in flight). depth 0: does not fit.
+// The smallest cluster whose blocks keep x in 80 KB beside a ring of two slots a warp, else 8, and the ring that the
+// rest holds (at most 8 slots a warp, 256 KB in flight). depth 0: does not fit.
 template <int NG, int TOK>
 Fit fit(Int4Args const& a) {
-  Fit f = {1, 0, 0, {}};
   const int kb = (a.k + kUnitK<TOK> - 1) / kUnitK<TOK>;
-  auto units = [&] { return (kb + f.cluster - 1) / f.cluster; };
-  while (f.cluster < 8 && size_t(units()) * kXBytes<NG, TOK> > 80 * 1024) f.cluster *= 2;
-  Int4Args b = a;
-  for (int depth = 2; depth <= 8; ++depth) {
-    const size_t bytes = lay_out<NG, TOK>(b, depth, units(), f.cluster);
-    if (bytes > size_t(kSmemLimit)) break;
-    f.depth = depth;
-    f.bytes = bytes;
-    f.args = b;
+  Fit f = {1, 0, 0, {}};
+  for (;; f.cluster *= 2) {
+    const int units = (kb + f.cluster - 1) / f.cluster;
+    Int4Args b = a;
+    for (int depth = 2; depth <= 8; ++depth) {
+      const size_t bytes = lay_out<NG, TOK>(b, depth, units, f.cluster);
+      if (bytes > size_t(kSmemLimit)) break;
+      f.depth = depth;
+      f.bytes = bytes;
+      f.args = b;
+    }
+    if (f.cluster == 8 || (f.depth >= 2 && size_t(units) * kXBytes<NG, TOK> <= 80 * 1024)) return f;
+    f.depth = 0;
   }
-  return f;
 }
 
 template <class T, int NG, int TOK, bool kZeros>
