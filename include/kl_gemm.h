@@ -276,10 +276,12 @@ KL_API kl_status kl_moe_combine_grad(const void* dout, int64_t ld_dout, const vo
  * out[t, n] = sum_i x[t, i] (q[n, i] - zeros[n, i / group]) scales[n, i / group], rounded once. With
  * ids, one matrix per expert: out row t topk + j uses expert ids[t, j] (the experts' products for
  * single tokens, straight from kl_moe_route's ids; an id may repeat); an id outside [0, experts)
- * gives zeros. x enters as a fixed-point number with 22 bits below the largest of its 128 neighbours
- * (what an fp32 sum with that neighbour would keep); the products of a scale group are summed exactly,
- * the groups in fp32. A NaN or infinity in a row of x makes that row of out NaN, and no other. The weights
- * stream once for up to 16 tokens of a matrix; more take a pass for every 16. Allocates nothing, keeps
+ * gives zeros. All sums are kept in fp32 or exactly: with up to two tokens to a matrix x enters as a
+ * fixed-point number with 22 bits below the largest of its 128 neighbours (what an fp32 sum with that
+ * neighbour would keep) and a scale group's products are summed exactly; with more, q - zeros and x enter
+ * as they are and every sum is fp32. A NaN or infinity in a row of x makes that row of out NaN or
+ * infinite, and no other. The weights stream once for up to 16 tokens of a matrix; more take a pass for
+ * every 16. Allocates nothing, keeps
  * nothing; stream-ordered; may be captured. No counterpart in the reference. */
 typedef struct kl_int4_desc {
   const void* x;        /* device [tokens, ldx], x_type KL_BF16 or KL_F16; 16-byte aligned, ldx % 8 == 0;
@@ -290,7 +292,7 @@ typedef struct kl_int4_desc {
   int64_t ldq, stride_q;
   const void* scales;   /* device [n, ld_scales], one per `group` K-elements, x_type or KL_F32 */
   int64_t ld_scales, stride_scales;
-  const uint8_t* zeros; /* device [n, ld_zeros], values 0 .. 127, or NULL: 8 everywhere */
+  const uint8_t* zeros; /* device [n, ld_zeros], or NULL: 8 everywhere */
   int64_t ld_zeros, stride_zeros;
   const int32_t* ids;   /* device [tokens, topk] or NULL: one matrix */
   int64_t experts, topk; /* with ids: tokens * topk <= 4096, experts <= 1024 */

@@ -2,21 +2,30 @@
 //   out[t, n] = sum_g s[n, g] sum_{i in g} (q[n, i] - z[n, g]) x[t, i],
 // with one matrix, or one per expert and the expert of every (token, slot) in `ids`.
 //
-// The weights' bytes should bound it, so a code may cost little: at 6.5 TB/s an SM gets 46 codes a
-// cycle. Turned into bf16, eight codes cost eleven instructions and the SM, not the memory, sets the
-// time (measured: 2.0 TB/s). As unsigned bytes they cost three (two masks and a shift), so the products
-// are integer ones (mma.sync.m16n8k32, u8 x s8 -> s32): every block first writes x as fixed-point numbers
-// X = round(x 2^e), |X| <= 2^22, one e for 128 K-elements of a token, in three signed digits of 8 bits,
-//   x ~ 2^-e (d_0 + 256 d_1 + 65536 d_2).
-// This rounding is at most 2^-22 of the 128 elements' largest |x|, what one addition in fp32 loses. The sums
-// of a scale group are exact: P_c = sum q d_c, and P_c - z D_c, D_c = sum d_c, takes the zero point off without
-// cancellation. Only then come fp32 and the scales: sum over the 128s of 2^-e sum_g s 256^c (P_c - z D_c).
+// The weights' bytes should bound it, so a code may cost little: at 6.5 TB/s an SM gets 46 codes a cycle and has 128
+// lanes' instructions for them.
+//
+// One and two tokens. As unsigned bytes eight codes cost three instructions (two masks and a shift), so the products are
+// integer ones (mma.sync.m16n8k32, u8 x s8 -> s32): every block first writes x as fixed-point numbers X = round(x 2^e),
+// |X| <= 2^22, one e for 128 K-elements of a token, in three signed digits of 8 bits, x ~ 2^-e (d_0 + 256 d_1 + 65536 d_2).
+// This rounding is at most 2^-22 of the 128 elements' largest |x|, what one addition in fp32 loses. The sums of a scale
+// group are exact: P_c = sum q d_c, and P_c - z D_c, D_c = sum d_c, takes the zero point off without cancellation. Only
+// then come fp32 and the scales: sum over the 128s of 2^-e sum_g s 256^c (P_c - z D_c).
+//
+// More tokens, 8 or 16 at a time. Three digits of 8 tokens would be three products and a longer sum, so here the
+// codes become q - z in x's type, exactly (eleven instructions for eight codes in bf16, nine in f16), and the products are
+// x's own (mma.sync.m16n8k16, sums in fp32); a group's sum is scaled once. Digits took 44 us for 8 tokens of
+// 28672 x 8192 and 83 for 16; this takes 43 and 60.
 //
 // Layout: a block per SM, 16 warps, each with its own ring of TMA loads (units of 16 rows x 512
 // codes, two boxes of 128 bytes a row), refilled as soon as a slot has been read, so that no warp waits for another
-// while the weights stream. ldmatrix hands a lane eight codes of a row at a time. Where x's digits for all of K
+// while the weights stream. ldmatrix hands a lane eight codes of a row at a time. Where x for all of K
 // would crowd out the ring, a cluster of 2, 4 or 8 blocks splits K and adds up through distributed
 // shared memory.
+//
+// Measured, bf16, groups of 128: 28672 x 8192 with one token 24.6 us (4.9 TB/s; 6.9 while it streams, 6 us before the first
+// unit and 2 after the last), 2 tokens 26.3, 8 tokens 43, 16 tokens 60 (instruction issue, four warps a scheduler); groups
+// of 32, one token 47 (a scale and a sum every 32 codes); 4096 x 4096, one token 6.5.
 
 #include <cooperative_groups.h>
 #include <cuda.h>
@@ -68,7 +77,7 @@ struct Int4Args {
   int f32_scales, f32_out;
   int tiles;  // 16-row tiles of one matrix
   int depth;  // slots of a warp's ring
-  uint32_t digits, sums, powers, pieces, block, records, bars, lists;  // offsets in shared memory
+  uint32_t x_at, sums, powers, pieces, block, records, bars, lists;  // offsets in shared memory
   int group_span, last_group;                           // 128-element runs of a group (groups of 128 and more); index of the last
   int* status;
   unsigned long long timeout_ns;
@@ -266,7 +275,8 @@ __device__ void build_lists(const Int4Args& a, Lists const& l, int* hist, int* a
 template <int TOK>
 constexpr bool kDigits = TOK <= 2;
 
-// Codes of a unit's row: two boxes' worth; with 16 tokens one.
+// Codes of a unit's row: two boxes' worth; with 16 tokens, whose x and sums leave the ring less room, one (16 tokens of
+// 28672 x 8192: 80 us with two boxes, 60 with one; 8 tokens 42.6 and 43.5).
 template <int TOK>
 constexpr int kUnitK = TOK <= 8 ? 512 : 256;
 template <int TOK>
@@ -298,7 +308,7 @@ constexpr int kEnd = 1;     // the last of the warp's run in the batch
 constexpr int kSecond = 2;  // the run's second
 constexpr int kNone = 4;    // the warp has no unit in this batch: a slot without loads
 
-// Shared memory, in order: rings, x's digits, sums and powers, pieces, the block's sums, stretch records, barriers,
+// Shared memory, in order: rings, x with its sums and powers, pieces, the block's sums, stretch records, barriers,
 // lists.
 template <int NG, int TOK>
 size_t lay_out(Int4Args& a, int depth, int units, int cluster) {
@@ -308,7 +318,7 @@ size_t lay_out(Int4Args& a, int depth, int units, int cluster) {
     offset = uint32_t(at);
     at += bytes;
   };
-  take(a.digits, size_t(units) * (kUnitK<TOK> / 32) * kXRow<TOK>);
+  take(a.x_at, size_t(units) * (kUnitK<TOK> / 32) * kXRow<TOK>);
   take(a.sums, size_t(units) * NG * kSumBytes<TOK>);
   take(a.powers, size_t(units) * (kUnitK<TOK> / 128) * kPowerBytes<TOK>);
   take(a.pieces, size_t(kWarps) * kPieces * kPiece<TOK> * 4);
@@ -319,7 +329,7 @@ size_t lay_out(Int4Args& a, int depth, int units, int cluster) {
   return at + 1024;  // the base is rounded up to 1024
 }
 
-// NG: scale groups of a unit (of 512 codes 16, 8, 4 for groups of 32, 64, multiples of 128).
+// NG: scale groups of a unit (a group of more than 128 counts for every 128).
 template <class T, int NG, int TOK, bool kZeros>
 __global__ void __launch_bounds__(kThreads, 1) gemv_int4_kernel(const __grid_constant__ Int4Args a) {
   constexpr int kPerGroup = kUnitK<TOK> / 32 / NG;  // 32-code chunks of a group
@@ -351,7 +361,7 @@ __global__ void __launch_bounds__(kThreads, 1) gemv_int4_kernel(const __grid_con
   int passes = (a.slots + TOK - 1) / TOK, active = 0;
   if (a.ids != nullptr) {
     griddep_wait();
-    build_lists<TOK>(a, l, reinterpret_cast<int*>(smem + a.digits), &active);
+    build_lists<TOK>(a, l, reinterpret_cast<int*>(smem + a.x_at), &active);
     passes = l.base[active];
   }
   // The tokens and the matrix of a pass.
@@ -485,7 +495,7 @@ __global__ void __launch_bounds__(kThreads, 1) gemv_int4_kernel(const __grid_con
     load_x += kUnitK<TOK> / 2;
   };
 
-  // x of a pass as digits: a warp takes 256 K-elements of a token at a time, a lane 8 of them, and loads
+  // x of a pass into shared memory: a warp takes 256 K-elements of a token at a time, a lane 8 of them, and loads
   // the next piece before it works on one.
   int x_token = 0, x_half = 0;  // of the piece that is loaded; halves of a unit: kbs * kHalves a token
   uint4 x_piece = make_uint4(0, 0, 0, 0);
@@ -511,7 +521,7 @@ __global__ void __launch_bounds__(kThreads, 1) gemv_int4_kernel(const __grid_con
       const uint4 u = x_piece;
       x_half += kWarps;
       fetch(p);
-      uint8_t* to = smem + a.digits + (half * 8 + lane / 4) * kXRow<TOK>;
+      uint8_t* to = smem + a.x_at + (half * 8 + lane / 4) * kXRow<TOK>;
       if constexpr (!kDigits<TOK>) {
         *reinterpret_cast<uint4*>(to + token * 64 + lane % 4 * 16) =
             make_uint4(__byte_perm(u.x, u.z, 0x5410), __byte_perm(u.x, u.z, 0x7632), __byte_perm(u.y, u.w, 0x5410), __byte_perm(u.y, u.w, 0x7632));
@@ -691,7 +701,7 @@ __global__ void __launch_bounds__(kThreads, 1) gemv_int4_kernel(const __grid_con
       }
       now_left = max(u.units, 1);
       k_at = (kb0 + u.kb) * kUnitK<TOK>;
-      xd = smem + a.digits + u.kb * (kUnitK<TOK> / 32) * kXRow<TOK> + x_lane;
+      xd = smem + a.x_at + u.kb * (kUnitK<TOK> / 32) * kXRow<TOK> + x_lane;
       xs = smem + a.sums + u.kb * NG * kSumBytes<TOK> + t * 8;
       xp = smem + a.powers + u.kb * (kUnitK<TOK> / 128) * kPowerBytes<TOK> + t * 8;
 #pragma unroll
@@ -897,7 +907,8 @@ struct Fit {
 };
 
 // The smallest cluster whose blocks keep x in 80 KB beside a ring of two slots a warp, else 8, and the ring that the
-// rest holds (at most 8 slots a warp, 256 KB in flight). depth 0: does not fit.
+// rest holds (at most 8 slots a warp). depth 0: does not fit. With x in 40 KB 16 tokens of 28672 x 8192 take 71.6 us
+// instead of 60.3 (a cluster's sums cost more than a deeper ring gains), 13 tokens of 10007 x 4128 21.8 instead of 20.4.
 template <int NG, int TOK>
 Fit fit(Int4Args const& a) {
   const int kb = (a.k + kUnitK<TOK> - 1) / kUnitK<TOK>;
@@ -921,7 +932,7 @@ template <class T, int NG, int TOK, bool kZeros>
 kl_status launch(Fit const& f, int device, cudaStream_t stream) {
   Int4Args const& a = f.args;
   auto* kernel = gemv_int4_kernel<T, NG, TOK, kZeros>;
-  static std::atomic<int> resident[64][4];  // clusters of 1, 2, 4, 8 that fit the device at once
+  static std::atomic<int> resident[64][4];  // by device: clusters of 1, 2, 4, 8 that fit at once
   const int which = f.cluster == 1 ? 0 : f.cluster == 2 ? 1 : f.cluster == 4 ? 2 : 3;
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute attr[2];
@@ -957,7 +968,8 @@ kl_status launch(Fit const& f, int device, cudaStream_t stream) {
   return e == cudaSuccess ? KL_OK : cuda_fail(e, "kl_gemv_int4 launch");
 }
 
-// Tokens of a pass by what a matrix meets (with ids: on average), fewer where x's digits would not fit.
+// Tokens of a pass by what a matrix meets (with ids: on average), fewer where x would not fit. 28672 x 8192: 2
+// tokens 26 us, in the form for 8 42; 4 tokens 42, in two passes of 2 47; 16 tokens 60, in two passes of 8 85.
 template <class T, int GROUP, bool kZeros>
 kl_status by_tokens(Int4Args& a, int device, cudaStream_t stream) {
   const int tokens = a.ids != nullptr ? (a.slots + a.experts - 1) / a.experts : a.slots;

@@ -2,6 +2,10 @@
 // sort of the slots by expert, each expert padded to whole blocks), kl_moe_dispatch (copy every
 // token's row to its experts), kl_moe_combine (weighted sum of the experts' rows) and
 // kl_moe_combine_grad.
+//
+// The last three move rows and are bound by memory. Measured on 8192 tokens, 4 experts each, rows of 4096 bf16:
+// dispatch 83.6 us (70.5 at the copy rate), combine 57.0 (5.9 TB/s), its gradient 110.4 (6.1 TB/s). The plan is a
+// latency: 5.8 us for 662 slots, 10.7 for 32768.
 
 #include <cooperative_groups.h>
 #include <cuda_runtime.h>
@@ -63,7 +67,8 @@ __device__ __forceinline__ int block_scan(int v, int* red) {
 // One cluster sorts all slots. Every warp counts the experts of its own run of consecutive slots;
 // sums over the warps, then (through distributed shared memory) over the blocks, give each (warp,
 // expert) the row of its first slot; a second walk over the same slots hands the rows out. Slots of
-// one expert keep their order, and nothing depends on the timing of atomics.
+// one expert keep their order, and nothing depends on the timing of atomics. A grid of its own for each step
+// would cost two more launches, which take as long as the whole.
 __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const PlanArgs a) {
   extern __shared__ int hist[];  // [kPlanWarps][experts]
   __shared__ int block_count[kMaxExperts], starts[kMaxExperts], counts[kMaxExperts];
@@ -191,7 +196,8 @@ __device__ __forceinline__ void zero_padding(const RowArgs& a, long long part) {
 }
 
 // A copy knows no element type: V is the widest of 16, 8, 4, 2 or 1 bytes that the row's bytes,
-// pitches and addresses allow. A token's row is read once and written to each of its experts.
+// pitches and addresses allow. A token's row is read once and written to each of its experts; a block to a token,
+// since whole rows in turn are what memory takes best.
 template <class V>
 __global__ void __launch_bounds__(kRowThreads) dispatch_kernel(const RowArgs a) {
   griddep_wait();
@@ -236,6 +242,7 @@ __device__ __forceinline__ long long row_of(const RowArgs& a, long long slot) {
   return r >= 0 && r < a.m ? r : -1;
 }
 
+// A thread has one vector of a token's row and takes its slots four at a time, all their loads before the first sum.
 template <class T, bool Vec>
 __global__ void __launch_bounds__(kRowThreads) combine_kernel(const RowArgs a) {
   using C = Cells<T, Vec>;
@@ -359,7 +366,7 @@ int type_bytes(int32_t t) { return t == KL_F32 ? 4 : t == KL_BF16 || t == KL_F16
 kl_status check_rows(char const* who, int64_t tokens, int64_t k, int64_t m, int64_t width) {
   if (tokens < 0 || k < 1 || k > kMaxTopK || m < 0 || width < 0)
     return fail(KL_ERR_INVALID_ARGUMENT, std::string(who) + ": extents must not be negative, k in [1, 32]");
-  if (tokens * k > INT32_MAX || m > INT32_MAX || tokens + (m + kPadRows - 1) / kPadRows > INT32_MAX)
+  if (tokens > INT32_MAX || m > INT32_MAX || tokens * k > INT32_MAX || tokens + (m + kPadRows - 1) / kPadRows > INT32_MAX)
     return fail(KL_ERR_INVALID_ARGUMENT, std::string(who) + ": more than 2^31 - 1 rows");
   return KL_OK;
 }
@@ -394,8 +401,9 @@ extern "C" kl_status kl_moe_plan(const int32_t* ids, int64_t tokens, int64_t k, 
   a.rows = rows;
   a.slots = slots;
   a.blocks = m_block_group;
-  // One block while it has at most four turns of 32 slots for each warp.
-  const int cluster = a.total <= 4 * 32 * kPlanWarps ? 1 : kPlanBlocks;
+  // One block while a warp has one turn of 32 slots. One block against a cluster, 64 experts: 1024 slots 7.5 and
+  // 7.7 us, 4096 slots 12.7 and 7.9, 8192 slots 19.5 and 7.8.
+  const int cluster = a.total <= 32 * kPlanWarps ? 1 : kPlanBlocks;
   const long long warps = (long long)cluster * kPlanWarps;
   a.warp_span = (a.total + warps * 32 - 1) / (warps * 32) * 32;
   const size_t smem = size_t(kPlanWarps) * size_t(experts) * sizeof(int);

@@ -285,12 +285,12 @@ def moe_combine_grad(dout, y, weights=None, *, rows=None, slots=None, stream=Non
 def gemv_int4(x, q, scales, zeros=None, *, group: int = 128, ids=None, out=None, out_dtype=None, stream=None):
     """out = x @ ((q - zeros) * scales).T for few tokens: x bf16 / f16 [tokens, K]; q uint8 [N, K / 2],
     two 4-bit codes a byte, the lower K in the low nibble; scales [N, ceil(K / group)] of x's type or fp32;
-    zeros uint8 of the scales' shape (0 .. 127), None = 8. group: 32, 64 or a multiple of 128; K a
+    zeros uint8 of the scales' shape, None = 8. group: 32, 64 or a multiple of 128; K a
     multiple of 32. With int32 ids [tokens, k]: q [E, N, K / 2], scales and zeros [E, N, ...], x [tokens, K]
     or [tokens, k, K], out [tokens, k, N] with expert ids[t, j] (rows of zeros for ids outside 0 .. E - 1;
-    at most 4096 ids, 1024 experts). out in x's type or fp32. x enters with 22 bits below the largest of its 128
-    neighbours, a scale group's products are summed exactly, the groups in fp32; a NaN or infinity makes its row
-    NaN. Up to 16 tokens of a matrix read the weights once. K up to 65536."""
+    at most 4096 ids, 1024 experts). out in x's type or fp32. Sums are exact or fp32 (with up to two
+    tokens to a matrix x enters with 22 bits below the largest of its 128 neighbours); a NaN or infinity makes its
+    row NaN or infinite. Up to 16 tokens of a matrix read the weights once. K up to 65536."""
     dtype, bits = x.dtype, x.dim()
     if dtype is not torch.bfloat16 and dtype is not torch.float16:
         raise ValueError("x must be bf16 or f16")

@@ -3,6 +3,9 @@
 Tolerances count roundings. u = 2^-24 is half a step of fp32, relative to the value."""
 
 import math
+import pathlib
+import subprocess
+import sys
 
 import pytest
 import torch
@@ -344,7 +347,9 @@ def int4_case(cuda, n, k, group, dtype, zeros, experts=0, seed=0, scale_dtype=No
 def gemv_tol(x, w, want, k, dtype):
     """x enters as fixed-point numbers, off by at most 2^-22 of its group's largest. A group's products are
     summed exactly; each group's sum takes 3 roundings to scale and 3 to join its three digits, then at
-    most k / 32 sums, 16 warps and 8 blocks are added in fp32; one rounding to the type."""
+    most k / 32 sums, 16 warps and 8 blocks are added in fp32; one rounding to the type. With three tokens
+    and more, x and q - z enter as they are; a group of up to 128 is 8 steps of 16 products, each step's sum cut off
+    below 2 U of what the group's products sum to, so 16 U a group, one rounding to scale it, and the same sums after."""
     x = x.to(F64).abs()
     if x.shape[0] == 0:
         return torch.zeros_like(want)
@@ -421,6 +426,24 @@ def test_gemv_int4_every_code(cuda):
             assert torch.equal(got.cpu().to(F64), oracle.int4_weights(q, s, z, group).T)
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("tokens", [1, 2, 5, 16])
+def test_gemv_int4_any_zero_point(cuda, dtype, tokens):
+    """Zero points up to 255, which 8 bits of a bf16 cannot hold beside a code."""
+    n, k, group = 50, 640, 64
+    q, s, _ = int4_case(cuda, n, k, group, dtype, None, seed=tokens)
+    z = torch.randint(0, 256, s.shape, generator=gen(tokens), dtype=torch.uint8)
+    z[:, 0], z[:16], z[3, 1] = 127, z[:16] % 128, 128
+    x = torch.randn((tokens, k), generator=gen(9)).to(dtype)
+    w = oracle.int4_weights(q, s, z, group)
+    want = x.to(F64) @ w.T
+    close(kl.gemv_int4(x.to(cuda), q, s, z.to(cuda), group=group), want, gemv_tol(x, w, want, k, dtype))
+    # Codes and zero points alone: every weight exactly.
+    eye = torch.eye(k, dtype=dtype, device=cuda)[:tokens]
+    got = kl.gemv_int4(eye, q, torch.ones_like(s), z.to(cuda), group=group, out_dtype=torch.float32)
+    assert torch.equal(got.cpu().to(F64), oracle.int4_weights(q, torch.ones_like(s), z, group).T[:tokens])
+
+
 def test_gemv_int4_strides(cuda):
     n, k = 48, 512
     q, s, z = int4_case(cuda, 2 * n, 2 * k, 64, torch.bfloat16, "narrow", seed=3)
@@ -481,6 +504,33 @@ def test_gemv_int4_by_expert(cuda, group, tokens, k, experts, n, width):
 
 
 # ------------------------------------------------------------------------------------ streams, graphs, together
+
+FIRST_IN_CAPTURE = """
+import torch
+import maia_b200 as kl
+d = torch.device("cuda", 0)
+x = torch.randn((100, 64), device=d)
+q = torch.randint(0, 256, (4096, 1024), device=d, dtype=torch.uint8)
+s, v = torch.rand((4096, 16), device=d).bfloat16(), torch.randn((3, 2048), device=d).bfloat16()
+torch.cuda.synchronize()
+def step():
+    r = kl.moe_route(x, 4, renormalize=True)
+    plan = kl.moe_plan(r.ids, 64)
+    return kl.moe_combine(kl.moe_dispatch(x, plan), r.weights, rows=plan.rows), kl.gemv_int4(v, q, s)
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    got = step()
+g.replay()
+torch.cuda.synchronize()
+assert all(torch.equal(a, b) for a, b in zip(got, step()))
+"""
+
+
+def test_first_call_may_be_captured(cuda):
+    """A process whose first call of each operator is made while a graph is captured."""
+    done = subprocess.run([sys.executable, "-c", FIRST_IN_CAPTURE], cwd=pathlib.Path(__file__).parent.parent, capture_output=True, text=True, timeout=300)
+    assert done.returncode == 0, done.stderr[-2000:]
+
 
 def test_graph_replay_and_streams(cuda):
     """The whole path captured on a side stream and replayed with new inputs in place: the results
