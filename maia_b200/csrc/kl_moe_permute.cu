@@ -4,8 +4,8 @@
 // kl_moe_combine_grad.
 //
 // The last three move rows and are bound by memory. Measured on 8192 tokens, 4 experts each, rows of 4096 bf16:
-// dispatch 83.6 us (70.5 at the copy rate), combine 57.0 (5.9 TB/s), its gradient 110.4 (6.1 TB/s). The plan is a
-// latency: 5.8 us for 662 slots, 10.7 for 32768.
+// dispatch 83.6 us (5.6 TB/s; 72.5 us at the copy rate), combine 57.0 (5.4 TB/s), its gradient 110.4 (5.8 TB/s). The
+// plan is a latency: 5.8 us for 662 slots, 10.7 for 32768.
 
 #include <cooperative_groups.h>
 #include <cuda_runtime.h>
@@ -67,8 +67,7 @@ __device__ __forceinline__ int block_scan(int v, int* red) {
 // One cluster sorts all slots. Every warp counts the experts of its own run of consecutive slots;
 // sums over the warps, then (through distributed shared memory) over the blocks, give each (warp,
 // expert) the row of its first slot; a second walk over the same slots hands the rows out. Slots of
-// one expert keep their order, and nothing depends on the timing of atomics. A grid of its own for each step
-// would cost two more launches, which take as long as the whole.
+// one expert keep their order, and nothing depends on the timing of atomics.
 __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const PlanArgs a) {
   extern __shared__ int hist[];  // [kPlanWarps][experts]
   __shared__ int block_count[kMaxExperts], starts[kMaxExperts], counts[kMaxExperts];
@@ -196,8 +195,7 @@ __device__ __forceinline__ void zero_padding(const RowArgs& a, long long part) {
 }
 
 // A copy knows no element type: V is the widest of 16, 8, 4, 2 or 1 bytes that the row's bytes,
-// pitches and addresses allow. A token's row is read once and written to each of its experts; a block to a token,
-// since whole rows in turn are what memory takes best.
+// pitches and addresses allow. A token's row is read once and written to each of its experts.
 template <class V>
 __global__ void __launch_bounds__(kRowThreads) dispatch_kernel(const RowArgs a) {
   griddep_wait();
