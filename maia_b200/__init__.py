@@ -158,14 +158,14 @@ def lib() -> ctypes.CDLL:
             "kl_comm_is_aborted": (i32, [vp]),
             "kl_comm_destroy": (i32, [vp, i64]),
             "kl_moe_route_workspace_size": (i32, [i64, i64, P(ctypes.c_size_t)]),
-            "kl_moe_route": (i32, [P(MoeRouteDesc), vp, ctypes.c_size_t, vp]),
-            "kl_moe_route_grad": (i32, [P(MoeRouteDesc), vp, vp, vp, i64, vp]),
+            "kl_moe_route": (i32, [vp, vp, ctypes.c_size_t, vp]),
+            "kl_moe_route_grad": (i32, [vp, vp, vp, vp, i64, vp]),
             "kl_moe_rows": (i64, [i64, i64, i32]),
             "kl_moe_plan": (i32, [vp, i64, i64, i64, i32, i64, vp, vp, vp, vp]),
             "kl_moe_dispatch": (i32, [vp, i64, i64, i64, i64, vp, vp, i64, vp, i64, vp]),
             "kl_moe_combine": (i32, [vp, i32, i64, i64, vp, vp, i64, i64, i64, vp, i64, vp]),
             "kl_moe_combine_grad": (i32, [vp, i64, vp, i32, i64, i64, vp, vp, vp, i64, i64, i64, vp, i64, vp, vp]),
-            "kl_gemv_int4": (i32, [P(Int4Desc), vp]),
+            "kl_gemv_int4": (i32, [vp, vp]),
         }
         for name, (res, args) in sig.items():
             fn = getattr(L, name)

@@ -14,6 +14,7 @@ through torch. No counterpart in the reference (kernel_lib has no GEMM and no ro
 from __future__ import annotations
 
 import ctypes
+import struct
 from functools import lru_cache
 from typing import NamedTuple
 
@@ -44,6 +45,17 @@ _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda i:
 _current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
 
 
+def _packer(desc):
+    """desc(*fields) as bytes, at a quarter of the structure's cost."""
+    kinds = {ctypes.c_void_p: "P", ctypes.c_int64: "q", ctypes.c_int32: "i"}
+    packed = struct.Struct("@" + "".join(kinds[kind] for _, kind in desc._fields_))
+    assert packed.size == ctypes.sizeof(desc)
+    return packed.pack
+
+
+_pack_route, _pack_int4 = _packer(MoeRouteDesc), _packer(Int4Desc)
+
+
 def _refuse(ok: bool, message: str) -> None:
     if not ok:
         raise ValueError(message)
@@ -63,8 +75,8 @@ def _whole(name: str, t, shape, dtype) -> None:
 
 def _pitch(t) -> int:
     """Row pitch in elements; of a single row, whose stride torch leaves open, at least the row."""
-    pitch = t.stride(-2)
-    return pitch if pitch >= t.shape[-1] or t.shape[-2] > 1 else t.shape[-1]
+    pitch, shape = t.stride(-2), t.shape
+    return pitch if pitch >= shape[-1] or shape[-2] > 1 else shape[-1]
 
 
 def _ptr(t):
@@ -108,9 +120,9 @@ def _route_workspace(tokens: int, experts: int) -> int:
 
 
 def _route_desc(logits, k, renormalize, valid, ids, weights, counts, routed, loss):
-    return MoeRouteDesc(logits.data_ptr(), _pitch(logits), logits.shape[0], logits.shape[1], k, _FLOATS[logits.dtype],
-                        int(bool(renormalize)), _ptr(valid), ids.data_ptr(), weights.data_ptr(), counts.data_ptr(),
-                        routed.data_ptr(), _ptr(loss))
+    return _pack_route(logits.data_ptr(), _pitch(logits), logits.shape[0], logits.shape[1], k, _FLOATS[logits.dtype],
+                       bool(renormalize), _ptr(valid) or 0, ids.data_ptr(), weights.data_ptr(), counts.data_ptr(),
+                       routed.data_ptr(), _ptr(loss) or 0)
 
 
 def _check_logits(logits, valid) -> None:
@@ -144,7 +156,7 @@ def moe_route(logits, k: int, *, renormalize: bool = True, valid=None, stream=No
         work = logits.new_empty((size,), dtype=torch.uint8)
         owned = (*out, work)
     d = _route_desc(logits, k, renormalize, valid, ids, weights, counts, routed, loss)
-    _queue(device, stream, owned, lib().kl_moe_route, ctypes.byref(d), _ptr(work), size)
+    _queue(device, stream, owned, lib().kl_moe_route, d, _ptr(work), size)
     return out
 
 
@@ -171,7 +183,7 @@ def moe_route_grad(logits, route: MoeRoute, dweights=None, dloss=None, *, renorm
     _refuse(out.shape == logits.shape, "out must have the logits' shape")
     device = _device(logits, valid, route.ids, route.weights, route.counts, route.tokens, dweights, dloss, out)
     d = _route_desc(logits, k, renormalize, valid, route.ids, route.weights, route.counts, route.tokens, None)
-    _queue(device, stream, (out,), lib().kl_moe_route_grad, ctypes.byref(d), _ptr(dweights), _ptr(dloss), out.data_ptr(),
+    _queue(device, stream, (out,), lib().kl_moe_route_grad, d, _ptr(dweights), _ptr(dloss), out.data_ptr(),
            _pitch(out))
     return out
 
@@ -318,14 +330,19 @@ def gemv_int4(x, q, scales, zeros=None, *, group: int = 128, ids=None, out=None,
         _refuse(not per_slot or x.is_contiguous(), "x of [tokens, k, K] must be contiguous")
         result, ldx = (tokens, topk, n), k if per_slot else _pitch(x)
     if out is None:
-        out = x.new_empty(result, dtype=out_dtype or dtype)
-    if out.shape != result or (out.dtype is not dtype and out.dtype is not torch.float32):
-        raise ValueError(f"out must have the shape {result} and x's type or fp32")
-    _refuse(out.stride(-1) == 1 or n <= 1 if ids is None else out.is_contiguous(), "out must be contiguous in its last dimension")
-    d = Int4Desc(x.data_ptr(), ldx, q.data_ptr(), _pitch(q), 0 if ids is None else q.stride(0),
-                 scales.data_ptr(), _pitch(scales), 0 if ids is None else scales.stride(0),
-                 _ptr(zeros), 0 if zeros is None else _pitch(zeros), 0 if ids is None or zeros is None else zeros.stride(0),
-                 _ptr(ids), 0 if ids is None else q.shape[0], topk, out.data_ptr(), _pitch(out) if ids is None else n,
-                 tokens, n, k, group, _FLOATS[dtype], _FLOATS[scales.dtype], _FLOATS[out.dtype], per_slot)
-    _queue(_device(x, q, scales, zeros, ids, out), stream, (out,), lib().kl_gemv_int4, ctypes.byref(d))
+        out_dtype = out_dtype or dtype
+        out = x.new_empty(result) if out_dtype is dtype else x.new_empty(result, dtype=out_dtype)
+    elif out.shape != result:
+        raise ValueError(f"out must have the shape {result}")
+    else:
+        _refuse(out.stride(-1) == 1 or n <= 1 if ids is None else out.is_contiguous(), "out must be contiguous in its last dimension")
+    if out.dtype is not dtype and out.dtype is not torch.float32:
+        raise ValueError("out must have x's type or fp32")
+    one = ids is None
+    zero_fields = (0, 0, 0) if zeros is None else (zeros.data_ptr(), _pitch(zeros), 0 if one else zeros.stride(0))
+    d = _pack_int4(x.data_ptr(), ldx, q.data_ptr(), _pitch(q), 0 if one else q.stride(0),
+                   scales.data_ptr(), _pitch(scales), 0 if one else scales.stride(0), *zero_fields,
+                   0 if one else ids.data_ptr(), 0 if one else q.shape[0], topk, out.data_ptr(), _pitch(out) if one else n,
+                   tokens, n, k, group, _FLOATS[dtype], _FLOATS[scales.dtype], _FLOATS[out.dtype], per_slot)
+    _queue(_device(x, q, scales, zeros, ids, out), stream, (out,), lib().kl_gemv_int4, d)
     return out
