@@ -692,3 +692,39 @@ def test_gradients_that_only_one_output_uses(cuda):
     q, s, _ = int4_case(cuda, 16, 64, 32, torch.bfloat16, None)
     x = torch.randn((2, 64), generator=gen(3)).bfloat16().to(cuda)
     assert torch.equal(torch.ops.kl.gemv_int4(x, q, s, None, 32), kl.gemv_int4(x, q, s, group=32))
+
+
+def test_training_step_in_a_graph(cuda):
+    """Forward and backward through torch.ops.kl, captured and replayed on new values: the eager step's bits."""
+    import maia_b200.torch_ops  # noqa: F401
+
+    tokens, experts, k, width = 70, 16, 3, 136
+    logits = torch.empty((tokens, experts), device=cuda, requires_grad=True)
+    x = torch.empty((tokens, width), device=cuda, dtype=torch.bfloat16, requires_grad=True)
+
+    def fill(seed):
+        with torch.no_grad():
+            logits.copy_(torch.randn(logits.shape, generator=gen(seed)))
+            x.copy_(torch.randn(x.shape, generator=gen(seed + 1)))
+
+    def step():
+        ids, weights, _, _, loss = torch.ops.kl.moe_route(logits, k)
+        rows, slots, _ = torch.ops.kl.moe_plan(ids, experts)
+        y = torch.ops.kl.moe_dispatch(x, rows, slots)
+        out = torch.ops.kl.moe_combine(y, weights, rows, slots)
+        return torch.autograd.grad(out.float().square().sum() + loss, [logits, x])
+
+    fill(0)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        got = step()
+    for seed in (3, 9):
+        fill(seed)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, step()))
