@@ -25,7 +25,7 @@
 //
 // Measured, bf16, groups of 128: 28672 x 8192 with one token 24.6 us (4.9 TB/s; 6.9 while it streams, 6 us before the first
 // unit and 2 after the last), 2 tokens 26.3, 8 tokens 43, 16 tokens 60 (instruction issue, four warps a scheduler); groups
-// of 32, one token 47 (a scale and a sum every 32 codes); 4096 x 4096, one token 6.5.
+// of 32 with zero points, one token 37 (a scale, a zero point and a sum every 32 codes); 4096 x 4096, one token 6.5.
 
 #include <cooperative_groups.h>
 #include <cuda.h>
@@ -78,6 +78,7 @@ struct Int4Args {
   int tiles;  // 16-row tiles of one matrix
   int depth;  // slots of a warp's ring
   uint32_t x_at, sums, powers, pieces, block, records, bars, lists;  // offsets in shared memory
+  int wide_scales;                                      // a lane's scales and zero points come by one load
   int group_span, last_group;                           // 128-element runs of a group (groups of 128 and more); index of the last
   int* status;
   unsigned long long timeout_ns;
@@ -587,10 +588,11 @@ __global__ void __launch_bounds__(kThreads, 1) gemv_int4_kernel(const __grid_con
     }
   };
 
-  // A unit's scales and zero points, loaded one unit ahead: lane t of a row's four holds groups t, t + 4, ...
+  // A unit's scales and zero points, loaded one unit ahead: lane t of a row's four holds kHeld groups from t kHeld.
   // Rows behind the matrix and groups behind K read the last ones: the first are not stored, the second multiply
-  // zeros.
-  struct Scales {
+  // zeros. Where the layout allows, a lane's groups come by one load (one token of 28672 x 8192 with zero points, groups
+  // of 32: 37.2 us, else 47.1; groups of 64: 30.6 and 33.9).
+  struct __align__(16) Scales {
     uint32_t s[2][kHeld];  // as loaded: nothing waits for them before the unit that uses them
     uint32_t z[2][kHeld];
   };
@@ -608,16 +610,32 @@ __global__ void __launch_bounds__(kThreads, 1) gemv_int4_kernel(const __grid_con
     }
   };
   auto load_scales = [&] {
-#pragma unroll
-    for (int h = 0; h < kHeld; ++h) {
-      int gi = s_kb * NG + t + 4 * h;
-      if (kPerGroup == 4 && a.group_span != 1) gi /= a.group_span;
-      gi = min(gi, a.last_group);
+    if (kHeld > 1 && a.wide_scales) {
+      const int gi = min(s_kb * NG + t * kHeld, a.last_group + 1 - kHeld);
 #pragma unroll
       for (int r = 0; r < 2; ++r) {
-        if (a.f32_scales) raw.s[r][h] = reinterpret_cast<const uint32_t*>(s_row[r])[gi];
-        else raw.s[r][h] = reinterpret_cast<const uint16_t*>(s_row[r])[gi];
-        if (kZeros) raw.z[r][h] = z_row[r][gi];
+        if constexpr (kHeld == 4) {
+          if (a.f32_scales) *reinterpret_cast<uint4*>(raw.s[r]) = *reinterpret_cast<const uint4*>(s_row[r] + 4 * gi);
+          else *reinterpret_cast<uint2*>(raw.s[r]) = *reinterpret_cast<const uint2*>(s_row[r] + 2 * gi);
+          if (kZeros) raw.z[r][0] = *reinterpret_cast<const uint32_t*>(z_row[r] + gi);
+        } else {
+          if (a.f32_scales) *reinterpret_cast<uint2*>(raw.s[r]) = *reinterpret_cast<const uint2*>(s_row[r] + 4 * gi);
+          else raw.s[r][0] = *reinterpret_cast<const uint32_t*>(s_row[r] + 2 * gi);
+          if (kZeros) raw.z[r][0] = *reinterpret_cast<const uint16_t*>(z_row[r] + gi);
+        }
+      }
+    } else {
+#pragma unroll
+      for (int h = 0; h < kHeld; ++h) {
+        int gi = s_kb * NG + t * kHeld + h;
+        if (kPerGroup == 4 && a.group_span != 1) gi /= a.group_span;
+        gi = min(gi, a.last_group);
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+          if (a.f32_scales) raw.s[r][h] = reinterpret_cast<const uint32_t*>(s_row[r])[gi];
+          else raw.s[r][h] = reinterpret_cast<const uint16_t*>(s_row[r])[gi];
+          if (kZeros) raw.z[r][h] = z_row[r][gi];
+        }
       }
     }
     ++s_kb;
@@ -708,14 +726,22 @@ __global__ void __launch_bounds__(kThreads, 1) gemv_int4_kernel(const __grid_con
       for (int set = 0; set < kSets; ++set) acc[set][0] = acc[set][1] = acc[set][2] = acc[set][3] = 0.0f;
     }
     float s_now[2][kHeld];
-    uint32_t z_now[2][kHeld];
+    uint32_t z_now[2];  // a byte a group
 #pragma unroll
-    for (int r = 0; r < 2; ++r)
+    for (int r = 0; r < 2; ++r) {
+      if (kHeld > 1 && a.wide_scales) {
 #pragma unroll
-      for (int h = 0; h < kHeld; ++h) {
-        s_now[r][h] = scale_of(raw.s[r][h]);
-        z_now[r][h] = raw.z[r][h];
+        for (int h = 0; h < kHeld; ++h) s_now[r][h] = scale_of(a.f32_scales ? raw.s[r][h] : raw.s[r][h / 2] >> 16 * (h % 2) & 0xFFFFu);
+        z_now[r] = raw.z[r][0];
+      } else {
+        z_now[r] = 0;
+#pragma unroll
+        for (int h = 0; h < kHeld; ++h) {
+          s_now[r][h] = scale_of(raw.s[r][h]);
+          z_now[r] |= raw.z[r][h] << 8 * h;
+        }
       }
+    }
     if (now_left > 1) {
       load_scales();
     } else if (done + 1 < issued) {
@@ -736,7 +762,7 @@ __global__ void __launch_bounds__(kThreads, 1) gemv_int4_kernel(const __grid_con
           float sum[4] = {};                      // of the quarter
           float dot[kSets][4];                    // of a group
           float sc[2];
-          uint32_t z[2] = {8, 8};
+          uint32_t z[2] = {8, 8}, z_four[2];
 #pragma unroll
           for (int pair = 0; pair < 2; ++pair) {
             // Matrices: rows 0-7 and 8-15 of chunk 2 pair, then of chunk 2 pair + 1.
@@ -748,11 +774,12 @@ __global__ void __launch_bounds__(kThreads, 1) gemv_int4_kernel(const __grid_con
               const bool begins = c % kPerGroup == 0, ends = c % kPerGroup == kPerGroup - 1;
               const uint8_t* xc = xd + (quarter * 4 + c) * kXRow<TOK>;
               if (begins) {
-                const int from = (lane & 28) | ((quarter * kGroups + gj) & 3);
+                const int from = (lane & 28) | (quarter * kGroups + gj) / kHeld, held = (quarter * kGroups + gj) % kHeld;
 #pragma unroll
                 for (int r = 0; r < 2; ++r) {
-                  sc[r] = __shfl_sync(0xFFFFFFFFu, s_now[r][0], from);
-                  if (kZeros) z[r] = __shfl_sync(0xFFFFFFFFu, z_now[r][0], from);
+                  sc[r] = __shfl_sync(0xFFFFFFFFu, s_now[r][held], from);
+                  if (kZeros && held == 0) z_four[r] = __shfl_sync(0xFFFFFFFFu, z_now[r], from);
+                  if (kZeros) z[r] = z_four[r] >> 8 * held & 0xFF;
                 }
               }
               if constexpr (kDigits<TOK>) {
@@ -799,16 +826,6 @@ __global__ void __launch_bounds__(kThreads, 1) gemv_int4_kernel(const __grid_con
             const float2 q = *reinterpret_cast<const float2*>(xp + quarter * kPowerBytes<TOK>);
 #pragma unroll
             for (int i = 0; i < 4; ++i) acc[0][i] = fmaf(i % 2 ? q.y : q.x, sum[i], acc[0][i]);
-          }
-          // The next quarter's groups in front, where this one's were a lane's last.
-          if (kHeld > 1 && (quarter + 1) * (4 / kPerGroup) % 4 == 0) {
-#pragma unroll
-            for (int r = 0; r < 2; ++r)
-#pragma unroll
-              for (int h = 0; h + 1 < kHeld; ++h) {
-                s_now[r][h] = s_now[r][h + 1];
-                z_now[r][h] = z_now[r][h + 1];
-              }
           }
         }
         xd += kUnitK<TOK> / 32 * kXRow<TOK>;
@@ -930,10 +947,15 @@ Fit fit(Int4Args const& a) {
 
 template <class T, int NG, int TOK, bool kZeros>
 kl_status launch(Fit const& f, int device, cudaStream_t stream) {
-  Int4Args const& a = f.args;
+  Int4Args a = f.args;
   auto* kernel = gemv_int4_kernel<T, NG, TOK, kZeros>;
   static std::atomic<int> resident[64][4];  // by device: clusters of 1, 2, 4, 8 that fit at once
   const int which = f.cluster == 1 ? 0 : f.cluster == 2 ? 1 : f.cluster == 4 ? 2 : 3;
+  constexpr uint64_t kHeld = NG >= 4 ? NG / 4 : 1;  // as in the kernel
+  const uint64_t scale_bytes = a.f32_scales ? 4 : 2;
+  a.wide_scales = (a.last_group + 1) % kHeld == 0 && a.lds % kHeld == 0 && a.stride_s % kHeld == 0 &&
+                  reinterpret_cast<uintptr_t>(a.scales) % (kHeld * scale_bytes) == 0 &&
+                  (!kZeros || (a.ldz % kHeld == 0 && a.stride_z % kHeld == 0 && reinterpret_cast<uintptr_t>(a.zeros) % kHeld == 0));
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute attr[2];
   cfg.blockDim = dim3(kThreads, 1, 1);
