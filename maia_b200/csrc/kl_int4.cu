@@ -23,7 +23,7 @@
 // would crowd out the ring, a cluster of 2, 4 or 8 blocks splits K and adds up through distributed
 // shared memory.
 //
-// Measured, bf16, groups of 128: 28672 x 8192 with one token 24.6 us (4.9 TB/s; 6.9 while it streams, 6 us before the first
+// Measured, bf16, groups of 128: 28672 x 8192 with one token 25 us (4.9 TB/s; 6.9 while it streams, 6 us before the first
 // unit and 2 after the last), 2 tokens 26.3, 8 tokens 43, 16 tokens 60 (instruction issue, four warps a scheduler); groups
 // of 32 with zero points, one token 37 (a scale, a zero point and a sum every 32 codes); 4096 x 4096, one token 6.5.
 

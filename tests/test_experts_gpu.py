@@ -378,6 +378,7 @@ def test_gemv_int4(cuda, dtype, group, tokens, n, k):
     (2, 16 * 148 * 21, 512, 32),          # a full batch of 16 tiles and a rest, one unit a tile
     (1, 16 * 148 * 3, 1536, 64), (5, 16 * 300 + 1, 2560, 64), (13, 10007, 4128, 64), (16, 16 * 700, 8192, 128),
     (33, 16 * 200, 1056, 32), (3, 40, 16384, 128), (16, 64, 32768, 32), (1, 32, 65536, 64), (2, 8192, 8192, 256),
+    (5, 40, 65536, 64), (12, 24, 40960, 128), (3, 16 * 148, 36896, 32),    # x of 8 or 16 tokens does not fit
 ])
 def test_gemv_int4_many_tiles(cuda, tokens, n, k, group):
     """Sizes at which blocks have several tiles, tiles are shared between warps, K is split over a cluster."""
