@@ -1091,6 +1091,8 @@ extern "C" kl_status kl_gemv_int4(const kl_int4_desc* d, void* stream) {
   if (d->out == nullptr || (d->k > 0 && (d->x == nullptr || d->q == nullptr || d->scales == nullptr))) return bad("null pointer");
   if (d->k > 0 && (!aligned16(d->x) || !aligned16(d->q) || d->ldx % 8 != 0 || d->ldq % 16 != 0))
     return bad("x and q must be 16-byte aligned with row pitches that are multiples of 16 bytes");
+  if (!aligned(d->scales, d->scale_type == KL_F32 ? 4 : 2) || !aligned(d->out, d->out_type == KL_F32 ? 4 : 2) || !aligned(d->ids, 4))
+    return bad("scales, out and ids must be aligned to their elements");
   if (by_expert && d->experts > 1 && (d->stride_q % 16 != 0 || d->stride_q <= 0 || d->stride_scales < 0 || d->stride_zeros < 0))
     return bad("expert strides must not be negative, stride_q a positive multiple of 16 bytes");
   if (d->k == 0) {  // a sum of nothing

@@ -475,6 +475,8 @@ extern "C" kl_status kl_moe_combine(const void* y, int32_t type, int64_t ldy, in
   if (rows == nullptr && m != tokens * k)
     return fail(KL_ERR_INVALID_ARGUMENT, "kl_moe_combine: without rows, y has tokens * k rows");
   if (out == nullptr || (m > 0 && y == nullptr)) return fail(KL_ERR_INVALID_ARGUMENT, "kl_moe_combine: null pointer");
+  if (!aligned(y, size) || !aligned(out, size))
+    return fail(KL_ERR_INVALID_ARGUMENT, "kl_moe_combine: y and out must be aligned to their elements");
   RowArgs a = {};
   a.src = y;
   a.ld_src = ldy * size;
@@ -516,6 +518,8 @@ extern "C" kl_status kl_moe_combine_grad(const void* dout, int64_t ld_dout, cons
   if (tokens == 0 && m == 0) return KL_OK;
   if ((tokens > 0 && width > 0 && dout == nullptr) || (m > 0 && width > 0 && (dy == nullptr || (dweights != nullptr && y == nullptr))))
     return fail(KL_ERR_INVALID_ARGUMENT, "kl_moe_combine_grad: null pointer");
+  if (!aligned(dout, size) || !aligned(y, size) || !aligned(dy, size))
+    return fail(KL_ERR_INVALID_ARGUMENT, "kl_moe_combine_grad: dout, y and dy must be aligned to their elements");
   RowArgs a = {};
   a.src = y;
   a.ld_src = ldy * size;

@@ -634,6 +634,8 @@ extern "C" kl_status kl_moe_route(const kl_moe_route_desc* d, void* workspace, s
   if (d->counts == nullptr || d->routed == nullptr || d->loss == nullptr ||
       (d->tokens > 0 && (d->logits == nullptr || d->ids == nullptr || d->weights == nullptr)))
     return fail(KL_ERR_INVALID_ARGUMENT, "kl_moe_route: null pointer");
+  if (!aligned(d->logits, d->logits_type == KL_F32 ? 4 : 2))
+    return fail(KL_ERR_INVALID_ARGUMENT, "kl_moe_route: logits must be aligned to their elements");
   const int blocks = route_blocks(d->tokens, int(d->experts));
   size_t need = 0;
   kl_moe_route_workspace_size(d->tokens, d->experts, &need);
@@ -686,6 +688,8 @@ extern "C" kl_status kl_moe_route_grad(const kl_moe_route_desc* d, const float* 
   if (d->logits == nullptr || d->ids == nullptr || d->weights == nullptr || d->counts == nullptr || d->routed == nullptr ||
       dlogits == nullptr)
     return fail(KL_ERR_INVALID_ARGUMENT, "kl_moe_route_grad: null pointer");
+  if (!aligned(d->logits, d->logits_type == KL_F32 ? 4 : 2) || !aligned(dlogits, d->logits_type == KL_F32 ? 4 : 2))
+    return fail(KL_ERR_INVALID_ARGUMENT, "kl_moe_route_grad: logits and their gradient must be aligned to their elements");
   RouteGradArgs a = {};
   a.logits = d->logits;
   a.ld = d->ld_logits;

@@ -50,6 +50,7 @@ __device__ __forceinline__ uint4 pack(const float* v) {
   return u;
 }
 
+inline bool aligned(const void* p, size_t bytes) { return reinterpret_cast<uintptr_t>(p) % bytes == 0; }
 inline bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
 
 }  // namespace kl::capi

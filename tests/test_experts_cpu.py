@@ -32,6 +32,7 @@ def route_desc(**over):
     (dict(counts=None), kl.KL_ERR_INVALID_ARGUMENT, "null"),
     (dict(logits=None), kl.KL_ERR_INVALID_ARGUMENT, "null"),
     (dict(tokens=100000), kl.KL_ERR_INVALID_ARGUMENT, "workspace"),
+    (dict(logits=P + 1), kl.KL_ERR_INVALID_ARGUMENT, "aligned"),
 ])
 def test_route_refusals(over, status, what):
     d = route_desc(**over)
@@ -96,6 +97,8 @@ def test_row_movers_refusals():
         (lambda: L.kl_moe_combine(P, kl.KL_E4M3, 8, 128, P, P, 4, 2, 8, P, 8, None), "bf16"),
         (lambda: L.kl_moe_combine(P, kl.KL_BF16, 7, 128, P, P, 4, 2, 8, P, 8, None), "pitch"),
         (lambda: L.kl_moe_combine(P, kl.KL_BF16, 8, 9, None, P, 4, 2, 8, P, 8, None), "tokens * k"),
+        (lambda: L.kl_moe_combine(P + 1, kl.KL_BF16, 8, 128, P, P, 4, 2, 8, P, 8, None), "aligned"),
+        (lambda: L.kl_moe_combine_grad(P, 8, P, kl.KL_F32, 8, 8, None, None, P, 4, 2, 8, P + 2, 8, P, None), "aligned"),
         (lambda: L.kl_moe_combine(None, kl.KL_BF16, 8, 8, None, P, 4, 2, 8, P, 8, None), "null"),
         (lambda: L.kl_moe_combine_grad(P, 8, P, kl.KL_BF16, 8, 8, P, None, P, 4, 2, 8, P, 8, P, None), "together"),
         (lambda: L.kl_moe_combine_grad(P, 7, P, kl.KL_BF16, 8, 8, None, None, P, 4, 2, 8, P, 8, P, None), "pitch"),
@@ -116,6 +119,8 @@ def test_row_movers_refusals():
     (dict(ids=P, experts=0, topk=1), "experts"), (dict(ids=P, experts=4, topk=0), "topk"),
     (dict(ids=P, experts=4, topk=2049, tokens=2), "4096"), (dict(ids=P, experts=1025, topk=1), "1024 experts"),
     (dict(ids=P, experts=4, topk=1, stride_q=8), "stride"),
+    (dict(scales=P + 1), "aligned"), (dict(out=P + 1), "aligned"), (dict(out=P + 2, out_type=kl.KL_F32), "aligned"),
+    (dict(ids=P + 2, experts=1, topk=1), "aligned"),
 ])
 def test_gemv_int4_refusals(over, what):
     d = dict(x=P, ldx=4096, q=P, ldq=2048, scales=P, ld_scales=32, out=P, ldo=64, tokens=1, n=64, k=4096, group=128,
