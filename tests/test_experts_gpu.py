@@ -504,6 +504,36 @@ def test_gemv_int4_by_expert(cuda, group, tokens, k, experts, n, width):
                     close(got[t, j][None], want, gemv_tol(row, m, want, width, dtype))
 
 
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
+@pytest.mark.parametrize("width", [2, 7, 1023, 2046, 4095, 4100, 4104])
+@pytest.mark.parametrize("shift", [0, 1])
+def test_rows_of_any_alignment(cuda, dtype, width, shift):
+    """Rows that begin anywhere, in pitches that fit no vector: copies exactly, sums against 64 bits, nothing beside
+    the rows written."""
+    tokens, experts, k = 37, 5, 2
+    ids = torch.randint(-1, experts, (tokens, k), generator=gen(width), dtype=torch.int32).to(cuda)
+    plan = kl.moe_plan(ids, experts)
+    m = plan.slots.shape[0]
+    x = torch.randn((tokens, width + 3), generator=gen(1)).to(dtype).to(cuda)[:, shift:shift + width]
+    room = torch.full((m, width + 5), 9.0, dtype=dtype, device=cuda)
+    y = kl.moe_dispatch(x, plan, out=room[:, shift:shift + width])
+    slots = plan.slots.long()
+    want = torch.where((slots >= 0)[:, None], x[slots.clamp(min=0) // k], 0)
+    assert torch.equal(y, want) and (room[:, :shift] == 9).all() and (room[:, shift + width:] == 9).all()
+    weights = torch.rand((tokens, k), generator=gen(2)).to(cuda)
+    live = (plan.rows >= 0).double() * weights.double()
+    rows = plan.rows.long().clamp(min=0)
+    out = kl.moe_combine(y, weights, rows=plan.rows)
+    want = (live[..., None] * y.double()[rows]).sum(1)
+    close(out, want.cpu(), (want.abs() * HALF[dtype] * 1.001 + 3 * U * (live[..., None] * y.double()[rows].abs()).sum(1) + 2.0 ** -25).cpu())
+    dy, dw = kl.moe_combine_grad(x, y, weights, rows=plan.rows, slots=plan.slots)
+    wanted = x.double()[slots.clamp(min=0) // k] * weights.double().flatten()[slots.clamp(min=0)][:, None] * (slots >= 0)[:, None]
+    close(dy, wanted.cpu(), (wanted.abs() * (HALF[dtype] * 1.001 + U) + 2.0 ** -25).cpu())
+    products = x.double()[:, None] * y.double()[rows] * (plan.rows >= 0)[..., None]
+    # A thread's products one after another, then 8 exchanges: at most width / 256 + 16 + 16 roundings.
+    close(dw, products.sum(-1).cpu(), (products.abs().sum(-1) * (width / 256 + 32) * U).cpu())
+
+
 # ------------------------------------------------------------------------------------ streams, graphs, together
 
 FIRST_IN_CAPTURE = """
