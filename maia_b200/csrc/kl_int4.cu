@@ -1018,6 +1018,12 @@ kl_status by_zeros(Int4Args& a, int device, cudaStream_t stream) {
   return a.zeros != nullptr ? by_group<T, true>(a, device, stream) : by_group<T, false>(a, device, stream);
 }
 
+// The group as the kernel counts it, in 32 bits: one that is longer than a row is the row, in whole 128s.
+int64_t group_within(kl_int4_desc const& d) {
+  const int64_t row = d.k > 128 ? (d.k + 127) / 128 * 128 : 128;
+  return d.group < row ? d.group : row;
+}
+
 kl_status run(kl_int4_desc const& d, int64_t slots, cudaStream_t stream) {
   const bool by_expert = d.ids != nullptr;
   int device = 0;
@@ -1048,7 +1054,7 @@ kl_status run(kl_int4_desc const& d, int64_t slots, cudaStream_t stream) {
   a.ldo = d.ldo;
   a.n = int(d.n);
   a.k = int(d.k);
-  a.group = int(d.group);
+  a.group = int(group_within(d));
   a.f32_scales = d.scale_type == KL_F32;
   a.f32_out = d.out_type == KL_F32;
   a.tiles = (a.n + kRows - 1) / kRows;
@@ -1084,7 +1090,7 @@ extern "C" kl_status kl_gemv_int4(const kl_int4_desc* d, void* stream) {
   if (d->k % 32 != 0) return bad("k must be a multiple of 32");
   if (d->k > kMaxK) return fail(KL_ERR_NOT_SUPPORTED, "kl_gemv_int4: k up to 65536");
   if (slots == 0 || d->n == 0) return KL_OK;
-  const int64_t groups = (d->k + d->group - 1) / d->group;
+  const int64_t group = group_within(*d), groups = (d->k + group - 1) / group;
   if (d->ldo < d->n || d->ldx < d->k || d->ldq < d->k / 2 || d->ld_scales < groups || (d->zeros != nullptr && d->ld_zeros < groups))
     return bad("row pitch below the row's extent");
   if (d->ld_scales > INT32_MAX / 4 || d->ld_zeros > INT32_MAX) return bad("row pitch too large");
