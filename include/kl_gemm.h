@@ -196,7 +196,8 @@ KL_API kl_status kl_nv_quantize(const void* x, int32_t x_type, int64_t rows, int
  * kl_moe_route chooses every token's experts and measures their balance; kl_moe_plan turns the ids
  * into the row layout that kl_gemm takes with m_block_group, kl_moe_dispatch copies the tokens' rows
  * into it and kl_moe_combine sums the experts' rows back. No counterpart in the reference. All are
- * stream-ordered, allocate nothing and may be captured; the current device must be the stream's.
+ * stream-ordered, allocate nothing and may be captured; the current device must be the stream's. Every
+ * array is aligned to its elements (else refused).
  * Launches overlap the end of the kernel before them (programmatic dependent launch) and touch
  * global memory only once it has completed. */
 

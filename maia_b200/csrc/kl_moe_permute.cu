@@ -443,6 +443,8 @@ extern "C" kl_status kl_moe_plan(const int32_t* ids, int64_t tokens, int64_t k, 
   if (m == 0) return KL_OK;
   if ((tokens > 0 && (ids == nullptr || rows == nullptr)) || slots == nullptr || m_block_group == nullptr)
     return fail(KL_ERR_INVALID_ARGUMENT, "kl_moe_plan: null pointer");
+  if (!words_aligned({ids, rows, slots, m_block_group}))
+    return fail(KL_ERR_INVALID_ARGUMENT, "kl_moe_plan: ids, rows, slots and m_block_group must be 4-byte aligned");
   PlanArgs a = {};
   a.ids = ids;
   a.total = tokens * k;
@@ -476,6 +478,7 @@ extern "C" kl_status kl_moe_dispatch(const void* x, int64_t ldx_bytes, int64_t t
   if (m == 0 || row_bytes == 0) return KL_OK;
   if ((tokens > 0 && (x == nullptr || rows == nullptr)) || slots == nullptr || a_out == nullptr)
     return fail(KL_ERR_INVALID_ARGUMENT, "kl_moe_dispatch: null pointer");
+  if (!words_aligned({rows, slots})) return fail(KL_ERR_INVALID_ARGUMENT, "kl_moe_dispatch: rows and slots must be 4-byte aligned");
   if (ldx_bytes < row_bytes || lda_bytes < row_bytes)
     return fail(KL_ERR_INVALID_ARGUMENT, "kl_moe_dispatch: row pitch below the row's bytes");
   RowArgs a = {};
@@ -537,6 +540,7 @@ extern "C" kl_status kl_moe_combine(const void* y, int32_t type, int64_t ldy, in
   if (out == nullptr || (m > 0 && y == nullptr)) return fail(KL_ERR_INVALID_ARGUMENT, "kl_moe_combine: null pointer");
   if (!aligned(y, size) || !aligned(out, size))
     return fail(KL_ERR_INVALID_ARGUMENT, "kl_moe_combine: y and out must be aligned to their elements");
+  if (!words_aligned({rows, weights})) return fail(KL_ERR_INVALID_ARGUMENT, "kl_moe_combine: rows and weights must be 4-byte aligned");
   RowArgs a = {};
   a.src = y;
   a.ld_src = ldy * size;
@@ -581,6 +585,8 @@ extern "C" kl_status kl_moe_combine_grad(const void* dout, int64_t ld_dout, cons
     return fail(KL_ERR_INVALID_ARGUMENT, "kl_moe_combine_grad: null pointer");
   if (!aligned(dout, size) || !aligned(y, size) || !aligned(dy, size))
     return fail(KL_ERR_INVALID_ARGUMENT, "kl_moe_combine_grad: dout, y and dy must be aligned to their elements");
+  if (!words_aligned({rows, slots, weights, dweights}))
+    return fail(KL_ERR_INVALID_ARGUMENT, "kl_moe_combine_grad: rows, slots, weights and dweights must be 4-byte aligned");
   RowArgs a = {};
   a.src = y;
   a.ld_src = ldy * size;

@@ -636,6 +636,8 @@ extern "C" kl_status kl_moe_route(const kl_moe_route_desc* d, void* workspace, s
     return fail(KL_ERR_INVALID_ARGUMENT, "kl_moe_route: null pointer");
   if (!aligned(d->logits, d->logits_type == KL_F32 ? 4 : 2))
     return fail(KL_ERR_INVALID_ARGUMENT, "kl_moe_route: logits must be aligned to their elements");
+  if (!words_aligned({d->ids, d->weights, d->counts, d->routed, d->loss}))
+    return fail(KL_ERR_INVALID_ARGUMENT, "kl_moe_route: ids, weights, counts, routed and loss must be 4-byte aligned");
   const int blocks = route_blocks(d->tokens, int(d->experts));
   size_t need = 0;
   kl_moe_route_workspace_size(d->tokens, d->experts, &need);
@@ -690,6 +692,8 @@ extern "C" kl_status kl_moe_route_grad(const kl_moe_route_desc* d, const float* 
     return fail(KL_ERR_INVALID_ARGUMENT, "kl_moe_route_grad: null pointer");
   if (!aligned(d->logits, d->logits_type == KL_F32 ? 4 : 2) || !aligned(dlogits, d->logits_type == KL_F32 ? 4 : 2))
     return fail(KL_ERR_INVALID_ARGUMENT, "kl_moe_route_grad: logits and their gradient must be aligned to their elements");
+  if (!words_aligned({d->ids, d->weights, d->counts, d->routed, dweights, dloss}))
+    return fail(KL_ERR_INVALID_ARGUMENT, "kl_moe_route_grad: ids, weights, counts, routed, dweights and dloss must be 4-byte aligned");
   RouteGradArgs a = {};
   a.logits = d->logits;
   a.ld = d->ld_logits;

@@ -8,6 +8,8 @@
 #include <cuda_runtime.h>
 
 #include <cstdint>
+#include <cstring>
+#include <initializer_list>
 
 namespace kl::capi {
 
@@ -51,6 +53,12 @@ __device__ __forceinline__ uint4 pack(const float* v) {
 }
 
 inline bool aligned(const void* p, size_t bytes) { return reinterpret_cast<uintptr_t>(p) % bytes == 0; }
+// The 32-bit arrays of a call; NULL = not given.
+inline bool words_aligned(std::initializer_list<const void*> arrays) {
+  for (const void* p : arrays)
+    if (!aligned(p, 4)) return false;
+  return true;
+}
 inline bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
 
 }  // namespace kl::capi

@@ -1,0 +1,37 @@
+"""The expert layer's refusals and host-side rules beside those of test_experts_cpu.py; nothing here reaches a GPU."""
+
+import ctypes
+
+import pytest
+
+import maia_b200 as kl
+from test_experts_cpu import P, route_desc
+
+
+def refused(status, what):
+    with pytest.raises(kl.KlError) as e:
+        kl.check(status)
+    assert e.value.status == kl.KL_ERR_INVALID_ARGUMENT and what in e.value.message, e.value.message
+
+
+@pytest.mark.parametrize("field", ["ids", "weights", "counts", "routed", "loss"])
+@pytest.mark.parametrize("off", [1, 2])
+def test_route_misaligned_arrays(field, off):
+    refused(kl.lib().kl_moe_route(ctypes.byref(route_desc(**{field: P + off})), None, 0, None), "4-byte aligned")
+    if field != "loss":  # not the gradient's
+        refused(kl.lib().kl_moe_route_grad(ctypes.byref(route_desc(**{field: P + off})), P, P, P, 64, None), "4-byte aligned")
+
+
+def test_route_grad_misaligned_gradients():
+    for dweights, dloss in ((P + 2, P), (P, P + 1), (P + 1, None), (None, P + 2)):
+        refused(kl.lib().kl_moe_route_grad(ctypes.byref(route_desc()), dweights, dloss, P, 64, None), "4-byte aligned")
+
+
+@pytest.mark.parametrize("at", range(4))
+def test_row_movers_misaligned_arrays(at):
+    L, w = kl.lib(), [P + 2 * (i == at) for i in range(4)]
+    refused(L.kl_moe_plan(w[0], 64, 4, 8, 128, 1280, w[1], w[2], w[3], None), "4-byte aligned")
+    refused(L.kl_moe_combine_grad(P, 8, P, kl.KL_BF16, 8, 8, w[0], w[1], w[2], 4, 2, 8, P, 8, w[3], None), "4-byte aligned")
+    if at < 2:
+        refused(L.kl_moe_dispatch(P, 16, 4, 16, 2, w[0], w[1], 128, P, 16, None), "4-byte aligned")
+        refused(L.kl_moe_combine(P, kl.KL_BF16, 8, 128, w[0], w[1], 4, 2, 8, P, 8, None), "4-byte aligned")
