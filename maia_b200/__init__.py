@@ -175,6 +175,32 @@ def lib() -> ctypes.CDLL:
     return _lib
 
 
+def _on_stream(stream: int, tensors, call):
+    """call() with the raw handle `stream` as torch's current stream on the tensors' device. What the call allocates
+    comes from that stream's memory, since a block of the current stream's may still be in use there; the
+    tensors outlive their use on `stream`, and what is returned its use on the current one."""
+    import torch
+
+    tensors = [t for t in tensors if t is not None]
+    device = tensors[0].device
+    if device.type != "cuda":
+        return call()  # refuses them
+    current = torch.cuda.current_stream(device)
+    if stream == current.cuda_stream:
+        return call()
+    # ExternalStream takes 0, the legacy default stream, for a new one.
+    there = torch.cuda.ExternalStream(stream, device=device) if stream else torch.cuda.default_stream(device)
+    with torch.cuda.stream(there):
+        result = call()
+    for t in tensors:
+        t.record_stream(there)
+    for t in result if isinstance(result, tuple) else (result,):
+        if t is not None:
+            t.record_stream(there)
+            t.record_stream(current)
+    return result
+
+
 def last_error() -> str:
     return lib().kl_last_error().decode()
 

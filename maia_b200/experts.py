@@ -7,8 +7,10 @@
     out = moe_combine(y, r.weights, rows=plan.rows)
 
 For a few tokens, without a layout: y = gemv_int4(x, q, scales, ids=r.ids); out = moe_combine(y, r.weights).
-Every call is queued on the tensors' current CUDA stream (or `stream`) and allocates only its outputs,
-through torch. No counterpart in the reference (kernel_lib has no GEMM and no routing).
+Every call is queued on the tensors' current CUDA stream and allocates only its outputs (moe_route a workspace too),
+through torch. With `stream`, a raw handle, it runs as with that stream current: the caller orders the two streams, as
+for torch's own calls, and keeps the handle valid while tensors of the call live. No counterpart in the reference
+(kernel_lib has no GEMM and no routing).
 """
 
 from __future__ import annotations
@@ -20,7 +22,7 @@ from typing import NamedTuple
 
 import torch
 
-from . import Int4Desc, KL_BF16, KL_F16, KL_F32, KL_OK, MoeRouteDesc, check, lib
+from . import Int4Desc, KL_BF16, KL_F16, KL_F32, KL_OK, MoeRouteDesc, _on_stream, check, lib
 
 _FLOATS = {torch.bfloat16: KL_BF16, torch.float16: KL_F16, torch.float32: KL_F32}
 
@@ -94,20 +96,13 @@ def _device(first, *others) -> int:
     return index
 
 
-def _queue(device: int, stream, owned, fn, *args) -> None:
-    """fn(*args, stream) with `device` current; `owned` tensors of this call outlive their use on a `stream`
-    that is not torch's current one."""
-    current = _raw_stream(device)
-    if stream is None:
-        stream = current
-    elif stream != current:
-        for t in owned:
-            t.record_stream(torch.cuda.ExternalStream(stream, torch.device("cuda", device)))
+def _queue(device: int, fn, *args) -> None:
+    """fn(*args, the device's current stream) with `device` current."""
     if device == _current_device():
-        status = fn(*args, stream)
+        status = fn(*args, _raw_stream(device))
     else:
         with torch.cuda.device(device):
-            status = fn(*args, stream)
+            status = fn(*args, _raw_stream(device))
     if status != KL_OK:
         check(status)
 
@@ -140,6 +135,8 @@ def moe_route(logits, k: int, *, renormalize: bool = True, valid=None, stream=No
     for N = 0). A logit of -inf closes that expert to the token; a slot left without an expert has id
     -1 and weight 0. Tokens with valid = False, or with every logit -inf, are not routed, and what
     padding tokens hold is not read. For gradients: moe_route_grad, or torch.ops.kl.moe_route."""
+    if stream is not None:
+        return _on_stream(stream, (logits, valid), lambda: moe_route(logits, k, renormalize=renormalize, valid=valid))
     _check_logits(logits, valid)
     tokens, experts = logits.shape
     if not 1 <= k <= experts:
@@ -150,14 +147,11 @@ def moe_route(logits, k: int, *, renormalize: bool = True, valid=None, stream=No
     counts = logits.new_empty((experts,), dtype=torch.int32)
     routed = logits.new_empty((), dtype=torch.int32)
     loss = logits.new_empty((), dtype=torch.float32)
-    out = MoeRoute(ids, weights, counts, routed, loss)
-    owned, work, size = out, None, _route_workspace(tokens, experts)
-    if size:
-        work = logits.new_empty((size,), dtype=torch.uint8)
-        owned = (*out, work)
+    size = _route_workspace(tokens, experts)
+    work = logits.new_empty((size,), dtype=torch.uint8) if size else None
     d = _route_desc(logits, k, renormalize, valid, ids, weights, counts, routed, loss)
-    _queue(device, stream, owned, lib().kl_moe_route, d, _ptr(work), size)
-    return out
+    _queue(device, lib().kl_moe_route, d, _ptr(work), size)
+    return MoeRoute(ids, weights, counts, routed, loss)
 
 
 def moe_route_grad(logits, route: MoeRoute, dweights=None, dloss=None, *, renormalize: bool = True, valid=None,
@@ -165,6 +159,9 @@ def moe_route_grad(logits, route: MoeRoute, dweights=None, dloss=None, *, renorm
     """The gradient of moe_route's logits from those of its weights (fp32 [tokens, k]) and loss (fp32
     scalar); None = 0. `route` is moe_route's result for the same logits, renormalize and valid; its
     counts are constants. `out` may be the logits themselves."""
+    if stream is not None:
+        return _on_stream(stream, (logits, *route, dweights, dloss, valid, out),
+                          lambda: moe_route_grad(logits, route, dweights, dloss, renormalize=renormalize, valid=valid, out=out))
     _check_logits(logits, valid)
     tokens, experts = logits.shape
     _refuse(route.ids.dim() == 2, "route.ids must be 2-D")
@@ -183,8 +180,7 @@ def moe_route_grad(logits, route: MoeRoute, dweights=None, dloss=None, *, renorm
     _refuse(out.shape == logits.shape, "out must have the logits' shape")
     device = _device(logits, valid, route.ids, route.weights, route.counts, route.tokens, dweights, dloss, out)
     d = _route_desc(logits, k, renormalize, valid, route.ids, route.weights, route.counts, route.tokens, None)
-    _queue(device, stream, (out,), lib().kl_moe_route_grad, d, _ptr(dweights), _ptr(dloss), out.data_ptr(),
-           _pitch(out))
+    _queue(device, lib().kl_moe_route_grad, d, _ptr(dweights), _ptr(dloss), out.data_ptr(), _pitch(out))
     return out
 
 
@@ -200,13 +196,15 @@ def moe_plan(ids, experts: int, *, block: int = 128, stream=None) -> MoePlan:
     expert): the slots sorted by expert, in their order within one, each expert padded to `block`
     rows (256 for gemm_grouped's algo=ALGO_2CTA). Its m = moe_rows(tokens * k, experts, block) rows fit any
     ids, so nothing is read back; blocks behind the last expert have m_block_group -1."""
+    if stream is not None:
+        return _on_stream(stream, (ids,), lambda: moe_plan(ids, experts, block=block))
     _refuse(ids.dim() == 2, "ids must be 2-D")
     _whole("ids", ids, ids.shape, torch.int32)
     tokens, k = ids.shape
     m = moe_rows(tokens * k, experts, block)
     device = _device(ids)
     plan = MoePlan(torch.empty_like(ids), ids.new_empty((m,)), ids.new_empty((m // 128,)))
-    _queue(device, stream, plan, lib().kl_moe_plan, ids.data_ptr(), tokens, k, experts, block, m, plan.rows.data_ptr(),
+    _queue(device, lib().kl_moe_plan, ids.data_ptr(), tokens, k, experts, block, m, plan.rows.data_ptr(),
            plan.slots.data_ptr(), plan.m_block_group.data_ptr())
     return plan
 
@@ -220,6 +218,8 @@ def _check_plan(rows, slots) -> None:
 def moe_dispatch(x, plan: MoePlan, out=None, *, stream=None):
     """out[row] = x[slots[row] // k]: the tokens' rows (2-D, any type) in the m-grouped layout, every padding row
     zero. Its gradient is moe_combine(dout, rows=plan.rows)."""
+    if stream is not None:
+        return _on_stream(stream, (x, plan.rows, plan.slots, out), lambda: moe_dispatch(x, plan, out))
     rows, slots = plan.rows, plan.slots
     _matrix("x", x)
     _check_plan(rows, slots)
@@ -232,7 +232,7 @@ def moe_dispatch(x, plan: MoePlan, out=None, *, stream=None):
     else:
         _matrix("out", out, (x.dtype,))
         _refuse(out.shape == (m, width), f"out must have the shape {(m, width)}")
-    _queue(_device(x, rows, slots, out), stream, (out,), lib().kl_moe_dispatch, x.data_ptr(), _pitch(x) * size, tokens,
+    _queue(_device(x, rows, slots, out), lib().kl_moe_dispatch, x.data_ptr(), _pitch(x) * size, tokens,
            width * size, max(k, 1), rows.data_ptr(), slots.data_ptr(), m, out.data_ptr(), _pitch(out) * size)
     return out
 
@@ -260,6 +260,8 @@ def moe_combine(y, weights=None, *, rows=None, out=None, stream=None):
     """out[t] = sum_j weights[t, j] * y[rows[t, j]] in fp32, rounded once to y's type (bf16, f16, fp32). y
     is [m, width] with int32 rows [tokens, k] (-1 adds nothing), or [tokens, k, width] without rows.
     weights: fp32 [tokens, k], None = 1."""
+    if stream is not None:
+        return _on_stream(stream, (y, weights, rows, out), lambda: moe_combine(y, weights, rows=rows, out=out))
     tokens, k, m, width, pitch = _rows_of(y, rows, weights)
     if out is None:
         out = y.new_empty((tokens, width))
@@ -269,7 +271,7 @@ def moe_combine(y, weights=None, *, rows=None, out=None, stream=None):
     device = _device(y, rows, weights, out)
     if k == 0:
         return out.zero_()
-    _queue(device, stream, (out,), lib().kl_moe_combine, y.data_ptr(), _FLOATS[y.dtype], pitch, m, _ptr(rows), _ptr(weights),
+    _queue(device, lib().kl_moe_combine, y.data_ptr(), _FLOATS[y.dtype], pitch, m, _ptr(rows), _ptr(weights),
            tokens, k, width, out.data_ptr(), _pitch(out))
     return out
 
@@ -278,6 +280,9 @@ def moe_combine_grad(dout, y, weights=None, *, rows=None, slots=None, stream=Non
     """(dy, dweights) of moe_combine from dout [tokens, width] of y's type: dy in y's shape and type,
     zero in padding rows; dweights fp32, or None where weights is None. rows and slots are moe_plan's, or
     both None."""
+    if stream is not None:
+        return _on_stream(stream, (dout, y, weights, rows, slots),
+                          lambda: moe_combine_grad(dout, y, weights, rows=rows, slots=slots))
     tokens, k, m, width, pitch = _rows_of(y, rows, weights)
     _refuse((rows is None) == (slots is None), "rows and slots come together")
     if slots is not None:
@@ -288,8 +293,7 @@ def moe_combine_grad(dout, y, weights=None, *, rows=None, slots=None, stream=Non
     device = _device(dout, y, weights, rows, slots)
     dy = y.new_empty(y.shape)
     dweights = None if weights is None else torch.empty_like(weights)
-    _queue(device, stream, (dy,) if dweights is None else (dy, dweights), lib().kl_moe_combine_grad, dout.data_ptr(),
-           _pitch(dout), y.data_ptr(), _FLOATS[y.dtype], pitch, m, _ptr(rows), _ptr(slots), _ptr(weights), tokens, max(k, 1),
+    _queue(device, lib().kl_moe_combine_grad, dout.data_ptr(), _pitch(dout), y.data_ptr(), _FLOATS[y.dtype], pitch, m, _ptr(rows), _ptr(slots), _ptr(weights), tokens, max(k, 1),
            width, dy.data_ptr(), width, _ptr(dweights))
     return dy, dweights
 
@@ -303,6 +307,9 @@ def gemv_int4(x, q, scales, zeros=None, *, group: int = 128, ids=None, out=None,
     at most 4096 ids, 1024 experts). out in x's type or fp32. Sums are exact or fp32 (with up to two
     tokens to a matrix x enters with 22 bits below the largest of its 128 neighbours); a NaN or infinity makes its
     row NaN or infinite. Up to 16 tokens of a matrix read the weights once. K up to 65536."""
+    if stream is not None:
+        return _on_stream(stream, (x, q, scales, zeros, ids, out),
+                          lambda: gemv_int4(x, q, scales, zeros, group=group, ids=ids, out=out, out_dtype=out_dtype))
     dtype, bits = x.dtype, x.dim()
     if dtype is not torch.bfloat16 and dtype is not torch.float16:
         raise ValueError("x must be bf16 or f16")
@@ -344,5 +351,5 @@ def gemv_int4(x, q, scales, zeros=None, *, group: int = 128, ids=None, out=None,
                    scales.data_ptr(), _pitch(scales), 0 if one else scales.stride(0), *zero_fields,
                    0 if one else ids.data_ptr(), 0 if one else q.shape[0], topk, out.data_ptr(), _pitch(out) if one else n,
                    tokens, n, k, group, _FLOATS[dtype], _FLOATS[scales.dtype], _FLOATS[out.dtype], per_slot)
-    _queue(_device(x, q, scales, zeros, ids, out), stream, (out,), lib().kl_gemv_int4, d)
+    _queue(_device(x, q, scales, zeros, ids, out), lib().kl_gemv_int4, d)
     return out

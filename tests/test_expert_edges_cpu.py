@@ -35,3 +35,13 @@ def test_row_movers_misaligned_arrays(at):
     if at < 2:
         refused(L.kl_moe_dispatch(P, 16, 4, 16, 2, w[0], w[1], 128, P, 16, None), "4-byte aligned")
         refused(L.kl_moe_combine(P, kl.KL_BF16, 8, 128, w[0], w[1], 4, 2, 8, P, 8, None), "4-byte aligned")
+
+
+def test_host_tensors_are_refused_on_any_stream():
+    import torch
+
+    x, q, s = torch.zeros((2, 64), dtype=torch.bfloat16), torch.zeros((8, 32), dtype=torch.uint8), torch.ones((8, 1), dtype=torch.bfloat16)
+    for call in (lambda: kl.moe_route(torch.zeros((2, 4)), 1, stream=16), lambda: kl.gemv_int4(x, q, s, group=64, stream=0),
+                 lambda: kl.moe_combine(torch.zeros((2, 2, 8)), stream=16)):
+        with pytest.raises(ValueError):
+            call()

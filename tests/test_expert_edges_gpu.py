@@ -54,3 +54,122 @@ def test_gemv_int4_group_longer_than_32_bits(cuda, tokens, group):
     within(got, want, slack)
     for j in range(2):
         within(by_expert[:, j], want, slack)
+
+
+# ------------------------------------------------------------------------------------ streams
+
+PENDING = 100_000_000  # cycles that a stream is kept busy: 50 ms
+
+
+def calls(cuda):
+    """name -> (a call on a stream, fresh tensors that it reads)."""
+    tokens, experts, k, width = 3000, 64, 4, 264
+    logits = torch.randn((tokens, experts), generator=gen(1)).to(cuda)
+    x = torch.randn((tokens, width), generator=gen(2)).bfloat16().to(cuda)
+    route = kl.moe_route(logits, k)
+    plan = kl.moe_plan(route.ids, experts)
+    y = kl.moe_dispatch(x, plan)
+    dw = torch.randn((tokens, k), generator=gen(3)).to(cuda)
+    q = torch.randint(0, 256, (4096, 256), generator=gen(4), dtype=torch.uint8).to(cuda)
+    s = torch.ones((4096, 4), device=cuda).bfloat16()
+    v = torch.randn((300, 512), generator=gen(5)).bfloat16().to(cuda)
+    some = torch.randint(-1, 2, (300, 2), generator=gen(6), dtype=torch.int32).to(cuda)
+    return {
+        "route": (lambda st, t: kl.moe_route(t, k, stream=st), logits),
+        "route_grad": (lambda st, t: kl.moe_route_grad(t, route, dw, route.loss, stream=st), logits),
+        "plan": (lambda st, t: kl.moe_plan(t, experts, stream=st), route.ids),
+        "dispatch": (lambda st, t: kl.moe_dispatch(t, plan, stream=st), x),
+        "combine": (lambda st, t: kl.moe_combine(t, dw, rows=plan.rows, stream=st), y),
+        "combine_grad": (lambda st, t: kl.moe_combine_grad(t, y, dw, rows=plan.rows, slots=plan.slots, stream=st), x),
+        "gemv": (lambda st, t: kl.gemv_int4(t, q, s, stream=st), v),
+        "gemv_by_expert": (lambda st, t: kl.gemv_int4(v, q.view(2, 2048, 256), s.view(2, 2048, 4), ids=t, stream=st), some),
+    }
+
+
+def several(result):
+    return [t for t in (result if isinstance(result, tuple) else (result,)) if t is not None]
+
+
+NAMES = ["route", "route_grad", "plan", "dispatch", "combine", "combine_grad", "gemv", "gemv_by_expert"]
+
+
+@pytest.mark.parametrize("name", NAMES)
+def test_memory_that_the_current_stream_still_uses(cuda, name):
+    """A call on another stream takes none of the blocks that were just given back while work queued on the
+    current stream still reads them, its workspace's among them."""
+    call, t = calls(cuda)[name]
+    want = [r.clone() for r in several(call(None, t))]
+    need = kl.experts._route_workspace(3000, 64)
+    sizes = [r.numel() * r.element_size() for r in want] + [need]
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    for _ in range(2):
+        freed = [torch.full((size,), 7, dtype=torch.uint8, device=cuda) for size in sizes for _ in range(2)]
+        torch.cuda._sleep(PENDING)
+        copies = [f.clone() for f in freed]
+        del freed
+        got = several(call(side.cuda_stream, t))
+        side.synchronize()
+        same = [g.clone() for g in got]
+        torch.cuda.synchronize()
+        assert all((c == 7).all() for c in copies)
+        assert all(torch.equal(a, b) for a, b in zip(same, want))
+
+
+@pytest.mark.parametrize("name", [n for n in NAMES if n not in ("plan", "gemv_by_expert")])
+def test_inputs_dropped_while_another_stream_reads_them(cuda, name):
+    call, t = calls(cuda)[name]
+    want = [r.clone() for r in several(call(None, t))]
+    side = torch.cuda.Stream()
+    mine = t.clone()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(PENDING)
+    got = several(call(side.cuda_stream, mine))
+    del mine
+    over = [torch.full_like(t, 3) for _ in range(4)]  # would take the block that was given back
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(got, want)) and len(over) == 4
+
+
+@pytest.mark.parametrize("name", NAMES)
+def test_outputs_dropped_while_the_current_stream_reads_them(cuda, name):
+    """What a call on another stream returns may be used on the current stream and dropped there."""
+    call, t = calls(cuda)[name]
+    want = [r.clone() for r in several(call(None, t))]
+    side, zero = torch.cuda.Stream(), torch.zeros_like(t)
+    torch.cuda.synchronize()
+    got = several(call(side.cuda_stream, t))
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda._sleep(PENDING)
+    copies = [g.clone() for g in got]
+    del got
+    call(side.cuda_stream, zero)  # would write where the first results lay
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(copies, want))
+
+
+def test_the_default_stream_by_its_handle(cuda):
+    x = torch.randn((3000, 64), generator=gen(1)).to(cuda)
+    want = kl.moe_route(x, 4)
+    torch.cuda.synchronize()
+    with torch.cuda.stream(torch.cuda.Stream()):
+        got = kl.moe_route(x, 4, stream=0)
+        torch.cuda.default_stream().synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+    torch.cuda.synchronize()
+
+
+def test_nothing_to_add_on_another_stream(cuda):
+    """No slots at all: the zeros are written on the stream that was asked for."""
+    side = torch.cuda.Stream()
+    out = torch.full((50, 64), 5.0, device=cuda)
+    torch.cuda.synchronize()
+    torch.cuda._sleep(PENDING)
+    kl.moe_combine(torch.empty((50, 0, 64), device=cuda), out=out, stream=side.cuda_stream)
+    side.synchronize()
+    with torch.cuda.stream(side):
+        zero = (out == 0).all()
+        side.synchronize()
+    assert bool(zero)
+    torch.cuda.synchronize()
