@@ -201,6 +201,16 @@ def _on_stream(stream: int, tensors, call):
     return result
 
 
+def _new(stream, tensors, shape, dtype):
+    """An output beside the first of `tensors`, for a call that reads them on `stream` (None: the current one)."""
+    import torch
+
+    def make():
+        return torch.empty(shape, dtype=dtype, device=tensors[0].device)
+
+    return make() if stream is None else _on_stream(stream, tensors, make)
+
+
 def last_error() -> str:
     return lib().kl_last_error().decode()
 
@@ -373,7 +383,7 @@ def gemm(a, b, out=None, *, out_dtype=None, alpha=1.0, scale_a=None, scale_b=Non
         m = a.shape[-1] if a_major else a.shape[-2]
         n = b.shape[-1] if b_major else b.shape[-2]
         shape = (a.shape[0], m, n) if a.dim() == 3 else (m, n)
-        out = torch.empty(shape, dtype=out_dtype or torch.bfloat16, device=a.device)
+        out = _new(stream, (a, b, scale_a, scale_b, sfa, sfb, workspace), shape, out_dtype or torch.bfloat16)
     d = gemm_desc(a, b, out, alpha, scale_a, scale_b, algo, group_m, max_ctas, variant, prefetch, a_major, b_major,
                   int(bool(accumulate)), swizzle, sfa, sfb, scale_vec, ab_type, stream_k, overlap)
     s = stream if stream is not None else torch.cuda.current_stream(a.device).cuda_stream
@@ -430,7 +440,7 @@ def gemm_grouped(a, b, m_block_group, out=None, *, out_dtype=None, alpha=1.0, sc
     if accumulate and out is None:
         raise ValueError("accumulate=True adds into `out`, which must be given")
     if out is None:
-        out = torch.empty((a.shape[0], b.shape[1]), dtype=out_dtype or torch.bfloat16, device=a.device)
+        out = _new(stream, (a, b, m_block_group, scale_a, scale_b, sfa, sfb), (a.shape[0], b.shape[1]), out_dtype or torch.bfloat16)
     d = gemm_desc(a, b[0], out, alpha, scale_a, scale_b, algo, c_reduce=int(bool(accumulate)), sfa=sfa, sfb=sfb,
                   scale_vec=scale_vec, ab_type=ab_type, stream_k=stream_k)
     d.groups = b.shape[0]
@@ -454,7 +464,7 @@ def pack_block_scales(scales, k: int, vec: int = 32, out=None, stream=None):
     if scales.dtype != torch.uint8 or scales.dim() != 2 or scales.stride(1) != 1:
         raise ValueError("scales must be a 2-D uint8 tensor with a contiguous last dimension")
     if out is None:
-        out = torch.empty(block_scale_bytes(rows, k, vec), dtype=torch.uint8, device=scales.device)
+        out = _new(stream, (scales,), (block_scale_bytes(rows, k, vec),), torch.uint8)
     s = stream if stream is not None else torch.cuda.current_stream(scales.device).cuda_stream
     check(lib().kl_pack_block_scales(ctypes.c_void_p(scales.data_ptr()), rows, int(k), int(vec), scales.stride(0),
                                      ctypes.c_void_p(out.data_ptr()), ctypes.c_void_p(s)))
@@ -468,6 +478,8 @@ def mx_quantize(x, kind: str = "e4m3", stream=None):
     blocked UE8M0 array, ready for gemm(..., sfa=scales) (with ab_type=kind for fp6)."""
     import torch
 
+    if stream is not None:
+        return _on_stream(stream, (x,), lambda: mx_quantize(x, kind))
     rows, k = x.shape
     if x.stride(1) != 1:
         raise ValueError("x must have a contiguous last dimension")
@@ -496,6 +508,8 @@ def nv_quantize(x, stream=None):
     scale_a=g, scale_vec=16)."""
     import torch
 
+    if stream is not None:
+        return _on_stream(stream, (x,), lambda: nv_quantize(x))
     rows, k = x.shape
     if x.stride(1) != 1:
         raise ValueError("x must have a contiguous last dimension")

@@ -173,3 +173,40 @@ def test_nothing_to_add_on_another_stream(cuda):
         side.synchronize()
     assert bool(zero)
     torch.cuda.synchronize()
+
+
+def products(cuda):
+    """name -> a call on a stream of the package's GEMMs and quantisers that make their own outputs."""
+    x = torch.randn((512, 1024), generator=gen(1)).bfloat16().to(cuda)
+    w = torch.randn((2, 768, 1024), generator=gen(2)).bfloat16().to(cuda)
+    blocks = torch.tensor([0, 1, 1, 0], dtype=torch.int32, device=cuda)
+    scales = torch.randint(100, 140, (512, 32), generator=gen(3), dtype=torch.uint8).to(cuda)
+    return {
+        "gemm": lambda st: kl.gemm(x, w[0], stream=st),
+        "gemm_grouped": lambda st: kl.gemm_grouped(x, w, blocks, stream=st),
+        "pack_block_scales": lambda st: kl.pack_block_scales(scales, 1024, stream=st),
+        "mx_quantize": lambda st: kl.mx_quantize(x, stream=st),
+        "nv_quantize": lambda st: kl.nv_quantize(x, stream=st),
+    }
+
+
+@pytest.mark.parametrize("name", ["gemm", "gemm_grouped", "pack_block_scales", "mx_quantize", "nv_quantize"])
+def test_outputs_of_products_on_another_stream(cuda, name):
+    """Likewise for the calls around the GEMMs that make their outputs: none lies where the current stream still reads."""
+    call = products(cuda)[name]
+    bits = lambda t: t.contiguous().view(torch.uint8).clone()  # noqa: E731
+    want = [bits(r) for r in several(call(None))]
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    for _ in range(2):
+        freed = [torch.full((w.numel(),), 7, dtype=torch.uint8, device=cuda) for w in want for _ in range(2)]
+        torch.cuda._sleep(PENDING)
+        copies = [f.clone() for f in freed]
+        del freed
+        got = several(call(side.cuda_stream))
+        side.synchronize()
+        with torch.cuda.stream(side):
+            same = [bits(g) for g in got]
+        torch.cuda.synchronize()
+        assert all((c == 7).all() for c in copies)
+        assert all(torch.equal(a, b) for a, b in zip(same, want))
