@@ -277,10 +277,8 @@ KL_API kl_status kl_moe_combine_grad(const void* dout, int64_t ld_dout, const vo
  * out[t, n] = sum_i x[t, i] (q[n, i] - zeros[n, i / group]) scales[n, i / group], rounded once. With
  * ids, one matrix per expert: out row t topk + j uses expert ids[t, j] (the experts' products for
  * single tokens, straight from kl_moe_route's ids; an id may repeat); an id outside [0, experts)
- * gives zeros. All sums are kept in fp32 or exactly: with up to two tokens to a matrix x enters as a
- * fixed-point number with 22 bits below the largest of its 128 neighbours (what an fp32 sum with that
- * neighbour would keep) and a scale group's products are summed exactly; with more, q - zeros and x enter
- * as they are and every sum is fp32. A NaN or infinity in a row of x makes that row of out NaN or
+ * gives zeros. x and q - zeros enter with all their bits and every sum is exact or fp32, in an order that
+ * depends on the shape and on the tokens that a matrix meets. A NaN or infinity in a row of x makes that row of out NaN or
  * infinite, and no other. The weights stream once for up to 16 tokens of a matrix; more take a pass for
  * every 16. Allocates nothing, keeps
  * nothing; stream-ordered; may be captured. No counterpart in the reference. */

@@ -7,15 +7,18 @@
 //
 // One and two tokens. As unsigned bytes eight codes cost three instructions (two masks and a shift), so the products are
 // integer ones (mma.sync.m16n8k32, u8 x s8 -> s32): every block first writes x as fixed-point numbers X = round(x 2^e),
-// |X| <= 2^22, one e for 128 K-elements of a token, in three signed digits of 8 bits, x ~ 2^-e (d_0 + 256 d_1 + 65536 d_2).
-// This rounding is at most 2^-22 of the 128 elements' largest |x|, what one addition in fp32 loses. The sums of a scale
-// group are exact: P_c = sum q d_c, and P_c - z D_c, D_c = sum d_c, takes the zero point off without cancellation. Only
-// then come fp32 and the scales: sum over the 128s of 2^-e sum_g s 256^c (P_c - z D_c).
+// |X| <= 2^30, one e for 128 K-elements of a token, in four signed digits of 8 bits, x = 2^-e (d_0 + 256 d_1 + ...) + r.
+// The sums of a scale group are exact: P_c = sum q d_c, and P_c - z D_c, D_c = sum d_c, takes the zero point off without
+// cancellation. Only then come fp32 and the scales: sum over the 128s of 2^-e sum_g s 256^c (P_c - z D_c).
+// A rest r is left where an element lies far below the largest of its 128 (2^-22 of it in bf16; in f16 only beside one of
+// 64 and more). It may be all that counts, where the large one meets a code equal to its zero point, so 128s with a rest
+// are marked, and r, which x's type holds exactly, is multiplied as below and added. One of 28000 128s of normal bf16
+// values has a rest, one of 1000 of gated ones; three digits would leave one in 120 and 7 of them, in f16 15 and 1.7.
 //
-// More tokens, 8 or 16 at a time. Three digits of 8 tokens would be three products and a longer sum, so here the
+// More tokens, 8 or 16 at a time. Four digits of 8 tokens would be four products and a longer sum, so here the
 // codes become q - z in x's type, exactly (eleven instructions for eight codes in bf16, nine in f16), and the products are
-// x's own (mma.sync.m16n8k16, sums in fp32); a group's sum is scaled once. Digits took 44 us for 8 tokens of
-// 28672 x 8192 and 83 for 16; this takes 43 and 60.
+// x's own (mma.sync.m16n8k16, sums in fp32); a group's sum is scaled once. Three digits took 44 us for 8 tokens of
+// 28672 x 8192 and 83 for 16; this takes 42 and 60.
 //
 // Layout: a block per SM, 16 warps, each with its own ring of TMA loads (units of 16 rows x 512
 // codes, two boxes of 128 bytes a row), refilled as soon as a slot has been read, so that no warp waits for another
@@ -23,9 +26,9 @@
 // would crowd out the ring, a cluster of 2, 4 or 8 blocks splits K and adds up through distributed
 // shared memory.
 //
-// Measured, bf16, groups of 128: 28672 x 8192 with one token 25 us (4.9 TB/s; 6.9 while it streams, 6 us before the first
-// unit and 2 after the last), 2 tokens 26.3, 8 tokens 43, 16 tokens 60 (instruction issue, four warps a scheduler); groups
-// of 32 with zero points, one token 37 (a scale, a zero point and a sum every 32 codes); 4096 x 4096, one token 6.5.
+// Measured, bf16, groups of 128: 28672 x 8192 with one token 24.3 us (5.0 TB/s; 6.9 while it streams, 6 us before the first
+// unit and 2 after the last), 2 tokens 25.7, 8 tokens 42, 16 tokens 60 (instruction issue, four warps a scheduler); groups
+// of 32 with zero points, one token 38 (a scale, a zero point and a sum every 32 codes); 4096 x 4096, one token 6.8.
 
 #include <cooperative_groups.h>
 #include <cuda.h>
@@ -77,7 +80,7 @@ struct Int4Args {
   int f32_scales, f32_out;
   int tiles;  // 16-row tiles of one matrix
   int depth;  // slots of a warp's ring
-  uint32_t x_at, sums, powers, pieces, block, records, bars, lists;  // offsets in shared memory
+  uint32_t x_at, sums, powers, rests, pieces, block, records, bars, lists;  // offsets in shared memory
   int wide_scales;                                      // a lane's scales and zero points come by one load
   int group_span, last_group;                           // 128-element runs of a group (groups of 128 and more); index of the last
   int* status;
@@ -188,6 +191,44 @@ struct Codes<__half> {
   }
 };
 
+// 32 codes - z of rows g and g + 8 as the A operands of two products in x's type.
+template <class T, bool kZeros>
+struct CodesOf32 {
+  // bf16 has 128 + z for z up to 127; what is above goes into a product of its own.
+  static constexpr uint32_t kMaxZ = std::is_same_v<T, __nv_bfloat16> ? 127 : 255;
+  uint32_t low[4], high[4];
+  uint32_t z[2];
+  bool more = false;
+  __device__ __forceinline__ CodesOf32(Codes<T> const& codes, uint32_t w0, uint32_t w1, const uint32_t (&zero)[2]) : z{zero[0], zero[1]} {
+    const auto z0 = codes.zero(kZeros ? min(z[0], kMaxZ) * 0x10001u : 0x00080008u);
+    const auto z1 = codes.zero(kZeros ? min(z[1], kMaxZ) * 0x10001u : 0x00080008u);
+    uint32_t f0[4], f1[4];
+    codes.minus(w0, z0, f0);
+    codes.minus(w1, z1, f1);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      low[2 * i] = f0[i];
+      low[2 * i + 1] = f1[i];
+      high[2 * i] = f0[2 + i];
+      high[2 * i + 1] = f1[2 + i];
+    }
+    if (kZeros && kMaxZ < 255) more = __any_sync(0xFFFFFFFFu, max(z[0], z[1]) > kMaxZ);
+  }
+  // dot = or += the products with eight tokens' 32 elements of x.
+  __device__ __forceinline__ void times(float (&dot)[4], uint4 x, bool first) const {
+    mma_16<T>(dot, low, x.x, x.y, first);
+    mma_16<T>(dot, high, x.z, x.w, false);
+    if (more) {
+      uint32_t rest[2];
+#pragma unroll
+      for (int r = 0; r < 2; ++r) rest[r] = pack_two<T>(-float(max(z[r], kMaxZ) - kMaxZ));
+      const uint32_t fr[4] = {rest[0], rest[1], rest[0], rest[1]};
+      mma_16<T>(dot, fr, x.x, x.y, false);
+      mma_16<T>(dot, fr, x.z, x.w, false);
+    }
+  }
+};
+
 // With ids: the experts that some slot names, each with its slots, in shared memory.
 struct Lists {
   int* base;        // [experts + 1]: token passes before an active expert
@@ -270,8 +311,8 @@ __device__ void build_lists(const Int4Args& a, Lists const& l, int* hist, int* a
   *active_out = active;
 }
 
-// TOK: tokens of a pass, 1, 2, 8 or 16. Up to two go by the integer products: three digits of two tokens fit one
-// 8-column tile, digit c of token i in column 2 c + i, and the digits meet by shuffles. 8 and 16 would take three and six
+// TOK: tokens of a pass, 1, 2, 8 or 16. Up to two go by the integer products: four digits of two tokens fill one
+// 8-column tile, digit c of token i in column 2 c + i, and the digits meet by shuffles. 8 and 16 would take four and eight
 // tiles; with them the codes are turned into x's type and each 8 tokens are one tile.
 template <int TOK>
 constexpr bool kDigits = TOK <= 2;
@@ -283,17 +324,21 @@ constexpr int kUnitK = TOK <= 8 ? 512 : 256;
 template <int TOK>
 constexpr int kUnitBytes = kRows * kUnitK<TOK> / 2;
 
-// x in shared memory, by 32 K-elements. Digits: a row of 32 bytes for each column that is used; sums D of a scale
-// group, an int a column; powers 2^-e of 128 elements, times 256^c, a float a column. Else: 64 bytes a token, every eight
+// x in shared memory, by 32 K-elements. Digits: a row of 32 bytes for each column that is used, and 16 bytes between, so
+// that the lanes that write them meet other banks (without, 4096 x 4096 with one token 6.9 us instead of 6.8); sums D of a scale
+// group, an int a column; powers 2^-e of 128 elements, times 256^c, a float a column; rests, a byte a token and 128
+// elements: not 0 where some r is not. Else: 64 bytes a token, every eight
 // elements in the order of the codes' pairs.
 template <int TOK>
-constexpr int kXRow = kDigits<TOK> ? TOK * 96 : TOK * 64;  // bytes of 32 K-elements
+constexpr int kXRow = kDigits<TOK> ? TOK * 128 + 16 : TOK * 64;  // bytes of 32 K-elements
 template <int TOK>
 constexpr int kSumBytes = kDigits<TOK> ? 32 : 0;  // of a group
 template <int TOK>
 constexpr int kPowerBytes = kDigits<TOK> ? 32 : 0;  // of 128 K-elements
+template <int TOK>
+constexpr int kRestBytes = kDigits<TOK> ? 8 : 0;  // of a unit
 template <int NG, int TOK>
-constexpr int kXBytes = kUnitK<TOK> / 32 * kXRow<TOK> + NG * kSumBytes<TOK> + kUnitK<TOK> / 128 * kPowerBytes<TOK>;  // of a unit
+constexpr int kXBytes = kUnitK<TOK> / 32 * kXRow<TOK> + NG * kSumBytes<TOK> + kUnitK<TOK> / 128 * kPowerBytes<TOK> + kRestBytes<TOK>;  // of a unit
 
 constexpr int kPieces = 2;  // tiles that a warp's run of units can touch
 template <int TOK>
@@ -322,6 +367,7 @@ size_t lay_out(Int4Args& a, int depth, int units, int cluster) {
   take(a.x_at, size_t(units) * (kUnitK<TOK> / 32) * kXRow<TOK>);
   take(a.sums, size_t(units) * NG * kSumBytes<TOK>);
   take(a.powers, size_t(units) * (kUnitK<TOK> / 128) * kPowerBytes<TOK>);
+  take(a.rests, (size_t(units) * kRestBytes<TOK> + 15) / 16 * 16);
   take(a.pieces, size_t(kWarps) * kPieces * kPiece<TOK> * 4);
   take(a.block, cluster > 1 ? size_t(2) * kWarps * kPiece<TOK> * 4 : 0);
   take(a.records, size_t(kWarps) * depth * sizeof(Stretch));
@@ -514,7 +560,9 @@ __global__ void __launch_bounds__(kThreads, 1) gemv_int4_kernel(const __grid_con
     x_half = warp;
     fetch(p);
   };
+  bool marked = false;  // a 128 that this warp wrote has a rest; after the pass's barrier, one of the block's
   auto convert = [&](Pass const& p) {
+    marked = false;
     constexpr int kLanes = kUnitK<TOK> / NG / 8;  // lanes of a scale group
 #pragma unroll 1
     while (x_token < p.count) {
@@ -537,53 +585,62 @@ __global__ void __launch_bounds__(kThreads, 1) gemv_int4_kernel(const __grid_con
       memcpy(&top_t, &top16, 2);
       const float top = to_f32(top_t);
       const bool bad = !(top < INFINITY);  // an infinity or a NaN makes the token's results NaN
-      // Largest |X| in [2^21, 2^22]; below 2^-105 the steps stay at 2^-126.
-      const int e = min(21 + 127 - int(__float_as_uint(top) >> 23), 126);
-      const float up = bad ? 0.0f : __int_as_float((e + 127) << 23);
+      // Largest |X| in [2^29, 2^30]; below 2^-97 the steps stay at 2^-126.
+      const int e = min(29 + 127 - int(__float_as_uint(top) >> 23), 126);
+      const float up = bad ? 0.0f : __int_as_float((e + 127) << 23), down = __int_as_float((127 - e) << 23);
       float v[8];
       unpack<T>(u, v);
-      // 1.5 2^23 + X has X in its low bits; adding 0x80 to each byte and flipping its top bit leaves X's
-      // digits, each in [-128, 127], in three bytes.
-      uint32_t y[8];
+      // Adding 0x80 to each byte and flipping its top bit leaves X's digits, each in [-128, 127], in four bytes. Of an
+      // element whose last place is 2^-e or more nothing is left (f16 has none below 2^-24); 2 bits - 1 orders the others by
+      // size, with zeros behind them.
+      constexpr bool kBf16 = std::is_same_v<T, __nv_bfloat16>;
+      const uint32_t whole = bad || (!kBf16 && e >= 24) ? 0 : (uint32_t(127 + (kBf16 ? 7 : 10) - e) << 24) - 1;
+      uint32_t y[8], least = 0xFFFFFFFFu;
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        const uint32_t x = __float_as_uint(fmaf(bad ? 0.0f : v[j], up, 12582912.0f));
-        y[j] = (x + (0x00808080u - 0x4B400000u)) ^ 0x00808080u;
+        least = min(least, 2 * __float_as_uint(v[j]) - 1);
+        y[j] = (uint32_t(__float2int_rn((bad ? 0.0f : v[j]) * up)) + 0x80808080u) ^ 0x80808080u;
       }
+      const unsigned rests = __ballot_sync(0xFFFFFFFFu, least < whole);
+      marked |= rests != 0;
       // By digit, the even elements (low nibbles) before the odd ones, as the masks leave the codes.
-      uint2 d[3];
+      uint2 d[4];
 #pragma unroll
       for (int odd = 0; odd < 2; ++odd) {
         const uint32_t a01 = __byte_perm(y[odd], y[odd + 2], 0x5140), b01 = __byte_perm(y[odd + 4], y[odd + 6], 0x5140);
-        const uint32_t a2 = __byte_perm(y[odd], y[odd + 2], 0x7362), b2 = __byte_perm(y[odd + 4], y[odd + 6], 0x7362);
+        const uint32_t a23 = __byte_perm(y[odd], y[odd + 2], 0x7362), b23 = __byte_perm(y[odd + 4], y[odd + 6], 0x7362);
         (odd ? d[0].y : d[0].x) = __byte_perm(a01, b01, 0x5410);
         (odd ? d[1].y : d[1].x) = __byte_perm(a01, b01, 0x7632);
-        (odd ? d[2].y : d[2].x) = __byte_perm(a2, b2, 0x5410);
+        (odd ? d[2].y : d[2].x) = __byte_perm(a23, b23, 0x5410);
+        (odd ? d[3].y : d[3].x) = __byte_perm(a23, b23, 0x7632);
       }
-      int sum[3];
+      int sum[4];
 #pragma unroll
-      for (int c = 0; c < 3; ++c) sum[c] = __dp4a(int(d[c].x), 0x01010101, __dp4a(int(d[c].y), 0x01010101, 0));
-      int low = sum[0] + sum[1] * 65536, high = sum[2];
+      for (int c = 0; c < 4; ++c) sum[c] = __dp4a(int(d[c].x), 0x01010101, __dp4a(int(d[c].y), 0x01010101, 0));
+      int low = sum[0] + sum[1] * 65536, high = sum[2] + sum[3] * 65536;
 #pragma unroll
       for (int o = kLanes / 2; o > 0; o /= 2) {
         low += __shfl_xor_sync(0xFFFFFFFFu, low, o);
         high += __shfl_xor_sync(0xFFFFFFFFu, high, o);
       }
 #pragma unroll
-      for (int c = 0; c < 3; ++c) *reinterpret_cast<uint2*>(to + (c * TOK + token) * 32 + lane % 4 * 8) = d[c];
-      const int s0 = int(int16_t(low)), s1 = (low - s0) >> 16;
+      for (int c = 0; c < 4; ++c) *reinterpret_cast<uint2*>(to + (c * TOK + token) * 32 + lane % 4 * 8) = d[c];
+      const int s0 = int(int16_t(low)), s1 = (low - s0) >> 16, s2 = int(int16_t(high)), s3 = (high - s2) >> 16;
       if (lane % kLanes == 0) {
         int* f = reinterpret_cast<int*>(smem + a.sums + (half * (32 / kLanes) + lane / kLanes) * kSumBytes<TOK>) + token;
         f[0] = s0;
         f[2] = s1;
-        f[4] = high;
+        f[4] = s2;
+        f[6] = s3;
       }
       if (lane % 16 == 0) {
-        const float down = bad ? NAN : __int_as_float((127 - e) << 23);
+        const float step = bad ? NAN : down;
         float* f = reinterpret_cast<float*>(smem + a.powers + (half * 2 + lane / 16) * kPowerBytes<TOK>) + token;
-        f[0] = down;
-        f[2] = down * 256.0f;
-        f[4] = down * 65536.0f;
+        f[0] = step;
+        f[2] = step * 256.0f;
+        f[4] = step * 65536.0f;
+        f[6] = step * 16777216.0f;
+        smem[a.rests + (half * 2 + lane / 16) * 2 + token] = (rests >> (lane & 16) & 0xFFFFu) != 0;
       }
     }
   };
@@ -654,10 +711,10 @@ __global__ void __launch_bounds__(kThreads, 1) gemv_int4_kernel(const __grid_con
   };
 
   constexpr int kSets = TOK <= 8 ? 1 : TOK / 8;  // of up to 8 tokens
-  // Where a lane reads: its ldmatrix rows in a box (swizzled by 16 bytes), its column's digits (a column that
-  // nothing uses reads another's) or its token's elements.
+  // Where a lane reads: its ldmatrix rows in a box (swizzled by 16 bytes), its column's digits (of one token, the unused
+  // columns read their neighbours') or its token's elements.
   const uint32_t in_box = lane % 16 * 128 + ((lane / 16 ^ (lane & 7)) * 16);
-  const int x_lane = !kDigits<TOK> ? lane * 16 : t * 8 + (g >= 6 ? 0 : TOK == 2 ? g * 32 : g % 2 ? 0 : g / 2 * 32);
+  const int x_lane = !kDigits<TOK> ? lane * 16 : t * 8 + (TOK == 2 ? g * 32 : g / 2 * 32);
   // A batch's sums of the cluster's blocks, a tile to a block in turn. They are gathered a batch later, when the
   // others' have long arrived; two buffers: by then every block has left the one that is written next.
   Stretch gathers = {};
@@ -684,6 +741,45 @@ __global__ void __launch_bounds__(kThreads, 1) gemv_int4_kernel(const __grid_con
   uint32_t parity = 0;
   const uint8_t *xd = smem, *xs = smem, *xp = smem;
   int k_at = 0;
+  // The rests of a unit's marked 128s, in the form for more tokens: column i is token i, so the sums join digit 0's.
+  auto add_rests = [&](uint32_t base, const float (&s_now)[2][kHeld], const uint32_t (&z_now)[2], uint2 marks) {
+    const Codes<T> codes;
+#pragma unroll 1
+    for (int quarter = 0; quarter < 4; ++quarter) {
+      if (((quarter < 2 ? marks.x : marks.y) >> quarter % 2 * 16 & 0xFFFFu) == 0) continue;
+      const float down = *reinterpret_cast<const float*>(xp - t * 8 + quarter * kPowerBytes<TOK> + g % TOK * 4);
+      const float up = __uint_as_float(0x7F000000u - __float_as_uint(down));
+#pragma unroll 1
+      for (int c = 0; c < 4; ++c) {
+        const int k = k_at + quarter * 128 + c * 32 + t * 8, group = quarter * (NG / 4) + c / kPerGroup;
+        uint4 q = make_uint4(0, 0, 0, 0);
+        if (g < p.count && k < a.k) {
+          float v[8];
+          unpack<T>(*reinterpret_cast<const uint4*>(row_of(p, g) + k), v);
+#pragma unroll
+          for (int j = 0; j < 8; ++j) v[j] = fmaf(-float(__float2int_rn(v[j] * up)), down, v[j]);
+          q = pack<T>(v);
+        }
+        q = make_uint4(__byte_perm(q.x, q.z, 0x5410), __byte_perm(q.x, q.z, 0x7632), __byte_perm(q.y, q.w, 0x5410), __byte_perm(q.y, q.w, 0x7632));
+        uint32_t w[4];
+        ldmatrix_x4(w, (base + quarter / 2 * kBoxBytes) ^ (quarter % 2 * 64 + c / 2 * 32));
+        float sc[2], dot[4];
+        uint32_t z[2];
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+          const int from = (lane & 28) | group / kHeld;
+          float s = s_now[r][0];
+#pragma unroll
+          for (int h = 1; h < kHeld; ++h) s = group % kHeld == h ? s_now[r][h] : s;
+          sc[r] = __shfl_sync(0xFFFFFFFFu, s, from);
+          z[r] = kZeros ? __shfl_sync(0xFFFFFFFFu, z_now[r], from) >> 8 * (group % kHeld) & 0xFF : 8;
+        }
+        CodesOf32<T, kZeros>(codes, c % 2 ? w[2] : w[0], c % 2 ? w[3] : w[1], z).times(dot, q, true);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) acc[0][i] = fmaf(sc[i / 2], dot[i], acc[0][i]);
+      }
+    }
+  };
   if (a.ids == nullptr) griddep_wait();
   griddep_launch_dependents();
   if (remaining > 0) {  // x first: what the start waits for goes before the weights
@@ -714,7 +810,8 @@ __global__ void __launch_bounds__(kThreads, 1) gemv_int4_kernel(const __grid_con
           __syncthreads();
         }
         convert(p);
-        __syncthreads();
+        if constexpr (kDigits<TOK>) marked = __syncthreads_or(marked);
+        else __syncthreads();
         if (start) continue;  // to fill the ring
       }
       now_left = max(u.units, 1);
@@ -791,30 +888,11 @@ __global__ void __launch_bounds__(kThreads, 1) gemv_int4_kernel(const __grid_con
 #pragma unroll
                 for (int i = 0; i < 4; ++i) sum[i] = fmaf(sc[i / 2], float(part[i] - int(z[i / 2]) * (i % 2 ? q.y : q.x)), sum[i]);
               } else {
-                // bf16 has 128 + z for z up to 127; what is above goes into a product of its own.
-                constexpr uint32_t kMaxZ = std::is_same_v<T, __nv_bfloat16> ? 127 : 255;
-                const auto z0 = codes.zero(kZeros ? min(z[0], kMaxZ) * 0x10001u : 0x00080008u);
-                const auto z1 = codes.zero(kZeros ? min(z[1], kMaxZ) * 0x10001u : 0x00080008u);
-                uint32_t f0[4], f1[4];
-                codes.minus(w[2 * cc], z0, f0);
-                codes.minus(w[2 * cc + 1], z1, f1);
-                const uint32_t fa[4] = {f0[0], f1[0], f0[1], f1[1]}, fb[4] = {f0[2], f1[2], f0[3], f1[3]};
-                bool more = false;
-                if (kZeros && kMaxZ < 255) more = __any_sync(0xFFFFFFFFu, max(z[0], z[1]) > kMaxZ);
+                const CodesOf32<T, kZeros> f(codes, w[2 * cc], w[2 * cc + 1], z);
 #pragma unroll
                 for (int set = 0; set < kSets; ++set) {
                   if (set > 0 && p.count <= 8) continue;
-                  const uint4 q = *reinterpret_cast<const uint4*>(xc + set * 512);
-                  mma_16<T>(dot[set], fa, q.x, q.y, begins);
-                  mma_16<T>(dot[set], fb, q.z, q.w, false);
-                  if (more) {
-                    uint32_t rest[2];
-#pragma unroll
-                    for (int r = 0; r < 2; ++r) rest[r] = pack_two<T>(-float(max(z[r], kMaxZ) - kMaxZ));
-                    const uint32_t fr[4] = {rest[0], rest[1], rest[0], rest[1]};
-                    mma_16<T>(dot[set], fr, q.x, q.y, false);
-                    mma_16<T>(dot[set], fr, q.z, q.w, false);
-                  }
+                  f.times(dot[set], *reinterpret_cast<const uint4*>(xc + set * 512), begins);
                   if (!ends) continue;
 #pragma unroll
                   for (int i = 0; i < 4; ++i) acc[set][i] = fmaf(sc[i / 2], dot[set][i], acc[set][i]);
@@ -826,6 +904,13 @@ __global__ void __launch_bounds__(kThreads, 1) gemv_int4_kernel(const __grid_con
             const float2 q = *reinterpret_cast<const float2*>(xp + quarter * kPowerBytes<TOK>);
 #pragma unroll
             for (int i = 0; i < 4; ++i) acc[0][i] = fmaf(i % 2 ? q.y : q.x, sum[i], acc[0][i]);
+          }
+        }
+        if constexpr (kDigits<TOK>) {
+          if (marked) {
+            uint2 rests = *reinterpret_cast<const uint2*>(smem + a.rests + (k_at / kUnitK<TOK> - kb0) * kRestBytes<TOK>);
+            if (p.count == 1) rests = make_uint2(rests.x & 0x00FF00FFu, rests.y & 0x00FF00FFu);
+            if (rests.x | rests.y) add_rests(base, s_now, z_now, rests);
           }
         }
         xd += kUnitK<TOK> / 32 * kXRow<TOK>;
@@ -844,9 +929,10 @@ __global__ void __launch_bounds__(kThreads, 1) gemv_int4_kernel(const __grid_con
         if constexpr (kDigits<TOK>) {
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            const float v0 = __shfl_sync(0xFFFFFFFFu, acc[0][i], lane & 28), v1 = __shfl_sync(0xFFFFFFFFu, acc[0][i], (lane & 28) | 1),
-                        v2 = __shfl_sync(0xFFFFFFFFu, acc[0][i], (lane & 28) | 2);
-            if (t == 0 && i % 2 < TOK) f(i % 2 * kRows + i / 2 * 8 + g, v0 + v1 + v2);
+            float v = acc[0][i];  // digits 0 and 1, 2 and 3, then the two sums
+            v += __shfl_xor_sync(0xFFFFFFFFu, v, 1);
+            v += __shfl_xor_sync(0xFFFFFFFFu, v, 2);
+            if (t == 0 && i % 2 < TOK) f(i % 2 * kRows + i / 2 * 8 + g, v);
           }
         } else {
 #pragma unroll

@@ -304,9 +304,8 @@ def gemv_int4(x, q, scales, zeros=None, *, group: int = 128, ids=None, out=None,
     zeros uint8 of the scales' shape, None = 8. group: 32, 64 or a multiple of 128; K a
     multiple of 32. With int32 ids [tokens, k]: q [E, N, K / 2], scales and zeros [E, N, ...], x [tokens, K]
     or [tokens, k, K], out [tokens, k, N] with expert ids[t, j] (rows of zeros for ids outside 0 .. E - 1;
-    at most 4096 ids, 1024 experts). out in x's type or fp32. Sums are exact or fp32 (with up to two
-    tokens to a matrix x enters with 22 bits below the largest of its 128 neighbours); a NaN or infinity makes its
-    row NaN or infinite. Up to 16 tokens of a matrix read the weights once. K up to 65536."""
+    at most 4096 ids, 1024 experts). out in x's type or fp32. x enters with all its bits, sums are exact or fp32; a NaN
+    or infinity makes its row NaN or infinite. Up to 16 tokens of a matrix read the weights once. K up to 65536."""
     if stream is not None:
         return _on_stream(stream, (x, q, scales, zeros, ids, out),
                           lambda: gemv_int4(x, q, scales, zeros, group=group, ids=ids, out=out, out_dtype=out_dtype))

@@ -25,11 +25,14 @@ def within(got, want, tol, what=""):
     assert got.shape == want.shape and bool((off <= tol.cpu()).all()), f"{what}: off by {(off / tol.cpu().clamp(min=1e-300)).max().item():.2f} of the tolerance"
 
 
-def product_tol(x, w, want, dtype, groups):
-    """An element of x enters whole, so only fp32 sums of exact products are off, relative to the products' sizes: 16
-    steps within a group's product, 4 roundings for its scale and its digits, a sum a group, 16 warps and 8 blocks."""
+def product_tol(x, w, want, dtype):
+    """An element of x enters whole, so only fp32 sums are off, relative to the products' sizes. With up to two tokens
+    x is taken apart into signed digits, whose sizes add up to at most three times its own (every digit below the first is at
+    most half of its base). A sum meets at most one rounding for every 32 elements and scale, and 32 for
+    a group's 8 products of 16, its scale, the digits, 16 warps and 8 blocks; what is a tensor core's own cuts at 2 U."""
     size = x.to(F64).abs() @ w.abs().transpose(-1, -2)
-    return size * (groups + 48) * U + want.abs() * HALF[dtype] * 1.001 + torch.finfo(dtype).smallest_normal * HALF[dtype] * 2
+    k = x.shape[-1]
+    return 3 * size * (k / 32 + 32) * U + want.abs() * HALF[dtype] * 1.001 + torch.finfo(dtype).smallest_normal * HALF[dtype] * 2
 
 
 # ------------------------------------------------------------------------------------ 4-bit products
@@ -49,11 +52,104 @@ def test_gemv_int4_group_longer_than_32_bits(cuda, tokens, group):
     ids = torch.tensor([[0, 1]] * tokens, dtype=torch.int32, device=cuda)
     by_expert = kl.gemv_int4(x, torch.stack([q, q]), torch.stack([s, s]), torch.stack([z, z]), group=group, ids=ids)
     want = x.cpu().to(F64) @ oracle.int4_weights(q, s, z, 1152).T
-    # Two forms of one product: each rounds fp32 sums of it once to bf16.
-    slack = product_tol(x.cpu(), oracle.int4_weights(q, s, z, 1152), want, torch.bfloat16, 9) + 2.0 ** -21 * x.abs().max().item() * oracle.int4_weights(q, s, z, 1152).abs().sum(1)
+    slack = product_tol(x.cpu(), oracle.int4_weights(q, s, z, 1152), want, torch.bfloat16)
     within(got, want, slack)
     for j in range(2):
         within(by_expert[:, j], want, slack)
+
+
+
+def check_products(x, q, s, z, group, cuda, what=""):
+    """Every row of x by itself, in pairs and all together, dense and by expert, into x's type and fp32."""
+    w = oracle.int4_weights(q, s, z, group)
+    want = x.to(F64) @ w.T
+    xd, tokens = x.to(cuda), x.shape[0]
+    on = [None if t is None else t.to(cuda) for t in (q, s, z)]
+    for step in (1, 2, tokens):
+        for dtype in (x.dtype, torch.float32):
+            got = torch.cat([kl.gemv_int4(xd[i:i + step], *on, group=group, out_dtype=dtype) for i in range(0, tokens, step)])
+            within(got, want, product_tol(x, w, want, dtype), f"{what}, {step} tokens into {dtype}")
+    two = [None if t is None else torch.stack([t, t]) for t in on]
+    ids = torch.arange(tokens, dtype=torch.int32, device=cuda)[:, None] % 2
+    for i in range(0, tokens, 4):  # two tokens to an expert
+        got = kl.gemv_int4(xd[i:i + 4], *two, group=group, ids=ids[i:i + 4], out_dtype=torch.float32)[:, 0]
+        within(got, want[i:i + 4], product_tol(x[i:i + 4], w, want[i:i + 4], torch.float32), f"{what}, by expert")
+
+
+@pytest.mark.parametrize("dtype, outlier", [(torch.bfloat16, 1000.0), (torch.bfloat16, 1e30), (torch.float16, 1000.0),
+                                            (torch.float16, 4096.0), (torch.float16, 60000.0)])
+@pytest.mark.parametrize("group, zeros", [(32, True), (64, True), (64, False), (128, False), (256, True)])
+def test_gemv_int4_small_beside_large(cuda, dtype, outlier, group, zeros):
+    """An element far above its neighbours that meets a code equal to the zero point: the neighbours alone make the
+    result, and keep every bit."""
+    n, k, tokens = 40, 1056, 8
+    q = torch.randint(0, 256, (n, k // 2), generator=gen(group), dtype=torch.uint8)
+    s = (torch.rand((n, -(-k // group)), generator=gen(2)) * 0.02 + 0.001).to(dtype)
+    z = torch.randint(0, 256 if group == 64 else 16, s.shape, generator=gen(3), dtype=torch.uint8) % 16 if zeros else None
+    x = (torch.randn((tokens, k), generator=gen(4)) * 0.01).to(dtype)
+    codes = torch.stack([q % 16, q // 16], -1).flatten(-2)
+    for i in range(0, k, 128):
+        at = i + (37 * i // 128) % min(128, k - i)
+        x[i // 128 % tokens:, at] = outlier    # some tokens' and not others'
+        codes[:, at] = 8 if z is None else z[:, at // group]
+    q = codes[:, 0::2] | codes[:, 1::2] << 4
+    check_products(x, q, s, z, group, cuda, f"outlier {outlier}")
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("group", [32, 128])
+@pytest.mark.parametrize("high_zeros", [False, True])
+def test_gemv_int4_values_of_all_sizes(cuda, dtype, group, high_zeros):
+    """Elements spread over the exponents of the type, zero points up to 255: each counts with all its bits, alone (the
+    others' codes at the zero point) and together."""
+    n, k, tokens = 72, 640, 6
+    low, high = (-60, 60) if dtype is torch.bfloat16 else (-24, 15)
+    x = (torch.randn((tokens, k), generator=gen(1)).clamp(-1.9, 1.9) * 2.0 ** torch.randint(low, high, (tokens, k), generator=gen(2))).to(dtype)
+    z = torch.randint(0, 16, (n, k // group), generator=gen(3), dtype=torch.uint8)
+    codes = torch.randint(0, 16, (n, k), generator=gen(4), dtype=torch.uint8)
+    at = torch.arange(k) // group
+    codes[8:] = z[8:][:, at]
+    codes[torch.arange(8, n), torch.randint(0, k, (n - 8,), generator=gen(5))] = 3
+    if high_zeros:
+        z[4:8] = torch.randint(120, 256, z[4:8].shape, generator=gen(6), dtype=torch.uint8)
+    q = codes[:, 0::2] | codes[:, 1::2] << 4
+    s = torch.ones(z.shape).to(dtype)
+    # f16 holds no sum of these: what it would round to infinity is left to fp32's comparison.
+    if dtype is torch.float16:
+        s = s / 4096
+        x = x.clamp(-2048, 2048)
+    check_products(x, q, s, z, group, cuda)
+
+
+@pytest.mark.parametrize("tokens", [1, 2])
+def test_gemv_int4_small_beside_large_over_a_cluster(cuda, tokens):
+    """K cut over blocks, tiles shared between warps, some 128s with and most without a large element."""
+    n, k, group = 16 * 160 + 5, 24576, 64
+    g = torch.Generator("cuda").manual_seed(1)
+    codes = torch.randint(0, 16, (n, k), generator=g, device=cuda, dtype=torch.uint8)
+    s = (torch.rand((n, k // group), generator=g, device=cuda) * 0.02 + 0.001).bfloat16()
+    x = (torch.randn((tokens, k), generator=g, device=cuda) * 0.01).bfloat16()
+    for i in range(5, k, 1408):
+        x[i % tokens, i] = 2.0 ** 40
+        codes[:, i] = 8
+    w = (codes.double() - 8) * s.double().repeat_interleave(group, 1)
+    want = x.double() @ w.T
+    got = kl.gemv_int4(x, codes[:, 0::2] | codes[:, 1::2] << 4, s, group=group, out_dtype=torch.float32)
+    within(got, want, product_tol(x, w, want, torch.float32))
+
+
+def test_gemv_int4_bad_rows_beside_rests(cuda):
+    """A token with a NaN or an infinity beside one whose elements leave rests: the second is not touched."""
+    n, k = 40, 512
+    q = torch.randint(0, 256, (n, k // 2), generator=gen(1), dtype=torch.uint8).to(cuda)
+    s = torch.ones((n, 4), dtype=torch.bfloat16, device=cuda)
+    x = (torch.randn((2, k), generator=gen(2)) * 1e-9).bfloat16().to(cuda)
+    x[1, ::128] = 4.0
+    alone = kl.gemv_int4(x, q, s, out_dtype=torch.float32)
+    for bad in (math.nan, math.inf):
+        x[0, 3] = bad
+        got = kl.gemv_int4(x, q, s, out_dtype=torch.float32)
+        assert not got[0].isfinite().any() and torch.equal(got[1], alone[1])
 
 
 # ------------------------------------------------------------------------------------ streams
