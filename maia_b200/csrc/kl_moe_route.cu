@@ -156,8 +156,9 @@ __device__ __forceinline__ void values(Row<T, NV> const& r, float (&v)[8 * NV]) 
   for (int i = 0; i < NV * 8 / kPerVec<T>; ++i) unpack<T>(r.u[i], v + i * kPerVec<T>);
 }
 
-// exp(x) for x <= 0 as one product and one ex2: off by |x| + 4 times 2^-24, relative. A row's large
-// probabilities have small |x|.
+// exp(x) for x <= 0 as one product and one ex2: off by |x| + 4 times 2^-24, relative, and 0 below 2^-126. For a row's sum
+// and what adds up over tokens, where the large probabilities count and have small |x|. The k weights, which a user
+// sees one by one, take expf (131072 tokens of 256 experts: 63.9 us instead of 63.2).
 __device__ __forceinline__ float exp_neg(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x * 1.44269504f));
@@ -281,7 +282,7 @@ __global__ void __launch_bounds__(kRouteThreads, NV == 1 ? 2 : 1) route_kernel(c
     float w[kHeld], part = 0.0f;
 #pragma unroll
     for (int h = 0; h < kHeld; ++h) {
-      w[h] = h * L + lane < a.k && pick[h] > Key::kClosed ? exp_neg(Key::value(pick[h]) - top) : 0.0f;
+      w[h] = h * L + lane < a.k && pick[h] > Key::kClosed ? expf(Key::value(pick[h]) - top) : 0.0f;
       part += w[h];
     }
     if (a.renormalize) inv = 1.0f / group_sum<L>(part);

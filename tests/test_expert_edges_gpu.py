@@ -35,6 +35,27 @@ def product_tol(x, w, want, dtype):
     return 3 * size * (k / 32 + 32) * U + want.abs() * HALF[dtype] * 1.001 + torch.finfo(dtype).smallest_normal * HALF[dtype] * 2
 
 
+# ------------------------------------------------------------------------------------ routing
+
+
+@pytest.mark.parametrize("experts", [4, 64, 300])
+def test_route_weights_far_below_the_largest(cuda, experts):
+    """Chosen experts whose probabilities go down through fp32's subnormals: each keeps its own bits."""
+    tokens, k = 40, 3
+    x = torch.full((tokens, experts), -300.0)
+    x[:, 0] = torch.randn(tokens, generator=gen(1))
+    x[:, 2] = x[:, 0] - torch.linspace(1, 102, tokens)
+    x[:, 3] = x[:, 2] - 0.5
+    p = torch.softmax(x.to(F64), 1)[:, [0, 2, 3]]
+    reach = (x[:, :1] - x[:, [0, 2, 3]]).to(F64)
+    for renormalize in (False, True):
+        r = kl.moe_route(x.to(cuda), k, renormalize=renormalize)
+        assert r.ids.cpu().tolist() == [[0, 2, 3]] * tokens
+        want = p / p.sum(1, keepdim=True) if renormalize else p
+        # The difference's rounding (|l - max| U), expf's two steps, sum, reciprocal and product; the last step of a subnormal.
+        within(r.weights, want, want * (reach + 16) * U + 2.0 ** -149, f"renormalize {renormalize}")
+
+
 # ------------------------------------------------------------------------------------ 4-bit products
 
 
