@@ -64,7 +64,7 @@ def _refuse(ok: bool, message: str) -> None:
 
 
 def _matrix(name: str, t, dtypes=None) -> None:
-    if t.dim() != 2 or (t.stride(1) != 1 and t.shape[1] > 1):
+    if t.dim() != 2 or (t.stride(1) != 1 and t.shape[1] > 1 and t.shape[0] > 0):  # torch leaves an empty tensor's strides open
         raise ValueError(f"{name} must be 2-D with a contiguous last dimension")
     if dtypes is not None and t.dtype not in dtypes:
         raise ValueError(f"{name} has the type {t.dtype}")

@@ -56,6 +56,25 @@ def test_route_weights_far_below_the_largest(cuda, experts):
         within(r.weights, want, want * (reach + 16) * U + 2.0 ** -149, f"renormalize {renormalize}")
 
 
+# ------------------------------------------------------------------------------------ nothing to do
+
+
+def test_no_tokens_through_torch_ops(cuda):
+    """A batch without tokens, forward and backward from a broadcast gradient, whose strides torch leaves at 0."""
+    import maia_b200.torch_ops  # noqa: F401
+
+    logits = torch.empty((0, 8), device=cuda, requires_grad=True)
+    x = torch.empty((0, 64), device=cuda, requires_grad=True)
+    ids, weights, _, _, loss = torch.ops.kl.moe_route(logits, 2)
+    rows, slots, _ = torch.ops.kl.moe_plan(ids, 8)
+    y = torch.ops.kl.moe_dispatch(x, rows, slots)
+    (torch.ops.kl.moe_combine(y, weights, rows, slots).sum() + loss + y.sum()).backward()
+    assert x.grad.shape == (0, 64) and logits.grad.shape == (0, 8)
+    y = torch.empty((0, 2, 64), device=cuda, requires_grad=True)
+    torch.ops.kl.moe_combine(y).sum().backward()
+    assert y.grad.shape == y.shape
+
+
 # ------------------------------------------------------------------------------------ 4-bit products
 
 
