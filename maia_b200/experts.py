@@ -204,6 +204,8 @@ def moe_plan(ids, experts: int, *, block: int = 128, stream=None) -> MoePlan:
     m = moe_rows(tokens * k, experts, block)
     device = _device(ids)
     plan = MoePlan(torch.empty_like(ids), ids.new_empty((m,)), ids.new_empty((m // 128,)))
+    if k == 0:
+        return plan
     _queue(device, lib().kl_moe_plan, ids.data_ptr(), tokens, k, experts, block, m, plan.rows.data_ptr(),
            plan.slots.data_ptr(), plan.m_block_group.data_ptr())
     return plan
@@ -232,8 +234,10 @@ def moe_dispatch(x, plan: MoePlan, out=None, *, stream=None):
     else:
         _matrix("out", out, (x.dtype,))
         _refuse(out.shape == (m, width), f"out must have the shape {(m, width)}")
-    _queue(_device(x, rows, slots, out), lib().kl_moe_dispatch, x.data_ptr(), _pitch(x) * size, tokens,
-           width * size, max(k, 1), rows.data_ptr(), slots.data_ptr(), m, out.data_ptr(), _pitch(out) * size)
+    device = _device(x, rows, slots, out)
+    if k == 0:
+        return out.zero_()
+    _queue(device, lib().kl_moe_dispatch, x.data_ptr(), _pitch(x) * size, tokens, width * size, k, rows.data_ptr(), slots.data_ptr(), m, out.data_ptr(), _pitch(out) * size)
     return out
 
 
@@ -291,9 +295,11 @@ def moe_combine_grad(dout, y, weights=None, *, rows=None, slots=None, stream=Non
     if dout.shape != (tokens, width):
         raise ValueError(f"dout must have the shape {(tokens, width)}")
     device = _device(dout, y, weights, rows, slots)
+    if k == 0:
+        return y.new_zeros(y.shape), None if weights is None else torch.empty_like(weights)
     dy = y.new_empty(y.shape)
     dweights = None if weights is None else torch.empty_like(weights)
-    _queue(device, lib().kl_moe_combine_grad, dout.data_ptr(), _pitch(dout), y.data_ptr(), _FLOATS[y.dtype], pitch, m, _ptr(rows), _ptr(slots), _ptr(weights), tokens, max(k, 1),
+    _queue(device, lib().kl_moe_combine_grad, dout.data_ptr(), _pitch(dout), y.data_ptr(), _FLOATS[y.dtype], pitch, m, _ptr(rows), _ptr(slots), _ptr(weights), tokens, k,
            width, dy.data_ptr(), width, _ptr(dweights))
     return dy, dweights
 
@@ -344,11 +350,14 @@ def gemv_int4(x, q, scales, zeros=None, *, group: int = 128, ids=None, out=None,
         _refuse(out.stride(-1) == 1 or n <= 1 if ids is None else out.is_contiguous(), "out must be contiguous in its last dimension")
     if out.dtype is not dtype and out.dtype is not torch.float32:
         raise ValueError("out must have x's type or fp32")
+    device = _device(x, q, scales, zeros, ids, out)
+    if topk == 0:
+        return out
     one = ids is None
     zero_fields = (0, 0, 0) if zeros is None else (zeros.data_ptr(), _pitch(zeros), 0 if one else zeros.stride(0))
     d = _pack_int4(x.data_ptr(), ldx, q.data_ptr(), _pitch(q), 0 if one else q.stride(0),
                    scales.data_ptr(), _pitch(scales), 0 if one else scales.stride(0), *zero_fields,
                    0 if one else ids.data_ptr(), 0 if one else q.shape[0], topk, out.data_ptr(), _pitch(out) if one else n,
                    tokens, n, k, group, _FLOATS[dtype], _FLOATS[scales.dtype], _FLOATS[out.dtype], per_slot)
-    _queue(_device(x, q, scales, zeros, ids, out), lib().kl_gemv_int4, d)
+    _queue(device, lib().kl_gemv_int4, d)
     return out

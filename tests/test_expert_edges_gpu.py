@@ -75,6 +75,40 @@ def test_no_tokens_through_torch_ops(cuda):
     assert y.grad.shape == y.shape
 
 
+@pytest.mark.parametrize("tokens", [0, 3])
+def test_no_slots_at_all(cuda, tokens):
+    """k = 0 through plan, dispatch, combine, their gradients and the products by expert: empty or zero everywhere."""
+    import maia_b200.torch_ops  # noqa: F401
+
+    ids = torch.empty((tokens, 0), dtype=torch.int32, device=cuda)
+    plan = kl.moe_plan(ids, 8)
+    assert plan.rows.shape == (tokens, 0) and plan.slots.shape == (0,) and plan.m_block_group.shape == (0,)
+    x = torch.randn((tokens, 64), device=cuda)
+    a = kl.moe_dispatch(x, plan)
+    assert a.shape == (0, 64)
+    w = torch.empty((tokens, 0), device=cuda)
+    padding = torch.randn((256, 64), device=cuda)       # a layout with padding alone
+    slots = torch.full((256,), -1, dtype=torch.int32, device=cuda)
+    out = torch.full((256, 64), 5.0, device=cuda)
+    assert kl.moe_dispatch(x, kl.MoePlan(ids, slots, None), out) is out and (out == 0).all()
+    for weights in (w, None):
+        for y, rows, at in ((a, plan.rows, plan.slots), (padding, ids, slots), (torch.empty((tokens, 0, 64), device=cuda), None, None)):
+            assert torch.equal(kl.moe_combine(y, weights, rows=rows), torch.zeros_like(x))
+            dy, dw = kl.moe_combine_grad(x, y, weights, rows=rows, slots=at)
+            assert torch.equal(dy, torch.zeros_like(y)) and (dw is None if weights is None else dw.shape == (tokens, 0))
+            leaf = y.clone().requires_grad_()
+            torch.ops.kl.moe_combine(leaf, weights, rows, at).sum().backward()
+            assert torch.equal(leaf.grad, torch.zeros_like(y))
+    leaf = x.clone().requires_grad_()
+    torch.ops.kl.moe_dispatch(leaf, plan.rows, plan.slots).sum().backward()
+    assert torch.equal(leaf.grad, torch.zeros_like(x))
+    q = torch.zeros((4, 16, 32), dtype=torch.uint8, device=cuda)
+    s = torch.ones((4, 16, 2), dtype=torch.bfloat16, device=cuda)
+    for v in (x.bfloat16(), torch.empty((tokens, 0, 64), dtype=torch.bfloat16, device=cuda)):
+        assert kl.gemv_int4(v, q, s, group=32, ids=ids).shape == (tokens, 0, 16)
+    torch.cuda.synchronize()
+
+
 # ------------------------------------------------------------------------------------ 4-bit products
 
 
