@@ -76,9 +76,9 @@ def _whole(name: str, t, shape, dtype) -> None:
 
 
 def _pitch(t) -> int:
-    """Row pitch in elements; of a single row, whose stride torch leaves open, at least the row."""
-    pitch, shape = t.stride(-2), t.shape
-    return pitch if pitch >= shape[-1] or shape[-2] > 1 else shape[-1]
+    """Row pitch in elements; of a single row, which has none, the row."""
+    shape = t.shape
+    return t.stride(-2) if shape[-2] > 1 else shape[-1]
 
 
 def _ptr(t):

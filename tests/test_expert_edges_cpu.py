@@ -45,3 +45,14 @@ def test_host_tensors_are_refused_on_any_stream():
                  lambda: kl.moe_combine(torch.zeros((2, 2, 8)), stream=16)):
         with pytest.raises(ValueError):
             call()
+
+
+def test_a_single_row_has_no_pitch():
+    """Whatever buffer one token's row was cut from, its pitch is its own length: no alignment is asked of the buffer's."""
+    import torch
+
+    from maia_b200.experts import _pitch
+
+    base = torch.empty((6, 4100))
+    assert _pitch(base[:1, :4096]) == 4096 and _pitch(base[:2, :4096]) == 4100 and _pitch(base[::5][:1]) == 4100
+    assert _pitch(base[:0, :64]) == 64 and _pitch(torch.empty((3, 1, 48))[..., :32]) == 32

@@ -226,6 +226,26 @@ def test_gemv_int4_bad_rows_beside_rests(cuda):
         assert not got[0].isfinite().any() and torch.equal(got[1], alone[1])
 
 
+
+def test_one_row_of_a_wider_buffer(cuda):
+    """One token, one weight row: cut from buffers whose pitch fits no load, with a base that does."""
+    k, n = 256, 24
+    x = torch.randn((4, k + 4), generator=gen(1)).bfloat16()
+    q = torch.randint(0, 256, (n, k // 2 + 3), generator=gen(2), dtype=torch.uint8)
+    s = torch.ones((n, 2), dtype=torch.bfloat16)
+    xd, qd, sd = x.to(cuda)[:1, :k], q.to(cuda)[:1, :k // 2], s.to(cuda)[:1]
+    w = oracle.int4_weights(q[:1, :k // 2], s[:1], None, 128)
+    want = x[:1, :k].to(F64) @ w.T
+    within(kl.gemv_int4(xd, qd, sd), want, product_tol(x[:1, :k], w, want, torch.bfloat16))
+    got = kl.gemv_int4(xd, qd[None], sd[None], ids=torch.zeros((1, 1), dtype=torch.int32, device=cuda))
+    within(got[0], want, product_tol(x[:1, :k], w, want, torch.bfloat16))
+    logits = torch.randn((2, 67), generator=gen(3)).to(cuda)
+    r, whole = kl.moe_route(logits[:1, :64], 4), kl.moe_route(logits[:1, :64].contiguous(), 4)
+    assert all(torch.equal(a, b) for a, b in zip(r, whole))
+    dw = torch.randn((1, 4), generator=gen(4)).to(cuda)
+    assert torch.equal(kl.moe_route_grad(logits[:1, :64], r, dw), kl.moe_route_grad(logits[:1, :64].contiguous(), r, dw))
+
+
 # ------------------------------------------------------------------------------------ streams
 
 PENDING = 100_000_000  # cycles that a stream is kept busy: 50 ms
