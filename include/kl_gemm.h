@@ -266,8 +266,9 @@ KL_API kl_status kl_moe_combine(const void* y, int32_t type, int64_t ldy, int64_
                                 void* stream);
 
 /* The gradients of kl_moe_combine: dy[row] = weights[slots[row]] dout[slots[row] / k] (zeros for padding rows),
- * dweights[t, j] = <dout[t], y[rows[t, j]]> in fp32 (0 where rows is -1; NULL = not wanted, y is then
- * not read). rows and slots are kl_moe_plan's, or both NULL for slot order. dy must not be y. */
+ * dweights[t, j] = <dout[t], y[rows[t, j]]> in fp32 (0 where rows is -1). One of them may be NULL, not wanted:
+ * without dweights y is not read. rows and slots are kl_moe_plan's, or both NULL for slot order. dy must
+ * not be y. */
 KL_API kl_status kl_moe_combine_grad(const void* dout, int64_t ld_dout, const void* y, int32_t type, int64_t ldy,
                                      int64_t m, const int32_t* rows, const int32_t* slots, const float* weights,
                                      int64_t tokens, int64_t k, int64_t width, void* dy, int64_t ld_dy, float* dweights,

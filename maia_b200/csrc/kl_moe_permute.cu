@@ -168,7 +168,7 @@ constexpr int kRowThreads = 256;
 struct RowArgs {
   const void* src;      // dispatch: x [tokens]; combine: y [m]; combine_grad: y [m]
   long long ld_src;     // row pitches in bytes
-  void* dst;            // dispatch: a [m]; combine: out [tokens]; combine_grad: dy [m]
+  void* dst;            // dispatch: a [m]; combine: out [tokens]; combine_grad: dy [m] or NULL
   long long ld_dst;
   const void* dout;     // combine_grad: [tokens]
   long long ld_dout;
@@ -331,8 +331,8 @@ __global__ void __launch_bounds__(kRowThreads) combine_grad_kernel(const RowArgs
     const long long s = t * a.k + threadIdx.x, r = row_of(a, s);
     row[threadIdx.x] = r;
     weight[threadIdx.x] = a.weights != nullptr ? a.weights[s] : 1.0f;
-    // A row's gradient is written by its own slot alone.
-    writes[threadIdx.x] = r >= 0 && (a.slots == nullptr || a.slots[r] == s);
+    // A row's gradient, where it is wanted, is written by its own slot alone.
+    writes[threadIdx.x] = r >= 0 && a.dst != nullptr && (a.slots == nullptr || a.slots[r] == s);
   }
   __syncthreads();
   const V* dout = reinterpret_cast<const V*>(static_cast<const char*>(a.dout) + t * a.ld_dout);
@@ -578,10 +578,11 @@ extern "C" kl_status kl_moe_combine_grad(const void* dout, int64_t ld_dout, cons
     return fail(KL_ERR_INVALID_ARGUMENT, "kl_moe_combine_grad: rows and slots come together");
   if (rows == nullptr && m != tokens * k)
     return fail(KL_ERR_INVALID_ARGUMENT, "kl_moe_combine_grad: without rows, y has tokens * k rows");
-  if (ldy < width || ld_dout < width || ld_dy < width)
+  if (ldy < width || ld_dout < width || (dy != nullptr && ld_dy < width))
     return fail(KL_ERR_INVALID_ARGUMENT, "kl_moe_combine_grad: row pitch below the width");
-  if (tokens == 0 && m == 0) return KL_OK;
-  if ((tokens > 0 && width > 0 && dout == nullptr) || (m > 0 && width > 0 && (dy == nullptr || (dweights != nullptr && y == nullptr))))
+  if (tokens == 0 && (m == 0 || dy == nullptr)) return KL_OK;
+  if ((tokens > 0 && width > 0 && dout == nullptr) ||
+      (m > 0 && width > 0 && ((dy == nullptr && dweights == nullptr) || (dweights != nullptr && y == nullptr))))
     return fail(KL_ERR_INVALID_ARGUMENT, "kl_moe_combine_grad: null pointer");
   if (!aligned(dout, size) || !aligned(y, size) || !aligned(dy, size))
     return fail(KL_ERR_INVALID_ARGUMENT, "kl_moe_combine_grad: dout, y and dy must be aligned to their elements");
@@ -604,7 +605,7 @@ extern "C" kl_status kl_moe_combine_grad(const void* dout, int64_t ld_dout, cons
   const int g = common_granule({reinterpret_cast<uintptr_t>(y), reinterpret_cast<uintptr_t>(dy), reinterpret_cast<uintptr_t>(dout),
                                 uint64_t(a.ld_src), uint64_t(a.ld_dst), uint64_t(a.ld_dout), uint64_t(width * size)});
   a.width = width * size / g;
-  const int64_t pad_parts = slots != nullptr ? (m + kPadRows - 1) / kPadRows : 0;
+  const int64_t pad_parts = slots != nullptr && dy != nullptr ? (m + kPadRows - 1) / kPadRows : 0;
   cudaError_t e = cudaSuccess;
   by_cells(type, g, [&](auto t, auto v) {
     void* args[] = {&a};

@@ -280,13 +280,14 @@ def moe_combine(y, weights=None, *, rows=None, out=None, stream=None):
     return out
 
 
-def moe_combine_grad(dout, y, weights=None, *, rows=None, slots=None, stream=None):
+def moe_combine_grad(dout, y, weights=None, *, rows=None, slots=None, want_dy=True, want_dweights=True, stream=None):
     """(dy, dweights) of moe_combine from dout [tokens, width] of y's type: dy in y's shape and type,
     zero in padding rows; dweights fp32, or None where weights is None. rows and slots are moe_plan's, or
-    both None."""
+    both None. What is not wanted is None and not computed; without dweights y is not read."""
     if stream is not None:
         return _on_stream(stream, (dout, y, weights, rows, slots),
-                          lambda: moe_combine_grad(dout, y, weights, rows=rows, slots=slots))
+                          lambda: moe_combine_grad(dout, y, weights, rows=rows, slots=slots, want_dy=want_dy,
+                                                   want_dweights=want_dweights))
     tokens, k, m, width, pitch = _rows_of(y, rows, weights)
     _refuse((rows is None) == (slots is None), "rows and slots come together")
     if slots is not None:
@@ -295,12 +296,14 @@ def moe_combine_grad(dout, y, weights=None, *, rows=None, slots=None, stream=Non
     if dout.shape != (tokens, width):
         raise ValueError(f"dout must have the shape {(tokens, width)}")
     device = _device(dout, y, weights, rows, slots)
+    dweights = torch.empty_like(weights) if want_dweights and weights is not None else None
     if k == 0:
-        return y.new_zeros(y.shape), None if weights is None else torch.empty_like(weights)
-    dy = y.new_empty(y.shape)
-    dweights = None if weights is None else torch.empty_like(weights)
+        return y.new_zeros(y.shape) if want_dy else None, dweights
+    dy = y.new_empty(y.shape) if want_dy else None
+    if dy is None and dweights is None:
+        return None, None
     _queue(device, lib().kl_moe_combine_grad, dout.data_ptr(), _pitch(dout), y.data_ptr(), _FLOATS[y.dtype], pitch, m, _ptr(rows), _ptr(slots), _ptr(weights), tokens, k,
-           width, dy.data_ptr(), width, _ptr(dweights))
+           width, _ptr(dy), width, _ptr(dweights))
     return dy, dweights
 
 

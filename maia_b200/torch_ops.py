@@ -179,30 +179,35 @@ def _(y, weights=None, rows=None, slots=None):
 
 @torch.library.custom_op("kl::moe_combine_grad", mutates_args=())
 def moe_combine_grad(dout: torch.Tensor, y: torch.Tensor, weights: torch.Tensor, rows: Optional[torch.Tensor],
-                     slots: Optional[torch.Tensor]) -> Tuple[torch.Tensor, torch.Tensor]:
-    """The gradients of kl::moe_combine's y and weights: maia_b200.moe_combine_grad."""
-    return tuple(_experts.moe_combine_grad(dout, y, weights, rows=rows, slots=slots))
+                     slots: Optional[torch.Tensor], want_dy: bool = True, want_dweights: bool = True
+                     ) -> Tuple[torch.Tensor, torch.Tensor]:
+    """The gradients of kl::moe_combine's y and weights: maia_b200.moe_combine_grad. What is not wanted is empty."""
+    both = _experts.moe_combine_grad(dout, y, weights, rows=rows, slots=slots, want_dy=want_dy, want_dweights=want_dweights)
+    return tuple(t.new_empty((0,)) if g is None else g for g, t in zip(both, (y, weights)))
 
 
 @moe_combine_grad.register_fake
-def _(dout, y, weights, rows, slots):
-    return y.new_empty(y.shape), weights.new_empty(weights.shape)
+def _(dout, y, weights, rows, slots, want_dy=True, want_dweights=True):
+    return y.new_empty(y.shape if want_dy else (0,)), weights.new_empty(weights.shape if want_dweights else (0,))
 
 
 def _combine_context(ctx, inputs, output):
-    ctx.save_for_backward(*inputs)
+    y, weights, rows, slots = inputs
+    ctx.shape = y.shape
+    ctx.save_for_backward(None if weights is None else y, weights, rows, slots)
 
 
 def _combine_backward(ctx, dout):
     y, weights, rows, slots = ctx.saved_tensors
     if rows is not None and slots is None:
         raise RuntimeError("kl::moe_combine with rows needs kl::moe_plan's slots for its gradient")
-    plain = weights is None
-    if plain:
-        tokens, k = y.shape[:2] if rows is None else rows.shape
-        weights = torch.ones((tokens, k), dtype=torch.float32, device=y.device)
-    dy, dweights = torch.ops.kl.moe_combine_grad(dout.contiguous(), y, weights, rows, slots)
-    return dy, None if plain else dweights, None, None
+    if weights is None:  # a copy of dout for every slot
+        if rows is None:
+            return dout[:, None].expand(ctx.shape), None, None, None
+        return torch.ops.kl.moe_dispatch(dout.contiguous(), rows, slots), None, None, None
+    want_dy, want_dweights = ctx.needs_input_grad[:2]
+    dy, dweights = torch.ops.kl.moe_combine_grad(dout.contiguous(), y, weights, rows, slots, want_dy, want_dweights)
+    return dy if want_dy else None, dweights if want_dweights else None, None, None
 
 
 moe_combine.register_autograd(_combine_backward, setup_context=_combine_context)

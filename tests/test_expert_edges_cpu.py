@@ -56,3 +56,12 @@ def test_a_single_row_has_no_pitch():
     base = torch.empty((6, 4100))
     assert _pitch(base[:1, :4096]) == 4096 and _pitch(base[:2, :4096]) == 4100 and _pitch(base[::5][:1]) == 4100
     assert _pitch(base[:0, :64]) == 64 and _pitch(torch.empty((3, 1, 48))[..., :32]) == 32
+
+
+def test_combine_grad_of_one_output():
+    """dy or dweights may be left out, not both; what is left out is not checked, what is read is."""
+    L = kl.lib()
+    refused(L.kl_moe_combine_grad(P, 8, P, kl.KL_BF16, 8, 8, None, None, P, 4, 2, 8, None, 8, None, None), "null")
+    refused(L.kl_moe_combine_grad(P, 8, None, kl.KL_BF16, 8, 8, None, None, P, 4, 2, 8, None, 8, P, None), "null")
+    refused(L.kl_moe_combine_grad(None, 8, P, kl.KL_BF16, 8, 8, None, None, P, 4, 2, 8, None, 0, P, None), "null")
+    assert L.kl_moe_combine_grad(None, 8, None, kl.KL_BF16, 8, 128, P, P, P, 0, 2, 8, None, 0, P, None) == kl.KL_OK  # no tokens

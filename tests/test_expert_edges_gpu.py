@@ -56,6 +56,54 @@ def test_route_weights_far_below_the_largest(cuda, experts):
         within(r.weights, want, want * (reach + 16) * U + 2.0 ** -149, f"renormalize {renormalize}")
 
 
+# ------------------------------------------------------------------------------------ combine's gradients, one by one
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("tokens, k, width", [(1, 1, 1), (37, 3, 1001), (70, 8, 264)])
+@pytest.mark.parametrize("grouped", [True, False])
+def test_combine_gradients_one_by_one(cuda, dtype, tokens, k, width, grouped):
+    """Each gradient by itself is what both calls give, bit for bit, in the C call and through autograd, and the one that is
+    not asked for reads nothing of its own."""
+    import maia_b200.torch_ops  # noqa: F401
+
+    rows = slots = None
+    y = torch.randn((tokens, k, width), generator=gen(1)).to(dtype).to(cuda)
+    if grouped:
+        plan = kl.moe_plan(torch.randint(-1, 5, (tokens, k), generator=gen(2), dtype=torch.int32).to(cuda), 5)
+        rows, slots = plan.rows, plan.slots
+        y = torch.randn((slots.shape[0], width), generator=gen(3)).to(dtype).to(cuda)
+    w = torch.rand((tokens, k), generator=gen(4)).to(cuda)
+    dout = torch.randn((tokens, width), generator=gen(5)).to(dtype).to(cuda)
+    dy, dw = kl.moe_combine_grad(dout, y, w, rows=rows, slots=slots)
+    only, none = kl.moe_combine_grad(dout, torch.full_like(y, math.nan), w, rows=rows, slots=slots, want_dweights=False)
+    assert none is None and torch.equal(only, dy)
+    none, only = kl.moe_combine_grad(dout, y, w, rows=rows, slots=slots, want_dy=False)
+    assert none is None and torch.equal(only, dw)
+    assert kl.moe_combine_grad(dout, y, w, rows=rows, slots=slots, want_dy=False, want_dweights=False) == (None, None)
+    plain, _ = kl.moe_combine_grad(dout, y, rows=rows, slots=slots)
+    for needs_y, needs_w in ((True, True), (True, False), (False, True)):
+        leaves = [y.clone().requires_grad_(needs_y), w.clone().requires_grad_(needs_w)]
+        torch.ops.kl.moe_combine(*leaves, rows, slots).backward(dout)
+        assert torch.equal(leaves[0].grad, dy) if needs_y else leaves[0].grad is None
+        assert torch.equal(leaves[1].grad, dw) if needs_w else leaves[1].grad is None
+    leaf = y.clone().requires_grad_()
+    torch.ops.kl.moe_combine(leaf, None, rows, slots).backward(dout)
+    assert torch.equal(leaf.grad, plain)
+
+
+def test_unweighted_combine_keeps_nothing_of_its_rows(cuda):
+    """y itself is not needed for its gradient without weights: it may be written over before the backward pass."""
+    import maia_b200.torch_ops  # noqa: F401
+
+    leaf = torch.randn((5, 2, 16), device=cuda, requires_grad=True)
+    y = leaf * 1
+    out = torch.ops.kl.moe_combine(y)
+    y.detach().zero_()
+    out.backward(torch.ones_like(out))
+    assert (leaf.grad == 1).all()
+
+
 # ------------------------------------------------------------------------------------ nothing to do
 
 
