@@ -295,7 +295,7 @@ typedef struct kl_int4_desc {
   const uint8_t* zeros; /* device [n, ld_zeros], or NULL: 8 everywhere */
   int64_t ld_zeros, stride_zeros;
   const int32_t* ids;   /* device [tokens, topk] or NULL: one matrix */
-  int64_t experts, topk; /* with ids: tokens * topk <= 4096, experts <= 1024 */
+  int64_t experts, topk; /* with ids: tokens * topk <= 4096 (more: several calls), experts <= 1024 */
   void* out;            /* device [tokens (* topk), ldo], x_type or KL_F32 */
   int64_t ldo;
   int64_t tokens, n, k; /* k a multiple of 32, at most 65536 */

@@ -1165,7 +1165,7 @@ extern "C" kl_status kl_gemv_int4(const kl_int4_desc* d, void* stream) {
   if (d->tokens > INT32_MAX / 64 || d->n > INT32_MAX / 2 || d->k > INT32_MAX / 2 || topk > kMaxSlots) return bad("extent too large");
   const int64_t slots = d->tokens * topk;
   if (by_expert && (slots > kMaxSlots || d->experts > kMaxExperts))
-    return fail(KL_ERR_NOT_SUPPORTED, "kl_gemv_int4: at most 4096 (token, expert) pairs and 1024 experts (more tokens: kl_moe_plan and the m-grouped GEMM)");
+    return fail(KL_ERR_NOT_SUPPORTED, "kl_gemv_int4: at most 4096 (token, expert) pairs and 1024 experts a call (more tokens: in calls of some of them)");
   if (d->x_type != KL_BF16 && d->x_type != KL_F16) return fail(KL_ERR_NOT_SUPPORTED, "kl_gemv_int4: x must be bf16 or f16");
   if (d->scale_type != d->x_type && d->scale_type != KL_F32)
     return fail(KL_ERR_NOT_SUPPORTED, "kl_gemv_int4: scales must have x's type or f32");

@@ -65,3 +65,13 @@ def test_combine_grad_of_one_output():
     refused(L.kl_moe_combine_grad(P, 8, None, kl.KL_BF16, 8, 8, None, None, P, 4, 2, 8, None, 8, P, None), "null")
     refused(L.kl_moe_combine_grad(None, 8, P, kl.KL_BF16, 8, 8, None, None, P, 4, 2, 8, None, 0, P, None), "null")
     assert L.kl_moe_combine_grad(None, 8, None, kl.KL_BF16, 8, 128, P, P, P, 0, 2, 8, None, 0, P, None) == kl.KL_OK  # no tokens
+
+
+def test_gemv_int4_refusal_names_a_way():
+    """Too many pairs: the message names what takes them, which no other product of the library does with 4-bit codes."""
+    d = kl.Int4Desc(x=P, ldx=4096, q=P, ldq=2048, scales=P, ld_scales=32, out=P, ldo=64, tokens=2049, n=64, k=4096, group=128,
+                    ids=P, experts=4, topk=2, stride_q=64 * 2048, stride_scales=64 * 32,
+                    x_type=kl.KL_BF16, scale_type=kl.KL_BF16, out_type=kl.KL_BF16)
+    with pytest.raises(kl.KlError) as e:
+        kl.check(kl.lib().kl_gemv_int4(ctypes.byref(d), None))
+    assert "calls of some of them" in e.value.message and "GEMM" not in e.value.message
