@@ -75,3 +75,39 @@ def test_gemv_int4_refusal_names_a_way():
     with pytest.raises(kl.KlError) as e:
         kl.check(kl.lib().kl_gemv_int4(ctypes.byref(d), None))
     assert "calls of some of them" in e.value.message and "GEMM" not in e.value.message
+
+
+@pytest.mark.parametrize("renormalize", [True, False])
+@pytest.mark.parametrize("dloss", [None, 2.0])
+def test_the_oracles_gradient_against_differences(renormalize, dloss):
+    """expert_oracle.route_grad, which the kernel's gradient is held to, against central differences of expert_oracle.route:
+    closed experts, fewer open ones than k, a row with none, padding. The choice is held by gaps between the logits."""
+    import math
+
+    import torch
+
+    import expert_oracle as oracle
+
+    tokens, experts, k, h = 6, 9, 3, 1e-5
+    rng = lambda i: torch.Generator().manual_seed(i)  # noqa: E731
+    x = torch.stack([torch.randperm(experts, generator=rng(i)).double() * 0.3 for i in range(tokens)])
+    x[1, ::2] = -math.inf
+    x[2, 2:] = -math.inf                       # two open experts for three slots
+    x[3] = -math.inf
+    valid = torch.tensor([True, True, True, True, False, True])
+    dw = torch.randn((tokens, k), generator=rng(9)).double()
+
+    def value(z):
+        ids, w, _, _, loss, _ = oracle.route(z, k, renormalize, valid)
+        return (w * dw)[ids >= 0].sum().item() + (dloss or 0.0) * loss
+
+    got = oracle.route_grad(x, k, dw, dloss, renormalize, valid)
+    assert (got[3:5] == 0).all()
+    for t in range(tokens):
+        for e in range(experts):
+            up, down = x.clone(), x.clone()
+            up[t, e] += h
+            down[t, e] -= h
+            want = (value(up) - value(down)) / (2 * h)
+            # A third derivative below 50 by h^2 / 6, and values below 50 rounded to 2^-53 each over 2 h.
+            assert abs(got[t, e].item() - want) <= 50 * h * h / 6 + 64 * 50 * 2.0 ** -53 / h, (t, e)
