@@ -461,7 +461,10 @@ extern "C" kl_status kl_moe_plan(const int32_t* ids, int64_t tokens, int64_t k, 
   a.warp_span = (a.total + warps * 32 - 1) / (warps * 32) * 32;
   const size_t smem = size_t(kPlanWarps) * size_t(experts) * sizeof(int);
   cudaError_t e = cudaSuccess;
-  if (smem > 32 * 1024) e = cudaFuncSetAttribute(plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem));
+  // Always to the most: a limit of this call's own would undercut a call of more experts that another thread is about
+  // to launch, or one captured into the same graph.
+  if (smem > 32 * 1024)
+    e = cudaFuncSetAttribute(plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(kPlanWarps * kMaxExperts * sizeof(int)));
   if (e != cudaSuccess) return cuda_fail(e, "kl_moe_plan shared memory");
   void* args[] = {&a};
   e = launch(static_cast<cudaStream_t>(stream), dim3(unsigned(cluster)), kPlanThreads, smem, cluster,

@@ -56,6 +56,51 @@ def test_route_weights_far_below_the_largest(cuda, experts):
         within(r.weights, want, want * (reach + 16) * U + 2.0 ** -149, f"renormalize {renormalize}")
 
 
+# ------------------------------------------------------------------------------------ plans of several sizes
+
+
+def test_plans_of_many_and_few_experts_in_one_graph(cuda):
+    many, few = (torch.randint(-1, e, (700, 3), generator=gen(e), dtype=torch.int32).to(cuda) for e in (1024, 300))
+    want = (*kl.moe_plan(many, 1024), *kl.moe_plan(few, 300))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = (*kl.moe_plan(many, 1024), *kl.moe_plan(few, 300))
+    kl.moe_plan(few, 300)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_plans_of_many_and_few_experts_from_two_threads(cuda):
+    """Every call keeps the shared memory that it needs, whatever another thread plans."""
+    import threading
+
+    sizes = (1024, 300)
+    ids = [torch.randint(-1, e, (700, 3), generator=gen(e), dtype=torch.int32).to(cuda) for e in sizes]
+    want = [kl.moe_plan(i, e) for i, e in zip(ids, sizes)]
+    torch.cuda.synchronize()
+    wrong = []
+
+    def plan(at):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                for _ in range(2000):
+                    got = kl.moe_plan(ids[at], sizes[at])
+                torch.cuda.current_stream().synchronize()
+                if not all(torch.equal(a, b) for a, b in zip(got, want[at])):
+                    wrong.append("another plan")
+                torch.cuda.current_stream().synchronize()
+        except Exception as e:
+            wrong.append(e)
+
+    threads = [threading.Thread(target=plan, args=(at,)) for at in (0, 1)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong, wrong
+
+
 # ------------------------------------------------------------------------------------ combine's gradients, one by one
 
 
