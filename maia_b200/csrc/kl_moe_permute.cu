@@ -15,6 +15,7 @@
 #include <kl/arch/griddep.hpp>
 #include <kl_gemm.h>
 
+#include "kl_experts.cuh"
 #include "kl_internal.cuh"
 #include "kl_vec.cuh"
 
@@ -23,8 +24,6 @@ namespace cg = cooperative_groups;
 namespace kl::capi {
 namespace {
 
-constexpr int kMaxExperts = 1024;
-constexpr int kMaxTopK = 32;
 constexpr int kPlanThreads = 1024;
 constexpr int kPlanWarps = kPlanThreads / 32;
 constexpr int kPlanBlocks = 8;  // of the cluster, where one does not do
@@ -387,24 +386,6 @@ __global__ void __launch_bounds__(kRowThreads) combine_grad_kernel(const RowArgs
   }
 }
 
-cudaError_t launch(cudaStream_t stream, dim3 grid, int threads, size_t smem, int cluster, void const* kernel, void** args) {
-  cudaLaunchConfig_t cfg = {};
-  cudaLaunchAttribute attr[2];
-  cfg.gridDim = grid;
-  cfg.blockDim = dim3(unsigned(threads), 1, 1);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = stream;
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  attr[1].id = cudaLaunchAttributeClusterDimension;
-  attr[1].val.clusterDim.x = unsigned(cluster);
-  attr[1].val.clusterDim.y = 1;
-  attr[1].val.clusterDim.z = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = cluster > 1 ? 2 : 1;
-  return cudaLaunchKernelExC(&cfg, kernel, args);
-}
-
 // Bytes that every one of the values is a multiple of: 16, 8, 4, 2 or 1.
 int common_granule(std::initializer_list<uint64_t> values) {
   uint64_t all = 16;
@@ -460,14 +441,8 @@ extern "C" kl_status kl_moe_plan(const int32_t* ids, int64_t tokens, int64_t k, 
   const long long warps = (long long)cluster * kPlanWarps;
   a.warp_span = (a.total + warps * 32 - 1) / (warps * 32) * 32;
   const size_t smem = size_t(kPlanWarps) * size_t(experts) * sizeof(int);
-  cudaError_t e = cudaSuccess;
-  // Always to the most: a limit of this call's own would undercut a call of more experts that another thread is about
-  // to launch, or one captured into the same graph.
-  if (smem > 32 * 1024)
-    e = cudaFuncSetAttribute(plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(kPlanWarps * kMaxExperts * sizeof(int)));
-  if (e != cudaSuccess) return cuda_fail(e, "kl_moe_plan shared memory");
   void* args[] = {&a};
-  e = launch(static_cast<cudaStream_t>(stream), dim3(unsigned(cluster)), kPlanThreads, smem, cluster,
+  cudaError_t e = launch_dependent(static_cast<cudaStream_t>(stream), dim3(unsigned(cluster)), kPlanThreads, smem, cluster,
              reinterpret_cast<void const*>(&plan_kernel), args);
   return e == cudaSuccess ? KL_OK : cuda_fail(e, "kl_moe_plan launch");
 }
@@ -503,7 +478,7 @@ extern "C" kl_status kl_moe_dispatch(const void* x, int64_t ldx_bytes, int64_t t
                        : g == 2 ? reinterpret_cast<void const*>(&dispatch_kernel<2>)
                                 : reinterpret_cast<void const*>(&dispatch_kernel<1>);
   void* args[] = {&a};
-  cudaError_t e = launch(static_cast<cudaStream_t>(stream), dim3(unsigned(tokens + (m + kPadRows - 1) / kPadRows)),
+  cudaError_t e = launch_dependent(static_cast<cudaStream_t>(stream), dim3(unsigned(tokens + (m + kPadRows - 1) / kPadRows)),
                          kRowThreads, 0, 1, kernel, args);
   return e == cudaSuccess ? KL_OK : cuda_fail(e, "kl_moe_dispatch launch");
 }
@@ -563,7 +538,7 @@ extern "C" kl_status kl_moe_combine(const void* y, int32_t type, int64_t ldy, in
   cudaError_t e = cudaSuccess;
   by_cells(type, g, [&](auto t, auto v) {
     void* args[] = {&a};
-    e = launch(static_cast<cudaStream_t>(stream), dim3(unsigned(tokens), unsigned(parts)), kRowThreads, 0, 1,
+    e = launch_dependent(static_cast<cudaStream_t>(stream), dim3(unsigned(tokens), unsigned(parts)), kRowThreads, 0, 1,
                reinterpret_cast<void const*>(&combine_kernel<decltype(t), decltype(v)::value>), args);
   });
   return e == cudaSuccess ? KL_OK : cuda_fail(e, "kl_moe_combine launch");
@@ -612,7 +587,7 @@ extern "C" kl_status kl_moe_combine_grad(const void* dout, int64_t ld_dout, cons
   cudaError_t e = cudaSuccess;
   by_cells(type, g, [&](auto t, auto v) {
     void* args[] = {&a};
-    e = launch(static_cast<cudaStream_t>(stream), dim3(unsigned(tokens + pad_parts)), kRowThreads, 0, 1,
+    e = launch_dependent(static_cast<cudaStream_t>(stream), dim3(unsigned(tokens + pad_parts)), kRowThreads, 0, 1,
                reinterpret_cast<void const*>(&combine_grad_kernel<decltype(t), decltype(v)::value>), args);
   });
   return e == cudaSuccess ? KL_OK : cuda_fail(e, "kl_moe_combine_grad launch");

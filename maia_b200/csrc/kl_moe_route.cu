@@ -23,6 +23,7 @@
 #include <kl/arch/griddep.hpp>
 #include <kl_gemm.h>
 
+#include "kl_experts.cuh"
 #include "kl_internal.cuh"
 #include "kl_vec.cuh"
 
@@ -33,8 +34,6 @@ namespace {
 
 constexpr int kRouteThreads = 512;
 constexpr int kRouteWarps = kRouteThreads / 32;
-constexpr int kMaxExperts = 1024;
-constexpr int kMaxTopK = 32;
 
 // Ordering keys: larger key = earlier choice. The value's bits in an order-preserving form sit above
 // 1023 - e, so one integer maximum gives the largest value and, among equals, the lowest expert.
@@ -592,28 +591,6 @@ bool vector_rows(const void* p, int64_t ld, int64_t experts, int32_t type) {
   return aligned16(p) && ld * size % 16 == 0 && experts % 8 == 0;
 }
 
-cudaError_t launch(cudaStream_t stream, int grid, int threads, size_t smem, int cluster, void const* kernel, void** args) {
-  cudaLaunchConfig_t cfg = {};
-  cudaLaunchAttribute attr[2];
-  cfg.gridDim = dim3(unsigned(grid), 1, 1);
-  cfg.blockDim = dim3(unsigned(threads), 1, 1);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = stream;
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  attr[1].id = cudaLaunchAttributeClusterDimension;
-  attr[1].val.clusterDim.x = unsigned(cluster);
-  attr[1].val.clusterDim.y = 1;
-  attr[1].val.clusterDim.z = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = cluster > 1 ? 2 : 1;
-  if (smem > 48 * 1024) {
-    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem));
-    if (e != cudaSuccess) return e;
-  }
-  return cudaLaunchKernelExC(&cfg, kernel, args);
-}
-
 }  // namespace
 }  // namespace kl::capi
 
@@ -669,13 +646,13 @@ extern "C" kl_status kl_moe_route(const kl_moe_route_desc* d, void* workspace, s
       using T = decltype(t);
       void const* kernel = a.k <= 8 ? reinterpret_cast<void const*>(&route_kernel<T, l(), nv(), 8>)
                                     : reinterpret_cast<void const*>(&route_kernel<T, l(), nv(), kMaxTopK>);
-      e = launch(st, blocks, kRouteThreads, size_t(kRouteWarps) * l() * 8 * nv() * sizeof(float), 1, kernel, args);
+      e = launch_dependent(st, blocks, kRouteThreads, size_t(kRouteWarps) * l() * 8 * nv() * sizeof(float), 1, kernel, args);
     });
   });
   if (e == cudaSuccess && blocks > 1) {
     int b = blocks;
     void* args[] = {&a, &b};
-    e = launch(st, kFinishBlocks, kFinishThreads, 0, kFinishBlocks, reinterpret_cast<void const*>(&route_finish_kernel), args);
+    e = launch_dependent(st, kFinishBlocks, kFinishThreads, 0, kFinishBlocks, reinterpret_cast<void const*>(&route_finish_kernel), args);
   }
   return e == cudaSuccess ? KL_OK : cuda_fail(e, "kl_moe_route launch");
 }
@@ -720,7 +697,7 @@ extern "C" kl_status kl_moe_route_grad(const kl_moe_route_desc* d, const float* 
   by_type(d->logits_type, [&](auto t) {
     by_width(a.experts, [&](auto l, auto nv) {
       void* args[] = {&a};
-      e = launch(static_cast<cudaStream_t>(stream), blocks, kGradThreads, 0, 1,
+      e = launch_dependent(static_cast<cudaStream_t>(stream), blocks, kGradThreads, 0, 1,
                  reinterpret_cast<void const*>(&route_grad_kernel<decltype(t), l(), nv()>), args);
     });
   });
