@@ -280,9 +280,11 @@ KL_API kl_status kl_moe_combine_grad(const void* dout, int64_t ld_dout, const vo
  * single tokens, straight from kl_moe_route's ids; an id may repeat); an id outside [0, experts)
  * gives zeros. x and q - zeros enter with all their bits and every sum is exact or fp32, in an order that
  * depends on the shape and on the tokens that a matrix meets. A NaN or infinity in a row of x makes that row of out NaN or
- * infinite, and no other. The weights stream once for up to 16 tokens of a matrix; more take a pass for
- * every 16. Allocates nothing, keeps
- * nothing; stream-ordered; may be captured. No counterpart in the reference. */
+ * infinite, and no other. A pass over a matrix takes up to 1, 2, 8 or 16 of its tokens: the least that holds
+ * them, else 16; with ids the least that holds ceil(tokens topk / experts), so an expert with more tokens
+ * than that has several passes. 16 at a time need k <= 22528, 8 at a time k <= 28672 (18432 and 20480 do
+ * with any ids); with longer rows 8, then 2 go at a time. Allocates nothing, keeps nothing;
+ * stream-ordered; may be captured. No counterpart in the reference. */
 typedef struct kl_int4_desc {
   const void* x;        /* device [tokens, ldx], x_type KL_BF16 or KL_F16; 16-byte aligned, ldx % 8 == 0;
                          * x_per_slot: [tokens topk, ldx] */

@@ -1077,8 +1077,10 @@ kl_status launch(Fit const& f, int device, cudaStream_t stream) {
   return e == cudaSuccess ? KL_OK : cuda_fail(e, "kl_gemv_int4 launch");
 }
 
-// Tokens of a pass by what a matrix meets (with ids: on average), fewer where x would not fit. 28672 x 8192: 2
-// tokens 26 us, in the form for 8 42; 4 tokens 42, in two passes of 2 47; 16 tokens 60, in two passes of 8 85.
+// Tokens of a pass by what a matrix meets (with ids: on average), fewer where x would not fit: 16 above K = 22528, 8 above
+// 28672, a little less with long lists. 28672 x 8192: 2 tokens 26 us, in the form for 8 42; 4 tokens 42, in two passes of 2
+// 47; 16 tokens 60, in two passes of 8 85. 8192 rows, 16 tokens: K = 22528 52, 24576 71 (two passes of 8), 32768 200
+// (eight of 2). 16 tokens x 4 of 64, 4096 x 1536, groups of 32: 53 us with even ids, 51 where one expert has every token.
 template <class T, int GROUP, bool kZeros>
 kl_status by_tokens(Int4Args& a, int device, cudaStream_t stream) {
   const int tokens = a.ids != nullptr ? (a.slots + a.experts - 1) / a.experts : a.slots;

@@ -4,8 +4,9 @@
 // kl_moe_combine_grad.
 //
 // The last three move rows and are bound by memory. Measured on 8192 tokens, 4 experts each, rows of 4096 bf16:
-// dispatch 83.9 us (5.6 TB/s; 72.5 us at the copy rate), combine 57.0 (5.4 TB/s), its gradient 112.4 (5.7 TB/s). The
-// plan is a latency: 5.8 us for 662 slots, 10.7 for 32768.
+// dispatch 83.6 us (5.6 TB/s; 72.5 us at the copy rate), combine 56.4 (5.4 TB/s), its gradient 112.0 (5.7 TB/s). The
+// plan is a latency: 5.2 us for 662 slots, 10.3 for 32768 (64 experts); one cluster takes all sizes, 131072 slots 35 us, 2^20 240
+// (256 experts: 42 and 281).
 
 #include <cooperative_groups.h>
 #include <cuda_runtime.h>

@@ -12,8 +12,9 @@
 // eight keys once (19 exchanges), after which each of the k rounds takes one warp-wide maximum and a shift in the lane that
 // held it (two sorted keys a lane, enough for four tokens of ten, and a second search for the rest: 69 us instead
 // of 62).
-// Measured, 131072 tokens of 256 bf16 experts, k = 8: routing and its sums 62 us (353 instructions a token, half of
-// them on the integer pipe, which is full), gradient 45 us (280 a token). One token of 64 fp32 experts: 3.8 us.
+// Measured, 131072 tokens of 256 bf16 experts, k = 8: routing and its sums 61 us (361 instructions a token, half of
+// them on the integer pipe, which is full), gradient 44 us (280 a token). One token of 64 fp32 experts: 3.3 us. Above 512
+// experts fp32 keys and values do not fit the registers (300 bytes a thread spill): 32768 x 1024 112 and 77 us.
 
 #include <cooperative_groups.h>
 #include <cuda_runtime.h>

@@ -314,7 +314,9 @@ def gemv_int4(x, q, scales, zeros=None, *, group: int = 128, ids=None, out=None,
     multiple of 32. With int32 ids [tokens, k]: q [E, N, K / 2], scales and zeros [E, N, ...], x [tokens, K]
     or [tokens, k, K], out [tokens, k, N] with expert ids[t, j] (rows of zeros for ids outside 0 .. E - 1;
     at most 4096 ids, 1024 experts). out in x's type or fp32. x enters with all its bits, sums are exact or fp32; a NaN
-    or infinity makes its row NaN or infinite. Up to 16 tokens of a matrix read the weights once. K up to 65536."""
+    or infinity makes its row NaN or infinite. K up to 65536. Up to 16 tokens of a matrix read its weights once (8 where
+    K > 22528, 2 where K > 28672, by ids a little earlier). With ids the number goes by the average of ids to an expert,
+    rounded up to 1, 2, 8 or 16; an expert with more reads its weights several times."""
     if stream is not None:
         return _on_stream(stream, (x, q, scales, zeros, ids, out),
                           lambda: gemv_int4(x, q, scales, zeros, group=group, ids=ids, out=out, out_dtype=out_dtype))
