@@ -193,7 +193,8 @@ def _on_stream(stream: int, tensors, call):
     with torch.cuda.stream(there):
         result = call()
     for t in tensors:
-        t.record_stream(there)
+        if t.is_cuda:  # not a scale in mapped host memory
+            t.record_stream(there)
     for t in result if isinstance(result, tuple) else (result,):
         if t is not None:
             t.record_stream(there)

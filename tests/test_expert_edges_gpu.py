@@ -56,6 +56,48 @@ def test_route_weights_far_below_the_largest(cuda, experts):
         within(r.weights, want, want * (reach + 16) * U + 2.0 ** -149, f"renormalize {renormalize}")
 
 
+# ------------------------------------------------------------------------------------ offsets behind 2^31
+
+
+def test_rows_behind_2_to_the_31_elements(cuda):
+    """Dispatch, combine and its gradient on matrices of more than 2^31 elements."""
+    tokens, width = 67000, 32776
+    x = torch.empty((tokens, width), dtype=torch.bfloat16, device=cuda)
+    x.copy_(torch.arange(width, device=cuda)[None] % 64)
+    x[:, 0] = (torch.arange(tokens, device=cuda) % 256).bfloat16()
+    x[:, 1] = (torch.arange(tokens, device=cuda) // 256).bfloat16()  # both exact: every row has its own
+    ids = torch.randint(0, 3, (tokens, 1), generator=gen(1), dtype=torch.int32).to(cuda)
+    plan = kl.moe_plan(ids, 3)
+    a = kl.moe_dispatch(x, plan)
+    assert a.numel() > 2 ** 31
+    slots = plan.slots.long()
+    live = slots >= 0
+    assert torch.equal(a[live, :2], x[slots[live], :2]) and not a[~live].any()
+    assert torch.equal(a[-200:], torch.where(live[-200:, None], x[slots[-200:].clamp(min=0)], 0))
+    w = torch.full((tokens, 1), 0.5, device=cuda)
+    out = kl.moe_combine(a, w, rows=plan.rows)
+    assert torch.equal(out[-200:], x[-200:] / 2) and torch.equal(out[:, :2], x[:, :2] / 2)
+    del out
+    dy, dw = kl.moe_combine_grad(x, a, w, rows=plan.rows, slots=plan.slots)
+    assert torch.equal(dy[live, :2], x[slots[live], :2] / 2) and not dy[~live].any()
+    tail = x[-200:].double().square().sum(1)
+    within(dw[-200:, 0], tail, tail * (width / 256 + 32) * U)
+
+
+def test_routing_behind_2_to_the_31_logits(cuda):
+    tokens, experts, k = 2 ** 21 + 300, 1024, 2
+    x = torch.empty((tokens, experts), dtype=torch.bfloat16, device=cuda).uniform_(-1, 1)
+    assert x.numel() > 2 ** 31
+    x[-300:, 7], x[-300:, 1000] = 3.0, 2.5
+    r = kl.moe_route(x, k)
+    assert r.tokens.item() == tokens and r.counts.sum().item() == tokens * k
+    assert (r.ids[-300:] == torch.tensor([7, 1000], device=cuda)).all()
+    g = kl.moe_route_grad(x, r, torch.ones_like(r.weights) * torch.tensor([1.0, -1.0], device=cuda))
+    w = r.weights[-300:].double()
+    want = 2 * w[:, 0] * w[:, 1]      # w0 (1 - (w0 - w1)) = 2 w0 w1
+    within(g[-300:, 7], want, want * (HALF[torch.bfloat16] * 1.001 + 64 * U) + 2.0 ** -24)
+
+
 # ------------------------------------------------------------------------------------ plans of several sizes
 
 
@@ -337,6 +379,22 @@ def test_one_row_of_a_wider_buffer(cuda):
     assert all(torch.equal(a, b) for a, b in zip(r, whole))
     dw = torch.randn((1, 4), generator=gen(4)).to(cuda)
     assert torch.equal(kl.moe_route_grad(logits[:1, :64], r, dw), kl.moe_route_grad(logits[:1, :64].contiguous(), r, dw))
+
+
+
+@pytest.mark.parametrize("tokens", [1, 20])
+def test_gemv_int4_weights_behind_2_to_the_31_bytes(cuda, tokens):
+    """The last of the experts lies 2 GB behind the first, its scales 2^27 elements."""
+    experts, n, k, group = 130, 16384, 2048, 32
+    q = torch.empty((experts, n, k // 2), dtype=torch.uint8, device=cuda).random_(0, 256)
+    s = torch.empty((experts, n, k // group), dtype=torch.bfloat16, device=cuda).uniform_(0.001, 0.02)
+    ids = torch.tensor([[experts - 1, 0]], dtype=torch.int32, device=cuda).repeat(tokens, 1)
+    x = torch.randn((tokens, k), generator=gen(1)).bfloat16().to(cuda)
+    got = kl.gemv_int4(x, q, s, group=group, ids=ids, out_dtype=torch.float32)
+    for j, e in enumerate((experts - 1, 0)):
+        w = (torch.stack([q[e] & 15, q[e] >> 4], -1).flatten(-2).double() - 8) * s[e].double().repeat_interleave(group, 1)
+        want = x.double() @ w.T
+        within(got[:, j], want, product_tol(x, w, want, torch.float32), f"expert {e}")
 
 
 # ------------------------------------------------------------------------------------ streams
